@@ -7,7 +7,7 @@ operations in 32 bits (angles of decays in 64); with ``own`` true it calls the
 package.  ``exact`` is the operator's definition in 64 bits.  The kinds:
 
 * ``chunk``  the gated delta rule over packed sequences, forward alone
-             (``ssla_amd.delta.chunk_gated_delta_rule``), or with ``grad``
+             (``ssla_amd.delta.chunk_gated_delta``), or with ``grad``
              forward and backward;
 * ``sites``  ragged histories of many sites at once, their states gathered from
              and written back to a resident table
@@ -256,8 +256,8 @@ def run(s):
         return y.detach(), *torch.autograd.grad(y, (s["x"], s["w"], s["b"]), s["dy"])
     x = s["q"], s["k"], s["v"], s["g"], s["beta"]
     if own:
-        from ssla_amd.delta import chunk_gated_delta_rule
-        o, ht = chunk_gated_delta_rule(*x, s["cu"], scale=s["scale"], initial_state=s["h0"], output_final_state=True)
+        from ssla_amd.delta import chunk_gated_delta
+        o, ht = chunk_gated_delta(*x, s["cu"], scale=s["scale"], initial_state=s["h0"], output_final_state=True)
     else:
         o, ht = _plain_chunk(*x, s["cu"], s["longest"], s["scale"], s["h0"])
         o = o.to(s["v"].dtype)
