@@ -228,6 +228,51 @@ int ssla_gla_recurrent_fwd(const void *q, const void *k, const void *v,
 int ssla_seq_bounds_async(const int64_t *cu_seqlens, int n_seq, int64_t *host_out, void *event, void *stream);
 
 /* ------------------------------------------------------------------------
+ * Gated delta rule (no reference counterpart): per sequence and head
+ *   S <- exp(g_t) S;  u_t = beta_t (v_t - S^T k_t);  S <- S + k_t u_t^T;
+ *   o_t = scale S^T q_t
+ * q, k: [T, Hk, K]; v, o: [T, H, V] (all of dtype `dtype`), H a multiple of
+ * Hk: value head h reads key head h / (H / Hk).  g (log-gates, -inf empties
+ * the state), beta: fp32 [T, H].  States fp32 [n_seq, H, K, V]; h0 NULL =
+ * zeros, ht NULL = not wanted.  Sequences are clamped to [0, T) on the
+ * device; rows of o outside [cu_seqlens[0], cu_seqlens[n_seq]) are left as
+ * they were.
+ * ------------------------------------------------------------------------ */
+
+/* Token by token, the state in registers: K <= 256, any V.  cu_seqlens NULL
+ * (with T == n_seq): sequence n is row n.  state_idx (int32 [n_seq] or NULL)
+ * redirects the states as for ssla_gla_recurrent_fwd: h0 and ht may be the same
+ * table of n_state_rows rows; an entry out of range or not above the one
+ * before it is skipped (zero o rows, no state touched, SSLA_ERR_ARG in
+ * *status).  Entries that are equal without being neighbours, which only a
+ * list that is not increasing holds, leave their row's state unspecified. */
+int ssla_gated_delta_recurrent(const void *q, const void *k, const void *v, const float *g, const float *beta,
+                               const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,
+                               float scale, const float *h0, void *o, float *ht, const int32_t *state_idx,
+                               int n_state_rows, int32_t *status, int dtype, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Group norm with an activation, channels last (no reference counterpart):
+ *   y = act((x - mean) / sqrt(var + eps) * weight + bias)
+ * x, y: [N, L, C] of dtype `dtype`; mean and variance over the L positions of a
+ * sample and the C / G channels of a group (fp32).  weight, bias: fp32 [C] or
+ * NULL.  act: SSLA_ACT_*.  stats (fp32 [N, G, 2], or NULL when no backward
+ * follows) receives each group's mean and 1 / sqrt(var + eps).
+ * The backward takes dy in x's dtype and x and stats of the forward; dx (x's
+ * dtype), dweight and dbias (fp32 [C], summed in a fixed order) may be NULL.
+ * Workspaces: the queried bytes, 16-byte aligned, no initialisation; 0: none.
+ * ------------------------------------------------------------------------ */
+enum { SSLA_ACT_NONE = 0, SSLA_ACT_RELU = 1, SSLA_ACT_SILU = 2 };
+size_t ssla_group_norm_workspace_size(int64_t N, int64_t L, int C, int G);
+int ssla_group_norm_fwd(const void *x, int64_t N, int64_t L, int C, int G, const float *weight, const float *bias,
+                        float eps, int act, void *y, float *stats, int dtype, void *workspace,
+                        size_t workspace_bytes, void *stream);
+size_t ssla_group_norm_bwd_workspace_size(int64_t N, int64_t L, int C, int G);
+int ssla_group_norm_bwd(const void *dy, const void *x, const float *stats, int64_t N, int64_t L, int C, int G,
+                        const float *weight, const float *bias, int act, void *dx, float *dweight, float *dbias,
+                        int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
  * G2 -- sparse sequential scans.
  * ------------------------------------------------------------------------ */
 

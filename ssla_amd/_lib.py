@@ -6,6 +6,7 @@ loaded every entry point raises -- there is no fallback implementation.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import os
 import threading
@@ -73,6 +74,13 @@ SIGNATURES = {
     "ssla_diag_scan_bwd": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp]),
     "ssla_sparse_gla_step": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
                                     _f32, _vp, _vp, _vp]),
+    "ssla_gated_delta_recurrent": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
+                                          _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
+    "ssla_group_norm_workspace_size": (_sz, [_i64, _i64, _i32, _i32]),
+    "ssla_group_norm_fwd": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _f32, _i32, _vp, _vp, _i32, _vp, _sz, _vp]),
+    "ssla_group_norm_bwd_workspace_size": (_sz, [_i64, _i64, _i32, _i32]),
+    "ssla_group_norm_bwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _sz,
+                                   _vp]),
     "ssla_status_read": (_i32, [_vp, C.POINTER(_i32), _vp]),
     "ssla_site_project": (_i32, [_vp, _i64, _i32, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _vp]),
     "ssla_site_finish": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _f32, _i32, _vp, _vp]),
@@ -204,6 +212,16 @@ def ptr(t: torch.Tensor | None) -> int | None:
 def stream_of(t: torch.Tensor) -> int:
     """The raw handle of the current stream of t's device."""
     return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+_SAME_DEVICE = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """A context in which t's device is the current one (a kernel is launched
+    on a stream of the current device)."""
+    dev = t.get_device()
+    return _SAME_DEVICE if torch.cuda.current_device() == dev else torch.cuda.device(dev)
 
 
 class HostWords:
