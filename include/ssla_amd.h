@@ -251,6 +251,18 @@ int ssla_gated_delta_recurrent(const void *q, const void *k, const void *v, cons
                                float scale, const float *h0, void *o, float *ht, const int32_t *state_idx,
                                int n_state_rows, int32_t *status, int dtype, void *stream);
 
+/* By chunks of 64 rows, all products on the matrix cores with the precision of
+ * fp32 (fp32 values as sums of bf16): K <= 128, any V.  A row whose k, g or beta
+ * is not finite (a g of -inf is) makes its head's o and state NaN from that
+ * row on, one of v its column; earlier rows keep their values.  Workspace:
+ * ssla_gated_delta_chunk_workspace_size bytes, 16-byte aligned, no
+ * initialisation. */
+size_t ssla_gated_delta_chunk_workspace_size(int n_seq, int64_t T, int H, int K, int V);
+int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, const float *g, const float *beta,
+                               const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,
+                               float scale, const float *h0, void *o, float *ht, int dtype, void *workspace,
+                               size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------------------------
  * Group norm with an activation, channels last (no reference counterpart):
  *   y = act((x - mean) / sqrt(var + eps) * weight + bias)

@@ -1,0 +1,703 @@
+// Chunked gated delta rule, forward, on gfx950.
+//
+// Per sequence and head, S <- e^(g_t) S, u_t = beta_t (v_t - S^T k_t),
+// S <- S + k_t u_t^T, o_t = scale S^T q_t.  In a chunk of 64 rows, with G the
+// inclusive sum of g from the chunk's start and S the state entering it,
+//   u = Tm X,  X_i = beta_i (v_i - e^(G_i) S^T k_i),
+//   Tm = (I + A)^-1,  A_ij = beta_i e^(G_i - G_j) k_i . k_j  (j < i),
+//   o_i = scale e^(G_i) S^T q_i + sum_(j <= i) P_ij u_j,
+//   P_ij = scale e^(G_i - G_j) q_i . k_j,
+//   S' = e^(G_last) S + sum_j k_j (e^(G_last - G_j) u_j)^T.
+// Tm needs no state: one kernel computes it for all chunks side by side (unit
+// lower triangular, by forward substitution in 16 x 16 blocks whose inverses
+// are joined: no power of A, so equal keys lose no digits).  The walk then
+// carries the states from chunk to chunk, one wavefront per 16 value columns,
+// which do not need each other.
+//
+// Long sequences are cut into segments that run side by side: over a segment
+// the state goes through an affine map S -> M S + L, and the columns of M are
+// columns of a state that enters as the identity with v = 0.  A pass over all
+// segments but a sequence's last computes L and M, a fold carries the states
+// over the segments, and the walk starts every segment from its state.
+//
+// Values that are not finite: a row whose k, beta or g is not finite makes all
+// columns of its head NaN from that row on, one in v or in a state its own
+// column; earlier rows are computed without them.
+#include "delta_tile.h"
+#include "seq_slots.h"
+
+namespace ssla {
+namespace {
+
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+
+// -------------------------------------------------- matrices of the chunks --
+// One workgroup per (chunk slot, head): the row factors and Tm.
+template <int DT, int KP>
+__global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict__ k, const float *__restrict__ g,
+                                                         const float *__restrict__ beta,
+                                                         const int64_t *__restrict__ cu, int n_seq, int64_t T, int Hk,
+                                                         int H, int K, int vec, float scale, float *__restrict__ tm,
+                                                         float *__restrict__ rowv) {
+  constexpr int NP = Parts<DT>::n, LD = 68;
+  __shared__ __align__(16) uint16_t sk[NP][kChunk * KP];
+  __shared__ __align__(16) float A[kChunk][LD];   // I + A, then Tm
+  __shared__ __align__(16) float Y[32][LD - 32];  // a product between two of the joins
+  __shared__ float sv[kRowVecs][kChunk];
+  __shared__ float diag[kChunk];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int h = static_cast<int>(blockIdx.x % H), hk = h / (H / Hk);
+  const int64_t slot = blockIdx.x / H;
+  int n;
+  int64_t bos, eos, first;
+  if (!seq_of_slot(cu, n_seq, T, kChunk, slot, n, bos, eos, first)) return;   // workgroup-uniform
+  const int64_t t0 = bos + (slot - first) * kChunk;
+  if (t0 >= eos) return;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+
+  RowTile<DT, KP> kt;
+  kt.fetch(k, t0, rows, Hk, hk, K, vec);
+  float gv = 0.f, bv = 0.f;
+  if (w == 0 && lane < rows) {
+    gv = g[(t0 + lane) * H + h];
+    bv = beta[(t0 + lane) * H + h];
+  }
+  kt.store(&sk[0][0], kChunk * KP);
+  __syncthreads();
+
+  // Gram matrix k k^T: wavefront w computes the row tile w
+  f32x4 acc[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < KP / 32; ++ks) {
+    bf16x8 a[NP];
+#pragma unroll
+    for (int i = 0; i < NP; ++i) a[i] = op_rows<KP>(sk[i], w, ks, lane);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j > (w | 1)) continue;   // columns past the rows' pair: above the diagonal
+      bf16x8 b[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) b[i] = op_rows<KP>(sk[i], j, ks, lane);
+      acc[j] = mul<2>(a, b, acc[j]);
+    }
+  }
+  {   // the diagonal tells whether a row of k is finite
+    const int r = (lane >> 4) * 4, m = lane & 15;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j == w && m >= r && m < r + 4) {
+        const f32x4 v4 = acc[j];
+        diag[idx_of(w, m)] = m == r ? v4[0] : m == r + 1 ? v4[1] : m == r + 2 ? v4[2] : v4[3];
+      }
+  }
+  __syncthreads();
+  if (w == 0) {
+    // a row that is not finite (a gate of -inf is: it empties the state) and
+    // those after it are left out of Tm; its beta becomes NaN, which the walk
+    // turns into NaN for all that follows
+    const bool bad = lane < rows && !(finite(diag[lane]) && finite(bv) && gv < 3.402823466e38f);
+    const unsigned long long any = __ballot(bad);
+    const int r0 = any ? __ffsll(static_cast<long long>(any)) - 1 : kChunk;
+    if (lane >= r0) {
+      gv = 0.f;
+      bv = lane == r0 ? __builtin_nanf("") : 0.f;
+    }
+    // e^-150 is 0 in fp32; sums in 64 bits, kept as two floats, so that
+    // differences of far sums stay exact
+    double G = static_cast<double>(fmaxf(gv, -150.f)) * 1.4426950408889634;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double up = __shfl_up(G, d);
+      if (lane >= d) G += up;
+    }
+    const float hi = static_cast<float>(G), lo = static_cast<float>(G - static_cast<double>(hi));
+    const float eg = fast_exp2(hi) * fast_exp2(lo), last = __shfl(hi, 63), last_lo = __shfl(lo, 63);
+    sv[kBeta][lane] = bv;
+    sv[kBetaG][lane] = bv * eg;
+    sv[kScaleG][lane] = scale * eg;
+    sv[kToEnd][lane] = fast_exp2((last - hi) + (last_lo - lo));
+    sv[kGHi][lane] = hi;
+    sv[kGLo][lane] = lo;
+    diag[lane] = lane < r0 ? bv : 0.f;   // now: beta of the rows that Tm takes
+  }
+  __syncthreads();
+  {
+    const int col = lane & 15, r = (lane >> 4) * 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = idx_of(w, r + i), c = idx_of(j, col);
+        float x = row == c ? 1.f : 0.f;
+        // (a selection, not a product: what is above the diagonal or left out may be NaN)
+        if (c < row && diag[row] != 0.f)
+          x = diag[row] * acc[j][i] * fast_exp2((sv[kGHi][row] - sv[kGHi][c]) + (sv[kGLo][row] - sv[kGLo][c]));
+        A[row][c] = x;
+      }
+  }
+  // (rows r0.. have beta 0, so row r0's NaN keys reach no other row: row > c >= r0 is left out by its own beta)
+  __syncthreads();
+  // the four diagonal blocks of 16, inverted in place: lane = (block, column)
+  if (w == 0) {
+    const int b = 16 * (lane >> 4), c = lane & 15;
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float s = i == c ? 1.f : 0.f;
+#pragma unroll
+      for (int j = 0; j < i; ++j) s = fmaf(-A[b + i][b + j], x[j], s);
+      x[i] = s;
+    }
+    // (one wavefront: all reads above are done before the writes)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) A[b + i][b + c] = i < c ? 0.f : x[i];
+  }
+  __syncthreads();
+  // joins: [[P, 0], [C, Q]]^-1 = [[P^-1, 0], [-Q^-1 C P^-1, Q^-1]]
+  {   // blocks of 16, two pairs: 128 threads each, a row and two columns
+    const int pr = tid >> 7, i = (tid & 127) >> 3, c = (tid & 7) * 2, b = 32 * pr;
+    float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float a = A[b + 16 + i][b + j];
+      y0 = fmaf(a, A[b + j][b + c], y0);
+      y1 = fmaf(a, A[b + j][b + c + 1], y1);
+    }
+    Y[16 * pr + i][c] = y0;
+    Y[16 * pr + i][c + 1] = y1;
+    __syncthreads();
+    y0 = y1 = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const float a = A[b + 16 + i][b + 16 + j];
+      y0 = fmaf(a, Y[16 * pr + j][c], y0);
+      y1 = fmaf(a, Y[16 * pr + j][c + 1], y1);
+    }
+    A[b + 16 + i][b + c] = -y0;
+    A[b + 16 + i][b + c + 1] = -y1;
+  }
+  __syncthreads();
+  {   // blocks of 32: a row and four columns of each thread
+    const int i = tid >> 3, c = (tid & 7) * 4;
+    f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) y += A[32 + i][j] * *reinterpret_cast<const f32x4 *>(&A[j][c]);
+    *reinterpret_cast<f32x4 *>(&Y[i][c]) = y;
+    __syncthreads();
+    y = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+    for (int j = 0; j < 32; ++j) y += A[32 + i][32 + j] * *reinterpret_cast<const f32x4 *>(&Y[j][c]);
+    *reinterpret_cast<f32x4 *>(&A[32 + i][c]) = -y;
+  }
+  __syncthreads();
+  float *dst = tm + (slot * H + h) * kTriFloats;
+  for (int e = tid; e < kTriFloats / 4; e += 256) {
+    const int set = e >> 7, ln = (e >> 1) & 63, half = e & 1;
+    const int t = set < 2 ? set : 2 + ((set - 2) >> 1), ks = set < 2 ? 0 : (set & 1);
+    reinterpret_cast<f32x4 *>(dst)[e] =
+        *reinterpret_cast<const f32x4 *>(&A[idx_of(t, ln & 15)][32 * ks + 8 * (ln >> 4) + 4 * half]);
+  }
+  float *dv = rowv + (slot * H + h) * kRowFloats;
+  for (int e = tid; e < kRowFloats; e += 256) dv[e] = (&sv[0][0])[e];
+}
+
+// ----------------------------------------------------------------- the walk --
+struct WalkArgs {
+  const void *q, *k, *v;
+  const int64_t *cu;
+  const float *tm, *rowv;
+  const float *h0;
+  void *o;
+  float *ht;
+  float *seg_state;       // per inner segment: L, after the fold the state entering the next segment
+  uint16_t *seg_map;      // per inner segment: M as operands of three bf16 parts
+  int64_t T;
+  int n_seq, Hk, H, K, V, per, vec;
+  float scale;
+};
+
+template <int DT, int KP, bool OUT>
+struct WalkSmem {
+  static constexpr int NP = Parts<DT>::n, NO = DT == SSLA_F32 ? 3 : 2;
+  uint16_t k[NP][kChunk * KP];
+  uint16_t q[OUT ? NP : 1][OUT ? kChunk * KP : 8];
+  uint16_t tm[3][kTriSets * 512];
+  uint16_t p[OUT ? NO : 1][OUT ? kTriSets * 512 : 8];
+  float rowv[kRowVecs][kChunk];
+};
+
+// OUT: walks a segment from its entering state and writes o (and ht behind the
+// sequence's last row).  Otherwise: walks an inner segment from zero and from
+// the identity and writes L and M.
+// Four wavefronts, each with 16 columns of the state (its rows: the keys).
+template <int DT, int KP, bool OUT>
+__global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void delta_walk_kernel(const WalkArgs a) {
+  constexpr int NP = Parts<DT>::n, NO = DT == SSLA_F32 ? 3 : 2, LIMO = NO - 1, NT = KP / 16;
+  typedef Elem<DT> E;
+  __shared__ __align__(16) WalkSmem<DT, KP, OUT> sm;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, G = lane >> 4;
+  const int n_vt = (a.V + 15) >> 4, n_groups = (n_vt + (OUT ? 0 : NT) + 3) >> 2;
+  int64_t b = blockIdx.x;
+  const int grp = static_cast<int>(b % n_groups);
+  b /= n_groups;
+  const int h = static_cast<int>(b % a.H), hk = h / (a.H / a.Hk);
+  const int64_t slot = b / a.H;
+  const int64_t unit = static_cast<int64_t>(a.per) * kChunk;
+  int n;
+  int64_t bos, eos, first;
+  if (!seq_of_slot<OUT>(a.cu, a.n_seq, a.T, unit, slot, n, bos, eos, first)) return;   // workgroup-uniform
+  const int64_t seg = slot - first, t_begin = bos + seg * unit;
+  if (OUT ? (t_begin >= eos && seg > 0) : t_begin + unit >= eos) return;
+  const int64_t t_end = min(t_begin + unit, eos);
+  const int tile = grp * 4 + w;
+  const bool is_map = !OUT && tile >= n_vt;                  // this wavefront's columns are M's
+  const int vcol = tile * 16 + col, mcol = (tile - n_vt) * 16 + col;
+  const bool active = is_map ? mcol < KP : tile < n_vt, v_ok = !is_map && vcol < a.V;
+  const int64_t KV = static_cast<int64_t>(a.K) * a.V;
+
+  f32x4 S[NT];
+  {
+    const float *src = nullptr;
+    if (OUT) {
+      if (seg == 0) src = a.h0 ? a.h0 + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr;
+      else src = a.seg_state + ((bos / unit + seg - 1) * a.H + h) * KV;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = idx_of(t, 4 * G + r);
+        float x = is_map && key == mcol ? 1.f : 0.f;
+        if (OUT && src && v_ok && key < a.K) x = src[static_cast<int64_t>(key) * a.V + vcol];
+        S[t][r] = x;
+      }
+  }
+
+  RowTile<DT, KP> kt, qt;
+  f32x4 tmr[3], rvr;
+  typename E::T vr[16];
+  auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+    kt.fetch(a.k, t0, rows, a.Hk, hk, a.K, a.vec);
+    if constexpr (OUT) qt.fetch(a.q, t0, rows, a.Hk, hk, a.K, a.vec);
+    const int64_t c = (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h);
+    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * kTriFloats);
+    tmr[0] = src[2 * tid];
+    tmr[1] = src[2 * tid + 1];
+    tmr[2] = src[512 + tid];
+    if (tid < kRowFloats / 4) rvr = reinterpret_cast<const f32x4 *>(a.rowv + c * kRowFloats)[tid];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int t = idx_of(i >> 2, 4 * G + (i & 3));
+      vr[i] = (v_ok && t < rows) ? static_cast<const typename E::T *>(a.v)[((t0 + t) * a.H + h) * a.V + vcol]
+                                 : typename E::T(0);
+    }
+  };
+  auto stage = [&]() __attribute__((always_inline)) {
+    kt.store(&sm.k[0][0], kChunk * KP);
+    if constexpr (OUT) qt.store(&sm.q[0][0], kChunk * KP);
+    {   // sets 0 .. 3: a lane's eight values of one thread
+      bf16x8 s[3];
+      split(join(tmr[0], tmr[1]), s);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4 *>(&sm.tm[i][tid * 8]) = to_bits(s[i]);
+    }
+    {   // sets 4, 5: half a lane's values of each thread
+      bf16x8 s[3];
+      split(join(tmr[2], f32x4{0.f, 0.f, 0.f, 0.f}), s);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) {
+        const uint4 x = to_bits(s[i]);
+        *reinterpret_cast<uint2 *>(&sm.tm[i][2048 + tid * 4]) = make_uint2(x.x, x.y);
+      }
+    }
+    if (tid < kRowFloats / 4) reinterpret_cast<f32x4 *>(&sm.rowv[0][0])[tid] = rvr;
+  };
+  auto row8 = [&](int vec, int p) __attribute__((always_inline)) {   // rows 32 p + 8 G .. + 7 of a row vector
+    const f32x4 *s = reinterpret_cast<const f32x4 *>(&sm.rowv[vec][32 * p + 8 * G]);
+    return join(s[0], s[1]);
+  };
+
+  if (t_begin < t_end) fetch(t_begin);
+  for (int64_t t0 = t_begin; t0 < t_end; t0 += kChunk) {
+    stage();
+    f32x8 vv[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (DT == SSLA_BF16) vv[i >> 3][i & 7] = bf16_bits_to_f32(vr[i]);
+      else if constexpr (DT == SSLA_F16) vv[i >> 3][i & 7] = f16_bits_to_f32(vr[i]);
+      else vv[i >> 3][i & 7] = vr[i];
+    }
+    __syncthreads();
+    if (t0 + kChunk < t_end) fetch(t0 + kChunk);   // the next chunk's, in flight meanwhile
+
+    if constexpr (OUT) {
+      // P of this wavefront's row tile: k q^T has row j of P^T in the lanes that
+      // the operand needs (columns: the rows i of P)
+      const int i = idx_of(w, col);
+      const float hi = sm.rowv[kGHi][i], lo = sm.rowv[kGLo][i];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks > (w >> 1)) continue;
+        f32x4 d[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int kk = 0; kk < KP / 32; ++kk) {
+          bf16x8 qb[NP];
+#pragma unroll
+          for (int j = 0; j < NP; ++j) qb[j] = op_rows<KP>(sm.q[j], w, kk, lane);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            bf16x8 ka[NP];
+#pragma unroll
+            for (int j = 0; j < NP; ++j) ka[j] = op_rows<KP>(sm.k[j], 2 * ks + x, kk, lane);
+            d[x] = mul<LIMO>(ka, qb, d[x]);
+          }
+        }
+        f32x8 pv = join(d[0], d[1]);
+        const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)   // (a selection: rows behind i may hold NaN)
+          pv[j] = 32 * ks + 8 * G + j <= i ? a.scale * pv[j] * fast_exp2((hi - ghi[j]) + (lo - glo[j])) : 0.f;
+        bf16x8 s[NO];
+        split(pv, s);
+#pragma unroll
+        for (int j = 0; j < NO; ++j)
+          *reinterpret_cast<uint4 *>(&sm.p[j][(tri_set(w, ks) * 64 + lane) * 8]) = to_bits(s[j]);
+      }
+    }
+
+    // R = k S (and q S): rows in pairs of tiles, this wavefront's columns
+    f32x4 R[4], O[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) R[t] = O[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KP / 32; ++ks) {
+      bf16x8 s[3];
+      split(join(S[2 * ks], S[2 * ks + 1]), s);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        bf16x8 x[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) x[j] = op_rows<KP>(sm.k[j], t, ks, lane);
+        R[t] = mul<2>(x, s, R[t]);
+        if constexpr (OUT) {
+#pragma unroll
+          for (int j = 0; j < NP; ++j) x[j] = op_rows<KP>(sm.q[j], t, ks, lane);
+          O[t] = mul<LIMO>(x, s, O[t]);
+        }
+      }
+    }
+    f32x8 X[2], U[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const f32x8 bt = row8(kBeta, p), bg = row8(kBetaG, p), r = join(R[2 * p], R[2 * p + 1]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) X[p][j] = fmaf(-bg[j], r[j], bt[j] * vv[p][j]);
+    }
+    int r0 = kChunk;   // this lane's column is not finite from this row on
+    for (bool sane = false;; sane = true) {
+      bf16x8 x[2][3];
+      f32x4 u[4];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) split(X[p], x[p]);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        u[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks <= t / 2; ++ks) {
+          bf16x8 m[3];
+#pragma unroll
+          for (int j = 0; j < 3; ++j)
+            m[j] = from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(&sm.tm[j][(tri_set(t, ks) * 64 + lane) * 8]));
+          u[t] = mul<2>(m, x[ks], u[t]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) U[p] = join(u[2 * p], u[2 * p + 1]);
+      // every row of tile 3 sums over all of X: one value tells
+      if (sane || __ballot(!finite(U[1][4])) == 0) break;   // wavefront-uniform
+#pragma unroll
+      for (int i = 15; i >= 0; --i)
+        if (!finite(X[i >> 3][i & 7])) r0 = 32 * (i >> 3) + 8 * G + (i & 7);
+      r0 = min(r0, __shfl_xor(r0, 16));
+      r0 = min(r0, __shfl_xor(r0, 32));
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (32 * (i >> 3) + 8 * G + (i & 7) >= r0) X[i >> 3][i & 7] = 0.f;
+    }
+    if (__ballot(r0 < kChunk)) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (32 * (i >> 3) + 8 * G + (i & 7) >= r0) U[i >> 3][i & 7] = 0.f;
+    }
+
+    if constexpr (OUT) {
+      bf16x8 us[2][NO];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) split(U[p], us[p]);
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const f32x8 eg = row8(kScaleG, p);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          O[2 * p][r] *= eg[r];
+          O[2 * p + 1][r] *= eg[4 + r];
+        }
+      }
+      __syncthreads();   // P is written
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int ks = 0; ks <= t / 2; ++ks) {
+          bf16x8 m[NO];
+#pragma unroll
+          for (int j = 0; j < NO; ++j)
+            m[j] = from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(&sm.p[j][(tri_set(t, ks) * 64 + lane) * 8]));
+          O[t] = mul<LIMO>(m, us[ks], O[t]);
+        }
+      const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = idx_of(i >> 2, 4 * G + (i & 3));
+        if (v_ok && t < rows) E::store(a.o, ((t0 + t) * a.H + h) * a.V + vcol, t >= r0 ? __builtin_nanf("") : O[i >> 2][i & 3]);
+      }
+    }
+
+    // S <- e^(G_last) S + k^T (e^(G_last - G) u)
+    bf16x8 ws[2][3];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) split(U[p] * row8(kToEnd, p), ws[p]);
+    const float through = fast_exp2(sm.rowv[kGHi][kChunk - 1]) * fast_exp2(sm.rowv[kGLo][kChunk - 1]);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      S[t] *= through;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        bf16x8 x[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) x[j] = op_cols<KP>(sm.k[j], t, ks, lane);
+        S[t] = mul<2>(x, ws[ks], S[t]);
+      }
+      if (r0 < kChunk) S[t] = f32x4{1.f, 1.f, 1.f, 1.f} * __builtin_nanf("");
+    }
+    __syncthreads();   // the chunk's tiles are read
+  }
+
+  if (OUT) {
+    if (a.ht && t_end == eos && v_ok) {
+      float *dst = a.ht + (static_cast<int64_t>(n) * a.H + h) * KV;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = idx_of(t, 4 * G + r);
+          if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = S[t][r];
+        }
+    }
+  } else if (is_map) {
+    if (active) {
+      uint16_t *dst = a.seg_map + (slot * a.H + h) * (3 * KP * KP);
+      const int ks = mcol >> 5, lg = 16 * ((mcol & 31) >> 3), j = mcol & 7;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = S[t][r];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            const uint16_t bits = f32_to_bf16_bits(x);
+            x -= bf16_bits_to_f32(bits);
+            dst[((t * (KP / 32) + ks) * 3 + p) * 512 + (lg + 4 * G + r) * 8 + j] = bits;
+          }
+        }
+    }
+  } else if (v_ok) {
+    float *dst = a.seg_state + (slot * a.H + h) * KV;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = idx_of(t, 4 * G + r);
+        if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = S[t][r];
+      }
+  }
+}
+
+// Carries the states over a sequence's segments: the L of segment j becomes
+// M_j E_j + L_j, the state entering segment j + 1 (E_0 = h0).
+template <int KP>
+__global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restrict__ cu, int64_t T, int H, int K, int V,
+                                                         int per, const float *__restrict__ h0,
+                                                         const uint16_t *__restrict__ seg_map,
+                                                         float *__restrict__ seg_state) {
+  constexpr int NT = KP / 16;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, G = lane >> 4;
+  const int n_groups = (((V + 15) >> 4) + 3) >> 2;
+  const int vcol = ((blockIdx.x % n_groups) * 4 + w) * 16 + col;
+  const int h = static_cast<int>((blockIdx.x / n_groups) % H);
+  const int64_t n = blockIdx.x / n_groups / H;
+  const int64_t bos = min(max(cu[n], (int64_t)0), T), eos = min(max(cu[n + 1], bos), T);
+  const int64_t unit = static_cast<int64_t>(per) * kChunk, KV = static_cast<int64_t>(K) * V;
+  const int64_t inner = (eos - bos + unit - 1) / unit - 1;   // segments but the last
+  const bool ok = vcol < V;
+  f32x4 S[NT];
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int key = idx_of(t, 4 * G + r);
+      S[t][r] = (h0 && ok && key < K) ? h0[(n * H + h) * KV + static_cast<int64_t>(key) * V + vcol] : 0.f;
+    }
+  for (int64_t j = 0; j < inner; ++j) {
+    const int64_t slot = (bos / unit + j) * H + h;
+    const uint16_t *m = seg_map + slot * (3 * KP * KP);
+    float *dst = seg_state + slot * KV;
+    bf16x8 s[NT / 2][3];
+#pragma unroll
+    for (int ks = 0; ks < NT / 2; ++ks) split(join(S[2 * ks], S[2 * ks + 1]), s[ks]);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = idx_of(t, 4 * G + r);
+        S[t][r] = (ok && key < K) ? dst[static_cast<int64_t>(key) * V + vcol] : 0.f;
+      }
+#pragma unroll
+      for (int ks = 0; ks < NT / 2; ++ks) {
+        bf16x8 x[3];
+#pragma unroll
+        for (int p = 0; p < 3; ++p)
+          x[p] = from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(m + ((t * (KP / 32) + ks) * 3 + p) * 512 + lane * 8));
+        S[t] = mul<2>(x, s[ks], S[t]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = idx_of(t, 4 * G + r);
+        if (ok && key < K) dst[static_cast<int64_t>(key) * V + vcol] = S[t][r];
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------ launches --
+inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
+
+// Chunks per segment: at least 4, and as many as leave about 512 workgroups
+// (two a CU) of 64 value columns.
+inline int seg_chunks(int64_t T, int H, int V) {
+  const int64_t work = (T / kChunk + 1) * H * ((V + 63) / 64);
+  return static_cast<int>(std::min<int64_t>(1 << 20, std::max<int64_t>(4, (work + 511) / 512)));
+}
+
+struct Layout {
+  size_t tm, rowv, state, map, total;
+  int64_t chunk_slots, seg_slots, inner_slots;
+  int per;
+  bool cut;
+};
+
+inline Layout layout_of(int n_seq, int64_t T, int H, int K, int V) {
+  Layout L{};
+  const int KP = padded_keys(K);
+  L.per = seg_chunks(T, H, V);
+  const int64_t unit = static_cast<int64_t>(L.per) * kChunk;
+  L.chunk_slots = T / kChunk + n_seq + 1;
+  L.seg_slots = T / unit + n_seq + 1;
+  L.inner_slots = T > 0 ? (T - 1) / unit : 0;   // no sequence has an inner segment where this is 0
+  L.cut = L.inner_slots > 0;
+  size_t p = 0;
+  L.tm = p;    p = align256(p + sizeof(float) * kTriFloats * L.chunk_slots * H);
+  L.rowv = p;  p = align256(p + sizeof(float) * kRowFloats * L.chunk_slots * H);
+  L.state = p; p = align256(p + sizeof(float) * L.inner_slots * H * K * V);
+  L.map = p;   p = align256(p + sizeof(uint16_t) * 3 * L.inner_slots * H * KP * KP);
+  L.total = p;
+  return L;
+}
+
+template <int DT, int KP>
+int launch_chunk(const Layout &L, WalkArgs a, const float *g, const float *beta, float scale, char *ws,
+                 hipStream_t st) {
+  float *tm = reinterpret_cast<float *>(ws + L.tm), *rowv = reinterpret_cast<float *>(ws + L.rowv);
+  a.tm = tm;
+  a.rowv = rowv;
+  a.seg_state = reinterpret_cast<float *>(ws + L.state);
+  a.seg_map = reinterpret_cast<uint16_t *>(ws + L.map);
+  a.per = L.per;
+  const int n_vt = (a.V + 15) / 16, vg = (n_vt + 3) / 4, sg = (n_vt + KP / 16 + 3) / 4;
+  const int64_t prep = L.chunk_slots * a.H, walk = L.seg_slots * a.H * vg, inner = L.inner_slots * a.H * sg;
+  const int64_t fold = static_cast<int64_t>(a.n_seq) * a.H * vg;
+  if (std::max({prep, walk, inner, fold}) > 0x7fffffff) {
+    set_error("gated_delta_chunk_fwd: too many workgroups");
+    return SSLA_ERR_UNSUPPORTED;
+  }
+  const dim3 block(256);
+  auto grid = [](int64_t n) { return dim3(static_cast<unsigned>(n)); };
+  hipLaunchKernelGGL((delta_prep_kernel<DT, KP>), grid(prep), block, 0, st, a.k, g, beta, a.cu, a.n_seq, a.T, a.Hk, a.H,
+                     a.K, a.vec, scale, tm, rowv);
+  if (L.cut) {
+    hipLaunchKernelGGL((delta_walk_kernel<DT, KP, false>), grid(inner), block, 0, st, a);
+    hipLaunchKernelGGL((delta_fold_kernel<KP>), grid(fold), block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per, a.h0,
+                       a.seg_map, a.seg_state);
+  }
+  hipLaunchKernelGGL((delta_walk_kernel<DT, KP, true>), grid(walk), block, 0, st, a);
+  return launch_status("gated_delta_chunk_fwd");
+}
+
+template <int DT>
+int launch_keys(const Layout &L, const WalkArgs &a, const float *g, const float *beta, float scale, char *ws,
+                hipStream_t st) {
+  switch (padded_keys(a.K)) {
+    case 32: return launch_chunk<DT, 32>(L, a, g, beta, scale, ws, st);
+    case 64: return launch_chunk<DT, 64>(L, a, g, beta, scale, ws, st);
+    default: return launch_chunk<DT, 128>(L, a, g, beta, scale, ws, st);
+  }
+}
+
+}  // namespace
+}  // namespace ssla
+
+extern "C" size_t ssla_gated_delta_chunk_workspace_size(int n_seq, int64_t T, int H, int K, int V) {
+  if (n_seq <= 0 || T < 0 || H <= 0 || K <= 0 || K > 128 || V <= 0) return 0;
+  return ssla::layout_of(n_seq, T, H, K, V).total;
+}
+
+extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, const float *g,
+                                          const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk,
+                                          int H, int K, int V, float scale, const float *h0, void *o, float *ht,
+                                          int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  using namespace ssla;
+  clear_error();
+  SSLA_CHECK_ARG(n_seq >= 0 && T >= 0 && Hk > 0 && H > 0 && H % Hk == 0 && K > 0 && V > 0,
+                 "gated_delta_chunk_fwd: bad sizes n_seq=%d T=%lld Hk=%d H=%d K=%d V=%d", n_seq, (long long)T, Hk, H, K,
+                 V);
+  if (K > 128) {
+    set_error("gated_delta_chunk_fwd: K=%d exceeds 128", K);
+    return SSLA_ERR_UNSUPPORTED;
+  }
+  if (n_seq == 0) return SSLA_OK;
+  SSLA_CHECK_ARG(cu_seqlens != nullptr, "gated_delta_chunk_fwd: cu_seqlens is NULL");
+  SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "gated_delta_chunk_fwd: null tensor pointer");
+  const Layout L = layout_of(n_seq, T, H, K, V);
+  if (!workspace || workspace_bytes < L.total || !aligned(workspace, 16)) {
+    set_error("gated_delta_chunk_fwd: needs %zu bytes of workspace, got %zu", L.total, workspace_bytes);
+    return SSLA_ERR_WORKSPACE;
+  }
+  const int es = dtype == SSLA_F32 ? 4 : 2;
+  const int vec = (static_cast<int64_t>(K) * es) % 16 == 0 && K % 8 == 0 && aligned(q, 16) && aligned(k, 16);
+  WalkArgs a{};
+  a.q = q; a.k = k; a.v = v; a.cu = cu_seqlens; a.h0 = h0; a.o = o; a.ht = ht;
+  a.T = T; a.n_seq = n_seq; a.Hk = Hk; a.H = H; a.K = K; a.V = V; a.vec = vec; a.scale = scale;
+  char *ws = static_cast<char *>(workspace);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case SSLA_F32: return launch_keys<SSLA_F32>(L, a, g, beta, scale, ws, st);
+    case SSLA_BF16: return launch_keys<SSLA_BF16>(L, a, g, beta, scale, ws, st);
+    case SSLA_F16: return launch_keys<SSLA_F16>(L, a, g, beta, scale, ws, st);
+  }
+  set_error("gated_delta_chunk_fwd: unsupported dtype %d", dtype);
+  return SSLA_ERR_DTYPE;
+}

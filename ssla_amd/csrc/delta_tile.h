@@ -1,0 +1,153 @@
+// Tiles and products of the chunked gated delta rule (forward and backward).
+//
+// Products run on v_mfma_f32_16x16x32_bf16.  An fp32 value is the exact sum of
+// three bf16 (a head and two rounded remainders, 24 bits in all), an fp16 value
+// of two, a bf16 value is one: a product of two operands is the sum of the
+// products of their parts whose orders add up to at most two, which leaves out
+// terms below 2^-26 of the operands' product.  States, sums and the values that
+// are carried on keep the precision of fp32 that way, at a sixth of the bf16
+// rate for two fp32 operands and a third where one is a bf16 input; the fp32
+// matrix instructions run at a sixteenth.
+//
+// Index order.  Rows (or keys) are taken 32 at a time as a pair of 16-row
+// accumulator tiles 2 p and 2 p + 1: row 4 G + r of tile 2 p + a is index
+// 32 p + 8 G + 4 a + r.  Lane group G (lanes 16 G .. 16 G + 15) then holds the
+// eight consecutive indices 32 p + 8 G .. + 7 of a column in its two
+// accumulators, which is what the next product's operand needs of it: results
+// go on to the next product without leaving their lanes.
+#pragma once
+#include "lds_tile.h"
+
+namespace ssla {
+
+constexpr int kChunk = 64;            // rows of a chunk
+constexpr int kTriSets = 6;           // 16 x 32 operands of a lower triangular 64 x 64 matrix
+constexpr int kTriFloats = kTriSets * 512;
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
+// Index of row m (0..15) of tile t in the order above.
+__device__ __forceinline__ int idx_of(int t, int m) { return 32 * (t >> 1) + 8 * (m >> 2) + 4 * (t & 1) + (m & 3); }
+// The operand set of row tile t (0..3), contraction half ks (<= t / 2), of a lower triangular matrix.
+__device__ __forceinline__ constexpr int tri_set(int t, int ks) { return t < 2 ? t : 2 * t - 2 + ks; }
+
+template <int DT> struct Parts { static constexpr int n = DT == SSLA_BF16 ? 1 : DT == SSLA_F16 ? 2 : 3; };
+
+// x as a sum of N bf16 vectors.
+template <int N>
+__device__ __forceinline__ void split(const f32x8 &x, bf16x8 (&p)[N]) {
+  f32x8 r = x;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    p[i] = __builtin_convertvector(r, bf16x8);
+    if (i + 1 < N) r = r - __builtin_convertvector(p[i], f32x8);
+  }
+}
+__device__ __forceinline__ f32x8 join(const f32x4 &a, const f32x4 &b) {
+  return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+
+// c += a b over the parts whose orders add up to at most LIM, small ones first.
+template <int LIM, int NA, int NB>
+__device__ __forceinline__ f32x4 mul(const bf16x8 (&a)[NA], const bf16x8 (&b)[NB], f32x4 c) {
+#pragma unroll
+  for (int s = LIM; s >= 0; --s)
+#pragma unroll
+    for (int i = 0; i < NA; ++i)
+      if (s - i >= 0 && s - i < NB) c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a[i], b[s - i], c, 0, 0, 0);
+  return c;
+}
+
+// A 64 x KP tile of bf16 in LDS: the 16-byte segments of a row are permuted so
+// that both the operand reads (rows idx_of(t, 0..7) of one segment) and the
+// transposing reads (four rows, four segments) spread over the banks.
+template <int KP>
+__device__ __forceinline__ int sw(int row, int col) {
+  const int a = row & 1, b = (row >> 1) & 1, c = (row >> 3) & 1;
+  const int key = KP == 32 ? (b << 1 | c) : KP == 64 ? (b << 2 | a << 1 | c) : (a << 3 | b << 2 | a << 1 | c);
+  return row * KP + ((((col >> 3) ^ key) << 3) | (col & 7));
+}
+// Operand with lane (m, G) = row idx_of(t, m), columns 32 ks + 8 G .. + 7.
+template <int KP>
+__device__ __forceinline__ bf16x8 op_rows(const uint16_t *t, int tile, int ks, int lane) {
+  return from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(t + sw<KP>(idx_of(tile, lane & 15), 32 * ks + 8 * (lane >> 4))));
+}
+// Operand with lane (m, G) = column idx_of(tile, m), rows 32 ks + 8 G .. + 7
+// (ds_read_b64_tr_b16: see tr_read4; source lane s reads row + s / 4, four
+// columns from 8 (s % 4)).
+template <int KP>
+__device__ __forceinline__ bf16x8 op_cols(const uint16_t *t, int tile, int ks, int lane) {
+  const int s = lane & 15, row = 32 * ks + 8 * (lane >> 4) + (s >> 2), col = 32 * (tile >> 1) + 8 * (s & 3) + 4 * (tile & 1);
+  uint2 u[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint16_t *p = t + sw<KP>(row + 4 * i, col);
+    u[i] = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<__attribute__((address_space(3))) s16x4 *>(reinterpret_cast<uintptr_t>(p))));
+  }
+  return from_bits<bf16x8>(make_uint4(u[0].x, u[0].y, u[1].x, u[1].y));
+}
+
+// Rows t0 .. of one head of a [T, heads, D] tensor, fetched into registers by
+// 256 threads and stored to LDS as Parts<DT>::n tiles of bf16; rows from
+// n_rows on and columns from D on are zero.  Rows of whole 16-byte pieces at
+// aligned addresses (vec) are read 16 bytes at a time.
+template <int DT, int KP>
+struct RowTile {
+  static constexpr int U = KP / 32;   // 8-column pieces of a thread
+  typedef typename Elem<DT>::T E;
+  struct Piece { E e[8]; };
+  Piece p[U];
+
+  __device__ __forceinline__ void fetch(const void *base, int64_t t0, int n_rows, int heads, int head, int D, bool vec) {
+    const E *x = static_cast<const E *>(base);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = threadIdx.x + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
+      const E *src = x + ((t0 + row) * heads + head) * D + col;
+      if (row < n_rows && vec && col + 8 <= D) {
+        constexpr int W = sizeof(Piece) / 16;
+        uint4 w[W];
+#pragma unroll
+        for (int j = 0; j < W; ++j) w[j] = reinterpret_cast<const uint4 *>(src)[j];
+        p[i] = __builtin_bit_cast(Piece, w);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[i].e[j] = (row < n_rows && col + j < D) ? src[j] : E(0);
+      }
+    }
+  }
+  // plane j at t + j * stride elements
+  __device__ __forceinline__ void store(uint16_t *t, int stride) const {
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      const int u = threadIdx.x + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
+      uint16_t *dst = t + sw<KP>(row, col);
+      if constexpr (DT == SSLA_BF16) {
+        *reinterpret_cast<uint4 *>(dst) = __builtin_bit_cast(uint4, p[i]);
+      } else {
+        f32x8 x;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          if constexpr (DT == SSLA_F16) x[j] = f16_bits_to_f32(p[i].e[j]);
+          else x[j] = p[i].e[j];
+        }
+        bf16x8 s[Parts<DT>::n];
+        split(x, s);
+#pragma unroll
+        for (int j = 0; j < Parts<DT>::n; ++j) *reinterpret_cast<uint4 *>(dst + j * stride) = to_bits(s[j]);
+      }
+    }
+  }
+};
+
+// The chunks' matrices and row factors that every pass reads, written once by
+// the first kernel: per (chunk slot, head) the operands of Tm = (I + A)^-1 in
+// fp32 (set by set, 64 lanes of 8 values) and kRowVecs vectors of 64 floats.
+enum { kBeta = 0, kBetaG, kScaleG, kToEnd, kGHi, kGLo, kRowVecs };
+constexpr int kRowFloats = kRowVecs * kChunk;
+
+// Chunk c (of 64 rows) of sequence n that starts at row bos has slot
+// bos / 64 + n + c; see seq_of_slot.
+__device__ __forceinline__ int64_t chunk_slot(int64_t bos, int n, int64_t c) { return bos / kChunk + n + c; }
+
+}  // namespace ssla

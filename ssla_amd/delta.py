@@ -10,6 +10,8 @@ fade.  Per sequence and head, with state S ``[K, V]``:
 It stands beside the gated linear attention of :mod:`ssla_amd.gla` (same packed
 layouts, same state tables) and has no counterpart in the reference.
 
+* :func:`chunk_gated_delta` -- packed sequences by chunks of 64 tokens, on the
+  matrix cores.
 * :func:`fused_recurrent_gated_delta` -- token by token, for short sequences.
 * :func:`sparse_delta_scan`, :func:`sparse_delta_step` -- per-site histories,
   and one token of each active site, on a resident state table.
@@ -27,7 +29,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["fused_recurrent_gated_delta", "sparse_delta_scan", "sparse_delta_step"]
+__all__ = ["chunk_gated_delta", "fused_recurrent_gated_delta", "sparse_delta_scan", "sparse_delta_step"]
 
 
 def _shapes(name, q, k, v, g, beta):
@@ -75,6 +77,60 @@ def _recurrent(q, k, v, g, beta, cu, n_seq, scale, h0, ht, state_idx=None, statu
             _lib.stream_of(q))
     _lib.check(st, "ssla_gated_delta_recurrent")
     return o
+
+
+def _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
+    """One ssla_gated_delta_chunk_fwd call on contiguous tensors."""
+    T, Hk, K = q.shape
+    H, V = v.shape[1:]
+    N = cu.numel() - 1
+    o = torch.empty_like(v)
+    ht = torch.empty(N, H, K, V, device=v.device, dtype=torch.float32) if output_final_state else None
+    lib, P = _lib.load(), _lib.ptr
+    with _lib.on_device_of(q):
+        nbytes = lib.ssla_gated_delta_chunk_workspace_size(N, T, H, K, V)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        st = lib.ssla_gated_delta_chunk_fwd(P(q), P(k), P(v), P(g), P(beta), P(cu), N, T, Hk, H, K, V, float(scale),
+                                            P(h0), P(o), P(ht), _lib.DTYPE_CODE[q.dtype], P(ws), nbytes,
+                                            _lib.stream_of(q))
+    _lib.check(st, "ssla_gated_delta_chunk_fwd")
+    return o, ht
+
+
+def chunk_gated_delta(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    g: torch.Tensor,
+    beta: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    scale: Optional[float] = None,
+    initial_state: Optional[torch.Tensor] = None,
+    output_final_state: bool = False,
+) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+    """The rule over packed sequences: o ``[T, H, V]`` in v's dtype and the fp32
+    final state ``[N, H, K, V]`` or None.  ``scale`` defaults to ``K ** -0.5``.
+    Rows of o outside ``[cu_seqlens[0], cu_seqlens[-1])`` are unspecified.
+
+    K up to 128 runs the chunk kernels, whose products keep the precision of
+    fp32 for every dtype; wider keys run the token-by-token kernel (K up to
+    256)."""
+    name = "chunk_gated_delta"
+    T, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
+    dev = _lib.require_cuda(q, k, v, g, beta, initial_state)
+    cu = _offsets(name, cu_seqlens, dev)
+    N = cu.numel() - 1
+    if initial_state is not None and initial_state.shape != (N, H, K, V):
+        raise ValueError(f"{name}: initial_state must be {(N, H, K, V)}, got {tuple(initial_state.shape)}")
+    _lib.require_no_grad(name, q, k, v, g, beta, initial_state)
+    scale = K ** -0.5 if scale is None else float(scale)
+    h0 = None if initial_state is None else initial_state.to(torch.float32).contiguous()
+    if K > 128 or N == 0 or T == 0:
+        ht = torch.empty(N, H, K, V, device=dev, dtype=torch.float32) if output_final_state else None
+        return _recurrent(q, k, v, g, beta, cu, N, scale, h0, ht), ht
+    q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
+    g, beta = g.to(torch.float32).contiguous(), beta.to(torch.float32).contiguous()
+    return _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
 
 
 def fused_recurrent_gated_delta(
