@@ -38,7 +38,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
                                                          const float *__restrict__ beta,
                                                          const int64_t *__restrict__ cu, int n_seq, int64_t T, int Hk,
                                                          int H, int K, int vec, float scale, float *__restrict__ tm,
-                                                         float *__restrict__ rowv) {
+                                                         int tm_floats, float *__restrict__ rowv) {
   constexpr int NP = Parts<DT>::n, LD = 68;
   __shared__ __align__(16) uint16_t sk[NP][kChunk * KP];
   __shared__ __align__(16) float A[kChunk][LD];   // I + A, then Tm
@@ -56,7 +56,8 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
   const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
 
   RowTile<DT, KP> kt;
-  kt.fetch(k, t0, rows, Hk, hk, K, vec);
+  typedef typename Elem<DT>::T E;
+  kt.fetch(static_cast<const E *>(k) + (t0 * Hk + hk) * K, static_cast<int64_t>(Hk) * K, rows, K, vec);
   float gv = 0.f, bv = 0.f;
   if (w == 0 && lane < rows) {
     gv = g[(t0 + lane) * H + h];
@@ -192,31 +193,33 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
     *reinterpret_cast<f32x4 *>(&A[32 + i][c]) = -y;
   }
   __syncthreads();
-  float *dst = tm + (slot * H + h) * kTriFloats;
+  float *dst = tm + (slot * H + h) * tm_floats;
   for (int e = tid; e < kTriFloats / 4; e += 256) {
     const int set = e >> 7, ln = (e >> 1) & 63, half = e & 1;
     const int t = set < 2 ? set : 2 + ((set - 2) >> 1), ks = set < 2 ? 0 : (set & 1);
     reinterpret_cast<f32x4 *>(dst)[e] =
         *reinterpret_cast<const f32x4 *>(&A[idx_of(t, ln & 15)][32 * ks + 8 * (ln >> 4) + 4 * half]);
   }
+  if (tm_floats > kTriFloats) {   // and Tm^T: row tiles 0, 1 need both halves, 2, 3 the second
+    for (int e = tid; e < kTriFloats / 4; e += 256) {
+      const int set = e >> 7, ln = (e >> 1) & 63, half = e & 1;
+      const int t = set < 4 ? set >> 1 : set - 2, ks = set < 4 ? (set & 1) : 1;
+      f32x4 x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = A[32 * ks + 8 * (ln >> 4) + 4 * half + i][idx_of(t, ln & 15)];
+      reinterpret_cast<f32x4 *>(dst + kTriFloats)[e] = x;
+    }
+  }
   float *dv = rowv + (slot * H + h) * kRowFloats;
   for (int e = tid; e < kRowFloats; e += 256) dv[e] = (&sv[0][0])[e];
 }
 
 // ----------------------------------------------------------------- the walk --
-struct WalkArgs {
-  const void *q, *k, *v;
-  const int64_t *cu;
-  const float *tm, *rowv;
-  const float *h0;
-  void *o;
-  float *ht;
-  float *seg_state;       // per inner segment: L, after the fold the state entering the next segment
-  uint16_t *seg_map;      // per inner segment: M as operands of three bf16 parts
-  int64_t T;
-  int n_seq, Hk, H, K, V, per, vec;
-  float scale;
-};
+// kOutput walks a segment from its entering state and writes o (and ht behind the
+// sequence's last row); kStates does so and writes every chunk's entering state
+// and u instead (for the backward); kSegment walks an inner segment from zero
+// and from the identity and writes L and M.
+enum { kOutput, kStates, kSegment };
 
 template <int DT, int KP, bool OUT>
 struct WalkSmem {
@@ -228,18 +231,17 @@ struct WalkSmem {
   float rowv[kRowVecs][kChunk];
 };
 
-// OUT: walks a segment from its entering state and writes o (and ht behind the
-// sequence's last row).  Otherwise: walks an inner segment from zero and from
-// the identity and writes L and M.
 // Four wavefronts, each with 16 columns of the state (its rows: the keys).
-template <int DT, int KP, bool OUT>
+template <int DT, int KP, int MODE>
 __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void delta_walk_kernel(const WalkArgs a) {
   constexpr int NP = Parts<DT>::n, NO = DT == SSLA_F32 ? 3 : 2, LIMO = NO - 1, NT = KP / 16;
+  constexpr bool OUT = MODE == kOutput, SEG = MODE == kSegment;
   typedef Elem<DT> E;
+  typedef typename E::T ET;
   __shared__ __align__(16) WalkSmem<DT, KP, OUT> sm;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, G = lane >> 4;
-  const int n_vt = (a.V + 15) >> 4, n_groups = (n_vt + (OUT ? 0 : NT) + 3) >> 2;
+  const int n_vt = (a.V + 15) >> 4, n_groups = (n_vt + (SEG ? NT : 0) + 3) >> 2;
   int64_t b = blockIdx.x;
   const int grp = static_cast<int>(b % n_groups);
   b /= n_groups;
@@ -248,12 +250,12 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   const int64_t unit = static_cast<int64_t>(a.per) * kChunk;
   int n;
   int64_t bos, eos, first;
-  if (!seq_of_slot<OUT>(a.cu, a.n_seq, a.T, unit, slot, n, bos, eos, first)) return;   // workgroup-uniform
+  if (!seq_of_slot<!SEG>(a.cu, a.n_seq, a.T, unit, slot, n, bos, eos, first)) return;   // workgroup-uniform
   const int64_t seg = slot - first, t_begin = bos + seg * unit;
-  if (OUT ? (t_begin >= eos && seg > 0) : t_begin + unit >= eos) return;
+  if (SEG ? t_begin + unit >= eos : (t_begin >= eos && seg > 0)) return;
   const int64_t t_end = min(t_begin + unit, eos);
   const int tile = grp * 4 + w;
-  const bool is_map = !OUT && tile >= n_vt;                  // this wavefront's columns are M's
+  const bool is_map = SEG && tile >= n_vt;                   // this wavefront's columns are M's
   const int vcol = tile * 16 + col, mcol = (tile - n_vt) * 16 + col;
   const bool active = is_map ? mcol < KP : tile < n_vt, v_ok = !is_map && vcol < a.V;
   const int64_t KV = static_cast<int64_t>(a.K) * a.V;
@@ -261,7 +263,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   f32x4 S[NT];
   {
     const float *src = nullptr;
-    if (OUT) {
+    if (!SEG) {
       if (seg == 0) src = a.h0 ? a.h0 + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr;
       else src = a.seg_state + ((bos / unit + seg - 1) * a.H + h) * KV;
     }
@@ -271,20 +273,21 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
       for (int r = 0; r < 4; ++r) {
         const int key = idx_of(t, 4 * G + r);
         float x = is_map && key == mcol ? 1.f : 0.f;
-        if (OUT && src && v_ok && key < a.K) x = src[static_cast<int64_t>(key) * a.V + vcol];
+        if (!SEG && src && v_ok && key < a.K) x = src[static_cast<int64_t>(key) * a.V + vcol];
         S[t][r] = x;
       }
   }
 
   RowTile<DT, KP> kt, qt;
   f32x4 tmr[3], rvr;
-  typename E::T vr[16];
+  ET vr[16];
   auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
-    kt.fetch(a.k, t0, rows, a.Hk, hk, a.K, a.vec);
-    if constexpr (OUT) qt.fetch(a.q, t0, rows, a.Hk, hk, a.K, a.vec);
+    const int64_t at = (t0 * a.Hk + hk) * a.K, stride = static_cast<int64_t>(a.Hk) * a.K;
+    kt.fetch(static_cast<const ET *>(a.k) + at, stride, rows, a.K, a.vec);
+    if constexpr (OUT) qt.fetch(static_cast<const ET *>(a.q) + at, stride, rows, a.K, a.vec);
     const int64_t c = (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h);
-    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * kTriFloats);
+    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * a.tm_floats);
     tmr[0] = src[2 * tid];
     tmr[1] = src[2 * tid + 1];
     tmr[2] = src[512 + tid];
@@ -292,8 +295,8 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
       const int t = idx_of(i >> 2, 4 * G + (i & 3));
-      vr[i] = (v_ok && t < rows) ? static_cast<const typename E::T *>(a.v)[((t0 + t) * a.H + h) * a.V + vcol]
-                                 : typename E::T(0);
+      vr[i] = (v_ok && t < rows) ? static_cast<const ET *>(a.v)[((t0 + t) * a.H + h) * a.V + vcol]
+                                 : ET(0);
     }
   };
   auto stage = [&]() __attribute__((always_inline)) {
@@ -330,6 +333,16 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
       if constexpr (DT == SSLA_BF16) vv[i >> 3][i & 7] = bf16_bits_to_f32(vr[i]);
       else if constexpr (DT == SSLA_F16) vv[i >> 3][i & 7] = f16_bits_to_f32(vr[i]);
       else vv[i >> 3][i & 7] = vr[i];
+    }
+    if constexpr (MODE == kStates) {
+      float *dst = a.chunk_state + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = idx_of(t, 4 * G + r);
+          if (v_ok && key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = S[t][r];
+        }
     }
     __syncthreads();
     if (t0 + kChunk < t_end) fetch(t0 + kChunk);   // the next chunk's, in flight meanwhile
@@ -466,6 +479,15 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
       }
     }
 
+    if constexpr (MODE == kStates) {
+      const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int t = idx_of(i >> 2, 4 * G + (i & 3));
+        if (v_ok && t < rows) a.u[((t0 + t) * a.H + h) * a.V + vcol] = t >= r0 ? __builtin_nanf("") : U[i >> 3][i & 7];
+      }
+    }
+
     // S <- e^(G_last) S + k^T (e^(G_last - G) u)
     bf16x8 ws[2][3];
 #pragma unroll
@@ -486,7 +508,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
     __syncthreads();   // the chunk's tiles are read
   }
 
-  if (OUT) {
+  if (!SEG) {
     if (a.ht && t_end == eos && v_ok) {
       float *dst = a.ht + (static_cast<int64_t>(n) * a.H + h) * KV;
 #pragma unroll
@@ -526,11 +548,12 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   }
 }
 
-// Carries the states over a sequence's segments: the L of segment j becomes
-// M_j E_j + L_j, the state entering segment j + 1 (E_0 = h0).
-template <int KP>
+// Carries the states over a sequence's segments: the L of inner segment j
+// becomes M_j E_j + L_j, the state entering segment j + 1 (E_0 = start or 0).
+// REV: from the last slot to the first.
+template <int KP, bool REV>
 __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restrict__ cu, int64_t T, int H, int K, int V,
-                                                         int per, const float *__restrict__ h0,
+                                                         int per, const float *__restrict__ start,
                                                          const uint16_t *__restrict__ seg_map,
                                                          float *__restrict__ seg_state) {
   constexpr int NT = KP / 16;
@@ -549,10 +572,10 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
       const int key = idx_of(t, 4 * G + r);
-      S[t][r] = (h0 && ok && key < K) ? h0[(n * H + h) * KV + static_cast<int64_t>(key) * V + vcol] : 0.f;
+      S[t][r] = (start && ok && key < K) ? start[(n * H + h) * KV + static_cast<int64_t>(key) * V + vcol] : 0.f;
     }
   for (int64_t j = 0; j < inner; ++j) {
-    const int64_t slot = (bos / unit + j) * H + h;
+    const int64_t slot = (bos / unit + (REV ? inner - 1 - j : j)) * H + h;
     const uint16_t *m = seg_map + slot * (3 * KP * KP);
     float *dst = seg_state + slot * KV;
     bf16x8 s[NT / 2][3];
@@ -583,86 +606,89 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
 }
 
 // ------------------------------------------------------------------ launches --
-inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
-inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
+inline dim3 grid_of(int64_t n) { return dim3(static_cast<unsigned>(n)); }
+inline int v_groups(int V) { return ((V + 15) / 16 + 3) / 4; }
 
-// Chunks per segment: at least 4, and as many as leave about 512 workgroups
-// (two a CU) of 64 value columns.
-inline int seg_chunks(int64_t T, int H, int V) {
-  const int64_t work = (T / kChunk + 1) * H * ((V + 63) / 64);
-  return static_cast<int>(std::min<int64_t>(1 << 20, std::max<int64_t>(4, (work + 511) / 512)));
-}
-
-struct Layout {
-  size_t tm, rowv, state, map, total;
-  int64_t chunk_slots, seg_slots, inner_slots;
-  int per;
-  bool cut;
-};
-
-inline Layout layout_of(int n_seq, int64_t T, int H, int K, int V) {
-  Layout L{};
-  const int KP = padded_keys(K);
-  L.per = seg_chunks(T, H, V);
-  const int64_t unit = static_cast<int64_t>(L.per) * kChunk;
-  L.chunk_slots = T / kChunk + n_seq + 1;
-  L.seg_slots = T / unit + n_seq + 1;
-  L.inner_slots = T > 0 ? (T - 1) / unit : 0;   // no sequence has an inner segment where this is 0
-  L.cut = L.inner_slots > 0;
-  size_t p = 0;
-  L.tm = p;    p = align256(p + sizeof(float) * kTriFloats * L.chunk_slots * H);
-  L.rowv = p;  p = align256(p + sizeof(float) * kRowFloats * L.chunk_slots * H);
-  L.state = p; p = align256(p + sizeof(float) * L.inner_slots * H * K * V);
-  L.map = p;   p = align256(p + sizeof(uint16_t) * 3 * L.inner_slots * H * KP * KP);
-  L.total = p;
-  return L;
+int check_grids(const char *what, const DeltaLayout &L, const WalkArgs &a) {
+  const int64_t walk = L.seg_slots * a.H * v_groups(a.V), prep = L.chunk_slots * a.H;
+  const int64_t inner = L.inner_slots * a.H * (v_groups(a.V) + L.KP / 64 + 1);
+  if (std::max({prep, walk, inner, static_cast<int64_t>(a.n_seq) * a.H * v_groups(a.V)}) > 0x7fffffff) {
+    set_error("%s: too many workgroups", what);
+    return SSLA_ERR_UNSUPPORTED;
+  }
+  return SSLA_OK;
 }
 
 template <int DT, int KP>
-int launch_chunk(const Layout &L, WalkArgs a, const float *g, const float *beta, float scale, char *ws,
-                 hipStream_t st) {
-  float *tm = reinterpret_cast<float *>(ws + L.tm), *rowv = reinterpret_cast<float *>(ws + L.rowv);
-  a.tm = tm;
-  a.rowv = rowv;
-  a.seg_state = reinterpret_cast<float *>(ws + L.state);
-  a.seg_map = reinterpret_cast<uint16_t *>(ws + L.map);
-  a.per = L.per;
-  const int n_vt = (a.V + 15) / 16, vg = (n_vt + 3) / 4, sg = (n_vt + KP / 16 + 3) / 4;
-  const int64_t prep = L.chunk_slots * a.H, walk = L.seg_slots * a.H * vg, inner = L.inner_slots * a.H * sg;
-  const int64_t fold = static_cast<int64_t>(a.n_seq) * a.H * vg;
-  if (std::max({prep, walk, inner, fold}) > 0x7fffffff) {
-    set_error("gated_delta_chunk_fwd: too many workgroups");
-    return SSLA_ERR_UNSUPPORTED;
-  }
+void launch_chunk(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, bool states,
+                  hipStream_t st) {
   const dim3 block(256);
-  auto grid = [](int64_t n) { return dim3(static_cast<unsigned>(n)); };
-  hipLaunchKernelGGL((delta_prep_kernel<DT, KP>), grid(prep), block, 0, st, a.k, g, beta, a.cu, a.n_seq, a.T, a.Hk, a.H,
-                     a.K, a.vec, scale, tm, rowv);
-  if (L.cut) {
-    hipLaunchKernelGGL((delta_walk_kernel<DT, KP, false>), grid(inner), block, 0, st, a);
-    hipLaunchKernelGGL((delta_fold_kernel<KP>), grid(fold), block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per, a.h0,
-                       a.seg_map, a.seg_state);
+  hipLaunchKernelGGL((delta_prep_kernel<DT, KP>), grid_of(L.chunk_slots * a.H), block, 0, st, a.k, g, beta, a.cu, a.n_seq,
+                     a.T, a.Hk, a.H, a.K, a.vec, a.scale, const_cast<float *>(a.tm), a.tm_floats,
+                     const_cast<float *>(a.rowv));
+  if (L.inner_slots > 0) {
+    const int groups = ((a.V + 15) / 16 + KP / 16 + 3) / 4;
+    hipLaunchKernelGGL((delta_walk_kernel<DT, KP, kSegment>), grid_of(L.inner_slots * a.H * groups), block, 0, st, a);
+    delta_fold(L, a, a.h0, false, st);
   }
-  hipLaunchKernelGGL((delta_walk_kernel<DT, KP, true>), grid(walk), block, 0, st, a);
-  return launch_status("gated_delta_chunk_fwd");
+  const dim3 grid = grid_of(L.seg_slots * a.H * v_groups(a.V));
+  if (states) hipLaunchKernelGGL((delta_walk_kernel<DT, KP, kStates>), grid, block, 0, st, a);
+  else hipLaunchKernelGGL((delta_walk_kernel<DT, KP, kOutput>), grid, block, 0, st, a);
 }
 
 template <int DT>
-int launch_keys(const Layout &L, const WalkArgs &a, const float *g, const float *beta, float scale, char *ws,
-                hipStream_t st) {
-  switch (padded_keys(a.K)) {
-    case 32: return launch_chunk<DT, 32>(L, a, g, beta, scale, ws, st);
-    case 64: return launch_chunk<DT, 64>(L, a, g, beta, scale, ws, st);
-    default: return launch_chunk<DT, 128>(L, a, g, beta, scale, ws, st);
+void launch_keys(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, bool states,
+                 hipStream_t st) {
+  switch (L.KP) {
+    case 32: return launch_chunk<DT, 32>(L, a, g, beta, states, st);
+    case 64: return launch_chunk<DT, 64>(L, a, g, beta, states, st);
+    default: return launch_chunk<DT, 128>(L, a, g, beta, states, st);
   }
 }
 
+int launch_dtype(const char *what, const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta,
+                 bool states, int dtype, hipStream_t st) {
+  if (const int e = check_grids(what, L, a)) return e;
+  if (dtype == SSLA_F32) launch_keys<SSLA_F32>(L, a, g, beta, states, st);
+  else if (dtype == SSLA_BF16) launch_keys<SSLA_BF16>(L, a, g, beta, states, st);
+  else if (dtype == SSLA_F16) launch_keys<SSLA_F16>(L, a, g, beta, states, st);
+  else {
+    set_error("%s: unsupported dtype %d", what, dtype);
+    return SSLA_ERR_DTYPE;
+  }
+  return launch_status(what);
+}
+
 }  // namespace
+
+int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, int dtype,
+                         hipStream_t st) {
+  return launch_dtype("gated_delta_chunk_bwd", L, a, g, beta, true, dtype, st);
+}
+
+int delta_fold(const DeltaLayout &L, const WalkArgs &a, const float *start, bool reverse, hipStream_t st) {
+  const dim3 grid = grid_of(static_cast<int64_t>(a.n_seq) * a.H * v_groups(a.V)), block(256);
+#define SSLA_FOLD(KP_)                                                                                               \
+  do {                                                                                                               \
+    if (reverse)                                                                                                     \
+      hipLaunchKernelGGL((delta_fold_kernel<KP_, true>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per, start,  \
+                         a.seg_map, a.seg_state);                                                                    \
+    else                                                                                                             \
+      hipLaunchKernelGGL((delta_fold_kernel<KP_, false>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per, start, \
+                         a.seg_map, a.seg_state);                                                                    \
+  } while (0)
+  if (L.KP == 32) SSLA_FOLD(32);
+  else if (L.KP == 64) SSLA_FOLD(64);
+  else SSLA_FOLD(128);
+#undef SSLA_FOLD
+  return launch_status("gated_delta_chunk");
+}
+
 }  // namespace ssla
 
 extern "C" size_t ssla_gated_delta_chunk_workspace_size(int n_seq, int64_t T, int H, int K, int V) {
-  if (n_seq <= 0 || T < 0 || H <= 0 || K <= 0 || K > 128 || V <= 0) return 0;
-  return ssla::layout_of(n_seq, T, H, K, V).total;
+  if (n_seq < 0 || T < 0 || H <= 0 || K <= 0 || K > 128 || V <= 0) return 0;
+  return ssla::delta_layout(n_seq, T, H, H, K, V, false).total;
 }
 
 extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, const float *g,
@@ -681,23 +707,14 @@ extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const vo
   if (n_seq == 0) return SSLA_OK;
   SSLA_CHECK_ARG(cu_seqlens != nullptr, "gated_delta_chunk_fwd: cu_seqlens is NULL");
   SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "gated_delta_chunk_fwd: null tensor pointer");
-  const Layout L = layout_of(n_seq, T, H, K, V);
+  const DeltaLayout L = delta_layout(n_seq, T, Hk, H, K, V, false);
   if (!workspace || workspace_bytes < L.total || !aligned(workspace, 16)) {
     set_error("gated_delta_chunk_fwd: needs %zu bytes of workspace, got %zu", L.total, workspace_bytes);
     return SSLA_ERR_WORKSPACE;
   }
-  const int es = dtype == SSLA_F32 ? 4 : 2;
-  const int vec = (static_cast<int64_t>(K) * es) % 16 == 0 && K % 8 == 0 && aligned(q, 16) && aligned(k, 16);
-  WalkArgs a{};
-  a.q = q; a.k = k; a.v = v; a.cu = cu_seqlens; a.h0 = h0; a.o = o; a.ht = ht;
-  a.T = T; a.n_seq = n_seq; a.Hk = Hk; a.H = H; a.K = K; a.V = V; a.vec = vec; a.scale = scale;
-  char *ws = static_cast<char *>(workspace);
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case SSLA_F32: return launch_keys<SSLA_F32>(L, a, g, beta, scale, ws, st);
-    case SSLA_BF16: return launch_keys<SSLA_BF16>(L, a, g, beta, scale, ws, st);
-    case SSLA_F16: return launch_keys<SSLA_F16>(L, a, g, beta, scale, ws, st);
-  }
-  set_error("gated_delta_chunk_fwd: unsupported dtype %d", dtype);
-  return SSLA_ERR_DTYPE;
+  WalkArgs a = walk_args(L, static_cast<char *>(workspace), q, k, v, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, dtype,
+                         false);
+  a.o = o;
+  a.ht = ht;
+  return launch_dtype("gated_delta_chunk_fwd", L, a, g, beta, false, dtype, static_cast<hipStream_t>(stream));
 }

@@ -1,0 +1,739 @@
+// Chunked gated delta rule, backward, on gfx950.
+//
+// Notation of delta_chunk.hip; do the gradient of o, D that of the state
+// leaving a chunk, S the state entering it.  Per chunk
+//   du = P^T do + e^(G_last - G) (k D),   dX = Tm^T du,   dv = beta dX,
+//   D' = e^(G_last) D + q^T (scale e^G do) - k^T (beta e^G dX)
+// (D' leaves the chunk before).  Each column of D goes its own way, so this is
+// the forward's walk in reverse: the same segments, the same affine map over a
+// segment, the same fold.  With the products' factors known for every chunk,
+//   dP_ij = scale e^(G_i - G_j) do_i . u_j (j <= i),
+//   dN_ij = -e^(G_i - G_j) dX_i . u_j (j < i),
+//   dq = scale e^G (do S^T) + dP k,
+//   dk = dP^T q + beta (dN k) + (beta dN)^T k - beta e^G (dX S^T)
+//        + e^(G_last - G) (u D^T),
+//   dbeta_i = dX_i . v_i - e^(G_i) k_i . (S dX_i) + k_i . (dN k)_i
+// for all chunks side by side.  A gate's gradient is the sum over everything its
+// step scales: the terms between rows i >= t > j of dP and dN, from the state to
+// rows i >= t, from rows j < t to the next state, and from state to state.  Row
+// and column sums of the first kind are dot products of the rows of q and k with
+// the pieces of dq and dk, so no second Gram matrix is formed.
+// Shared key heads: every value head's dq and dk in fp32, added in the order of
+// the heads.
+#include "delta_tile.h"
+#include "seq_slots.h"
+
+namespace ssla {
+namespace {
+
+struct GradArgs {
+  WalkArgs w;
+  const void *dout;
+  const float *dht;
+  float *chunk_grad;   // per chunk: D
+  float *dx;           // [T, H, V]
+  void *dq, *dk, *dv;
+  float *dq_part, *dk_part;   // [T, H, K] where key heads are shared
+  float *dg, *dbeta, *dh0;
+  int vvec, dvec;
+};
+
+// Operand set of row tile t, contraction half ks (>= t / 2), of an upper triangular matrix.
+__device__ __forceinline__ constexpr int upper_set(int t, int ks) { return t < 2 ? 2 * t + ks : t + 2; }
+
+template <int DT, int KP>
+struct ReverseSmem {
+  static constexpr int NP = Parts<DT>::n;
+  uint16_t k[NP][kChunk * KP];
+  uint16_t q[NP][kChunk * KP];
+  uint16_t tm[3][kTriSets * 512];
+  uint16_t p[3][kTriSets * 512];
+  float rowv[kRowVecs][kChunk];
+};
+
+// SEG: an inner segment (one with a predecessor) from zero and from the identity:
+// L and M of the gradient's map.  Otherwise: a segment from the gradient leaving
+// it; writes every chunk's D and dX, dv, and dh0 before the sequence's first row.
+template <int DT, int KP, bool SEG>
+__global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void delta_reverse_kernel(const GradArgs ga) {
+  constexpr int NP = Parts<DT>::n, NT = KP / 16;
+  typedef Elem<DT> E;
+  typedef typename E::T ET;
+  const WalkArgs &a = ga.w;
+  __shared__ __align__(16) ReverseSmem<DT, KP> sm;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, G = lane >> 4;
+  const int n_vt = (a.V + 15) >> 4, n_groups = (n_vt + (SEG ? NT : 0) + 3) >> 2;
+  int64_t b = blockIdx.x;
+  const int grp = static_cast<int>(b % n_groups);
+  b /= n_groups;
+  const int h = static_cast<int>(b % a.H), hk = h / (a.H / a.Hk);
+  const int64_t slot = b / a.H;
+  const int64_t unit = static_cast<int64_t>(a.per) * kChunk;
+  int n;
+  int64_t bos, eos, first;
+  if (!seq_of_slot<!SEG>(a.cu, a.n_seq, a.T, unit, slot, n, bos, eos, first)) return;   // workgroup-uniform
+  const int64_t seg = slot - first + (SEG ? 1 : 0), t_begin = bos + seg * unit;
+  if (t_begin >= eos && seg > 0) return;
+  const int64_t t_end = min(t_begin + unit, eos);
+  const int tile = grp * 4 + w;
+  const bool is_map = SEG && tile >= n_vt;
+  const int vcol = tile * 16 + col, mcol = (tile - n_vt) * 16 + col;
+  const bool active = is_map ? mcol < KP : tile < n_vt, v_ok = !is_map && vcol < a.V;
+  const int64_t KV = static_cast<int64_t>(a.K) * a.V;
+
+  f32x4 D[NT];
+  {
+    const float *src = nullptr;
+    if (!SEG) {
+      if (t_end == eos) src = ga.dht ? ga.dht + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr;
+      else src = a.seg_state + ((bos / unit + seg) * a.H + h) * KV;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = idx_of(t, 4 * G + r);
+        float x = is_map && key == mcol ? 1.f : 0.f;
+        if (!SEG && src && v_ok && key < a.K) x = src[static_cast<int64_t>(key) * a.V + vcol];
+        D[t][r] = x;
+      }
+  }
+
+  RowTile<DT, KP> kt, qt;
+  f32x4 tmr[3], rvr;
+  ET dr[16];
+  auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+    const int64_t at = (t0 * a.Hk + hk) * a.K, stride = static_cast<int64_t>(a.Hk) * a.K;
+    kt.fetch(static_cast<const ET *>(a.k) + at, stride, rows, a.K, a.vec);
+    qt.fetch(static_cast<const ET *>(a.q) + at, stride, rows, a.K, a.vec);
+    const int64_t c = (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h);
+    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * a.tm_floats + kTriFloats);
+    tmr[0] = src[2 * tid];
+    tmr[1] = src[2 * tid + 1];
+    tmr[2] = src[512 + tid];
+    if (tid < kRowFloats / 4) rvr = reinterpret_cast<const f32x4 *>(a.rowv + c * kRowFloats)[tid];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int t = idx_of(i >> 2, 4 * G + (i & 3));
+      dr[i] = (v_ok && t < rows) ? static_cast<const ET *>(ga.dout)[((t0 + t) * a.H + h) * a.V + vcol] : ET(0);
+    }
+  };
+  auto stage = [&]() __attribute__((always_inline)) {
+    kt.store(&sm.k[0][0], kChunk * KP);
+    qt.store(&sm.q[0][0], kChunk * KP);
+    bf16x8 s[3];
+    split(join(tmr[0], tmr[1]), s);   // sets 0 .. 3: a lane's eight values of one thread
+#pragma unroll
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4 *>(&sm.tm[i][tid * 8]) = to_bits(s[i]);
+    split(join(tmr[2], f32x4{0.f, 0.f, 0.f, 0.f}), s);   // sets 4, 5: half a lane's values
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const uint4 x = to_bits(s[i]);
+      *reinterpret_cast<uint2 *>(&sm.tm[i][2048 + tid * 4]) = make_uint2(x.x, x.y);
+    }
+    if (tid < kRowFloats / 4) reinterpret_cast<f32x4 *>(&sm.rowv[0][0])[tid] = rvr;
+  };
+  auto row8 = [&](int vec, int p) __attribute__((always_inline)) {
+    const f32x4 *s = reinterpret_cast<const f32x4 *>(&sm.rowv[vec][32 * p + 8 * G]);
+    return join(s[0], s[1]);
+  };
+  auto set_of = [&](const uint16_t (&m)[3][kTriSets * 512], int set, bf16x8 (&x)[3]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < 3; ++j) x[j] = from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(&m[j][(set * 64 + lane) * 8]));
+  };
+
+  const int64_t n_chunks = (t_end - t_begin + kChunk - 1) / kChunk;
+  if (n_chunks > 0) fetch(t_begin + (n_chunks - 1) * kChunk);
+  for (int64_t c = n_chunks - 1; c >= 0; --c) {
+    const int64_t t0 = t_begin + c * kChunk;
+    stage();
+    f32x8 dov[2];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if constexpr (DT == SSLA_BF16) dov[i >> 3][i & 7] = bf16_bits_to_f32(dr[i]);
+      else if constexpr (DT == SSLA_F16) dov[i >> 3][i & 7] = f16_bits_to_f32(dr[i]);
+      else dov[i >> 3][i & 7] = dr[i];
+    }
+    if constexpr (!SEG) {
+      float *dst = ga.chunk_grad + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = idx_of(t, 4 * G + r);
+          if (v_ok && key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = D[t][r];
+        }
+    }
+    __syncthreads();
+    if (c > 0) fetch(t0 - kChunk);   // the next chunk's, in flight meanwhile
+
+    {   // P^T of this wavefront's row tile (rows j): q k^T has row i of P in the lanes that the operand needs
+      const int j = idx_of(w, col);
+      const float hi = sm.rowv[kGHi][j], lo = sm.rowv[kGLo][j];
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks < (w >> 1)) continue;
+        f32x4 d[2] = {f32x4{0.f, 0.f, 0.f, 0.f}, f32x4{0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+        for (int kk = 0; kk < KP / 32; ++kk) {
+          bf16x8 kb[NP];
+#pragma unroll
+          for (int i = 0; i < NP; ++i) kb[i] = op_rows<KP>(sm.k[i], w, kk, lane);
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            bf16x8 qa[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) qa[i] = op_rows<KP>(sm.q[i], 2 * ks + x, kk, lane);
+            d[x] = mul<2>(qa, kb, d[x]);
+          }
+        }
+        f32x8 pv = join(d[0], d[1]);
+        const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          pv[i] = 32 * ks + 8 * G + i >= j ? a.scale * pv[i] * fast_exp2((ghi[i] - hi) + (glo[i] - lo)) : 0.f;
+        bf16x8 s[3];
+        split(pv, s);
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          *reinterpret_cast<uint4 *>(&sm.p[i][(upper_set(w, ks) * 64 + lane) * 8]) = to_bits(s[i]);
+      }
+    }
+
+    f32x4 u[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) u[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KP / 32; ++ks) {
+      bf16x8 s[3];
+      split(join(D[2 * ks], D[2 * ks + 1]), s);
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        bf16x8 x[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) x[j] = op_rows<KP>(sm.k[j], t, ks, lane);
+        u[t] = mul<2>(x, s, u[t]);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const f32x8 el = row8(kToEnd, p);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        u[2 * p][r] *= el[r];
+        u[2 * p + 1][r] *= el[4 + r];
+      }
+    }
+    {
+      bf16x8 d[2][NP];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) split(dov[p], d[p]);
+      __syncthreads();   // P^T is written
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int ks = t / 2; ks < 2; ++ks) {
+          bf16x8 m[3];
+          set_of(sm.p, upper_set(t, ks), m);
+          u[t] = mul<2>(m, d[ks], u[t]);
+        }
+    }
+    f32x8 dX[2];
+    {
+      bf16x8 x[2][3];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) split(join(u[2 * p], u[2 * p + 1]), x[p]);
+      f32x4 y[4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        y[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = t / 2; ks < 2; ++ks) {
+          bf16x8 m[3];
+          set_of(sm.tm, upper_set(t, ks), m);
+          y[t] = mul<2>(m, x[ks], y[t]);
+        }
+      }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) dX[p] = join(y[2 * p], y[2 * p + 1]);
+    }
+    if constexpr (!SEG) {
+      const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const f32x8 bt = row8(kBeta, p);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int t = 32 * p + 8 * G + i;
+          if (v_ok && t < rows) {
+            const int64_t at = ((t0 + t) * a.H + h) * a.V + vcol;
+            ga.dx[at] = dX[p][i];
+            E::store(ga.dv, at, bt[i] * dX[p][i]);
+          }
+        }
+      }
+    }
+    // D <- e^(G_last) D + q^T (scale e^G do) - k^T (beta e^G dX)
+    bf16x8 x1[2][3], x2[2][3];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      split(row8(kScaleG, p) * dov[p], x1[p]);
+      split(-row8(kBetaG, p) * dX[p], x2[p]);
+    }
+    const float through = fast_exp2(sm.rowv[kGHi][kChunk - 1]) * fast_exp2(sm.rowv[kGLo][kChunk - 1]);
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      D[t] *= through;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        bf16x8 x[NP];
+#pragma unroll
+        for (int j = 0; j < NP; ++j) x[j] = op_cols<KP>(sm.q[j], t, ks, lane);
+        D[t] = mul<2>(x, x1[ks], D[t]);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) x[j] = op_cols<KP>(sm.k[j], t, ks, lane);
+        D[t] = mul<2>(x, x2[ks], D[t]);
+      }
+    }
+    __syncthreads();   // the chunk's tiles are read
+  }
+
+  if (!SEG) {
+    if (ga.dh0 && seg == 0 && v_ok) {
+      float *dst = ga.dh0 + (static_cast<int64_t>(n) * a.H + h) * KV;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int key = idx_of(t, 4 * G + r);
+          if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = D[t][r];
+        }
+    }
+  } else if (is_map) {
+    if (active) {
+      uint16_t *dst = a.seg_map + (slot * a.H + h) * (3 * KP * KP);
+      const int ks = mcol >> 5, lg = 16 * ((mcol & 31) >> 3), j = mcol & 7;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float x = D[t][r];
+#pragma unroll
+          for (int p = 0; p < 3; ++p) {
+            const uint16_t bits = f32_to_bf16_bits(x);
+            x -= bf16_bits_to_f32(bits);
+            dst[((t * (KP / 32) + ks) * 3 + p) * 512 + (lg + 4 * G + r) * 8 + j] = bits;
+          }
+        }
+    }
+  } else if (v_ok) {
+    float *dst = a.seg_state + (slot * a.H + h) * KV;
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int key = idx_of(t, 4 * G + r);
+        if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = D[t][r];
+      }
+  }
+}
+
+// ------------------------------------------------------ the chunks' gradients --
+template <int DT, int KP>
+struct GradSmem {
+  static constexpr int NP = Parts<DT>::n, KR = KP < 64 ? 64 : KP;
+  union {
+    struct {   // 32 value columns at a time
+      uint16_t dout[NP][kChunk * 32], u[3][kChunk * 32], dx[3][kChunk * 32], S[3][KR * 32], D[3][KR * 32];
+    } v;
+    struct {
+      uint16_t q[NP][kChunk * KP], k[NP][kChunk * KP];
+    } k;
+  };
+  float rowv[kRowVecs][kChunk];
+  float base[kChunk], to_next[kChunk], dxv[kChunk];
+  float sd[4];
+};
+
+// One workgroup per (chunk slot, head); wavefront w owns the rows of tile w.
+template <int DT, int KP>
+__global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
+  constexpr int NP = Parts<DT>::n, KT = KP / 16;
+  typedef Elem<DT> E;
+  typedef typename E::T ET;
+  const WalkArgs &a = ga.w;
+  __shared__ __align__(16) GradSmem<DT, KP> sm;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, G = lane >> 4;
+  const int h = static_cast<int>(blockIdx.x % a.H), hk = h / (a.H / a.Hk);
+  const int64_t slot = blockIdx.x / a.H;
+  int n;
+  int64_t bos, eos, first;
+  if (!seq_of_slot(a.cu, a.n_seq, a.T, kChunk, slot, n, bos, eos, first)) return;   // workgroup-uniform
+  const int64_t t0 = bos + (slot - first) * kChunk;
+  if (t0 >= eos) return;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+  const int64_t KV = static_cast<int64_t>(a.K) * a.V;
+  const float *Sp = a.chunk_state + (slot * a.H + h) * KV, *Dp = ga.chunk_grad + (slot * a.H + h) * KV;
+  const int64_t vat = (t0 * a.H + h) * a.V, vstride = static_cast<int64_t>(a.H) * a.V;
+
+  f32x4 Z[KT], Y[KT], W[KT], C1[4], C2[4], C3[4], C4[4];
+  const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int i = 0; i < KT; ++i) Z[i] = Y[i] = W[i] = zero;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) C1[i] = C2[i] = C3[i] = C4[i] = zero;
+  float dxv = 0.f, sd = 0.f;
+  const int pair = w >> 1;
+  for (int c0 = 0; c0 < a.V; c0 += 32) {
+    {
+      const int nc = a.V - c0;
+      RowTile<DT, 32> dt, vt;
+      RowTile<SSLA_F32, 32> ut, xt, st, gt;
+      dt.fetch(static_cast<const ET *>(ga.dout) + vat + c0, vstride, rows, nc, ga.dvec);
+      vt.fetch(static_cast<const ET *>(a.v) + vat + c0, vstride, rows, nc, ga.dvec);
+      ut.fetch(a.u + vat + c0, vstride, rows, nc, ga.vvec);
+      xt.fetch(ga.dx + vat + c0, vstride, rows, nc, ga.vvec);
+      dt.store(&sm.v.dout[0][0], kChunk * 32);
+      ut.store(&sm.v.u[0][0], kChunk * 32);
+      xt.store(&sm.v.dx[0][0], kChunk * 32);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) dxv = fmaf(vt.value(0, j), xt.value(0, j), dxv);
+#pragma unroll
+      for (int k0 = 0; k0 < KP; k0 += 64) {
+        constexpr int KR = GradSmem<DT, KP>::KR;
+        st.fetch(Sp + static_cast<int64_t>(k0) * a.V + c0, a.V, a.K - k0, nc, ga.vvec);
+        gt.fetch(Dp + static_cast<int64_t>(k0) * a.V + c0, a.V, a.K - k0, nc, ga.vvec);
+        st.store(&sm.v.S[0][k0 * 32], KR * 32);
+        gt.store(&sm.v.D[0][k0 * 32], KR * 32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sd = fmaf(st.value(0, j), gt.value(0, j), sd);
+      }
+    }
+    __syncthreads();
+    bf16x8 od[NP], ou[3], ox[3];   // this wavefront's rows of do, u, dX
+#pragma unroll
+    for (int i = 0; i < NP; ++i) od[i] = op_rows<32>(sm.v.dout[i], w, 0, lane);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      ou[i] = op_rows<32>(sm.v.u[i], w, 0, lane);
+      ox[i] = op_rows<32>(sm.v.dx[i], w, 0, lane);
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      bf16x8 s[3];
+#pragma unroll
+      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.v.S[i], t, 0, lane);
+      Z[t] = mul<2>(od, s, Z[t]);
+      Y[t] = mul<2>(ox, s, Y[t]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.v.D[i], t, 0, lane);
+      W[t] = mul<2>(ou, s, W[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if ((t >> 1) <= pair) {   // rows j <= i: u do^T, u dX^T
+        bf16x8 x[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.v.u[i], t, 0, lane);
+        C1[t] = mul<2>(x, od, C1[t]);
+        C2[t] = mul<2>(x, ox, C2[t]);
+      }
+      if ((t >> 1) >= pair) {   // rows i >= j: do u^T, dX u^T
+        bf16x8 x[3], y[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) y[i] = op_rows<32>(sm.v.dout[i], t, 0, lane);
+        C3[t] = mul<2>(y, ou, C3[t]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.v.dx[i], t, 0, lane);
+        C4[t] = mul<2>(x, ou, C4[t]);
+      }
+    }
+    __syncthreads();
+  }
+
+  {
+    RowTile<DT, KP> x;
+    const int64_t at = (t0 * a.Hk + hk) * a.K, stride = static_cast<int64_t>(a.Hk) * a.K;
+    x.fetch(static_cast<const ET *>(a.q) + at, stride, rows, a.K, a.vec);
+    x.store(&sm.k.q[0][0], kChunk * KP);
+    x.fetch(static_cast<const ET *>(a.k) + at, stride, rows, a.K, a.vec);
+    x.store(&sm.k.k[0][0], kChunk * KP);
+    const float *src = a.rowv + (slot * a.H + h) * kRowFloats;
+    for (int e = tid; e < kRowFloats; e += 256) (&sm.rowv[0][0])[e] = src[e];
+    dxv += __shfl_xor(dxv, 1);
+    dxv += __shfl_xor(dxv, 2);
+    if ((tid & 3) == 0) sm.dxv[tid >> 2] = dxv;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sd += __shfl_xor(sd, d);
+    if (lane == 0) sm.sd[w] = sd;
+  }
+  __syncthreads();
+
+  auto row8 = [&](int vec, int p) __attribute__((always_inline)) {
+    const f32x4 *s = reinterpret_cast<const f32x4 *>(&sm.rowv[vec][32 * p + 8 * G]);
+    return join(s[0], s[1]);
+  };
+  // dP, dN with this wavefront's rows i in the lanes (contraction j), and their
+  // transposes with its rows j in the lanes (contraction i); halves beyond the
+  // diagonal stay zero
+  bf16x8 pA[2][3], nA[2][3], pT[2][3], nT[2][3];
+  {
+    const int me = idx_of(w, col);
+    const float hi = sm.rowv[kGHi][me], lo = sm.rowv[kGLo][me];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks), bt = row8(kBeta, ks);
+      f32x8 p1 = join(C1[2 * ks], C1[2 * ks + 1]), n1 = join(C2[2 * ks], C2[2 * ks + 1]);
+      f32x8 p2 = join(C3[2 * ks], C3[2 * ks + 1]), n2 = join(C4[2 * ks], C4[2 * ks + 1]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = 32 * ks + 8 * G + j;
+        const float e = fast_exp2(r <= me ? (hi - ghi[j]) + (lo - glo[j]) : (ghi[j] - hi) + (glo[j] - lo));
+        p1[j] = r <= me ? a.scale * p1[j] * e : 0.f;
+        n1[j] = r < me ? -n1[j] * e : 0.f;
+        p2[j] = r >= me ? a.scale * p2[j] * e : 0.f;
+        n2[j] = r > me ? -bt[j] * n2[j] * e : 0.f;
+      }
+      split(p1, pA[ks]);
+      split(n1, nA[ks]);
+      split(p2, pT[ks]);
+      split(n2, nT[ks]);
+    }
+  }
+  // per own row: q . (from the state), q . (dP k), k . (dP^T q), k . (dN k),
+  // k . ((beta dN)^T k), k . (dX S^T), k . (u D^T)
+  float qa[4], qb[4], kc[4], kd[4], ke[4], ky[4], kw[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) qa[r] = qb[r] = kc[r] = kd[r] = ke[r] = ky[r] = kw[r] = 0.f;
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    f32x4 b = zero, c = zero, d = zero, e = zero;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      bf16x8 x[NP];
+#pragma unroll
+      for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.k[i], t, ks, lane);
+      if (ks <= pair) {
+        b = mul<2>(pA[ks], x, b);
+        d = mul<2>(nA[ks], x, d);
+      }
+      if (ks >= pair) {
+        e = mul<2>(nT[ks], x, e);
+#pragma unroll
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.q[i], t, ks, lane);
+        c = mul<2>(pT[ks], x, c);
+      }
+    }
+    const int key = idx_of(t, col);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = idx_of(w, 4 * G + r);
+      float qv = 0.f, kv = 0.f;
+#pragma unroll
+      for (int j = NP - 1; j >= 0; --j) {
+        qv += bf16_bits_to_f32(sm.k.q[j][sw<KP>(i, key)]);
+        kv += bf16_bits_to_f32(sm.k.k[j][sw<KP>(i, key)]);
+      }
+      const float ia = sm.rowv[kScaleG][i] * Z[t][r], bt = sm.rowv[kBeta][i], hw = sm.rowv[kToEnd][i] * W[t][r];
+      qa[r] = fmaf(qv, ia, qa[r]);
+      qb[r] = fmaf(qv, b[r], qb[r]);
+      kc[r] = fmaf(kv, c[r], kc[r]);
+      kd[r] = fmaf(kv, d[r], kd[r]);
+      ke[r] = fmaf(kv, e[r], ke[r]);
+      ky[r] = fmaf(kv, Y[t][r], ky[r]);
+      kw[r] = fmaf(kv, hw, kw[r]);
+      const float dq = ia + b[r];
+      const float dk = (c[r] + e[r]) + fmaf(bt, d[r], fmaf(-sm.rowv[kBetaG][i], Y[t][r], hw));
+      if (i < rows && key < a.K) {
+        if (ga.dq_part) {
+          const int64_t at = ((t0 + i) * a.H + h) * a.K + key;
+          ga.dq_part[at] = dq;
+          ga.dk_part[at] = dk;
+        } else {
+          const int64_t at = ((t0 + i) * a.Hk + hk) * a.K + key;
+          E::store(ga.dq, at, dq);
+          E::store(ga.dk, at, dk);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int m = 1; m < 16; m <<= 1)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      qa[r] += __shfl_xor(qa[r], m);
+      qb[r] += __shfl_xor(qb[r], m);
+      kc[r] += __shfl_xor(kc[r], m);
+      kd[r] += __shfl_xor(kd[r], m);
+      ke[r] += __shfl_xor(ke[r], m);
+      ky[r] += __shfl_xor(ky[r], m);
+      kw[r] += __shfl_xor(kw[r], m);
+    }
+  if (col == 0) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int i = idx_of(w, 4 * G + r);
+      const float bt = sm.rowv[kBeta][i], eg = fast_exp2(sm.rowv[kGHi][i]) * fast_exp2(sm.rowv[kGLo][i]);
+      sm.base[i] = (qa[r] - sm.rowv[kBetaG][i] * ky[r]) + ((qb[r] - kc[r]) + (bt * kd[r] - ke[r]));
+      sm.to_next[i] = kw[r];
+      if (i < rows) ga.dbeta[(t0 + i) * a.H + h] = sm.dxv[i] + fmaf(-eg, ky[r], kd[r]);
+    }
+  }
+  __syncthreads();
+  if (w == 0) {
+    // dg_t = sum_(i >= t) base_i + sum_(j < t) to_next_j + e^(G_last) <S, D>
+    float s = sm.base[lane], p = sm.to_next[lane];
+    const float mine = p;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const float down = __shfl_down(s, d), up = __shfl_up(p, d);
+      if (lane + d < 64) s += down;
+      if (lane >= d) p += up;
+    }
+    const float through = fast_exp2(sm.rowv[kGHi][kChunk - 1]) * fast_exp2(sm.rowv[kGLo][kChunk - 1]);
+    const float sdt = (sm.sd[0] + sm.sd[1]) + (sm.sd[2] + sm.sd[3]);
+    if (lane < rows) ga.dg[(t0 + lane) * a.H + h] = s + fmaf(through, sdt, p - mine);
+  }
+}
+
+// dq, dk of the key heads: their value heads' in order.
+template <int DT>
+__global__ __launch_bounds__(256) void delta_heads_kernel(const int64_t *__restrict__ cu, int n_seq, int64_t T, int Hk,
+                                                          int rep, int K, const float *__restrict__ dq_part,
+                                                          const float *__restrict__ dk_part, void *__restrict__ dq,
+                                                          void *__restrict__ dk) {
+  const int64_t start = min(max(cu[0], (int64_t)0), T), end = min(max(cu[n_seq], start), T);
+  const int64_t per = static_cast<int64_t>(Hk) * K, n = (end - start) * per;
+  for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < n; e += static_cast<int64_t>(gridDim.x) * 256) {
+    const int64_t t = start + e / per, hk = (e % per) / K, key = e % K;
+    const int64_t src = ((t * Hk + hk) * rep) * K + key, dst = start * per + e;
+    float s = 0.f, x = 0.f;
+    for (int r = 0; r < rep; ++r) {
+      s += dq_part[src + static_cast<int64_t>(r) * K];
+      x += dk_part[src + static_cast<int64_t>(r) * K];
+    }
+    Elem<DT>::store(dq, dst, s);
+    Elem<DT>::store(dk, dst, x);
+  }
+}
+
+// Zeros in the rows of no sequence: n elements of `wide` 2- or 4-byte values a row.
+template <typename U>
+__device__ __forceinline__ void zero_rows(void *p, int64_t row, int64_t wide) {
+  for (int64_t i = threadIdx.x; i < wide; i += 256) static_cast<U *>(p)[row * wide + i] = U(0);
+}
+template <typename U>
+__global__ __launch_bounds__(256) void delta_outside_kernel(const GradArgs ga) {
+  const WalkArgs &a = ga.w;
+  const int64_t start = min(max(a.cu[0], (int64_t)0), a.T), end = min(max(a.cu[a.n_seq], start), a.T);
+  const int64_t n = start + (a.T - end);
+  for (int64_t i = blockIdx.x; i < n; i += gridDim.x) {
+    const int64_t row = i < start ? i : end + (i - start);
+    zero_rows<U>(ga.dq, row, static_cast<int64_t>(a.Hk) * a.K);
+    zero_rows<U>(ga.dk, row, static_cast<int64_t>(a.Hk) * a.K);
+    zero_rows<U>(ga.dv, row, static_cast<int64_t>(a.H) * a.V);
+    zero_rows<float>(ga.dg, row, a.H);
+    zero_rows<float>(ga.dbeta, row, a.H);
+  }
+}
+
+// ------------------------------------------------------------------ launches --
+inline dim3 grid_of(int64_t n) { return dim3(static_cast<unsigned>(n)); }
+
+template <int DT, int KP>
+int launch_bwd(const DeltaLayout &L, const GradArgs &ga, hipStream_t st) {
+  const WalkArgs &a = ga.w;
+  const dim3 block(256);
+  const int vg = ((a.V + 15) / 16 + 3) / 4;
+  if (L.inner_slots > 0) {
+    const int groups = ((a.V + 15) / 16 + KP / 16 + 3) / 4;
+    hipLaunchKernelGGL((delta_reverse_kernel<DT, KP, true>), grid_of(L.inner_slots * a.H * groups), block, 0, st, ga);
+    if (const int e = delta_fold(L, a, ga.dht, true, st)) return e;
+  }
+  hipLaunchKernelGGL((delta_reverse_kernel<DT, KP, false>), grid_of(L.seg_slots * a.H * vg), block, 0, st, ga);
+  hipLaunchKernelGGL((delta_grad_kernel<DT, KP>), grid_of(L.chunk_slots * a.H), block, 0, st, ga);
+  return launch_status("gated_delta_chunk_bwd");
+}
+
+template <int DT>
+int launch_keys(const DeltaLayout &L, const GradArgs &ga, hipStream_t st) {
+  int e;
+  if (L.KP == 32) e = launch_bwd<DT, 32>(L, ga, st);
+  else if (L.KP == 64) e = launch_bwd<DT, 64>(L, ga, st);
+  else e = launch_bwd<DT, 128>(L, ga, st);
+  if (e) return e;
+  const WalkArgs &a = ga.w;
+  if (ga.dq_part && a.T > 0) {
+    const int64_t n = a.T * a.Hk * a.K;
+    hipLaunchKernelGGL((delta_heads_kernel<DT>), grid_of(std::min<int64_t>((n + 255) / 256, 1 << 16)), dim3(256), 0, st,
+                       a.cu, a.n_seq, a.T, a.Hk, a.H / a.Hk, a.K, ga.dq_part, ga.dk_part, ga.dq, ga.dk);
+  }
+  return launch_status("gated_delta_chunk_bwd");
+}
+
+}  // namespace
+}  // namespace ssla
+
+extern "C" size_t ssla_gated_delta_chunk_bwd_workspace_size(int n_seq, int64_t T, int Hk, int H, int K, int V) {
+  if (n_seq < 0 || T < 0 || Hk <= 0 || H <= 0 || H % Hk || K <= 0 || K > 128 || V <= 0) return 0;
+  return ssla::delta_layout(n_seq, T, Hk, H, K, V, true).total;
+}
+
+extern "C" int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const void *v, const float *g,
+                                          const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk,
+                                          int H, int K, int V, float scale, const float *h0, const void *dout,
+                                          const float *dht, void *dq, void *dk, void *dv, float *dg, float *dbeta,
+                                          float *dh0, int dtype, void *workspace, size_t workspace_bytes,
+                                          void *stream) {
+  using namespace ssla;
+  clear_error();
+  SSLA_CHECK_ARG(n_seq >= 0 && T >= 0 && Hk > 0 && H > 0 && H % Hk == 0 && K > 0 && V > 0,
+                 "gated_delta_chunk_bwd: bad sizes n_seq=%d T=%lld Hk=%d H=%d K=%d V=%d", n_seq, (long long)T, Hk, H, K,
+                 V);
+  if (K > 128) {
+    set_error("gated_delta_chunk_bwd: K=%d exceeds 128", K);
+    return SSLA_ERR_UNSUPPORTED;
+  }
+  SSLA_CHECK_ARG(cu_seqlens != nullptr, "gated_delta_chunk_bwd: cu_seqlens is NULL");
+  SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && dout && dq && dk && dv && dg && dbeta),
+                 "gated_delta_chunk_bwd: null tensor pointer");
+  if (dtype != SSLA_F32 && dtype != SSLA_BF16 && dtype != SSLA_F16) {
+    set_error("gated_delta_chunk_bwd: unsupported dtype %d", dtype);
+    return SSLA_ERR_DTYPE;
+  }
+  const DeltaLayout L = delta_layout(n_seq, T, Hk, H, K, V, true);
+  if (!workspace || workspace_bytes < L.total || !aligned(workspace, 16)) {
+    set_error("gated_delta_chunk_bwd: needs %zu bytes of workspace, got %zu", L.total, workspace_bytes);
+    return SSLA_ERR_WORKSPACE;
+  }
+  char *ws = static_cast<char *>(workspace);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  GradArgs ga{};
+  ga.w = walk_args(L, ws, q, k, v, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, dtype, true);
+  ga.dout = dout;
+  ga.dht = dht;
+  ga.chunk_grad = reinterpret_cast<float *>(ws + L.chunk_grad);
+  ga.dx = reinterpret_cast<float *>(ws + L.dx);
+  ga.dq = dq; ga.dk = dk; ga.dv = dv; ga.dg = dg; ga.dbeta = dbeta; ga.dh0 = dh0;
+  if (H > Hk) {
+    ga.dq_part = reinterpret_cast<float *>(ws + L.dq);
+    ga.dk_part = reinterpret_cast<float *>(ws + L.dk);
+  }
+  ga.vvec = V % 4 == 0;
+  ga.dvec = (static_cast<int64_t>(V) * (dtype == SSLA_F32 ? 4 : 2)) % 16 == 0 && aligned(dout, 16) && aligned(v, 16);
+  if (T > 0) {
+    const dim3 grid = grid_of(std::min<int64_t>(T, 1024));
+    if (dtype == SSLA_F32) hipLaunchKernelGGL((delta_outside_kernel<float>), grid, dim3(256), 0, st, ga);
+    else hipLaunchKernelGGL((delta_outside_kernel<uint16_t>), grid, dim3(256), 0, st, ga);
+  }
+  if (n_seq == 0) return launch_status("gated_delta_chunk_bwd");
+  if (const int e = delta_forward_states(L, ga.w, g, beta, dtype, st)) return e;
+  switch (dtype) {
+    case SSLA_F32: return launch_keys<SSLA_F32>(L, ga, st);
+    case SSLA_BF16: return launch_keys<SSLA_BF16>(L, ga, st);
+    default: return launch_keys<SSLA_F16>(L, ga, st);
+  }
+}

@@ -87,10 +87,10 @@ __device__ __forceinline__ bf16x8 op_cols(const uint16_t *t, int tile, int ks, i
   return from_bits<bf16x8>(make_uint4(u[0].x, u[0].y, u[1].x, u[1].y));
 }
 
-// Rows t0 .. of one head of a [T, heads, D] tensor, fetched into registers by
-// 256 threads and stored to LDS as Parts<DT>::n tiles of bf16; rows from
-// n_rows on and columns from D on are zero.  Rows of whole 16-byte pieces at
-// aligned addresses (vec) are read 16 bytes at a time.
+// 64 rows of a matrix with row stride `stride`, fetched into registers by 256
+// threads and stored to LDS as Parts<DT>::n tiles of bf16; rows from n_rows on
+// and columns from n_cols on are zero.  Where rows are whole 16-byte pieces at
+// aligned addresses (vec) they are read 16 bytes at a time.
 template <int DT, int KP>
 struct RowTile {
   static constexpr int U = KP / 32;   // 8-column pieces of a thread
@@ -98,23 +98,27 @@ struct RowTile {
   struct Piece { E e[8]; };
   Piece p[U];
 
-  __device__ __forceinline__ void fetch(const void *base, int64_t t0, int n_rows, int heads, int head, int D, bool vec) {
-    const E *x = static_cast<const E *>(base);
+  __device__ __forceinline__ void fetch(const E *x, int64_t stride, int n_rows, int n_cols, bool vec) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int u = threadIdx.x + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
-      const E *src = x + ((t0 + row) * heads + head) * D + col;
-      if (row < n_rows && vec && col + 8 <= D) {
+      const E *src = x + row * stride + col;
+      if (row < n_rows && vec && col + 8 <= n_cols) {
         constexpr int W = sizeof(Piece) / 16;
-        uint4 w[W];
+        struct Raw { uint4 w[W]; } raw;
 #pragma unroll
-        for (int j = 0; j < W; ++j) w[j] = reinterpret_cast<const uint4 *>(src)[j];
-        p[i] = __builtin_bit_cast(Piece, w);
+        for (int j = 0; j < W; ++j) raw.w[j] = reinterpret_cast<const uint4 *>(src)[j];
+        p[i] = __builtin_bit_cast(Piece, raw);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[i].e[j] = (row < n_rows && col + j < D) ? src[j] : E(0);
+        for (int j = 0; j < 8; ++j) p[i].e[j] = (row < n_rows && col + j < n_cols) ? src[j] : E(0);
       }
     }
+  }
+  __device__ __forceinline__ float value(int i, int j) const {   // column j of piece i
+    if constexpr (DT == SSLA_BF16) return bf16_bits_to_f32(p[i].e[j]);
+    else if constexpr (DT == SSLA_F16) return f16_bits_to_f32(p[i].e[j]);
+    else return p[i].e[j];
   }
   // plane j at t + j * stride elements
   __device__ __forceinline__ void store(uint16_t *t, int stride) const {
@@ -127,10 +131,7 @@ struct RowTile {
       } else {
         f32x8 x;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if constexpr (DT == SSLA_F16) x[j] = f16_bits_to_f32(p[i].e[j]);
-          else x[j] = p[i].e[j];
-        }
+        for (int j = 0; j < 8; ++j) x[j] = value(i, j);
         bf16x8 s[Parts<DT>::n];
         split(x, s);
 #pragma unroll
@@ -142,12 +143,105 @@ struct RowTile {
 
 // The chunks' matrices and row factors that every pass reads, written once by
 // the first kernel: per (chunk slot, head) the operands of Tm = (I + A)^-1 in
-// fp32 (set by set, 64 lanes of 8 values) and kRowVecs vectors of 64 floats.
+// fp32 (set by set, 64 lanes of 8 values), for the backward those of its
+// transpose behind them, and kRowVecs vectors of 64 floats.
 enum { kBeta = 0, kBetaG, kScaleG, kToEnd, kGHi, kGLo, kRowVecs };
 constexpr int kRowFloats = kRowVecs * kChunk;
 
 // Chunk c (of 64 rows) of sequence n that starts at row bos has slot
 // bos / 64 + n + c; see seq_of_slot.
 __device__ __forceinline__ int64_t chunk_slot(int64_t bos, int n, int64_t c) { return bos / kChunk + n + c; }
+
+inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
+inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
+
+// Chunks per segment: at least 4, and as many as leave about 512 workgroups
+// (two a CU) of 64 value columns.
+inline int seg_chunks(int64_t T, int H, int V) {
+  const int64_t work = (T / kChunk + 1) * H * ((V + 63) / 64);
+  return static_cast<int>(std::min<int64_t>(1 << 20, std::max<int64_t>(4, (work + 511) / 512)));
+}
+
+// Workspace of the forward, and (grad) of the backward.
+struct DeltaLayout {
+  size_t tm, rowv, state, map, chunk_state, chunk_grad, u, dx, dq, dk, total;
+  int64_t chunk_slots, seg_slots, inner_slots;
+  int per, KP;
+};
+inline DeltaLayout delta_layout(int n_seq, int64_t T, int Hk, int H, int K, int V, bool grad) {
+  DeltaLayout L{};
+  L.KP = padded_keys(K);
+  L.per = seg_chunks(T, H, V);
+  const int64_t unit = static_cast<int64_t>(L.per) * kChunk;
+  L.chunk_slots = T / kChunk + n_seq + 1;
+  L.seg_slots = T / unit + n_seq + 1;
+  L.inner_slots = T > 0 ? (T - 1) / unit : 0;   // 0: no sequence is cut
+  size_t p = 0;
+  auto take = [&](size_t bytes) {
+    const size_t at = p;
+    p = align256(p + bytes);
+    return at;
+  };
+  const size_t kv = static_cast<size_t>(K) * V * sizeof(float);
+  L.tm = take(sizeof(float) * kTriFloats * (grad ? 2 : 1) * L.chunk_slots * H);
+  L.rowv = take(sizeof(float) * kRowFloats * L.chunk_slots * H);
+  L.state = take(kv * L.inner_slots * H);
+  L.map = take(sizeof(uint16_t) * 3 * L.inner_slots * H * L.KP * L.KP);
+  if (grad) {
+    L.chunk_state = take(kv * L.chunk_slots * H);
+    L.chunk_grad = take(kv * L.chunk_slots * H);
+    L.u = take(sizeof(float) * T * H * V);
+    L.dx = take(sizeof(float) * T * H * V);
+    L.dq = take(H > Hk ? sizeof(float) * T * H * K : 0);
+    L.dk = take(H > Hk ? sizeof(float) * T * H * K : 0);
+  }
+  L.total = p;
+  return L;
+}
+
+struct WalkArgs {
+  const void *q, *k, *v;
+  const int64_t *cu;
+  const float *tm, *rowv;
+  const float *h0;
+  void *o;
+  float *ht;
+  float *seg_state;       // per inner segment: L, after the fold the state entering the next segment
+  uint16_t *seg_map;      // per inner segment: M as operands of three bf16 parts
+  float *chunk_state;     // per chunk: the state entering it
+  float *u;               // [T, H, V]
+  int64_t T;
+  int n_seq, Hk, H, K, V, per, vec, tm_floats;
+  float scale;
+};
+
+inline WalkArgs walk_args(const DeltaLayout &L, char *ws, const void *q, const void *k, const void *v, const int64_t *cu,
+                          int n_seq, int64_t T, int Hk, int H, int K, int V, float scale, const float *h0, int dtype,
+                          bool grad) {
+  WalkArgs a{};
+  a.q = q; a.k = k; a.v = v; a.cu = cu; a.h0 = h0;
+  a.tm = reinterpret_cast<float *>(ws + L.tm);
+  a.rowv = reinterpret_cast<float *>(ws + L.rowv);
+  a.seg_state = reinterpret_cast<float *>(ws + L.state);
+  a.seg_map = reinterpret_cast<uint16_t *>(ws + L.map);
+  if (grad) {
+    a.chunk_state = reinterpret_cast<float *>(ws + L.chunk_state);
+    a.u = reinterpret_cast<float *>(ws + L.u);
+  }
+  a.T = T; a.n_seq = n_seq; a.Hk = Hk; a.H = H; a.K = K; a.V = V; a.per = L.per; a.scale = scale;
+  a.tm_floats = kTriFloats * (grad ? 2 : 1);
+  a.vec = (static_cast<int64_t>(K) * (dtype == SSLA_F32 ? 4 : 2)) % 16 == 0 && aligned(q, 16) && aligned(k, 16);
+  return a;
+}
+
+// The chunks' matrices, the segments' states and every chunk's entering state
+// and u (delta_chunk.hip), for the backward.
+int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, int dtype,
+                         hipStream_t st);
+
+// Carries states over a sequence's segments (delta_chunk.hip): forward, the L of
+// segment j becomes the state entering segment j + 1; in reverse the gradient's
+// L of segment j + 1 becomes the gradient leaving segment j.
+int delta_fold(const DeltaLayout &L, const WalkArgs &a, const float *start, bool reverse, hipStream_t st);
 
 }  // namespace ssla

@@ -29,7 +29,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["chunk_gated_delta", "fused_recurrent_gated_delta", "sparse_delta_scan", "sparse_delta_step"]
+__all__ = ["chunk_gated_delta", "ChunkGatedDeltaFunction", "fused_recurrent_gated_delta", "sparse_delta_scan", "sparse_delta_step"]
 
 
 def _shapes(name, q, k, v, g, beta):
@@ -97,6 +97,41 @@ def _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
     return o, ht
 
 
+class ChunkGatedDeltaFunction(torch.autograd.Function):
+    """Forward ``ssla_gated_delta_chunk_fwd``, backward
+    ``ssla_gated_delta_chunk_bwd``, which computes the states again from the
+    inputs.  dq, dk, dv have the inputs' dtype, dg, dbeta and dh0 are fp32."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, h0, cu, scale, output_final_state):
+        o, ht = _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
+        ctx.save_for_backward(q, k, v, g, beta, h0, cu)
+        ctx.scale = scale
+        ctx.set_materialize_grads(False)
+        return o, ht
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, do, dht):
+        q, k, v, g, beta, h0, cu = ctx.saved_tensors
+        T, Hk, K = q.shape
+        H, V = v.shape[1:]
+        N = cu.numel() - 1
+        do = torch.zeros_like(v) if do is None else do.to(v.dtype).contiguous()
+        dht = None if dht is None else dht.to(torch.float32).contiguous()
+        dq, dk, dv, dg, dbeta = (torch.empty_like(t) for t in (q, k, v, g, beta))
+        dh0 = None if h0 is None else torch.empty_like(h0)
+        lib, P = _lib.load(), _lib.ptr
+        with _lib.on_device_of(q):
+            nbytes = lib.ssla_gated_delta_chunk_bwd_workspace_size(N, T, Hk, H, K, V)
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+            st = lib.ssla_gated_delta_chunk_bwd(
+                P(q), P(k), P(v), P(g), P(beta), P(cu), N, T, Hk, H, K, V, ctx.scale, P(h0), P(do), P(dht), P(dq), P(dk),
+                P(dv), P(dg), P(dbeta), P(dh0), _lib.DTYPE_CODE[q.dtype], P(ws), nbytes, _lib.stream_of(q))
+        _lib.check(st, "ssla_gated_delta_chunk_bwd")
+        return dq, dk, dv, dg, dbeta, dh0, None, None, None
+
+
 def chunk_gated_delta(
     q: torch.Tensor,
     k: torch.Tensor,
@@ -113,8 +148,9 @@ def chunk_gated_delta(
     Rows of o outside ``[cu_seqlens[0], cu_seqlens[-1])`` are unspecified.
 
     K up to 128 runs the chunk kernels, whose products keep the precision of
-    fp32 for every dtype; wider keys run the token-by-token kernel (K up to
-    256)."""
+    fp32 for every dtype, and is differentiable in q, k, v, g, beta and the
+    initial state (once; rows in no sequence get zeros); wider keys run the
+    token-by-token kernel (K up to 256), forward only."""
     name = "chunk_gated_delta"
     T, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
     dev = _lib.require_cuda(q, k, v, g, beta, initial_state)
@@ -122,14 +158,19 @@ def chunk_gated_delta(
     N = cu.numel() - 1
     if initial_state is not None and initial_state.shape != (N, H, K, V):
         raise ValueError(f"{name}: initial_state must be {(N, H, K, V)}, got {tuple(initial_state.shape)}")
-    _lib.require_no_grad(name, q, k, v, g, beta, initial_state)
     scale = K ** -0.5 if scale is None else float(scale)
     h0 = None if initial_state is None else initial_state.to(torch.float32).contiguous()
-    if K > 128 or N == 0 or T == 0:
+    grad = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
+    if grad and K > 128:
+        raise NotImplementedError(f"{name}: the backward takes K up to 128 (got {K}; call it under torch.no_grad())")
+    if not grad and (K > 128 or N == 0 or T == 0):
         ht = torch.empty(N, H, K, V, device=dev, dtype=torch.float32) if output_final_state else None
         return _recurrent(q, k, v, g, beta, cu, N, scale, h0, ht), ht
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     g, beta = g.to(torch.float32).contiguous(), beta.to(torch.float32).contiguous()
+    if grad:
+        return ChunkGatedDeltaFunction.apply(q, k, v, g, beta, h0, cu, scale, output_final_state)
     return _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
 
 

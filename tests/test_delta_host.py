@@ -123,3 +123,22 @@ def test_chunk_entry_refuses():
     assert call(T=0, ws=16, nbytes=size(1, 0, 1, 16, 16), dtype=9) == _lib.SSLA_ERR_DTYPE
     assert size(1, 64, 1, 129, 16) == 0 and size(-1, 64, 1, 16, 16) == 0
     assert 0 < size(1, 64, 1, 16, 16) < size(2, 64, 1, 16, 16) < size(2, 640, 1, 16, 16) < size(2, 640, 2, 16, 16)
+
+
+def test_chunk_backward_entry_refuses():
+    lib = _lib.load()
+
+    def call(n=1, T=4, Hk=1, H=1, K=16, V=16, cu=8, dtype=0, ws=None, nbytes=0):
+        return lib.ssla_gated_delta_chunk_bwd(None, None, None, None, None, cu, n, T, Hk, H, K, V, 1.0, None, None, None,
+                                              None, None, None, None, None, None, dtype, ws, nbytes, None)
+
+    for bad in (dict(n=-1), dict(T=-1), dict(Hk=0), dict(H=0), dict(Hk=2, H=3), dict(K=0), dict(V=0)):
+        assert call(**bad) == _lib.SSLA_ERR_ARG, bad
+    assert call(K=129) == _lib.SSLA_ERR_UNSUPPORTED
+    assert call(cu=None) == _lib.SSLA_ERR_ARG and call() == _lib.SSLA_ERR_ARG
+    assert call(T=0, dtype=9) == _lib.SSLA_ERR_DTYPE
+    size = lib.ssla_gated_delta_chunk_bwd_workspace_size
+    assert call(T=0) == _lib.SSLA_ERR_WORKSPACE
+    assert call(T=0, ws=16, nbytes=size(1, 0, 1, 1, 16, 16) - 1) == _lib.SSLA_ERR_WORKSPACE
+    assert size(1, 64, 1, 1, 129, 16) == 0 and size(1, 64, 2, 3, 16, 16) == 0
+    assert size(1, 64, 2, 2, 16, 16) < size(1, 64, 1, 2, 16, 16)
