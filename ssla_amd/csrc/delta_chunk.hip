@@ -42,7 +42,6 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
   constexpr int NP = Parts<DT>::n, LD = 68;
   __shared__ __align__(16) uint16_t sk[NP][kChunk * KP];
   __shared__ __align__(16) float A[kChunk][LD];   // I + A, then Tm
-  __shared__ __align__(16) float Y[32][LD - 32];  // a product between two of the joins
   __shared__ float sv[kRowVecs][kChunk];
   __shared__ float diag[kChunk];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -56,8 +55,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
   const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
 
   RowTile<DT, KP> kt;
-  typedef typename Elem<DT>::T E;
-  kt.fetch(static_cast<const E *>(k) + (t0 * Hk + hk) * K, static_cast<int64_t>(Hk) * K, rows, K, vec);
+  kt.fetch(rows_rsrc(k, (t0 * Hk + hk) * K, rows, Hk * K, K, RowTile<DT, KP>::ES), Hk * K, K, vec);
   float gv = 0.f, bv = 0.f;
   if (w == 0 && lane < rows) {
     gv = g[(t0 + lane) * H + h];
@@ -125,18 +123,21 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
   }
   __syncthreads();
   {
-    const int col = lane & 15, r = (lane >> 4) * 4;
+    const int col = lane & 15, row = idx_of(w, (lane >> 4) * 4);   // and the three rows behind it
+    const f32x4 hi = *reinterpret_cast<const f32x4 *>(&sv[kGHi][row]), lo = *reinterpret_cast<const f32x4 *>(&sv[kGLo][row]);
+    const f32x4 bt = *reinterpret_cast<const f32x4 *>(&diag[row]);
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int j = 0; j < 4; ++j) {
+      if (j > (w | 1)) continue;
+      const int c = idx_of(j, col);
+      const float chi = sv[kGHi][c], clo = sv[kGLo][c];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = idx_of(w, r + i), c = idx_of(j, col);
-        float x = row == c ? 1.f : 0.f;
+        const float x = bt[i] * acc[j][i] * fast_exp2((hi[i] - chi) + (lo[i] - clo));
         // (a selection, not a product: what is above the diagonal or left out may be NaN)
-        if (c < row && diag[row] != 0.f)
-          x = diag[row] * acc[j][i] * fast_exp2((sv[kGHi][row] - sv[kGHi][c]) + (sv[kGLo][row] - sv[kGLo][c]));
-        A[row][c] = x;
+        A[row + i][c] = row + i == c ? 1.f : keep(c < row + i && bt[i] != 0.f, x);
       }
+    }
   }
   // (rows r0.. have beta 0, so row r0's NaN keys reach no other row: row > c >= r0 is left out by its own beta)
   __syncthreads();
@@ -156,41 +157,48 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
     for (int i = 0; i < 16; ++i) A[b + i][b + c] = i < c ? 0.f : x[i];
   }
   __syncthreads();
-  // joins: [[P, 0], [C, Q]]^-1 = [[P^-1, 0], [-Q^-1 C P^-1, Q^-1]]
-  {   // blocks of 16, two pairs: 128 threads each, a row and two columns
-    const int pr = tid >> 7, i = (tid & 127) >> 3, c = (tid & 7) * 2, b = 32 * pr;
-    float y0 = 0.f, y1 = 0.f;
+  // joins: [[P, 0], [C, Q]]^-1 = [[P^-1, 0], [-Q^-1 C P^-1, Q^-1]], in fp32
+  const int m = lane & 15, gr = lane >> 4;
+  if (w < 2) {   // blocks of 16, a pair for each of two wavefronts
+    const int b = 32 * w;
+    float x[4], y[4];
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float a = A[b + 16 + i][b + j];
-      y0 = fmaf(a, A[b + j][b + c], y0);
-      y1 = fmaf(a, A[b + j][b + c + 1], y1);
+    for (int j = 0; j < 4; ++j) {
+      x[j] = A[b + 16 + m][b + 4 * gr + j];
+      y[j] = A[b + 4 * gr + j][b + m];
     }
-    Y[16 * pr + i][c] = y0;
-    Y[16 * pr + i][c + 1] = y1;
-    __syncthreads();
-    y0 = y1 = 0.f;
+    f32x4 c = mul_f32(x, y, f32x4{0.f, 0.f, 0.f, 0.f});   // rows 4 gr + i = the next product's contraction
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float a = A[b + 16 + i][b + 16 + j];
-      y0 = fmaf(a, Y[16 * pr + j][c], y0);
-      y1 = fmaf(a, Y[16 * pr + j][c + 1], y1);
+    for (int j = 0; j < 4; ++j) {
+      x[j] = A[b + 16 + m][b + 16 + 4 * gr + j];
+      y[j] = c[j];
     }
-    A[b + 16 + i][b + c] = -y0;
-    A[b + 16 + i][b + c + 1] = -y1;
+    c = mul_f32(x, y, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+    for (int i = 0; i < 4; ++i) A[b + 16 + 4 * gr + i][b + m] = -c[i];
   }
   __syncthreads();
-  {   // blocks of 32: a row and four columns of each thread
-    const int i = tid >> 3, c = (tid & 7) * 4;
-    f32x4 y = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) y += A[32 + i][j] * *reinterpret_cast<const f32x4 *>(&A[j][c]);
-    *reinterpret_cast<f32x4 *>(&Y[i][c]) = y;
-    __syncthreads();
-    y = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 8
-    for (int j = 0; j < 32; ++j) y += A[32 + i][32 + j] * *reinterpret_cast<const f32x4 *>(&Y[j][c]);
-    *reinterpret_cast<f32x4 *>(&A[32 + i][c]) = -y;
+  {   // blocks of 32: wavefront w has 16 columns; both row tiles of C P^-1 feed its column of the second product
+    const int ct = 16 * (w & 1), rt = 16 * (w >> 1);
+    float x[8], y[8];
+    f32x4 c[2];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) y[j] = A[8 * gr + j][ct + m];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = A[32 + idx_of(t, m)][8 * gr + j];
+      c[t] = mul_f32(x, y, f32x4{0.f, 0.f, 0.f, 0.f});
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      x[j] = A[32 + rt + m][32 + 8 * gr + j];
+      y[j] = c[j >> 2][j & 3];
+    }
+    c[0] = mul_f32(x, y, f32x4{0.f, 0.f, 0.f, 0.f});
+    __syncthreads();   // C is read
+#pragma unroll
+    for (int i = 0; i < 4; ++i) A[32 + rt + 4 * gr + i][ct + m] = -c[0][i];
   }
   __syncthreads();
   float *dst = tm + (slot * H + h) * tm_floats;
@@ -260,44 +268,39 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   const bool active = is_map ? mcol < KP : tile < n_vt, v_ok = !is_map && vcol < a.V;
   const int64_t KV = static_cast<int64_t>(a.K) * a.V;
 
+  const StateCols<NT> cols(a.K, a.V, vcol, v_ok, G);
   f32x4 S[NT];
-  {
-    const float *src = nullptr;
-    if (!SEG) {
-      if (seg == 0) src = a.h0 ? a.h0 + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr;
-      else src = a.seg_state + ((bos / unit + seg - 1) * a.H + h) * KV;
-    }
+  if (!SEG) {
+    cols.load(seg > 0 ? a.seg_state + ((bos / unit + seg - 1) * a.H + h) * KV
+              : a.h0  ? a.h0 + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr, S);
+  } else {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = idx_of(t, 4 * G + r);
-        float x = is_map && key == mcol ? 1.f : 0.f;
-        if (!SEG && src && v_ok && key < a.K) x = src[static_cast<int64_t>(key) * a.V + vcol];
-        S[t][r] = x;
-      }
+      for (int r = 0; r < 4; ++r) S[t][r] = is_map && idx_of(t, 4 * G + r) == mcol ? 1.f : 0.f;
   }
+  // byte offset of row 8 G in this lane's column of v, o and u (in values of 4 bytes for u)
+  constexpr int ES = sizeof(ET);
+  const uint32_t vrow = static_cast<uint32_t>(a.H) * a.V, voff = v_ok ? (8 * G * vrow + vcol) * ES : kOutside;
 
   RowTile<DT, KP> kt, qt;
   f32x4 tmr[3], rvr;
   ET vr[16];
   auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
-    const int64_t at = (t0 * a.Hk + hk) * a.K, stride = static_cast<int64_t>(a.Hk) * a.K;
-    kt.fetch(static_cast<const ET *>(a.k) + at, stride, rows, a.K, a.vec);
-    if constexpr (OUT) qt.fetch(static_cast<const ET *>(a.q) + at, stride, rows, a.K, a.vec);
+    const int64_t at = (t0 * a.Hk + hk) * a.K;
+    const int stride = a.Hk * a.K;
+    kt.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
+    if constexpr (OUT) qt.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
     const int64_t c = (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h);
     const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * a.tm_floats);
     tmr[0] = src[2 * tid];
     tmr[1] = src[2 * tid + 1];
     tmr[2] = src[512 + tid];
     if (tid < kRowFloats / 4) rvr = reinterpret_cast<const f32x4 *>(a.rowv + c * kRowFloats)[tid];
+    const Rsrc rv = rows_rsrc(a.v, (t0 * a.H + h) * a.V, rows, vrow, a.V, ES);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = idx_of(i >> 2, 4 * G + (i & 3));
-      vr[i] = (v_ok && t < rows) ? static_cast<const ET *>(a.v)[((t0 + t) * a.H + h) * a.V + vcol]
-                                 : ET(0);
-    }
+    for (int i = 0; i < 16; ++i) vr[i] = load_one<ET>(rv, voff + idx_of(i >> 2, i & 3) * vrow * ES);
   };
   auto stage = [&]() __attribute__((always_inline)) {
     kt.store(&sm.k[0][0], kChunk * KP);
@@ -330,20 +333,10 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
     f32x8 vv[2];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-      if constexpr (DT == SSLA_BF16) vv[i >> 3][i & 7] = bf16_bits_to_f32(vr[i]);
-      else if constexpr (DT == SSLA_F16) vv[i >> 3][i & 7] = f16_bits_to_f32(vr[i]);
-      else vv[i >> 3][i & 7] = vr[i];
+      vv[i >> 3][i & 7] = of_elem<DT>(vr[i]);
     }
-    if constexpr (MODE == kStates) {
-      float *dst = a.chunk_state + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = idx_of(t, 4 * G + r);
-          if (v_ok && key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = S[t][r];
-        }
-    }
+    if constexpr (MODE == kStates)
+      cols.store(a.chunk_state + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV, S);
     __syncthreads();
     if (t0 + kChunk < t_end) fetch(t0 + kChunk);   // the next chunk's, in flight meanwhile
 
@@ -373,7 +366,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
         const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks);
 #pragma unroll
         for (int j = 0; j < 8; ++j)   // (a selection: rows behind i may hold NaN)
-          pv[j] = 32 * ks + 8 * G + j <= i ? a.scale * pv[j] * fast_exp2((hi - ghi[j]) + (lo - glo[j])) : 0.f;
+          pv[j] = keep(32 * ks + 8 * G + j <= i, a.scale * pv[j] * fast_exp2((hi - ghi[j]) + (lo - glo[j])));
         bf16x8 s[NO];
         split(pv, s);
 #pragma unroll
@@ -472,20 +465,24 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
           O[t] = mul<LIMO>(m, us[ks], O[t]);
         }
       const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+      const Rsrc ro = rows_rsrc(a.o, (t0 * a.H + h) * a.V, rows, vrow, a.V, ES);
+      if (__ballot(r0 < kChunk)) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = idx_of(i >> 2, 4 * G + (i & 3));
-        if (v_ok && t < rows) E::store(a.o, ((t0 + t) * a.H + h) * a.V + vcol, t >= r0 ? __builtin_nanf("") : O[i >> 2][i & 3]);
+        for (int i = 0; i < 16; ++i)
+          if (32 * (i >> 3) + 8 * G + (i & 7) >= r0) O[i >> 2][i & 3] = __builtin_nanf("");
       }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        store_one<ET>(ro, voff + idx_of(i >> 2, i & 3) * vrow * ES, to_elem<DT>(O[i >> 2][i & 3]));
     }
-
     if constexpr (MODE == kStates) {
       const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+      const Rsrc ru = rows_rsrc(a.u, (t0 * a.H + h) * a.V, rows, vrow, a.V, 4);
+      const uint32_t uoff = v_ok ? (8 * G * vrow + vcol) * 4 : kOutside;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int t = idx_of(i >> 2, 4 * G + (i & 3));
-        if (v_ok && t < rows) a.u[((t0 + t) * a.H + h) * a.V + vcol] = t >= r0 ? __builtin_nanf("") : U[i >> 3][i & 7];
-      }
+      for (int i = 0; i < 16; ++i)
+        store_one<float>(ru, uoff + idx_of(i >> 2, i & 3) * vrow * 4,
+                         32 * (i >> 3) + 8 * G + (i & 7) >= r0 ? __builtin_nanf("") : U[i >> 3][i & 7]);
     }
 
     // S <- e^(G_last) S + k^T (e^(G_last - G) u)
@@ -509,16 +506,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   }
 
   if (!SEG) {
-    if (a.ht && t_end == eos && v_ok) {
-      float *dst = a.ht + (static_cast<int64_t>(n) * a.H + h) * KV;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = idx_of(t, 4 * G + r);
-          if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = S[t][r];
-        }
-    }
+    if (a.ht && t_end == eos) cols.store(a.ht + (static_cast<int64_t>(n) * a.H + h) * KV, S);
   } else if (is_map) {
     if (active) {
       uint16_t *dst = a.seg_map + (slot * a.H + h) * (3 * KP * KP);
@@ -536,15 +524,8 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
           }
         }
     }
-  } else if (v_ok) {
-    float *dst = a.seg_state + (slot * a.H + h) * KV;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = idx_of(t, 4 * G + r);
-        if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = S[t][r];
-      }
+  } else {
+    cols.store(a.seg_state + (slot * a.H + h) * KV, S);
   }
 }
 
@@ -566,28 +547,20 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
   const int64_t unit = static_cast<int64_t>(per) * kChunk, KV = static_cast<int64_t>(K) * V;
   const int64_t inner = (eos - bos + unit - 1) / unit - 1;   // segments but the last
   const bool ok = vcol < V;
+  const StateCols<NT> cols(K, V, vcol, ok, G);
   f32x4 S[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int key = idx_of(t, 4 * G + r);
-      S[t][r] = (start && ok && key < K) ? start[(n * H + h) * KV + static_cast<int64_t>(key) * V + vcol] : 0.f;
-    }
+  cols.load(start ? start + (n * H + h) * KV : nullptr, S);
   for (int64_t j = 0; j < inner; ++j) {
     const int64_t slot = (bos / unit + (REV ? inner - 1 - j : j)) * H + h;
     const uint16_t *m = seg_map + slot * (3 * KP * KP);
-    float *dst = seg_state + slot * KV;
+    f32x4 L[NT];
+    cols.load(seg_state + slot * KV, L);
     bf16x8 s[NT / 2][3];
 #pragma unroll
     for (int ks = 0; ks < NT / 2; ++ks) split(join(S[2 * ks], S[2 * ks + 1]), s[ks]);
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = idx_of(t, 4 * G + r);
-        S[t][r] = (ok && key < K) ? dst[static_cast<int64_t>(key) * V + vcol] : 0.f;
-      }
+      S[t] = L[t];
 #pragma unroll
       for (int ks = 0; ks < NT / 2; ++ks) {
         bf16x8 x[3];
@@ -596,12 +569,8 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
           x[p] = from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(m + ((t * (KP / 32) + ks) * 3 + p) * 512 + lane * 8));
         S[t] = mul<2>(x, s[ks], S[t]);
       }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = idx_of(t, 4 * G + r);
-        if (ok && key < K) dst[static_cast<int64_t>(key) * V + vcol] = S[t][r];
-      }
     }
+    cols.store(seg_state + slot * KV, S);
   }
 }
 

@@ -82,43 +82,40 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   const bool active = is_map ? mcol < KP : tile < n_vt, v_ok = !is_map && vcol < a.V;
   const int64_t KV = static_cast<int64_t>(a.K) * a.V;
 
+  const StateCols<NT> cols(a.K, a.V, vcol, v_ok, G);
   f32x4 D[NT];
-  {
-    const float *src = nullptr;
-    if (!SEG) {
-      if (t_end == eos) src = ga.dht ? ga.dht + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr;
-      else src = a.seg_state + ((bos / unit + seg) * a.H + h) * KV;
-    }
+  if (!SEG) {
+    cols.load(t_end < eos ? a.seg_state + ((bos / unit + seg) * a.H + h) * KV
+              : ga.dht    ? ga.dht + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr, D);
+  } else {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = idx_of(t, 4 * G + r);
-        float x = is_map && key == mcol ? 1.f : 0.f;
-        if (!SEG && src && v_ok && key < a.K) x = src[static_cast<int64_t>(key) * a.V + vcol];
-        D[t][r] = x;
-      }
+      for (int r = 0; r < 4; ++r) D[t][r] = is_map && idx_of(t, 4 * G + r) == mcol ? 1.f : 0.f;
   }
+  // byte offset of row 8 G in this lane's column of do and dv, and of dX (4 bytes)
+  constexpr int ES = sizeof(ET);
+  const uint32_t vrow = static_cast<uint32_t>(a.H) * a.V;
+  const uint32_t voff = v_ok ? (8 * G * vrow + vcol) * ES : kOutside, xoff = v_ok ? (8 * G * vrow + vcol) * 4 : kOutside;
 
   RowTile<DT, KP> kt, qt;
   f32x4 tmr[3], rvr;
   ET dr[16];
   auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
-    const int64_t at = (t0 * a.Hk + hk) * a.K, stride = static_cast<int64_t>(a.Hk) * a.K;
-    kt.fetch(static_cast<const ET *>(a.k) + at, stride, rows, a.K, a.vec);
-    qt.fetch(static_cast<const ET *>(a.q) + at, stride, rows, a.K, a.vec);
+    const int64_t at = (t0 * a.Hk + hk) * a.K;
+    const int stride = a.Hk * a.K;
+    kt.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
+    qt.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
     const int64_t c = (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h);
     const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * a.tm_floats + kTriFloats);
     tmr[0] = src[2 * tid];
     tmr[1] = src[2 * tid + 1];
     tmr[2] = src[512 + tid];
     if (tid < kRowFloats / 4) rvr = reinterpret_cast<const f32x4 *>(a.rowv + c * kRowFloats)[tid];
+    const Rsrc rd = rows_rsrc(ga.dout, (t0 * a.H + h) * a.V, rows, vrow, a.V, ES);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int t = idx_of(i >> 2, 4 * G + (i & 3));
-      dr[i] = (v_ok && t < rows) ? static_cast<const ET *>(ga.dout)[((t0 + t) * a.H + h) * a.V + vcol] : ET(0);
-    }
+    for (int i = 0; i < 16; ++i) dr[i] = load_one<ET>(rd, voff + idx_of(i >> 2, i & 3) * vrow * ES);
   };
   auto stage = [&]() __attribute__((always_inline)) {
     kt.store(&sm.k[0][0], kChunk * KP);
@@ -151,21 +148,9 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
     stage();
     f32x8 dov[2];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      if constexpr (DT == SSLA_BF16) dov[i >> 3][i & 7] = bf16_bits_to_f32(dr[i]);
-      else if constexpr (DT == SSLA_F16) dov[i >> 3][i & 7] = f16_bits_to_f32(dr[i]);
-      else dov[i >> 3][i & 7] = dr[i];
-    }
-    if constexpr (!SEG) {
-      float *dst = ga.chunk_grad + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = idx_of(t, 4 * G + r);
-          if (v_ok && key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = D[t][r];
-        }
-    }
+    for (int i = 0; i < 16; ++i) dov[i >> 3][i & 7] = of_elem<DT>(dr[i]);
+    if constexpr (!SEG)
+      cols.store(ga.chunk_grad + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV, D);
     __syncthreads();
     if (c > 0) fetch(t0 - kChunk);   // the next chunk's, in flight meanwhile
 
@@ -193,7 +178,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
         const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          pv[i] = 32 * ks + 8 * G + i >= j ? a.scale * pv[i] * fast_exp2((ghi[i] - hi) + (glo[i] - lo)) : 0.f;
+          pv[i] = keep(32 * ks + 8 * G + i >= j, a.scale * pv[i] * fast_exp2((ghi[i] - hi) + (glo[i] - lo)));
         bf16x8 s[3];
         split(pv, s);
 #pragma unroll
@@ -261,17 +246,15 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
     }
     if constexpr (!SEG) {
       const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+      const int64_t at = (t0 * a.H + h) * a.V;
+      const Rsrc rv = rows_rsrc(ga.dv, at, rows, vrow, a.V, ES), rx = rows_rsrc(ga.dx, at, rows, vrow, a.V, 4);
 #pragma unroll
       for (int p = 0; p < 2; ++p) {
-        const f32x8 bt = row8(kBeta, p);
+        const f32x8 dv = row8(kBeta, p) * dX[p];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int t = 32 * p + 8 * G + i;
-          if (v_ok && t < rows) {
-            const int64_t at = ((t0 + t) * a.H + h) * a.V + vcol;
-            ga.dx[at] = dX[p][i];
-            E::store(ga.dv, at, bt[i] * dX[p][i]);
-          }
+          store_one<float>(rx, xoff + (32 * p + i) * vrow * 4, dX[p][i]);
+          store_one<ET>(rv, voff + (32 * p + i) * vrow * ES, to_elem<DT>(dv[i]));
         }
       }
     }
@@ -301,16 +284,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   }
 
   if (!SEG) {
-    if (ga.dh0 && seg == 0 && v_ok) {
-      float *dst = ga.dh0 + (static_cast<int64_t>(n) * a.H + h) * KV;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int key = idx_of(t, 4 * G + r);
-          if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = D[t][r];
-        }
-    }
+    if (ga.dh0 && seg == 0) cols.store(ga.dh0 + (static_cast<int64_t>(n) * a.H + h) * KV, D);
   } else if (is_map) {
     if (active) {
       uint16_t *dst = a.seg_map + (slot * a.H + h) * (3 * KP * KP);
@@ -328,15 +302,8 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
           }
         }
     }
-  } else if (v_ok) {
-    float *dst = a.seg_state + (slot * a.H + h) * KV;
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int key = idx_of(t, 4 * G + r);
-        if (key < a.K) dst[static_cast<int64_t>(key) * a.V + vcol] = D[t][r];
-      }
+  } else {
+    cols.store(a.seg_state + (slot * a.H + h) * KV, D);
   }
 }
 
@@ -377,7 +344,9 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
   const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
   const int64_t KV = static_cast<int64_t>(a.K) * a.V;
   const float *Sp = a.chunk_state + (slot * a.H + h) * KV, *Dp = ga.chunk_grad + (slot * a.H + h) * KV;
-  const int64_t vat = (t0 * a.H + h) * a.V, vstride = static_cast<int64_t>(a.H) * a.V;
+  const int64_t vat = (t0 * a.H + h) * a.V;
+  const int vrow = a.H * a.V;
+  constexpr int ES = sizeof(ET);
 
   f32x4 Z[KT], Y[KT], W[KT], C1[4], C2[4], C3[4], C4[4];
   const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -392,10 +361,13 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
       const int nc = a.V - c0;
       RowTile<DT, 32> dt, vt;
       RowTile<SSLA_F32, 32> ut, xt, st, gt;
-      dt.fetch(static_cast<const ET *>(ga.dout) + vat + c0, vstride, rows, nc, ga.dvec);
-      vt.fetch(static_cast<const ET *>(a.v) + vat + c0, vstride, rows, nc, ga.dvec);
-      ut.fetch(a.u + vat + c0, vstride, rows, nc, ga.vvec);
-      xt.fetch(ga.dx + vat + c0, vstride, rows, nc, ga.vvec);
+      auto slab = [&](const void *p, int es) __attribute__((always_inline)) {   // the rows from column c0 on
+        return rows_rsrc(p, vat + c0, rows, vrow, nc, es);
+      };
+      dt.fetch(slab(ga.dout, ES), vrow, nc, ga.dvec);
+      vt.fetch(slab(a.v, ES), vrow, nc, ga.dvec);
+      ut.fetch(slab(a.u, 4), vrow, nc, ga.vvec);
+      xt.fetch(slab(ga.dx, 4), vrow, nc, ga.vvec);
       dt.store(&sm.v.dout[0][0], kChunk * 32);
       ut.store(&sm.v.u[0][0], kChunk * 32);
       xt.store(&sm.v.dx[0][0], kChunk * 32);
@@ -404,8 +376,9 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
 #pragma unroll
       for (int k0 = 0; k0 < KP; k0 += 64) {
         constexpr int KR = GradSmem<DT, KP>::KR;
-        st.fetch(Sp + static_cast<int64_t>(k0) * a.V + c0, a.V, a.K - k0, nc, ga.vvec);
-        gt.fetch(Dp + static_cast<int64_t>(k0) * a.V + c0, a.V, a.K - k0, nc, ga.vvec);
+        const int64_t at = static_cast<int64_t>(k0) * a.V + c0;
+        st.fetch(rows_rsrc(Sp, at, a.K - k0, a.V, nc, 4), a.V, nc, ga.vvec);
+        gt.fetch(rows_rsrc(Dp, at, a.K - k0, a.V, nc, 4), a.V, nc, ga.vvec);
         st.store(&sm.v.S[0][k0 * 32], KR * 32);
         gt.store(&sm.v.D[0][k0 * 32], KR * 32);
 #pragma unroll
@@ -456,10 +429,11 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
 
   {
     RowTile<DT, KP> x;
-    const int64_t at = (t0 * a.Hk + hk) * a.K, stride = static_cast<int64_t>(a.Hk) * a.K;
-    x.fetch(static_cast<const ET *>(a.q) + at, stride, rows, a.K, a.vec);
+    const int64_t at = (t0 * a.Hk + hk) * a.K;
+    const int stride = a.Hk * a.K;
+    x.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
     x.store(&sm.k.q[0][0], kChunk * KP);
-    x.fetch(static_cast<const ET *>(a.k) + at, stride, rows, a.K, a.vec);
+    x.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
     x.store(&sm.k.k[0][0], kChunk * KP);
     const float *src = a.rowv + (slot * a.H + h) * kRowFloats;
     for (int e = tid; e < kRowFloats; e += 256) (&sm.rowv[0][0])[e] = src[e];
@@ -492,10 +466,10 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
       for (int j = 0; j < 8; ++j) {
         const int r = 32 * ks + 8 * G + j;
         const float e = fast_exp2(r <= me ? (hi - ghi[j]) + (lo - glo[j]) : (ghi[j] - hi) + (glo[j] - lo));
-        p1[j] = r <= me ? a.scale * p1[j] * e : 0.f;
-        n1[j] = r < me ? -n1[j] * e : 0.f;
-        p2[j] = r >= me ? a.scale * p2[j] * e : 0.f;
-        n2[j] = r > me ? -bt[j] * n2[j] * e : 0.f;
+        p1[j] = keep(r <= me, a.scale * p1[j] * e);
+        n1[j] = keep(r < me, -n1[j] * e);
+        p2[j] = keep(r >= me, a.scale * p2[j] * e);
+        n2[j] = keep(r > me, -bt[j] * n2[j] * e);
       }
       split(p1, pA[ks]);
       split(n1, nA[ks]);
@@ -503,6 +477,11 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
       split(n2, nT[ks]);
     }
   }
+  const bool part = ga.dq_part != nullptr;   // every value head's in fp32
+  const int krow = (part ? a.H : a.Hk) * a.K;
+  const int64_t kat = part ? (t0 * a.H + h) * a.K : (t0 * a.Hk + hk) * a.K;
+  const Rsrc rq = rows_rsrc(part ? static_cast<const void *>(ga.dq_part) : ga.dq, kat, rows, krow, a.K, part ? 4 : ES);
+  const Rsrc rk = rows_rsrc(part ? static_cast<const void *>(ga.dk_part) : ga.dk, kat, rows, krow, a.K, part ? 4 : ES);
   // per own row: q . (from the state), q . (dP k), k . (dP^T q), k . (dN k),
   // k . ((beta dN)^T k), k . (dX S^T), k . (u D^T)
   float qa[4], qb[4], kc[4], kd[4], ke[4], ky[4], kw[4];
@@ -547,16 +526,13 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
       kw[r] = fmaf(kv, hw, kw[r]);
       const float dq = ia + b[r];
       const float dk = (c[r] + e[r]) + fmaf(bt, d[r], fmaf(-sm.rowv[kBetaG][i], Y[t][r], hw));
-      if (i < rows && key < a.K) {
-        if (ga.dq_part) {
-          const int64_t at = ((t0 + i) * a.H + h) * a.K + key;
-          ga.dq_part[at] = dq;
-          ga.dk_part[at] = dk;
-        } else {
-          const int64_t at = ((t0 + i) * a.Hk + hk) * a.K + key;
-          E::store(ga.dq, at, dq);
-          E::store(ga.dk, at, dk);
-        }
+      const uint32_t off = static_cast<uint32_t>(i * krow + key);
+      if (part) {
+        store_one<float>(rq, key < a.K ? off * 4 : kOutside, dq);
+        store_one<float>(rk, key < a.K ? off * 4 : kOutside, dk);
+      } else {
+        store_one<ET>(rq, key < a.K ? off * ES : kOutside, to_elem<DT>(dq));
+        store_one<ET>(rk, key < a.K ? off * ES : kOutside, to_elem<DT>(dk));
       }
     }
   }

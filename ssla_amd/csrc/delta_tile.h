@@ -32,15 +32,32 @@ __device__ __forceinline__ constexpr int tri_set(int t, int ks) { return t < 2 ?
 
 template <int DT> struct Parts { static constexpr int n = DT == SSLA_BF16 ? 1 : DT == SSLA_F16 ? 2 : 3; };
 
-// x as a sum of N bf16 vectors.
+// x as a sum of N bf16 vectors.  (Two values a conversion, taken apart again by
+// a shift and a mask: the vector conversion back would convert each value anew.)
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 template <int N>
 __device__ __forceinline__ void split(const f32x8 &x, bf16x8 (&p)[N]) {
-  f32x8 r = x;
+  uint32_t w[N][4];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    p[i] = __builtin_convertvector(r, bf16x8);
-    if (i + 1 < N) r = r - __builtin_convertvector(p[i], f32x8);
+  for (int j = 0; j < 4; ++j) {
+    float a = x[2 * j], b = x[2 * j + 1];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      w[i][j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
+      if (i + 1 < N) {
+        a -= __uint_as_float(w[i][j] << 16);
+        b -= __uint_as_float(w[i][j] & 0xffff0000u);
+      }
+    }
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = from_bits<bf16x8>(make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]));
+}
+// x where on, else 0, also where x is not finite; without a branch around what computes x
+__device__ __forceinline__ float keep(bool on, float x) {
+  asm("" : "+v"(x));
+  return on ? x : 0.f;
 }
 __device__ __forceinline__ f32x8 join(const f32x4 &a, const f32x4 &b) {
   return f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -87,39 +104,74 @@ __device__ __forceinline__ bf16x8 op_cols(const uint16_t *t, int tile, int ks, i
   return from_bits<bf16x8>(make_uint4(u[0].x, u[0].y, u[1].x, u[1].y));
 }
 
-// 64 rows of a matrix with row stride `stride`, fetched into registers by 256
-// threads and stored to LDS as Parts<DT>::n tiles of bf16; rows from n_rows on
-// and columns from n_cols on are zero.  Where rows are whole 16-byte pieces at
-// aligned addresses (vec) they are read 16 bytes at a time.
+// Global memory goes through buffer resources that cover a chunk's rows (or one
+// state): the hardware reads zeros past their end and drops stores there, so
+// rows behind a sequence and columns behind a matrix need no branches.  Offsets
+// are 32 bits inside a resource; what is outside gets kOutside.
+constexpr uint32_t kOutside = 0x80000000u;
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+__device__ __forceinline__ Rsrc rsrc_of(const void *base, int64_t bytes) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(base), static_cast<short>(0), static_cast<int>(bytes),
+                                           0x00020000);   // raw 32-bit data, range checked
+}
+// rows of `width` values at a stride (in values of es bytes)
+__device__ __forceinline__ Rsrc rows_rsrc(const void *base, int64_t at, int rows, int64_t stride, int width, int es) {
+  return rsrc_of(static_cast<const char *>(base) + at * es, rows > 0 ? ((rows - 1) * stride + width) * es : 0);
+}
+template <typename E>
+__device__ __forceinline__ E load_one(const Rsrc &rs, uint32_t off) {
+  if constexpr (sizeof(E) == 2) return static_cast<E>(__builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0));
+  else return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
+}
+template <typename E>
+__device__ __forceinline__ void store_one(const Rsrc &rs, uint32_t off, E x) {
+  if constexpr (sizeof(E) == 2) __builtin_amdgcn_raw_buffer_store_b16(x, rs, off, 0, 0);
+  else __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), rs, off, 0, 0);
+}
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::T to_elem(float x) {
+  if constexpr (DT == SSLA_BF16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+  else if constexpr (DT == SSLA_F16) return f32_to_f16_bits(x);
+  else return x;
+}
+template <int DT>
+__device__ __forceinline__ float of_elem(typename Elem<DT>::T x) {
+  if constexpr (DT == SSLA_BF16) return bf16_bits_to_f32(x);
+  else if constexpr (DT == SSLA_F16) return f16_bits_to_f32(x);
+  else return x;
+}
+
+// 64 rows of a matrix with row stride `stride` (values), fetched into registers
+// by 256 threads and stored to LDS as Parts<DT>::n tiles of bf16; rows past the
+// resource and columns from n_cols on are zero.  Where rows are whole 16-byte
+// pieces at aligned addresses (vec) they are read 16 bytes at a time.
 template <int DT, int KP>
 struct RowTile {
   static constexpr int U = KP / 32;   // 8-column pieces of a thread
   typedef typename Elem<DT>::T E;
+  static constexpr int ES = sizeof(E), W = ES / 2;   // 16-byte loads of a piece
   struct Piece { E e[8]; };
   Piece p[U];
 
-  __device__ __forceinline__ void fetch(const E *x, int64_t stride, int n_rows, int n_cols, bool vec) {
+  __device__ __forceinline__ void fetch(const Rsrc &rs, int stride, int n_cols, bool vec) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int u = threadIdx.x + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
-      const E *src = x + row * stride + col;
-      if (row < n_rows && vec && col + 8 <= n_cols) {
-        constexpr int W = sizeof(Piece) / 16;
+      const uint32_t at = static_cast<uint32_t>(row * stride + col) * ES;
+      if (vec) {
         struct Raw { uint4 w[W]; } raw;
 #pragma unroll
-        for (int j = 0; j < W; ++j) raw.w[j] = reinterpret_cast<const uint4 *>(src)[j];
+        for (int j = 0; j < W; ++j)
+          raw.w[j] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(
+              rs, col + 8 / W * (j + 1) <= n_cols ? at + 16 * j : kOutside, 0, 0));
         p[i] = __builtin_bit_cast(Piece, raw);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[i].e[j] = (row < n_rows && col + j < n_cols) ? src[j] : E(0);
+        for (int j = 0; j < 8; ++j) p[i].e[j] = load_one<E>(rs, col + j < n_cols ? at + ES * j : kOutside);
       }
     }
   }
-  __device__ __forceinline__ float value(int i, int j) const {   // column j of piece i
-    if constexpr (DT == SSLA_BF16) return bf16_bits_to_f32(p[i].e[j]);
-    else if constexpr (DT == SSLA_F16) return f16_bits_to_f32(p[i].e[j]);
-    else return p[i].e[j];
-  }
+  __device__ __forceinline__ float value(int i, int j) const { return of_elem<DT>(p[i].e[j]); }   // column j of piece i
   // plane j at t + j * stride elements
   __device__ __forceinline__ void store(uint16_t *t, int stride) const {
 #pragma unroll
@@ -198,6 +250,40 @@ inline DeltaLayout delta_layout(int n_seq, int64_t T, int Hk, int H, int K, int 
   L.total = p;
   return L;
 }
+
+// 16 x 16 x 4 N product in fp32 (operand value j of lane group G: contraction
+// index N G + j), for the few products whose operands are not kept in parts.
+template <int N>
+__device__ __forceinline__ f32x4 mul_f32(const float (&a)[N], const float (&b)[N], f32x4 c) {
+#pragma unroll
+  for (int j = 0; j < N; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+  return c;
+}
+
+// 16 columns of a [K, V] fp32 state as accumulator tiles: lane = (key group,
+// column); keys from K on and columns from V on are zero and not stored.
+template <int NT>
+struct StateCols {
+  uint32_t off;   // of key 8 G in this lane's column
+  int K, V4;
+  __device__ __forceinline__ StateCols(int K_, int V, int vcol, bool on, int G)
+      : off(on ? static_cast<uint32_t>(8 * G * V + vcol) * 4u : kOutside), K(K_), V4(V * 4) {}
+  __device__ __forceinline__ Rsrc rs(const float *base) const { return rsrc_of(base, base ? static_cast<int64_t>(K) * V4 : 0); }
+  __device__ __forceinline__ void load(const float *base, f32x4 (&S)[NT]) const {
+    const Rsrc r = rs(base);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[t][i] = load_one<float>(r, off + idx_of(t, i) * V4);
+  }
+  __device__ __forceinline__ void store(float *base, const f32x4 (&S)[NT]) const {
+    const Rsrc r = rs(base);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store_one<float>(r, off + idx_of(t, i) * V4, S[t][i]);
+  }
+};
 
 struct WalkArgs {
   const void *q, *k, *v;
