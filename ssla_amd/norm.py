@@ -29,6 +29,13 @@ def _ws(nbytes: int, dev):
     return torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
 
 
+def _whole(t):
+    """t contiguous and, for the kernels' wide loads, not off a 16-byte boundary:
+    a view's sums are then taken in the order of a fresh tensor's."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 def _forward(x, num_groups, w, b, eps, act, stats):
     N, C = x.shape[0], x.shape[-1]
     L = x.numel() // max(N * C, 1)
@@ -63,7 +70,7 @@ class GroupNormFunction(torch.autograd.Function):
         x, weight, bias, stats = ctx.saved_tensors
         N, C, G = x.shape[0], x.shape[-1], ctx.num_groups
         L = x.numel() // max(N * C, 1)
-        dy = dy.contiguous()
+        dy = _whole(dy)
         need = ctx.needs_input_grad
         dx = torch.empty_like(x) if need[0] else None
         dw = torch.empty_like(weight) if need[1] else None
@@ -104,7 +111,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
         if t is not None and (t.shape != (C,) or not t.is_floating_point()):
             raise ValueError(f"group_norm_act: {nm} must be [{C}] floating point, got {tuple(t.shape)} {t.dtype}")
     _lib.require_cuda(x, weight, bias)
-    x = x.contiguous()
+    x = _whole(x)
     w, b = (None if t is None else t.to(torch.float32).contiguous() for t in (weight, bias))
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b)):
