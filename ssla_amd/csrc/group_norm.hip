@@ -80,6 +80,25 @@ __device__ __forceinline__ Point point_of(float x, float dy, float mean, float r
   return p;
 }
 
+// W values of a weight vector, or of its default.
+template <int W>
+__device__ __forceinline__ void load_row(const float *p, int c, bool on, float other, float (&x)[W]) {
+#pragma unroll
+  for (int e = 0; e < W; ++e) x[e] = other;
+  if (!p || !on) return;
+  if constexpr (W >= 4) {   // (rows of channels begin at a multiple of 16 bytes of an aligned vector: see widest)
+#pragma unroll
+    for (int e = 0; e < W; e += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(p + c + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[e + i] = v[i];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e) x[e] = p[c + e];
+  }
+}
+
 // --------------------------------------------------- groups of one wavefront --
 // Lane j of the SG lanes of a group has its vectors j, j + SG, ...; the lane
 // groups of a launch step over the samples, each with one group of channels.
@@ -88,7 +107,7 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(const NormArgs a, int S
   const int per = a.C / a.G, pv = per / W, nv = static_cast<int>(a.L) * pv;
   const int64_t sub = (static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x) / SG;
   const int j = threadIdx.x & (SG - 1), g = static_cast<int>(sub % a.G);
-  const bool on = sub < slots * a.G;   // (lanes behind take part in the shuffles only)
+  const bool on = sub < slots * a.G;
   const float inv = 1.f / static_cast<float>(a.L * per);
   int off[NV];
   bool ok[NV];
@@ -98,23 +117,42 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(const NormArgs a, int S
     const int v = j + SG * i, row = v / pv, c = g * per + (v - row * pv) * W;
     ok[i] = on && v < nv;
     off[i] = row * a.C + c;
+    load_row<W>(a.w, c, ok[i], 1.f, w[i]);
+    load_row<W>(a.b, c, ok[i], 0.f, b[i]);
+    if constexpr (BWD)
 #pragma unroll
-    for (int e = 0; e < W; ++e) {
-      w[i][e] = ok[i] && a.w ? a.w[c + e] : 1.f;
-      b[i][e] = ok[i] && a.b ? a.b[c + e] : 0.f;
-      if constexpr (BWD) sw[i][e] = sb[i][e] = 0.f;
-    }
+      for (int e = 0; e < W; ++e) sw[i][e] = sb[i][e] = 0.f;
   }
   auto sum = [&](float x) __attribute__((always_inline)) {
     for (int d = 1; d < SG; d <<= 1) x += __shfl_xor(x, d);
     return x;
   };
-  for (int64_t n = on ? sub / a.G : 0; n < a.N; n += slots) {
-    const int64_t base = n * a.L * a.C, st = 2 * (n * a.G + g);
-    Vec<DT, W> x[NV];
+  Vec<DT, W> x[NV], nx[NV], dy[BWD ? NV : 1], ndy[BWD ? NV : 1];
+  float nmean = 0.f, nrstd = 0.f;
+  auto fetch = [&](int64_t n) __attribute__((always_inline)) {
+    const int64_t base = n * a.L * a.C;
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (ok[i]) x[i] = load_vec<DT, W>(a.x, base + off[i]);
+      if (ok[i]) {
+        nx[i] = load_vec<DT, W>(a.x, base + off[i]);
+        if constexpr (BWD) ndy[i] = load_vec<DT, W>(a.dy, base + off[i]);
+      }
+    if constexpr (BWD) {
+      nmean = a.stats[2 * (n * a.G + g)];
+      nrstd = a.stats[2 * (n * a.G + g) + 1];
+    }
+  };
+  if (!on) return;   // (whole lane groups)
+  fetch(sub / a.G);
+  for (int64_t n = sub / a.G; n < a.N; n += slots) {
+    const int64_t base = n * a.L * a.C, st = 2 * (n * a.G + g);
+    const float mean_in = nmean, rstd_in = nrstd;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = nx[i];
+      if constexpr (BWD) dy[i] = ndy[i];
+    }
+    if (n + slots < a.N) fetch(n + slots);   // the next sample's, in flight meanwhile
     if constexpr (!BWD) {
       float s = 0.f;
 #pragma unroll
@@ -141,16 +179,12 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(const NormArgs a, int S
           for (int e = 0; e < W; ++e) y.set(e, act_of(a.act, fmaf((x[i][e] - mean) * rstd, w[i][e], b[i][e])));
           store_vec<DT, W>(a.y, base + off[i], y);
         }
-      if (a.stats && on && j == 0) {
+      if (a.stats && j == 0) {
         a.stats[st] = mean;
         a.stats[st + 1] = rstd;
       }
     } else {
-      Vec<DT, W> dy[NV];
-#pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (ok[i]) dy[i] = load_vec<DT, W>(a.dy, base + off[i]);
-      const float mean = on ? a.stats[st] : 0.f, rstd = on ? a.stats[st + 1] : 0.f;
+      const float mean = mean_in, rstd = rstd_in;
       float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -179,10 +213,9 @@ __global__ __launch_bounds__(256) void norm_lanes_kernel(const NormArgs a, int S
           }
       }
     }
-    if (!on) break;
   }
   if constexpr (BWD) {
-    if (a.cols && on) {
+    if (a.cols) {
       // row (slot, position): a position's channels of every slot
 #pragma unroll
       for (int i = 0; i < NV; ++i)
@@ -277,11 +310,8 @@ __global__ __launch_bounds__(256) void norm_slice_kernel(const NormArgs a) {
   const int64_t r0 = rb * s.RT * NR, rows = min(static_cast<int64_t>(s.RT) * NR, a.L - r0);
   const int64_t base = (n * a.L + r0) * a.C + c;
   float w[W], b[W];
-#pragma unroll
-  for (int e = 0; e < W; ++e) {
-    w[e] = on && a.w ? a.w[c + e] : 1.f;
-    b[e] = on && a.b ? a.b[c + e] : 0.f;
-  }
+  load_row<W>(a.w, c, on, 1.f, w);
+  load_row<W>(a.b, c, on, 0.f, b);
   Vec<DT, W> x[NR], dy[BWD ? NR : 1];
 #pragma unroll
   for (int i = 0; i < NR; ++i)
@@ -489,7 +519,7 @@ constexpr int kColSplits = 64;
 // The backward's lane groups keep their columns' sums over the samples they step
 // over: 512 workgroups (two a CU) leave 2,048 rows of sums of 8 heads of 64
 // channels to add.
-constexpr int64_t kBwdBlocks = 512;
+constexpr int64_t kBwdBlocks = 512, kFwdBlocks = 4096;
 
 NormPlan plan_of(int64_t N, int64_t L, int C, int G, int W, bool bwd) {
   NormPlan p{};
@@ -502,7 +532,7 @@ NormPlan plan_of(int64_t N, int64_t L, int C, int G, int W, bool bwd) {
     while (p.SG < 64 && p.SG < nv) p.SG *= 2;
     p.NV = 1;
     while (static_cast<int64_t>(p.SG) * p.NV < nv) p.NV *= 2;
-    p.slots = bwd ? std::min<int64_t>(N, std::max<int64_t>(1, kBwdBlocks * 256 / p.SG / G)) : N;
+    p.slots = std::min<int64_t>(N, std::max<int64_t>(1, (bwd ? kBwdBlocks : kFwdBlocks) * 256 / p.SG / G));
     p.col_rows = p.slots * L;
   } else {
     p.s = slice_of(L, C, W);
@@ -535,8 +565,10 @@ int check_sizes(const char *what, int64_t N, int64_t L, int C, int G, int act) {
   return SSLA_OK;
 }
 
-int widest(int per, int dtype, std::initializer_list<const void *> tensors) {
+int widest(int per, int dtype, std::initializer_list<const void *> tensors, std::initializer_list<const float *> rows) {
   const int es = dtype == SSLA_F32 ? 4 : 2;
+  for (const float *t : rows)
+    if (!aligned(t, 16)) return 1;   // (NULL is aligned)
   for (int W = 16 / es; W >= 4; W /= 2) {
     bool ok = per % W == 0;
     for (const void *t : tensors) ok = ok && aligned(t, W * es);
@@ -628,7 +660,7 @@ extern "C" int ssla_group_norm_fwd(const void *x, int64_t N, int64_t L, int C, i
   SSLA_CHECK_ARG(x && y, "group_norm_fwd: null pointer");
   if (const int e = check_dtype("group_norm_fwd", dtype)) return e;
   if (const int e = check_ws("group_norm_fwd", workspace, workspace_bytes, ws_bytes(N, L, C, G, false))) return e;
-  const NormPlan p = plan_of(N, L, C, G, widest(C / G, dtype, {x, y}), false);
+  const NormPlan p = plan_of(N, L, C, G, widest(C / G, dtype, {x, y}, {weight, bias}), false);
   float *part = static_cast<float *>(workspace);
   NormArgs a{};
   a.x = x; a.w = weight; a.b = bias; a.y = y; a.stats = stats; a.part = part;
@@ -660,7 +692,7 @@ extern "C" int ssla_group_norm_bwd(const void *dy, const void *x, const float *s
   if (!none) {
     if (!dx && !sums) return SSLA_OK;
     p = plan_of(N, L, C, G, widest(C / G, dtype, dx ? std::initializer_list<const void *>{x, dy, dx}
-                                                    : std::initializer_list<const void *>{x, dy}), true);
+                                                    : std::initializer_list<const void *>{x, dy}, {weight, bias}), true);
     cols = part + (p.part_floats + 3) / 4 * 4;
     split = cols + p.col_rows * 2 * C;
     NormArgs a{};

@@ -112,7 +112,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
             raise ValueError(f"group_norm_act: {nm} must be [{C}] floating point, got {tuple(t.shape)} {t.dtype}")
     _lib.require_cuda(x, weight, bias)
     x = _whole(x)
-    w, b = (None if t is None else t.to(torch.float32).contiguous() for t in (weight, bias))
+    w, b = (None if t is None else _whole(t.to(torch.float32)) for t in (weight, bias))
     act = ACTIVATIONS[activation]
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, b)):
         return GroupNormFunction.apply(x, w, b, num_groups, float(eps), act)
