@@ -66,7 +66,7 @@ struct NormArgs {
   float *part;         // moments or sums of the slices
   float *cols;         // backward: rows of dw and db sums, [rows][2][C]; NULL: not wanted
   int64_t N, L;
-  int C, G, act;
+  int C, G, act, join;
   float eps;
 };
 
@@ -293,9 +293,53 @@ __device__ __forceinline__ void group_sums(SliceSmem &sm, const Slice &s, int c0
   __syncthreads();
 }
 
+// Joins the slices of group i of all groups on one wavefront (every lane returns
+// the result): mean and centred squares, or the two sums.  A slice whose channels
+// lie elsewhere holds nothing of the group and wrote nothing.
+template <bool BWD>
+__device__ __forceinline__ void join_slices(const float *__restrict__ part, const Slice &s, int64_t i, int g, int pv,
+                                            float &u, float &v) {
+  const int lane = threadIdx.x & 63;
+  const int b0 = g * pv / s.CT, b1 = ((g + 1) * pv - 1) / s.CT, nb = b1 - b0 + 1;   // its channel blocks
+  float cnt = 0.f;
+  u = v = 0.f;
+  auto join = [&](float c2, float u2, float v2) __attribute__((always_inline)) {
+    if constexpr (BWD) {
+      u += u2;
+      v += v2;
+    } else if (c2 > 0.f) {
+      const float c = cnt + c2, d = u2 - u, f = c2 / c;
+      u = fmaf(d, f, u);
+      v += v2 + d * d * cnt * f;
+      cnt = c;
+    }
+  };
+  for (int64_t k = lane; k < static_cast<int64_t>(s.rblocks) * nb; k += 64) {
+    const float *p = part + ((i * s.rblocks + k / nb) * s.cblocks + b0 + k % nb) * (BWD ? 2 : 3);
+    if constexpr (BWD) join(0.f, p[0], p[1]);
+    else join(p[0], p[1], p[2]);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const float c2 = __shfl_xor(cnt, d), u2 = __shfl_xor(u, d), v2 = __shfl_xor(v, d);
+    if constexpr (!BWD) {   // both lanes join in the same order
+      const bool up = lane & d;
+      const float cx = up ? cnt : c2, ux = up ? u : u2, vx = up ? v : v2;
+      cnt = up ? c2 : cnt;
+      u = up ? u2 : u;
+      v = up ? v2 : v;
+      if (cnt == 0.f) { cnt = cx; u = ux; v = vx; }
+      else join(cx, ux, vx);
+    } else {
+      u += u2;
+      v += v2;
+    }
+  }
+}
+
 // STAGE 0: a sample is one slice, all in one pass; 1: the slices' moments (or
 // sums) and, in the backward, the columns' sums; 2: y (or dx) from the joined
-// ones.
+// ones, which a workgroup of a few slices joins itself (a.join: one launch less).
 template <int DT, int W, bool BWD, int STAGE>
 __global__ __launch_bounds__(256) void norm_slice_kernel(const NormArgs a) {
   constexpr int NR = kHold / W;
@@ -328,11 +372,27 @@ __global__ __launch_bounds__(256) void norm_slice_kernel(const NormArgs a) {
         for (int e = 0; e < W; ++e) f(i, e);
   };
   const int64_t st = 2 * (n * a.G + g);
+  if (STAGE == 2 && a.join) {
+    const int g0 = c0 / pv, ng = (c0 + cw - 1) / pv - g0 + 1;
+    for (int i = threadIdx.x >> 6; i < ng; i += 4) {
+      float u, v;
+      join_slices<BWD>(a.part, s, n * a.G + g0 + i, g0 + i, pv, u, v);
+      if ((threadIdx.x & 63) == 0) {
+        sm.sa[i] = u;
+        sm.sb[i] = BWD ? v : 1.f / sqrtf(v / (static_cast<float>(a.L) * per) + a.eps);
+      }
+    }
+    __syncthreads();
+  }
   if constexpr (!BWD) {
     float mean = 0.f, rstd = 0.f;
     if constexpr (STAGE == 2) {
-      mean = a.stats[st];
-      rstd = a.stats[st + 1];
+      mean = a.join ? sm.sa[k] : a.stats[st];
+      rstd = a.join ? sm.sb[k] : a.stats[st + 1];
+      if (a.join && a.stats && on && rb == 0 && rt == 0 && (c0 + cl) % pv == 0) {
+        a.stats[st] = mean;
+        a.stats[st + 1] = rstd;
+      }
     } else {
       const float cnt = static_cast<float>(rows) * W *
                         static_cast<float>(min((g + 1) * pv, c0 + cw) - max(g * pv, c0));   // values of the group in the slice
@@ -416,8 +476,8 @@ __global__ __launch_bounds__(256) void norm_slice_kernel(const NormArgs a) {
       }
       if constexpr (STAGE == 1) return;
     } else {
-      s0 = a.part[st];
-      s1 = a.part[st + 1];
+      s0 = a.join ? sm.sa[k] : a.part[st];
+      s1 = a.join ? sm.sb[k] : a.part[st + 1];
     }
     if (!a.y) return;
 #pragma unroll
@@ -434,68 +494,38 @@ __global__ __launch_bounds__(256) void norm_slice_kernel(const NormArgs a) {
   }
 }
 
-// Joins the slices of a group: one wavefront per (sample, group).  A slice whose
-// channels lie elsewhere holds nothing of the group and wrote nothing.
 template <bool BWD>
 __global__ __launch_bounds__(256) void norm_join_kernel(const float *__restrict__ part, int64_t groups, int G, int per,
                                                         int W, int64_t L, int C, float eps, float *__restrict__ out) {
   const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
   if (i >= groups) return;   // whole wavefront
-  const Slice s = slice_of(L, C, W);
-  const int lane = threadIdx.x & 63, g = static_cast<int>(i % G), pv = per / W;
-  const int b0 = g * pv / s.CT, b1 = ((g + 1) * pv - 1) / s.CT, nb = b1 - b0 + 1;   // its channel blocks
-  float cnt = 0.f, u = 0.f, v = 0.f;   // count, mean, centred squares; or two sums
-  auto join = [&](float c2, float u2, float v2) __attribute__((always_inline)) {
-    if constexpr (BWD) {
-      u += u2;
-      v += v2;
-    } else if (c2 > 0.f) {
-      const float c = cnt + c2, d = u2 - u, f = c2 / c;
-      u = fmaf(d, f, u);
-      v += v2 + d * d * cnt * f;
-      cnt = c;
-    }
-  };
-  for (int64_t k = lane; k < static_cast<int64_t>(s.rblocks) * nb; k += 64) {
-    const float *p = part + ((i * s.rblocks + k / nb) * s.cblocks + b0 + k % nb) * (BWD ? 2 : 3);
-    if constexpr (BWD) join(0.f, p[0], p[1]);
-    else join(p[0], p[1], p[2]);
-  }
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const float c2 = __shfl_xor(cnt, d), u2 = __shfl_xor(u, d), v2 = __shfl_xor(v, d);
-    if constexpr (!BWD) {   // both lanes join in the same order
-      const bool up = lane & d;
-      const float ca = up ? c2 : cnt, ua = up ? u2 : u, va = up ? v2 : v;
-      const float cx = up ? cnt : c2, ux = up ? u : u2, vx = up ? v : v2;
-      cnt = ca; u = ua; v = va;
-      if (ca == 0.f) { cnt = cx; u = ux; v = vx; }
-      else join(cx, ux, vx);
-    } else {
-      u += u2;
-      v += v2;
-    }
-  }
-  if (lane == 0) {
+  float u, v;
+  join_slices<BWD>(part, slice_of(L, C, W), i, static_cast<int>(i % G), per / W, u, v);
+  if ((threadIdx.x & 63) == 0) {
     out[2 * i] = u;
     out[2 * i + 1] = BWD ? v : 1.f / sqrtf(v / (static_cast<float>(L) * per) + eps);
   }
 }
 
-// Sums down R rows of [R][cols]: workgroup (64 columns, split s) takes rows s, s + S, ...
-__global__ __launch_bounds__(256) void norm_cols_kernel(const float *__restrict__ src, int64_t R, int64_t cols, int S,
-                                                        float *__restrict__ dst, int C, float *__restrict__ dw,
-                                                        float *__restrict__ db) {
-  __shared__ float sm[4][64];
+// Sums down R rows of [R][cols]: workgroup (64 columns, split s of S), 16
+// wavefronts with every 16 S-th row each.
+__global__ __launch_bounds__(1024) void norm_cols_kernel(const float *__restrict__ src, int64_t R, int64_t cols, int S,
+                                                         float *__restrict__ dst, int C, float *__restrict__ dw,
+                                                         float *__restrict__ db) {
+  __shared__ float sm[16][64];
   const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int64_t nb = (cols + 63) / 64, c = (blockIdx.x % nb) * 64 + lane, s = blockIdx.x / nb;
   float t = 0.f;
-  if (c < cols)
-    for (int64_t r = s * 4 + w; r < R; r += 4 * S) t += src[r * cols + c];
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = s * 16 + w; r < R; r += 16 * S) t += src[r * cols + c];
+  }
   sm[w][lane] = t;
   __syncthreads();
   if (w == 0 && c < cols) {
-    t = (sm[0][lane] + sm[1][lane]) + (sm[2][lane] + sm[3][lane]);
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += sm[i][lane];
     if (dst) dst[s * cols + c] = t;
     else if (c < C) {
       if (dw) dw[c] = t;
@@ -540,7 +570,8 @@ NormPlan plan_of(int64_t N, int64_t L, int C, int G, int W, bool bwd) {
     p.part_floats = p.one ? 0 : (bwd ? 2 : 3) * N * G * p.s.rblocks * p.s.cblocks + 2 * N * G;
     p.col_rows = N * p.s.rblocks;
   }
-  p.S = static_cast<int>(std::min<int64_t>(kColSplits, std::max<int64_t>(1, p.col_rows / 32)));
+  // (one step adds up to 64 rows a wavefront; more are split over the GPU first)
+  p.S = p.col_rows <= 1024 ? 1 : static_cast<int>(std::min<int64_t>(kColSplits, p.col_rows / 128));
   return p;
 }
 int64_t ws_floats(const NormPlan &p, int C, bool bwd) {
@@ -604,6 +635,12 @@ void launch_norm(const NormPlan &p, const NormArgs &a, float *joined, hipStream_
   hipLaunchKernelGGL((norm_slice_kernel<DT, W, BWD, 1>), grid, block, 0, st, a);
   if (BWD && !a.y) return;
   NormArgs second = a;
+  // up to 64 slices a sample (one a lane) are joined by each workgroup that needs them
+  second.join = p.s.rblocks * p.s.cblocks <= 64;
+  if (second.join) {
+    hipLaunchKernelGGL((norm_slice_kernel<DT, W, BWD, 2>), grid, block, 0, st, second);
+    return;
+  }
   if (BWD) second.part = joined;
   else second.stats = joined;
   hipLaunchKernelGGL((norm_join_kernel<BWD>), grid_of((a.N * a.G + 3) / 4), block, 0, st, a.part, a.N * a.G, a.G,
@@ -703,7 +740,7 @@ extern "C" int ssla_group_norm_bwd(const void *dy, const void *x, const float *s
   }
   if (sums) {
     const int64_t wide = 2 * static_cast<int64_t>(C), nb = (wide + 63) / 64;
-    const dim3 block(256);
+    const dim3 block(1024);
     if (p.S > 1) {
       hipLaunchKernelGGL(norm_cols_kernel, grid_of(nb * p.S), block, 0, st, cols, p.col_rows, wide, p.S, split, C,
                          dweight, dbias);
