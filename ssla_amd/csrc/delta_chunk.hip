@@ -676,6 +676,7 @@ extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const vo
   if (n_seq == 0) return SSLA_OK;
   SSLA_CHECK_ARG(cu_seqlens != nullptr, "gated_delta_chunk_fwd: cu_seqlens is NULL");
   SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "gated_delta_chunk_fwd: null tensor pointer");
+  if (const int e = check_widths("gated_delta_chunk_fwd", kChunk, Hk, H, K, V)) return e;
   const DeltaLayout L = delta_layout(n_seq, T, Hk, H, K, V, false);
   if (!workspace || workspace_bytes < L.total || !aligned(workspace, 16)) {
     set_error("gated_delta_chunk_fwd: needs %zu bytes of workspace, got %zu", L.total, workspace_bytes);

@@ -680,6 +680,7 @@ extern "C" int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const vo
     set_error("gated_delta_chunk_bwd: unsupported dtype %d", dtype);
     return SSLA_ERR_DTYPE;
   }
+  if (const int e = check_widths("gated_delta_chunk_bwd", kChunk, Hk, H, K, V)) return e;
   const DeltaLayout L = delta_layout(n_seq, T, Hk, H, K, V, true);
   if (!workspace || workspace_bytes < L.total || !aligned(workspace, 16)) {
     set_error("gated_delta_chunk_bwd: needs %zu bytes of workspace, got %zu", L.total, workspace_bytes);

@@ -320,6 +320,16 @@ inline WalkArgs walk_args(const DeltaLayout &L, char *ws, const void *q, const v
   return a;
 }
 
+// Offsets inside `rows` rows, or inside a state, are 32 bits.
+inline int check_widths(const char *what, int rows, int Hk, int H, int K, int V) {
+  if (std::max(static_cast<int64_t>(Hk) * K, static_cast<int64_t>(H) * std::max(K, V)) * rows * 4 > 0x7fffffff ||
+      static_cast<int64_t>(K) * V * 4 > 0x3fffffff) {
+    set_error("%s: rows of %d x %d or %d x %d values are too wide", what, Hk, K, H, V);
+    return SSLA_ERR_UNSUPPORTED;
+  }
+  return SSLA_OK;
+}
+
 // The chunks' matrices, the segments' states and every chunk's entering state
 // and u (delta_chunk.hip), for the backward.
 int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, int dtype,

@@ -142,3 +142,15 @@ def test_chunk_backward_entry_refuses():
     assert call(T=0, ws=16, nbytes=size(1, 0, 1, 1, 16, 16) - 1) == _lib.SSLA_ERR_WORKSPACE
     assert size(1, 64, 1, 1, 129, 16) == 0 and size(1, 64, 2, 3, 16, 16) == 0
     assert size(1, 64, 2, 2, 16, 16) < size(1, 64, 1, 2, 16, 16)
+
+
+def test_rows_too_wide_are_refused():
+    """Offsets inside a block of rows, or inside a state, are 32 bits."""
+    lib = _lib.load()
+    for H, K, V in ((1 << 17, 64, 128), (1, 128, 1 << 22)):
+        assert lib.ssla_gated_delta_chunk_fwd(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None, 0,
+                                              None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
+        assert lib.ssla_gated_delta_chunk_bwd(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None, None,
+                                              None, None, None, None, None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
+    assert lib.ssla_gated_delta_recurrent(None, None, None, None, None, 8, 1, 0, 1, 1 << 18, 64, 128, 1.0, None, None, None,
+                                          None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
