@@ -53,10 +53,15 @@ __device__ __forceinline__ void lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-// Sum over the lanes that share a lane's low four bits (the key groups).
+// Sum over the lanes that share a lane's low four bits (the key groups): lane
+// swaps on the VALU, where a shuffle would be a trip through LDS in every token's
+// chain.  A value swapped with itself gives both partners' values to both.
 __device__ __forceinline__ float sum_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
+  const uint32_t b = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
+  const uint32_t y = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+  const auto t = __builtin_amdgcn_permlane32_swap(y, y, false, false);
+  return __uint_as_float(t[0]) + __uint_as_float(t[1]);
 }
 
 // ROWS rows of `n` values (n <= N) at a stride, 16 bytes a lane and load where
@@ -190,29 +195,34 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
       if (t < BT && (lane & 3) == 0) m.gb[t][2] = s;
     }
     lds_order();
-    for (int t = 0; t < rows; ++t) {
-      const f32x4 gb = *reinterpret_cast<const f32x4 *>(&m.gb[t][0]);
-      const float vv = m.v[t][col], eg = gb[0];
-      float kk[KR], r0 = 0.f, r1 = 0.f, p0 = 0.f, p1 = 0.f;
+    f32x4 kx[KR / 4], qx[KR / 4], gb;
+    float vv;
+    auto token = [&](int t) __attribute__((always_inline)) {
+      gb = *reinterpret_cast<const f32x4 *>(&m.gb[t][0]);
+      vv = m.v[t][col];
 #pragma unroll
-      for (int i = 0; i < KR; i += 4) {
-        const f32x4 kx = *reinterpret_cast<const f32x4 *>(&m.k[t][kg * KR + i]);
-        const f32x4 qx = *reinterpret_cast<const f32x4 *>(&m.q[t][kg * KR + i]);
-#pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-          kk[i + j] = kx[j];
-          kk[i + j + 1] = kx[j + 1];
-          r0 = fmaf(kx[j], S[i + j], r0);
-          r1 = fmaf(kx[j + 1], S[i + j + 1], r1);
-          p0 = fmaf(qx[j], S[i + j], p0);
-          p1 = fmaf(qx[j + 1], S[i + j + 1], p1);
-        }
+      for (int i = 0; i < KR / 4; ++i) {
+        kx[i] = *reinterpret_cast<const f32x4 *>(&m.k[t][kg * KR + 4 * i]);
+        qx[i] = *reinterpret_cast<const f32x4 *>(&m.q[t][kg * KR + 4 * i]);
       }
-      const float r = sum_groups(r0 + r1), p = sum_groups(p0 + p1);
+    };
+    token(0);
+    for (int t = 0; t < rows; ++t) {
+      float r0 = 0.f, r1 = 0.f, p0 = 0.f, p1 = 0.f;
+#pragma unroll
+      for (int i = 0; i < KR; i += 2) {
+        r0 = fmaf(kx[i >> 2][i & 3], S[i], r0);
+        r1 = fmaf(kx[i >> 2][(i & 3) + 1], S[i + 1], r1);
+        p0 = fmaf(qx[i >> 2][i & 3], S[i], p0);
+        p1 = fmaf(qx[i >> 2][(i & 3) + 1], S[i + 1], p1);
+      }
+      const float eg = gb[0], r = sum_groups(r0 + r1), p = sum_groups(p0 + p1);
       const float u = gb[1] * fmaf(-eg, r, vv);
 #pragma unroll
-      for (int i = 0; i < KR; ++i) S[i] = fmaf(kk[i], u, eg * S[i]);
-      if (kg == 0) m.v[t][col] = a.scale * fmaf(gb[2], u, eg * p);   // o in the place of v
+      for (int i = 0; i < KR; ++i) S[i] = fmaf(kx[i >> 2][i & 3], u, eg * S[i]);
+      const float o = a.scale * fmaf(gb[2], u, eg * p);
+      token(min(t + 1, BT - 1));   // on its way while the sums above finish
+      if (kg == 0) m.v[t][col] = o;   // o in the place of v
     }
     lds_order();
     Rows<DT, BT, 16, 16>::put(&m.v[0][0], rows_rsrc(a.o, (t0 * a.H + h) * a.V + c0, rows, vstride, nc, ES), vstride, nc,
