@@ -256,25 +256,29 @@ int ssla_gated_delta_recurrent(const void *q, const void *k, const void *v, cons
  * is not finite (a g of -inf is) makes its head's o and state NaN from that
  * row on, one of v its column; earlier rows keep their values.  Workspace:
  * ssla_gated_delta_chunk_workspace_size bytes, 16-byte aligned, no
- * initialisation. */
+ * initialisation.  segments (NULL, or ssla_gated_delta_chunk_segments_size bytes,
+ * 16-byte aligned) receives the states and maps of the segments that long
+ * sequences are cut into, for ssla_gated_delta_chunk_bwd on the same inputs. */
 size_t ssla_gated_delta_chunk_workspace_size(int n_seq, int64_t T, int H, int K, int V);
+size_t ssla_gated_delta_chunk_segments_size(int n_seq, int64_t T, int H, int K, int V);
 int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, const float *g, const float *beta,
                                const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,
-                               float scale, const float *h0, void *o, float *ht, int dtype, void *workspace,
-                               size_t workspace_bytes, void *stream);
+                               float scale, const float *h0, void *o, float *ht, void *segments, int dtype,
+                               void *workspace, size_t workspace_bytes, void *stream);
 
 /* Gradients of ssla_gated_delta_chunk_fwd: dout [T, H, V] in `dtype`, dht fp32
  * [n_seq, H, K, V] or NULL; dq, dk, dv in `dtype` and the inputs' shapes (dq and
  * dk of a shared key head are the sums over its value heads), dg, dbeta fp32
  * [T, H], dh0 fp32 or NULL.  Rows in no sequence receive zeros.  The states are
- * computed again from the inputs.  A sequence's head with a value that is not
- * finite has gradients that are not.  Workspace as for the forward. */
+ * computed again from the inputs, and from the forward's segments if given.  A
+ * sequence's head with a value that is not finite has gradients that are not.
+ * Workspace as for the forward. */
 size_t ssla_gated_delta_chunk_bwd_workspace_size(int n_seq, int64_t T, int Hk, int H, int K, int V);
 int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const void *v, const float *g, const float *beta,
                                const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,
                                float scale, const float *h0, const void *dout, const float *dht, void *dq, void *dk,
-                               void *dv, float *dg, float *dbeta, float *dh0, int dtype, void *workspace,
-                               size_t workspace_bytes, void *stream);
+                               void *dv, float *dg, float *dbeta, float *dh0, const void *segments, int dtype,
+                               void *workspace, size_t workspace_bytes, void *stream);
 
 /* ------------------------------------------------------------------------
  * Group norm with an activation, channels last (no reference counterpart):

@@ -77,11 +77,12 @@ SIGNATURES = {
     "ssla_gated_delta_recurrent": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
                                           _vp, _vp, _vp, _i32, _vp, _i32, _vp]),
     "ssla_gated_delta_chunk_workspace_size": (_sz, [_i32, _i64, _i32, _i32, _i32]),
+    "ssla_gated_delta_chunk_segments_size": (_sz, [_i32, _i64, _i32, _i32, _i32]),
     "ssla_gated_delta_chunk_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
-                                          _vp, _vp, _i32, _vp, _sz, _vp]),
+                                          _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
     "ssla_gated_delta_chunk_bwd_workspace_size": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32]),
     "ssla_gated_delta_chunk_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
-                                          _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
+                                          _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
     "ssla_group_norm_workspace_size": (_sz, [_i64, _i64, _i32, _i32]),
     "ssla_group_norm_fwd": (_i32, [_vp, _i64, _i64, _i32, _i32, _vp, _vp, _f32, _i32, _vp, _vp, _i32, _vp, _sz, _vp]),
     "ssla_group_norm_bwd_workspace_size": (_sz, [_i64, _i64, _i32, _i32]),

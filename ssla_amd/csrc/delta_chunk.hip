@@ -17,8 +17,9 @@
 // Long sequences are cut into segments that run side by side: over a segment
 // the state goes through an affine map S -> M S + L, and the columns of M are
 // columns of a state that enters as the identity with v = 0.  A pass over all
-// segments but a sequence's last computes L and M, a fold carries the states
-// over the segments, and the walk starts every segment from its state.
+// segments but a sequence's last computes L and M (the first segment's from the
+// initial state, so it needs no M), a fold carries the states over the segments,
+// and the walk starts every segment from its state.
 //
 // Values that are not finite: a row whose k, beta or g is not finite makes all
 // columns of its head NaN from that row on, one in v or in a state its own
@@ -226,7 +227,8 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
 // kOutput walks a segment from its entering state and writes o (and ht behind the
 // sequence's last row); kStates does so and writes every chunk's entering state
 // and u instead (for the backward); kSegment walks an inner segment from zero
-// and from the identity and writes L and M.
+// (a sequence's first from its initial state) and from the identity and writes L
+// and M.
 enum { kOutput, kStates, kSegment };
 
 template <int DT, int KP, bool OUT>
@@ -261,6 +263,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   if (!seq_of_slot<!SEG>(a.cu, a.n_seq, a.T, unit, slot, n, bos, eos, first)) return;   // workgroup-uniform
   const int64_t seg = slot - first, t_begin = bos + seg * unit;
   if (SEG ? t_begin + unit >= eos : (t_begin >= eos && seg > 0)) return;
+  if (SEG && seg == 0 && grp * 4 >= n_vt) return;   // (a first segment's M)
   const int64_t t_end = min(t_begin + unit, eos);
   const int tile = grp * 4 + w;
   const bool is_map = SEG && tile >= n_vt;                   // this wavefront's columns are M's
@@ -270,14 +273,13 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
 
   const StateCols<NT> cols(a.K, a.V, vcol, v_ok, G);
   f32x4 S[NT];
-  if (!SEG) {
-    cols.load(seg > 0 ? a.seg_state + ((bos / unit + seg - 1) * a.H + h) * KV
-              : a.h0  ? a.h0 + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr, S);
-  } else {
+  cols.load(seg > 0 ? (SEG ? nullptr : a.seg_state + ((bos / unit + seg - 1) * a.H + h) * KV)
+            : a.h0  ? a.h0 + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr, S);
+  if (is_map) {
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) S[t][r] = is_map && idx_of(t, 4 * G + r) == mcol ? 1.f : 0.f;
+      for (int r = 0; r < 4; ++r) S[t][r] = idx_of(t, 4 * G + r) == mcol ? 1.f : 0.f;
   }
   // byte offset of row 8 G in this lane's column of v, o and u (in values of 4 bytes for u)
   constexpr int ES = sizeof(ET);
@@ -508,9 +510,8 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   if (!SEG) {
     if (a.ht && t_end == eos) cols.store(a.ht + (static_cast<int64_t>(n) * a.H + h) * KV, S);
   } else if (is_map) {
-    if (active) {
-      uint16_t *dst = a.seg_map + (slot * a.H + h) * (3 * KP * KP);
-      const int ks = mcol >> 5, lg = 16 * ((mcol & 31) >> 3), j = mcol & 7;
+    if (active && seg > 0) {
+      uint16_t *dst = a.seg_map + (slot * a.H + h) * (3 * KP * KP) + mcol;
 #pragma unroll
       for (int t = 0; t < NT; ++t)
 #pragma unroll
@@ -520,7 +521,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
           for (int p = 0; p < 3; ++p) {
             const uint16_t bits = f32_to_bf16_bits(x);
             x -= bf16_bits_to_f32(bits);
-            dst[((t * (KP / 32) + ks) * 3 + p) * 512 + (lg + 4 * G + r) * 8 + j] = bits;
+            dst[(p * KP + idx_of(t, 4 * G + r)) * KP] = bits;
           }
         }
     }
@@ -529,16 +530,16 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   }
 }
 
-// Carries the states over a sequence's segments: the L of inner segment j
-// becomes M_j E_j + L_j, the state entering segment j + 1 (E_0 = start or 0).
-// REV: from the last slot to the first.
+// The fold (see delta_fold): one workgroup per (sequence, head, 64 columns), a
+// segment after the other.  A segment's M is staged in LDS for the four
+// wavefronts, read by rows or (REV: M^T) by columns; the next one is in flight.
 template <int KP, bool REV>
 __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restrict__ cu, int64_t T, int H, int K, int V,
-                                                         int per, const float *__restrict__ start,
-                                                         const uint16_t *__restrict__ seg_map,
-                                                         float *__restrict__ seg_state) {
-  constexpr int NT = KP / 16;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, col = lane & 15, G = lane >> 4;
+                                                         int per, const uint16_t *__restrict__ seg_map,
+                                                         float *__restrict__ states) {
+  constexpr int NT = KP / 16, PLANE = KP * KP, N = (3 * PLANE / 8 + 255) / 256;
+  __shared__ __align__(16) uint16_t sm[3 * PLANE];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 15, G = lane >> 4;
   const int n_groups = (((V + 15) >> 4) + 3) >> 2;
   const int vcol = ((blockIdx.x % n_groups) * 4 + w) * 16 + col;
   const int h = static_cast<int>((blockIdx.x / n_groups) % H);
@@ -546,31 +547,45 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
   const int64_t bos = min(max(cu[n], (int64_t)0), T), eos = min(max(cu[n + 1], bos), T);
   const int64_t unit = static_cast<int64_t>(per) * kChunk, KV = static_cast<int64_t>(K) * V;
   const int64_t inner = (eos - bos + unit - 1) / unit - 1;   // segments but the last
-  const bool ok = vcol < V;
-  const StateCols<NT> cols(K, V, vcol, ok, G);
-  f32x4 S[NT];
-  cols.load(start ? start + (n * H + h) * KV : nullptr, S);
-  for (int64_t j = 0; j < inner; ++j) {
-    const int64_t slot = (bos / unit + (REV ? inner - 1 - j : j)) * H + h;
-    const uint16_t *m = seg_map + slot * (3 * KP * KP);
-    f32x4 L[NT];
-    cols.load(seg_state + slot * KV, L);
+  if (inner < 2) return;   // the only state is there already
+  const StateCols<NT> cols(K, V, vcol, vcol < V, G);
+  auto slot = [&](int64_t j) __attribute__((always_inline)) { return (bos / unit + j) * H + h; };
+  uint4 pm[N];
+  f32x4 S[NT], L[NT];
+  auto fetch = [&](int64_t i) __attribute__((always_inline)) {   // step i: M of segment i, or (REV) inner - i
+    const uint16_t *m = seg_map + slot(REV ? inner - i : i) * (3 * PLANE);
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (tid + 256 * e < 3 * PLANE / 8) pm[e] = reinterpret_cast<const uint4 *>(m)[tid + 256 * e];
+    cols.load(states + slot(REV ? inner - 1 - i : i) * KV, L);
+  };
+  cols.load(states + slot(REV ? inner - 1 : 0) * KV, S);
+  fetch(1);
+  for (int64_t i = 1; i < inner; ++i) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const int u = tid + 256 * e, p = u / (PLANE / 8), r = u % (PLANE / 8);
+      if (u < 3 * PLANE / 8)
+        *reinterpret_cast<uint4 *>(&sm[p * PLANE + sw<KP>(r / (KP / 8), (r % (KP / 8)) * 8)]) = pm[e];
+    }
     bf16x8 s[NT / 2][3];
 #pragma unroll
     for (int ks = 0; ks < NT / 2; ++ks) split(join(S[2 * ks], S[2 * ks + 1]), s[ks]);
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      S[t] = L[t];
+    for (int t = 0; t < NT; ++t) S[t] = L[t];
+    __syncthreads();
+    if (i + 1 < inner) fetch(i + 1);
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
 #pragma unroll
       for (int ks = 0; ks < NT / 2; ++ks) {
         bf16x8 x[3];
 #pragma unroll
-        for (int p = 0; p < 3; ++p)
-          x[p] = from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(m + ((t * (KP / 32) + ks) * 3 + p) * 512 + lane * 8));
+        for (int p = 0; p < 3; ++p) x[p] = REV ? op_cols<KP>(sm + p * PLANE, t, ks, lane) : op_rows<KP>(sm + p * PLANE, t, ks, lane);
         S[t] = mul<2>(x, s[ks], S[t]);
       }
-    }
-    cols.store(seg_state + slot * KV, S);
+    cols.store(states + slot(REV ? inner - 1 - i : i) * KV, S);
+    __syncthreads();   // M is read
   }
 }
 
@@ -590,15 +605,15 @@ int check_grids(const char *what, const DeltaLayout &L, const WalkArgs &a) {
 
 template <int DT, int KP>
 void launch_chunk(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, bool states,
-                  hipStream_t st) {
+                  bool have_segs, hipStream_t st) {
   const dim3 block(256);
   hipLaunchKernelGGL((delta_prep_kernel<DT, KP>), grid_of(L.chunk_slots * a.H), block, 0, st, a.k, g, beta, a.cu, a.n_seq,
                      a.T, a.Hk, a.H, a.K, a.vec, a.scale, const_cast<float *>(a.tm), a.tm_floats,
                      const_cast<float *>(a.rowv));
-  if (L.inner_slots > 0) {
+  if (L.inner_slots > 0 && !have_segs) {
     const int groups = ((a.V + 15) / 16 + KP / 16 + 3) / 4;
     hipLaunchKernelGGL((delta_walk_kernel<DT, KP, kSegment>), grid_of(L.inner_slots * a.H * groups), block, 0, st, a);
-    delta_fold(L, a, a.h0, false, st);
+    delta_fold(L, a, a.seg_state, false, st);
   }
   const dim3 grid = grid_of(L.seg_slots * a.H * v_groups(a.V));
   if (states) hipLaunchKernelGGL((delta_walk_kernel<DT, KP, kStates>), grid, block, 0, st, a);
@@ -607,20 +622,20 @@ void launch_chunk(const DeltaLayout &L, const WalkArgs &a, const float *g, const
 
 template <int DT>
 void launch_keys(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, bool states,
-                 hipStream_t st) {
+                 bool have_segs, hipStream_t st) {
   switch (L.KP) {
-    case 32: return launch_chunk<DT, 32>(L, a, g, beta, states, st);
-    case 64: return launch_chunk<DT, 64>(L, a, g, beta, states, st);
-    default: return launch_chunk<DT, 128>(L, a, g, beta, states, st);
+    case 32: return launch_chunk<DT, 32>(L, a, g, beta, states, have_segs, st);
+    case 64: return launch_chunk<DT, 64>(L, a, g, beta, states, have_segs, st);
+    default: return launch_chunk<DT, 128>(L, a, g, beta, states, have_segs, st);
   }
 }
 
 int launch_dtype(const char *what, const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta,
-                 bool states, int dtype, hipStream_t st) {
+                 bool states, bool have_segs, int dtype, hipStream_t st) {
   if (const int e = check_grids(what, L, a)) return e;
-  if (dtype == SSLA_F32) launch_keys<SSLA_F32>(L, a, g, beta, states, st);
-  else if (dtype == SSLA_BF16) launch_keys<SSLA_BF16>(L, a, g, beta, states, st);
-  else if (dtype == SSLA_F16) launch_keys<SSLA_F16>(L, a, g, beta, states, st);
+  if (dtype == SSLA_F32) launch_keys<SSLA_F32>(L, a, g, beta, states, have_segs, st);
+  else if (dtype == SSLA_BF16) launch_keys<SSLA_BF16>(L, a, g, beta, states, have_segs, st);
+  else if (dtype == SSLA_F16) launch_keys<SSLA_F16>(L, a, g, beta, states, have_segs, st);
   else {
     set_error("%s: unsupported dtype %d", what, dtype);
     return SSLA_ERR_DTYPE;
@@ -630,21 +645,21 @@ int launch_dtype(const char *what, const DeltaLayout &L, const WalkArgs &a, cons
 
 }  // namespace
 
-int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, int dtype,
-                         hipStream_t st) {
-  return launch_dtype("gated_delta_chunk_bwd", L, a, g, beta, true, dtype, st);
+int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, bool have_segs,
+                         int dtype, hipStream_t st) {
+  return launch_dtype("gated_delta_chunk_bwd", L, a, g, beta, true, have_segs, dtype, st);
 }
 
-int delta_fold(const DeltaLayout &L, const WalkArgs &a, const float *start, bool reverse, hipStream_t st) {
+int delta_fold(const DeltaLayout &L, const WalkArgs &a, float *states, bool reverse, hipStream_t st) {
   const dim3 grid = grid_of(static_cast<int64_t>(a.n_seq) * a.H * v_groups(a.V)), block(256);
 #define SSLA_FOLD(KP_)                                                                                               \
   do {                                                                                                               \
     if (reverse)                                                                                                     \
-      hipLaunchKernelGGL((delta_fold_kernel<KP_, true>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per, start,  \
-                         a.seg_map, a.seg_state);                                                                    \
+      hipLaunchKernelGGL((delta_fold_kernel<KP_, true>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per,         \
+                         a.seg_map, states);                                                                         \
     else                                                                                                             \
-      hipLaunchKernelGGL((delta_fold_kernel<KP_, false>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per, start, \
-                         a.seg_map, a.seg_state);                                                                    \
+      hipLaunchKernelGGL((delta_fold_kernel<KP_, false>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per,        \
+                         a.seg_map, states);                                                                         \
   } while (0)
   if (L.KP == 32) SSLA_FOLD(32);
   else if (L.KP == 64) SSLA_FOLD(64);
@@ -660,10 +675,15 @@ extern "C" size_t ssla_gated_delta_chunk_workspace_size(int n_seq, int64_t T, in
   return ssla::delta_layout(n_seq, T, H, H, K, V, false).total;
 }
 
+extern "C" size_t ssla_gated_delta_chunk_segments_size(int n_seq, int64_t T, int H, int K, int V) {
+  if (n_seq < 0 || T < 0 || H <= 0 || K <= 0 || K > 128 || V <= 0) return 0;
+  return ssla::delta_layout(n_seq, T, H, H, K, V, false).seg_bytes;
+}
+
 extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, const float *g,
                                           const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk,
                                           int H, int K, int V, float scale, const float *h0, void *o, float *ht,
-                                          int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+                                          void *segments, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
   using namespace ssla;
   clear_error();
   SSLA_CHECK_ARG(n_seq >= 0 && T >= 0 && Hk > 0 && H > 0 && H % Hk == 0 && K > 0 && V > 0,
@@ -682,9 +702,10 @@ extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const vo
     set_error("gated_delta_chunk_fwd: needs %zu bytes of workspace, got %zu", L.total, workspace_bytes);
     return SSLA_ERR_WORKSPACE;
   }
+  SSLA_CHECK_ARG(aligned(segments, 16), "gated_delta_chunk_fwd: segments must be 16-byte aligned");
   WalkArgs a = walk_args(L, static_cast<char *>(workspace), q, k, v, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, dtype,
-                         false);
+                         false, segments);
   a.o = o;
   a.ht = ht;
-  return launch_dtype("gated_delta_chunk_fwd", L, a, g, beta, false, dtype, static_cast<hipStream_t>(stream));
+  return launch_dtype("gated_delta_chunk_fwd", L, a, g, beta, false, false, dtype, static_cast<hipStream_t>(stream));
 }

@@ -5,8 +5,9 @@
 //   du = P^T do + e^(G_last - G) (k D),   dX = Tm^T du,   dv = beta dX,
 //   D' = e^(G_last) D + q^T (scale e^G do) - k^T (beta e^G dX)
 // (D' leaves the chunk before).  Each column of D goes its own way, so this is
-// the forward's walk in reverse: the same segments, the same affine map over a
-// segment, the same fold.  With the products' factors known for every chunk,
+// the forward's walk in reverse over the same segments: over a segment the
+// gradient goes through D -> M^T D + L with the forward's M, so only L is walked
+// for (the last segment's from the final state's gradient), then folded.  With the products' factors known for every chunk,
 //   dP_ij = scale e^(G_i - G_j) do_i . u_j (j <= i),
 //   dN_ij = -e^(G_i - G_j) dX_i . u_j (j < i),
 //   dq = scale e^G (do S^T) + dP k,
@@ -30,6 +31,7 @@ struct GradArgs {
   WalkArgs w;
   const void *dout;
   const float *dht;
+  float *seg_grad;     // per inner segment: after the fold the gradient leaving it
   float *chunk_grad;   // per chunk: D
   float *dx;           // [T, H, V]
   void *dq, *dk, *dv;
@@ -51,8 +53,8 @@ struct ReverseSmem {
   float rowv[kRowVecs][kChunk];
 };
 
-// SEG: an inner segment (one with a predecessor) from zero and from the identity:
-// L and M of the gradient's map.  Otherwise: a segment from the gradient leaving
+// SEG: a segment with a predecessor from zero (a sequence's last from dht): what it
+// adds to the gradient leaving that predecessor.  Otherwise: a segment from the gradient leaving
 // it; writes every chunk's D and dX, dv, and dh0 before the sequence's first row.
 template <int DT, int KP, bool SEG>
 __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void delta_reverse_kernel(const GradArgs ga) {
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   __shared__ __align__(16) ReverseSmem<DT, KP> sm;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, G = lane >> 4;
-  const int n_vt = (a.V + 15) >> 4, n_groups = (n_vt + (SEG ? NT : 0) + 3) >> 2;
+  const int n_vt = (a.V + 15) >> 4, n_groups = (n_vt + 3) >> 2;
   int64_t b = blockIdx.x;
   const int grp = static_cast<int>(b % n_groups);
   b /= n_groups;
@@ -77,22 +79,14 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   if (t_begin >= eos && seg > 0) return;
   const int64_t t_end = min(t_begin + unit, eos);
   const int tile = grp * 4 + w;
-  const bool is_map = SEG && tile >= n_vt;
-  const int vcol = tile * 16 + col, mcol = (tile - n_vt) * 16 + col;
-  const bool active = is_map ? mcol < KP : tile < n_vt, v_ok = !is_map && vcol < a.V;
+  const int vcol = tile * 16 + col;
+  const bool v_ok = vcol < a.V;
   const int64_t KV = static_cast<int64_t>(a.K) * a.V;
 
   const StateCols<NT> cols(a.K, a.V, vcol, v_ok, G);
   f32x4 D[NT];
-  if (!SEG) {
-    cols.load(t_end < eos ? a.seg_state + ((bos / unit + seg) * a.H + h) * KV
-              : ga.dht    ? ga.dht + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr, D);
-  } else {
-#pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) D[t][r] = is_map && idx_of(t, 4 * G + r) == mcol ? 1.f : 0.f;
-  }
+  cols.load(t_end < eos ? (SEG ? nullptr : ga.seg_grad + ((bos / unit + seg) * a.H + h) * KV)
+            : ga.dht    ? ga.dht + (static_cast<int64_t>(n) * a.H + h) * KV : nullptr, D);
   // byte offset of row 8 G in this lane's column of do and dv, and of dX (4 bytes)
   constexpr int ES = sizeof(ET);
   const uint32_t vrow = static_cast<uint32_t>(a.H) * a.V;
@@ -285,25 +279,8 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
 
   if (!SEG) {
     if (ga.dh0 && seg == 0) cols.store(ga.dh0 + (static_cast<int64_t>(n) * a.H + h) * KV, D);
-  } else if (is_map) {
-    if (active) {
-      uint16_t *dst = a.seg_map + (slot * a.H + h) * (3 * KP * KP);
-      const int ks = mcol >> 5, lg = 16 * ((mcol & 31) >> 3), j = mcol & 7;
-#pragma unroll
-      for (int t = 0; t < NT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float x = D[t][r];
-#pragma unroll
-          for (int p = 0; p < 3; ++p) {
-            const uint16_t bits = f32_to_bf16_bits(x);
-            x -= bf16_bits_to_f32(bits);
-            dst[((t * (KP / 32) + ks) * 3 + p) * 512 + (lg + 4 * G + r) * 8 + j] = bits;
-          }
-        }
-    }
   } else {
-    cols.store(a.seg_state + (slot * a.H + h) * KV, D);
+    cols.store(ga.seg_grad + (slot * a.H + h) * KV, D);
   }
 }
 
@@ -326,7 +303,7 @@ struct GradSmem {
 
 // One workgroup per (chunk slot, head); wavefront w owns the rows of tile w.
 template <int DT, int KP>
-__global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
+__global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(const GradArgs ga) {
   constexpr int NP = Parts<DT>::n, KT = KP / 16;
   typedef Elem<DT> E;
   typedef typename E::T ET;
@@ -450,90 +427,121 @@ __global__ __launch_bounds__(256, 1) void delta_grad_kernel(const GradArgs ga) {
     const f32x4 *s = reinterpret_cast<const f32x4 *>(&sm.rowv[vec][32 * p + 8 * G]);
     return join(s[0], s[1]);
   };
-  // dP, dN with this wavefront's rows i in the lanes (contraction j), and their
-  // transposes with its rows j in the lanes (contraction i); halves beyond the
-  // diagonal stay zero
-  bf16x8 pA[2][3], nA[2][3], pT[2][3], nT[2][3];
+  const bool part = ga.dq_part != nullptr;   // every value head's in fp32
+  const int krow = (part ? a.H : a.Hk) * a.K, GS = part ? 4 : ES;
+  const int64_t kat = part ? (t0 * a.H + h) * a.K : (t0 * a.Hk + hk) * a.K;
+  const Rsrc rq = rows_rsrc(part ? static_cast<const void *>(ga.dq_part) : ga.dq, kat, rows, krow, a.K, GS);
+  const Rsrc rk = rows_rsrc(part ? static_cast<const void *>(ga.dk_part) : ga.dk, kat, rows, krow, a.K, GS);
+  const int row0 = idx_of(w, 4 * G), me = idx_of(w, col);   // own rows row0 .. + 3 in accumulators, own row in operands
+  auto put = [&](const Rsrc &rs, int t, const f32x4 &x) __attribute__((always_inline)) {
+    const int key = idx_of(t, col);
+    const uint32_t off = key < a.K ? static_cast<uint32_t>(row0 * krow + key) * GS : kOutside;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (part) store_one<float>(rs, off + r * krow * 4, x[r]);
+      else store_one<ET>(rs, off + r * krow * ES, to_elem<DT>(x[r]));
+    }
+  };
+  // own rows of the column operands of half `pair`: elements 4 (w & 1) .. + 3
+  auto own = [&](const bf16x8 (&x)[NP]) __attribute__((always_inline)) {
+    f32x4 y = zero;
+#pragma unroll
+    for (int j = NP - 1; j >= 0; --j) {
+      const uint4 u = to_bits(x[j]);
+      const uint32_t lo = w & 1 ? u.z : u.x, hi = w & 1 ? u.w : u.y;
+      y += f32x4{__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u), __uint_as_float(hi << 16),
+                 __uint_as_float(hi & 0xffff0000u)};
+    }
+    return y;
+  };
+  const f32x4 sg = *reinterpret_cast<const f32x4 *>(&sm.rowv[kScaleG][row0]);
+  const f32x4 bt4 = *reinterpret_cast<const f32x4 *>(&sm.rowv[kBeta][row0]);
+  const f32x4 bg = *reinterpret_cast<const f32x4 *>(&sm.rowv[kBetaG][row0]);
+  const f32x4 te = *reinterpret_cast<const f32x4 *>(&sm.rowv[kToEnd][row0]);
+  const float mhi = sm.rowv[kGHi][me], mlo = sm.rowv[kGLo][me];
+  // per own row: q . (from the state), q . (dP k), k . (dP^T q), k . (dN k),
+  // k . ((beta dN)^T k), k . (dX S^T), k . (u D^T)
+  f32x4 qa = zero, qb = zero, kc = zero, kd = zero, ke = zero, ky = zero, kw = zero;
   {
-    const int me = idx_of(w, col);
-    const float hi = sm.rowv[kGHi][me], lo = sm.rowv[kGLo][me];
+    // dP, dN with this wavefront's rows i in the lanes (contraction j <= i)
+    bf16x8 pA[2][3], nA[2][3];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks);
+      f32x8 p1 = join(C1[2 * ks], C1[2 * ks + 1]), n1 = join(C2[2 * ks], C2[2 * ks + 1]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int r = 32 * ks + 8 * G + j;
+        const float e = fast_exp2((mhi - ghi[j]) + (mlo - glo[j]));
+        p1[j] = keep(r <= me, a.scale * p1[j] * e);
+        n1[j] = keep(r < me, -n1[j] * e);
+      }
+      split(p1, pA[ks]);
+      split(n1, nA[ks]);
+    }
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      f32x4 b = zero, d = zero, kv = zero, qv = zero;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks > pair) continue;
+        bf16x8 x[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.k[i], t, ks, lane);
+        b = mul<2>(pA[ks], x, b);
+        d = mul<2>(nA[ks], x, d);
+        if (ks == pair) {
+          kv = own(x);
+#pragma unroll
+          for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.q[i], t, ks, lane);
+          qv = own(x);
+        }
+      }
+      const f32x4 ia = sg * Z[t], hw = te * W[t];
+      qa += qv * ia;
+      qb += qv * b;
+      kd += kv * d;
+      ky += kv * Y[t];
+      kw += kv * hw;
+      put(rq, t, ia + b);
+      Z[t] = kv;                             // (from here on: the own rows of k)
+      Y[t] = bt4 * d + (hw - bg * Y[t]);     // (from here on: what dk has so far)
+    }
+  }
+  {
+    // their transposes with the own rows j in the lanes (contraction i >= j)
+    bf16x8 pT[2][3], nT[2][3];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks), bt = row8(kBeta, ks);
-      f32x8 p1 = join(C1[2 * ks], C1[2 * ks + 1]), n1 = join(C2[2 * ks], C2[2 * ks + 1]);
       f32x8 p2 = join(C3[2 * ks], C3[2 * ks + 1]), n2 = join(C4[2 * ks], C4[2 * ks + 1]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = 32 * ks + 8 * G + j;
-        const float e = fast_exp2(r <= me ? (hi - ghi[j]) + (lo - glo[j]) : (ghi[j] - hi) + (glo[j] - lo));
-        p1[j] = keep(r <= me, a.scale * p1[j] * e);
-        n1[j] = keep(r < me, -n1[j] * e);
+        const float e = fast_exp2((ghi[j] - mhi) + (glo[j] - mlo));
         p2[j] = keep(r >= me, a.scale * p2[j] * e);
         n2[j] = keep(r > me, -bt[j] * n2[j] * e);
       }
-      split(p1, pA[ks]);
-      split(n1, nA[ks]);
       split(p2, pT[ks]);
       split(n2, nT[ks]);
     }
-  }
-  const bool part = ga.dq_part != nullptr;   // every value head's in fp32
-  const int krow = (part ? a.H : a.Hk) * a.K;
-  const int64_t kat = part ? (t0 * a.H + h) * a.K : (t0 * a.Hk + hk) * a.K;
-  const Rsrc rq = rows_rsrc(part ? static_cast<const void *>(ga.dq_part) : ga.dq, kat, rows, krow, a.K, part ? 4 : ES);
-  const Rsrc rk = rows_rsrc(part ? static_cast<const void *>(ga.dk_part) : ga.dk, kat, rows, krow, a.K, part ? 4 : ES);
-  // per own row: q . (from the state), q . (dP k), k . (dP^T q), k . (dN k),
-  // k . ((beta dN)^T k), k . (dX S^T), k . (u D^T)
-  float qa[4], qb[4], kc[4], kd[4], ke[4], ky[4], kw[4];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) qa[r] = qb[r] = kc[r] = kd[r] = ke[r] = ky[r] = kw[r] = 0.f;
+    for (int t = 0; t < KT; ++t) {
+      f32x4 c = zero, e = zero;
 #pragma unroll
-  for (int t = 0; t < KT; ++t) {
-    f32x4 b = zero, c = zero, d = zero, e = zero;
+      for (int ks = 0; ks < 2; ++ks) {
+        if (ks < pair) continue;
+        bf16x8 x[NP];
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-      bf16x8 x[NP];
-#pragma unroll
-      for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.k[i], t, ks, lane);
-      if (ks <= pair) {
-        b = mul<2>(pA[ks], x, b);
-        d = mul<2>(nA[ks], x, d);
-      }
-      if (ks >= pair) {
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.k[i], t, ks, lane);
         e = mul<2>(nT[ks], x, e);
 #pragma unroll
         for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.q[i], t, ks, lane);
         c = mul<2>(pT[ks], x, c);
       }
-    }
-    const int key = idx_of(t, col);
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = idx_of(w, 4 * G + r);
-      float qv = 0.f, kv = 0.f;
-#pragma unroll
-      for (int j = NP - 1; j >= 0; --j) {
-        qv += bf16_bits_to_f32(sm.k.q[j][sw<KP>(i, key)]);
-        kv += bf16_bits_to_f32(sm.k.k[j][sw<KP>(i, key)]);
-      }
-      const float ia = sm.rowv[kScaleG][i] * Z[t][r], bt = sm.rowv[kBeta][i], hw = sm.rowv[kToEnd][i] * W[t][r];
-      qa[r] = fmaf(qv, ia, qa[r]);
-      qb[r] = fmaf(qv, b[r], qb[r]);
-      kc[r] = fmaf(kv, c[r], kc[r]);
-      kd[r] = fmaf(kv, d[r], kd[r]);
-      ke[r] = fmaf(kv, e[r], ke[r]);
-      ky[r] = fmaf(kv, Y[t][r], ky[r]);
-      kw[r] = fmaf(kv, hw, kw[r]);
-      const float dq = ia + b[r];
-      const float dk = (c[r] + e[r]) + fmaf(bt, d[r], fmaf(-sm.rowv[kBetaG][i], Y[t][r], hw));
-      const uint32_t off = static_cast<uint32_t>(i * krow + key);
-      if (part) {
-        store_one<float>(rq, key < a.K ? off * 4 : kOutside, dq);
-        store_one<float>(rk, key < a.K ? off * 4 : kOutside, dk);
-      } else {
-        store_one<ET>(rq, key < a.K ? off * ES : kOutside, to_elem<DT>(dq));
-        store_one<ET>(rk, key < a.K ? off * ES : kOutside, to_elem<DT>(dk));
-      }
+      kc += Z[t] * c;
+      ke += Z[t] * e;
+      put(rk, t, Y[t] + (c + e));
     }
   }
 #pragma unroll
@@ -625,9 +633,8 @@ int launch_bwd(const DeltaLayout &L, const GradArgs &ga, hipStream_t st) {
   const dim3 block(256);
   const int vg = ((a.V + 15) / 16 + 3) / 4;
   if (L.inner_slots > 0) {
-    const int groups = ((a.V + 15) / 16 + KP / 16 + 3) / 4;
-    hipLaunchKernelGGL((delta_reverse_kernel<DT, KP, true>), grid_of(L.inner_slots * a.H * groups), block, 0, st, ga);
-    if (const int e = delta_fold(L, a, ga.dht, true, st)) return e;
+    hipLaunchKernelGGL((delta_reverse_kernel<DT, KP, true>), grid_of(L.inner_slots * a.H * vg), block, 0, st, ga);
+    if (const int e = delta_fold(L, a, ga.seg_grad, true, st)) return e;
   }
   hipLaunchKernelGGL((delta_reverse_kernel<DT, KP, false>), grid_of(L.seg_slots * a.H * vg), block, 0, st, ga);
   hipLaunchKernelGGL((delta_grad_kernel<DT, KP>), grid_of(L.chunk_slots * a.H), block, 0, st, ga);
@@ -662,7 +669,7 @@ extern "C" int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const vo
                                           const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk,
                                           int H, int K, int V, float scale, const float *h0, const void *dout,
                                           const float *dht, void *dq, void *dk, void *dv, float *dg, float *dbeta,
-                                          float *dh0, int dtype, void *workspace, size_t workspace_bytes,
+                                          float *dh0, const void *segments, int dtype, void *workspace, size_t workspace_bytes,
                                           void *stream) {
   using namespace ssla;
   clear_error();
@@ -689,9 +696,11 @@ extern "C" int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const vo
   char *ws = static_cast<char *>(workspace);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   GradArgs ga{};
-  ga.w = walk_args(L, ws, q, k, v, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, dtype, true);
+  ga.w = walk_args(L, ws, q, k, v, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, dtype, true,
+                   const_cast<void *>(segments));
   ga.dout = dout;
   ga.dht = dht;
+  ga.seg_grad = reinterpret_cast<float *>(ws + L.seg_grad);
   ga.chunk_grad = reinterpret_cast<float *>(ws + L.chunk_grad);
   ga.dx = reinterpret_cast<float *>(ws + L.dx);
   ga.dq = dq; ga.dk = dk; ga.dv = dv; ga.dg = dg; ga.dbeta = dbeta; ga.dh0 = dh0;
@@ -707,7 +716,7 @@ extern "C" int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const vo
     else hipLaunchKernelGGL((delta_outside_kernel<uint16_t>), grid, dim3(256), 0, st, ga);
   }
   if (n_seq == 0) return launch_status("gated_delta_chunk_bwd");
-  if (const int e = delta_forward_states(L, ga.w, g, beta, dtype, st)) return e;
+  if (const int e = delta_forward_states(L, ga.w, g, beta, segments != nullptr, dtype, st)) return e;
   switch (dtype) {
     case SSLA_F32: return launch_keys<SSLA_F32>(L, ga, st);
     case SSLA_BF16: return launch_keys<SSLA_BF16>(L, ga, st);

@@ -210,13 +210,15 @@ inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
 // Chunks per segment: at least 4, and as many as leave about 512 workgroups
 // (two a CU) of 64 value columns.
 inline int seg_chunks(int64_t T, int H, int V) {
-  const int64_t work = (T / kChunk + 1) * H * ((V + 63) / 64);
+  const int64_t work = (T + kChunk - 1) / kChunk * H * ((V + 63) / 64);
   return static_cast<int>(std::min<int64_t>(1 << 20, std::max<int64_t>(4, (work + 511) / 512)));
 }
 
-// Workspace of the forward, and (grad) of the backward.
+// Workspace of the forward, and (grad) of the backward.  The segments' states and
+// maps come first in a block of their own (seg_bytes), which a forward can leave
+// to its backward.
 struct DeltaLayout {
-  size_t tm, rowv, state, map, chunk_state, chunk_grad, u, dx, dq, dk, total;
+  size_t map, seg_bytes, segs, tm, rowv, seg_grad, chunk_state, chunk_grad, u, dx, dq, dk, total;
   int64_t chunk_slots, seg_slots, inner_slots;
   int per, KP;
 };
@@ -237,9 +239,11 @@ inline DeltaLayout delta_layout(int n_seq, int64_t T, int Hk, int H, int K, int 
   const size_t kv = static_cast<size_t>(K) * V * sizeof(float);
   L.tm = take(sizeof(float) * kTriFloats * (grad ? 2 : 1) * L.chunk_slots * H);
   L.rowv = take(sizeof(float) * kRowFloats * L.chunk_slots * H);
-  L.state = take(kv * L.inner_slots * H);
-  L.map = take(sizeof(uint16_t) * 3 * L.inner_slots * H * L.KP * L.KP);
+  L.map = align256(kv * L.inner_slots * H);
+  L.seg_bytes = L.map + align256(sizeof(uint16_t) * 3 * L.inner_slots * H * L.KP * L.KP);
+  L.segs = take(L.seg_bytes);
   if (grad) {
+    L.seg_grad = take(kv * L.inner_slots * H);
     L.chunk_state = take(kv * L.chunk_slots * H);
     L.chunk_grad = take(kv * L.chunk_slots * H);
     L.u = take(sizeof(float) * T * H * V);
@@ -292,8 +296,10 @@ struct WalkArgs {
   const float *h0;
   void *o;
   float *ht;
-  float *seg_state;       // per inner segment: L, after the fold the state entering the next segment
-  uint16_t *seg_map;      // per inner segment: M as operands of three bf16 parts
+  // per inner segment (all but a sequence's last): L, after the fold the state
+  // entering the next segment, and (but for a sequence's first) M as three bf16 matrices
+  float *seg_state;
+  uint16_t *seg_map;
   float *chunk_state;     // per chunk: the state entering it
   float *u;               // [T, H, V]
   int64_t T;
@@ -303,13 +309,14 @@ struct WalkArgs {
 
 inline WalkArgs walk_args(const DeltaLayout &L, char *ws, const void *q, const void *k, const void *v, const int64_t *cu,
                           int n_seq, int64_t T, int Hk, int H, int K, int V, float scale, const float *h0, int dtype,
-                          bool grad) {
+                          bool grad, void *segs) {
   WalkArgs a{};
   a.q = q; a.k = k; a.v = v; a.cu = cu; a.h0 = h0;
   a.tm = reinterpret_cast<float *>(ws + L.tm);
   a.rowv = reinterpret_cast<float *>(ws + L.rowv);
-  a.seg_state = reinterpret_cast<float *>(ws + L.state);
-  a.seg_map = reinterpret_cast<uint16_t *>(ws + L.map);
+  char *sg = segs ? static_cast<char *>(segs) : ws + L.segs;
+  a.seg_state = reinterpret_cast<float *>(sg);
+  a.seg_map = reinterpret_cast<uint16_t *>(sg + L.map);
   if (grad) {
     a.chunk_state = reinterpret_cast<float *>(ws + L.chunk_state);
     a.u = reinterpret_cast<float *>(ws + L.u);
@@ -330,14 +337,16 @@ inline int check_widths(const char *what, int rows, int Hk, int H, int K, int V)
   return SSLA_OK;
 }
 
-// The chunks' matrices, the segments' states and every chunk's entering state
-// and u (delta_chunk.hip), for the backward.
-int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, int dtype,
-                         hipStream_t st);
+// The chunks' matrices, unless they are there (have_segs) the segments' states and
+// maps, and every chunk's entering state and u (delta_chunk.hip), for the backward.
+int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, bool have_segs,
+                         int dtype, hipStream_t st);
 
-// Carries states over a sequence's segments (delta_chunk.hip): forward, the L of
-// segment j becomes the state entering segment j + 1; in reverse the gradient's
-// L of segment j + 1 becomes the gradient leaving segment j.
-int delta_fold(const DeltaLayout &L, const WalkArgs &a, const float *start, bool reverse, hipStream_t st);
+// Carries states over a sequence's segments (delta_chunk.hip).  Forward: with M and
+// L of segments 1 .., and L of segment 0 the state behind it, L of segment j
+// becomes the state behind segment j.  In reverse (states: of the gradient, slot j
+// what segment j + 1 adds to the gradient leaving segment j) slot j becomes the
+// gradient leaving segment j.
+int delta_fold(const DeltaLayout &L, const WalkArgs &a, float *states, bool reverse, hipStream_t st);
 
 }  // namespace ssla

@@ -79,8 +79,9 @@ def _recurrent(q, k, v, g, beta, cu, n_seq, scale, h0, ht, state_idx=None, statu
     return o
 
 
-def _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
-    """One ssla_gated_delta_chunk_fwd call on contiguous tensors."""
+def _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state, keep=False):
+    """One ssla_gated_delta_chunk_fwd call on contiguous tensors: o, the final
+    states, and (keep) what its backward takes over."""
     T, Hk, K = q.shape
     H, V = v.shape[1:]
     N = cu.numel() - 1
@@ -90,22 +91,27 @@ def _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
     with _lib.on_device_of(q):
         nbytes = lib.ssla_gated_delta_chunk_workspace_size(N, T, H, K, V)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        segments = None
+        if keep:
+            segments = torch.empty(lib.ssla_gated_delta_chunk_segments_size(N, T, H, K, V), dtype=torch.uint8,
+                                   device=q.device)
         st = lib.ssla_gated_delta_chunk_fwd(P(q), P(k), P(v), P(g), P(beta), P(cu), N, T, Hk, H, K, V, float(scale),
-                                            P(h0), P(o), P(ht), _lib.DTYPE_CODE[q.dtype], P(ws), nbytes,
+                                            P(h0), P(o), P(ht), P(segments), _lib.DTYPE_CODE[q.dtype], P(ws), nbytes,
                                             _lib.stream_of(q))
     _lib.check(st, "ssla_gated_delta_chunk_fwd")
-    return o, ht
+    return o, ht, segments
 
 
 class ChunkGatedDeltaFunction(torch.autograd.Function):
     """Forward ``ssla_gated_delta_chunk_fwd``, backward
-    ``ssla_gated_delta_chunk_bwd``, which computes the states again from the
-    inputs.  dq, dk, dv have the inputs' dtype, dg, dbeta and dh0 are fp32."""
+    ``ssla_gated_delta_chunk_bwd``: keeps the inputs and, of long sequences, the
+    states and maps of their segments; every chunk's state is computed again.  dq, dk, dv have the inputs' dtype, dg, dbeta and dh0 are fp32."""
 
     @staticmethod
     def forward(ctx, q, k, v, g, beta, h0, cu, scale, output_final_state):
-        o, ht = _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
+        o, ht, segments = _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state, keep=True)
         ctx.save_for_backward(q, k, v, g, beta, h0, cu)
+        ctx.segments = segments if segments.numel() else None
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return o, ht
@@ -127,7 +133,7 @@ class ChunkGatedDeltaFunction(torch.autograd.Function):
             ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
             st = lib.ssla_gated_delta_chunk_bwd(
                 P(q), P(k), P(v), P(g), P(beta), P(cu), N, T, Hk, H, K, V, ctx.scale, P(h0), P(do), P(dht), P(dq), P(dk),
-                P(dv), P(dg), P(dbeta), P(dh0), _lib.DTYPE_CODE[q.dtype], P(ws), nbytes, _lib.stream_of(q))
+                P(dv), P(dg), P(dbeta), P(dh0), P(ctx.segments), _lib.DTYPE_CODE[q.dtype], P(ws), nbytes, _lib.stream_of(q))
         _lib.check(st, "ssla_gated_delta_chunk_bwd")
         return dq, dk, dv, dg, dbeta, dh0, None, None, None
 
@@ -171,7 +177,7 @@ def chunk_gated_delta(
     g, beta = g.to(torch.float32).contiguous(), beta.to(torch.float32).contiguous()
     if grad:
         return ChunkGatedDeltaFunction.apply(q, k, v, g, beta, h0, cu, scale, output_final_state)
-    return _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
+    return _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)[:2]
 
 
 def fused_recurrent_gated_delta(

@@ -109,7 +109,7 @@ def test_chunk_entry_refuses():
 
     def call(n=1, T=4, Hk=1, H=1, K=16, V=16, cu=8, dtype=0, ws=None, nbytes=0):
         return lib.ssla_gated_delta_chunk_fwd(None, None, None, None, None, cu, n, T, Hk, H, K, V, 1.0, None, None, None,
-                                              dtype, ws, nbytes, None)
+                                              None, dtype, ws, nbytes, None)
 
     for bad in (dict(n=-1), dict(T=-1), dict(Hk=0), dict(H=0), dict(Hk=2, H=3), dict(K=0), dict(V=0)):
         assert call(**bad) == _lib.SSLA_ERR_ARG, bad
@@ -130,7 +130,7 @@ def test_chunk_backward_entry_refuses():
 
     def call(n=1, T=4, Hk=1, H=1, K=16, V=16, cu=8, dtype=0, ws=None, nbytes=0):
         return lib.ssla_gated_delta_chunk_bwd(None, None, None, None, None, cu, n, T, Hk, H, K, V, 1.0, None, None, None,
-                                              None, None, None, None, None, None, dtype, ws, nbytes, None)
+                                              None, None, None, None, None, None, None, dtype, ws, nbytes, None)
 
     for bad in (dict(n=-1), dict(T=-1), dict(Hk=0), dict(H=0), dict(Hk=2, H=3), dict(K=0), dict(V=0)):
         assert call(**bad) == _lib.SSLA_ERR_ARG, bad
@@ -148,9 +148,9 @@ def test_rows_too_wide_are_refused():
     """Offsets inside a block of rows, or inside a state, are 32 bits."""
     lib = _lib.load()
     for H, K, V in ((1 << 17, 64, 128), (1, 128, 1 << 22)):
-        assert lib.ssla_gated_delta_chunk_fwd(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None, 0,
-                                              None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
+        assert lib.ssla_gated_delta_chunk_fwd(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None,
+                                              None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
         assert lib.ssla_gated_delta_chunk_bwd(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None, None,
-                                              None, None, None, None, None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
+                                              None, None, None, None, None, None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
     assert lib.ssla_gated_delta_recurrent(None, None, None, None, None, 8, 1, 0, 1, 1 << 18, 64, 128, 1.0, None, None, None,
                                           None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED

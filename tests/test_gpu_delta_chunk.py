@@ -130,8 +130,8 @@ def test_layouts(dev):
     o = torch.full((150, 2, 16), 7.0, device=dev)
     P, lib = _lib.ptr, _lib.load()
     ws = torch.empty(lib.ssla_gated_delta_chunk_workspace_size(1, 150, 2, 32, 16), dtype=torch.uint8, device=dev)
-    _lib.check(lib.ssla_gated_delta_chunk_fwd(*(P(t) for t in x), P(cu), 1, 150, 1, 2, 32, 16, 1.0, None, P(o), None, 0,
-                                              P(ws), ws.numel(), _lib.stream_of(o)), "chunk")
+    _lib.check(lib.ssla_gated_delta_chunk_fwd(*(P(t) for t in x), P(cu), 1, 150, 1, 2, 32, 16, 1.0, None, P(o), None, None,
+                                              0, P(ws), ws.numel(), _lib.stream_of(o)), "chunk")
     assert bool((o[:5] == 7).all()) and bool((o[140:] == 7).all()) and not bool((o[5:140] == 7).any())
 
 
