@@ -41,8 +41,10 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
                                                          int H, int K, int vec, float scale, float *__restrict__ tm,
                                                          int tm_floats, float *__restrict__ rowv) {
   constexpr int NP = Parts<DT>::n, LD = 68;
-  __shared__ __align__(16) uint16_t sk[NP][kChunk * KP];
-  __shared__ __align__(16) float A[kChunk][LD];   // I + A, then Tm
+  constexpr int SK = NP * kChunk * KP * 2, SA = kChunk * LD * 4;
+  __shared__ __align__(16) char buf[SK > SA ? SK : SA];
+  auto sk = reinterpret_cast<uint16_t(*)[kChunk * KP]>(buf);   // k, until its Gram matrix is in registers
+  auto A = reinterpret_cast<float(*)[LD]>(buf);                // then I + A, then Tm
   __shared__ float sv[kRowVecs][kChunk];
   __shared__ float diag[kChunk];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -202,21 +204,23 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
     for (int i = 0; i < 4; ++i) A[32 + rt + 4 * gr + i][ct + m] = -c[0][i];
   }
   __syncthreads();
-  float *dst = tm + (slot * H + h) * tm_floats;
-  for (int e = tid; e < kTriFloats / 4; e += 256) {
-    const int set = e >> 7, ln = (e >> 1) & 63, half = e & 1;
-    const int t = set < 2 ? set : 2 + ((set - 2) >> 1), ks = set < 2 ? 0 : (set & 1);
-    reinterpret_cast<f32x4 *>(dst)[e] =
-        *reinterpret_cast<const f32x4 *>(&A[idx_of(t, ln & 15)][32 * ks + 8 * (ln >> 4) + 4 * half]);
+  // operands: thread (b, lane, half of its eight values) has sets b, 2 + b, 4 + b
+  f32x4 *dst = reinterpret_cast<f32x4 *>(tm + (slot * H + h) * tm_floats) + tid;
+  const int b = tid >> 7, om = (tid >> 1) & 15, oc = 8 * ((tid >> 5) & 3) + 4 * (tid & 1);
+#pragma unroll
+  for (int i = 0; i < 3; ++i) {   // Tm: row tiles 0, 1 need the first half, 2, 3 both
+    const int t = i == 0 ? b : i + 1, ks = i == 0 ? 0 : b;
+    dst[256 * i] = *reinterpret_cast<const f32x4 *>(&A[idx_of(t, om)][32 * ks + oc]);
   }
   if (tm_floats > kTriFloats) {   // and Tm^T: row tiles 0, 1 need both halves, 2, 3 the second
-    for (int e = tid; e < kTriFloats / 4; e += 256) {
-      const int set = e >> 7, ln = (e >> 1) & 63, half = e & 1;
-      const int t = set < 4 ? set >> 1 : set - 2, ks = set < 4 ? (set & 1) : 1;
+    dst += kTriFloats / 4;
+#pragma unroll
+    for (int i = 0; i < 3; ++i) {
+      const int t = i == 2 ? 2 + b : i, ks = i == 2 ? 1 : b;
       f32x4 x;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = A[32 * ks + 8 * (ln >> 4) + 4 * half + i][idx_of(t, ln & 15)];
-      reinterpret_cast<f32x4 *>(dst + kTriFloats)[e] = x;
+      for (int j = 0; j < 4; ++j) x[j] = A[32 * ks + oc + j][idx_of(t, om)];
+      dst[256 * i] = x;
     }
   }
   float *dv = rowv + (slot * H + h) * kRowFloats;
@@ -550,13 +554,14 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
   if (inner < 2) return;   // the only state is there already
   const StateCols<NT> cols(K, V, vcol, vcol < V, G);
   auto slot = [&](int64_t j) __attribute__((always_inline)) { return (bos / unit + j) * H + h; };
-  uint4 pm[N];
+  typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+  u32x4 pm[N];
   f32x4 S[NT], L[NT];
   auto fetch = [&](int64_t i) __attribute__((always_inline)) {   // step i: M of segment i, or (REV) inner - i
     const uint16_t *m = seg_map + slot(REV ? inner - i : i) * (3 * PLANE);
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (tid + 256 * e < 3 * PLANE / 8) pm[e] = reinterpret_cast<const uint4 *>(m)[tid + 256 * e];
+      if (tid + 256 * e < 3 * PLANE / 8) pm[e] = reinterpret_cast<const u32x4 *>(m)[tid + 256 * e];
     cols.load(states + slot(REV ? inner - 1 - i : i) * KV, L);
   };
   cols.load(states + slot(REV ? inner - 1 : 0) * KV, S);
@@ -566,7 +571,7 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
     for (int e = 0; e < N; ++e) {
       const int u = tid + 256 * e, p = u / (PLANE / 8), r = u % (PLANE / 8);
       if (u < 3 * PLANE / 8)
-        *reinterpret_cast<uint4 *>(&sm[p * PLANE + sw<KP>(r / (KP / 8), (r % (KP / 8)) * 8)]) = pm[e];
+        *reinterpret_cast<u32x4 *>(&sm[p * PLANE + sw<KP>(r / (KP / 8), (r % (KP / 8)) * 8)]) = pm[e];
     }
     bf16x8 s[NT / 2][3];
 #pragma unroll

@@ -711,7 +711,7 @@ extern "C" int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const vo
   ga.vvec = V % 4 == 0;
   ga.dvec = (static_cast<int64_t>(V) * (dtype == SSLA_F32 ? 4 : 2)) % 16 == 0 && aligned(dout, 16) && aligned(v, 16);
   if (T > 0) {
-    const dim3 grid = grid_of(std::min<int64_t>(T, 1024));
+    const dim3 grid = grid_of(std::min<int64_t>(T, 256));
     if (dtype == SSLA_F32) hipLaunchKernelGGL((delta_outside_kernel<float>), grid, dim3(256), 0, st, ga);
     else hipLaunchKernelGGL((delta_outside_kernel<uint16_t>), grid, dim3(256), 0, st, ga);
   }
