@@ -545,25 +545,15 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
     }
   }
 #pragma unroll
-  for (int m = 1; m < 16; m <<= 1)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      qa[r] += __shfl_xor(qa[r], m);
-      qb[r] += __shfl_xor(qb[r], m);
-      kc[r] += __shfl_xor(kc[r], m);
-      kd[r] += __shfl_xor(kd[r], m);
-      ke[r] += __shfl_xor(ke[r], m);
-      ky[r] += __shfl_xor(ky[r], m);
-      kw[r] += __shfl_xor(kw[r], m);
-    }
-  if (col == 0) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int i = idx_of(w, 4 * G + r);
-      const float bt = sm.rowv[kBeta][i], eg = fast_exp2(sm.rowv[kGHi][i]) * fast_exp2(sm.rowv[kGLo][i]);
-      sm.base[i] = (qa[r] - sm.rowv[kBetaG][i] * ky[r]) + ((qb[r] - kc[r]) + (bt * kd[r] - ke[r]));
-      sm.to_next[i] = kw[r];
-      if (i < rows) ga.dbeta[(t0 + i) * a.H + h] = sm.dxv[i] + fmaf(-eg, ky[r], kd[r]);
+  for (int r = 0; r < 4; ++r) {   // the keys' sums, of what the row needs
+    const int i = row0 + r;
+    const float eg = fast_exp2(sm.rowv[kGHi][i]) * fast_exp2(sm.rowv[kGLo][i]);
+    const float base = row_sum((qa[r] - bg[r] * ky[r]) + ((qb[r] - kc[r]) + (bt4[r] * kd[r] - ke[r])));
+    const float next = row_sum(kw[r]), db = row_sum(fmaf(-eg, ky[r], kd[r]));
+    if (col == 0) {
+      sm.base[i] = base;
+      sm.to_next[i] = next;
+      if (i < rows) ga.dbeta[(t0 + i) * a.H + h] = sm.dxv[i] + db;
     }
   }
   __syncthreads();

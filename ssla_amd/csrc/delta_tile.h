@@ -16,6 +16,8 @@
 // accumulators, which is what the next product's operand needs of it: results
 // go on to the next product without leaving their lanes.
 #pragma once
+#include <type_traits>
+
 #include "lds_tile.h"
 
 namespace ssla {
@@ -53,6 +55,18 @@ __device__ __forceinline__ void split(const f32x8 &x, bf16x8 (&p)[N]) {
   }
 #pragma unroll
   for (int i = 0; i < N; ++i) p[i] = from_bits<bf16x8>(make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]));
+}
+// Sum over the 16 lanes of a DPP row, in every lane of it.
+__device__ __forceinline__ float row_sum(float x) {
+  auto turn = [&](auto n) __attribute__((always_inline)) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x120 + decltype(n)::value,
+                                                                 0xf, 0xf, false));
+  };
+  x += turn(std::integral_constant<int, 8>{});
+  x += turn(std::integral_constant<int, 4>{});
+  x += turn(std::integral_constant<int, 2>{});
+  x += turn(std::integral_constant<int, 1>{});
+  return x;
 }
 // x where on, else 0, also where x is not finite; without a branch around what computes x
 __device__ __forceinline__ float keep(bool on, float x) {
@@ -207,11 +221,17 @@ __device__ __forceinline__ int64_t chunk_slot(int64_t bos, int n, int64_t c) { r
 inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
 
-// Chunks per segment: at least 4, and as many as leave about 512 workgroups
-// (two a CU) of 64 value columns.
+// Chunks per segment: as many as leave about 512 workgroups (two a CU) of 64
+// value columns, and for a batch of few heads at least 4 and sqrt(chunks / 5),
+// where the two walks over a segment (3.5 us a chunk) take as long as the fold
+// over the segments (1.3 us each).  Measured: 8 x 4096 rows of 8 heads of 64 174
+// us at 8 chunks, 189-213 at 4, 6 and 16; one sequence of 16,384 rows and one
+// head 113 us at 7, 127 at 4, 195 at 2.
 inline int seg_chunks(int64_t T, int H, int V) {
-  const int64_t work = (T + kChunk - 1) / kChunk * H * ((V + 63) / 64);
-  return static_cast<int>(std::min<int64_t>(1 << 20, std::max<int64_t>(4, (work + 511) / 512)));
+  const int64_t chunks = (T + kChunk - 1) / kChunk, work = chunks * H * ((V + 63) / 64);
+  int64_t per = std::max<int64_t>(4, (work + 511) / 512);
+  while (per * per * 5 < chunks) ++per;
+  return static_cast<int>(std::min<int64_t>(1 << 20, per));
 }
 
 // Workspace of the forward, and (grad) of the backward.  The segments' states and

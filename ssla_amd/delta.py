@@ -102,6 +102,15 @@ def _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state, keep=False):
     return o, ht, segments
 
 
+def _token_rows(K: int) -> int:
+    """Rows of an average sequence up to which the token-by-token kernel is
+    faster: its time grows with K, the chunk kernels' hardly.  Measured at 32,768
+    rows and 4 heads, chunks against tokens: K = 32 fp32 80 / 36 us at 64 rows and
+    68 / 41 at 128, K = 64 bf16 118 / 103 at 32 and 80 / 101 at 64, K = 128 bf16 890 /
+    495 at 16 and 268 / 414 at 64."""
+    return max(16, min(64, 2048 // K))
+
+
 class ChunkGatedDeltaFunction(torch.autograd.Function):
     """Forward ``ssla_gated_delta_chunk_fwd``, backward
     ``ssla_gated_delta_chunk_bwd``: keeps the inputs and, of long sequences, the
@@ -153,10 +162,11 @@ def chunk_gated_delta(
     final state ``[N, H, K, V]`` or None.  ``scale`` defaults to ``K ** -0.5``.
     Rows of o outside ``[cu_seqlens[0], cu_seqlens[-1])`` are unspecified.
 
-    K up to 128 runs the chunk kernels, whose products keep the precision of
-    fp32 for every dtype, and is differentiable in q, k, v, g, beta and the
-    initial state (once; rows in no sequence get zeros); wider keys run the
-    token-by-token kernel (K up to 256), forward only."""
+    K up to 128 runs the chunk kernels (chunks of 64 tokens), whose products keep
+    the precision of fp32 for every dtype, and is differentiable in q, k, v, g, beta and the
+    initial state (once; rows in no sequence get zeros).  Without a
+    gradient, sequences so short on average that chunks stay mostly empty run
+    the token-by-token kernel; so do wider keys (K up to 256), forward only."""
     name = "chunk_gated_delta"
     T, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
     dev = _lib.require_cuda(q, k, v, g, beta, initial_state)
@@ -170,7 +180,7 @@ def chunk_gated_delta(
         t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
     if grad and K > 128:
         raise NotImplementedError(f"{name}: the backward takes K up to 128 (got {K}; call it under torch.no_grad())")
-    if not grad and (K > 128 or N == 0 or T == 0):
+    if not grad and (K > 128 or T <= N * _token_rows(K)):
         ht = torch.empty(N, H, K, V, device=dev, dtype=torch.float32) if output_final_state else None
         return _recurrent(q, k, v, g, beta, cu, N, scale, h0, ht), ht
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()

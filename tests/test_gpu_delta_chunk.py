@@ -219,3 +219,26 @@ def test_wide_keys_run_token_by_token(dev):
     x, cu, _ = inputs([4], 1, 1, 257, 8, torch.float32, seed=15)
     with pytest.raises(NotImplementedError):
         chunk_gated_delta(*(t.to(dev) for t in x), cu.to(dev))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("Hk,H,K,V", [(1, 2, 32, 16), (2, 4, 16, 17), (1, 1, 1, 1), (2, 2, 24, 40)])
+def test_chunk_kernels_on_short_sequences(dev, dtype, Hk, H, K, V):
+    """The chunk kernels on batches that chunk_gated_delta gives to the other
+    kernel, and both of them on either side of the rule."""
+    from ssla_amd.delta import _chunk_fwd, _token_rows, chunk_gated_delta
+    lens = [0, 1, 63, 64, 65, 30, 7, 0]
+    assert sum(lens) <= len(lens) * _token_rows(K)
+    x, cu, s0 = inputs(lens, Hk, H, K, V, dtype, seed=K + V)
+    d = [t.to(dev) for t in x]
+    o, ht, _ = _chunk_fwd(*d, cu.to(dev), 0.5, s0.to(dev), True)
+    ro, rs = gated_delta(*x, lens, 0.5, s0)
+    close(o, ro, K, max(lens), dtype, "o")
+    close(ht, rs, K, max(lens), torch.float32, "ht")
+    for n in (1, 2):   # T = n rows: token by token; 1 sequence of more: chunks
+        few = [t[:n * _token_rows(K) // 2 + 1] for t in x]
+        T = few[0].shape[0]
+        o, ht = run(dev, few, torch.tensor([0, T]), s0[:1], scale=0.5)
+        ro, rs = gated_delta(*few, [T], 0.5, s0[:1])
+        close(o, ro, K, T, dtype, "o")
+        close(ht, rs, K, T, torch.float32, "ht")
