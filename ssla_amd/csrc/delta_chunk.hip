@@ -247,7 +247,7 @@ struct WalkSmem {
 
 // Four wavefronts, each with 16 columns of the state (its rows: the keys).
 template <int DT, int KP, int MODE>
-__global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void delta_walk_kernel(const WalkArgs a) {
+__global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : MODE == kSegment && KP < 128 ? 3 : 2) void delta_walk_kernel(const WalkArgs a) {
   constexpr int NP = Parts<DT>::n, NO = DT == SSLA_F32 ? 3 : 2, LIMO = NO - 1, NT = KP / 16;
   constexpr bool OUT = MODE == kOutput, SEG = MODE == kSegment;
   typedef Elem<DT> E;
@@ -292,18 +292,20 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   RowTile<DT, KP> kt, qt;
   f32x4 tmr[3], rvr;
   ET vr[16];
+  // (a chunk past the segment: resources of no bytes, zeros and no traffic)
   auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
-    const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+    const int rows = t0 < t_end ? static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0)) : 0;
     const int64_t at = (t0 * a.Hk + hk) * a.K;
     const int stride = a.Hk * a.K;
     kt.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
     if constexpr (OUT) qt.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
-    const int64_t c = (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h);
-    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * a.tm_floats);
-    tmr[0] = src[2 * tid];
-    tmr[1] = src[2 * tid + 1];
-    tmr[2] = src[512 + tid];
-    if (tid < kRowFloats / 4) rvr = reinterpret_cast<const f32x4 *>(a.rowv + c * kRowFloats)[tid];
+    const int64_t c = chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h;
+    const Rsrc rt = rsrc_of(a.tm + c * a.tm_floats, rows > 0 ? kTriFloats * 4 : 0);
+    const Rsrc rr = rsrc_of(a.rowv + c * kRowFloats, rows > 0 ? kRowFloats * 4 : 0);
+    tmr[0] = load4(rt, tid * 32);
+    tmr[1] = load4(rt, tid * 32 + 16);
+    tmr[2] = load4(rt, 8192 + tid * 16);
+    rvr = load4(rr, tid * 16);   // (96 threads' worth)
     const Rsrc rv = rows_rsrc(a.v, (t0 * a.H + h) * a.V, rows, vrow, a.V, ES);
 #pragma unroll
     for (int i = 0; i < 16; ++i) vr[i] = load_one<ET>(rv, voff + idx_of(i >> 2, i & 3) * vrow * ES);
@@ -344,7 +346,6 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
     if constexpr (MODE == kStates)
       cols.store(a.chunk_state + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV, S);
     __syncthreads();
-    if (t0 + kChunk < t_end) fetch(t0 + kChunk);   // the next chunk's, in flight meanwhile
 
     if constexpr (OUT) {
       // P of this wavefront's row tile: k q^T has row j of P^T in the lanes that
@@ -490,6 +491,11 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
         store_one<float>(ru, uoff + idx_of(i >> 2, i & 3) * vrow * 4,
                          32 * (i >> 3) + 8 * G + (i & 7) >= r0 ? __builtin_nanf("") : U[i >> 3][i & 7]);
     }
+
+    // the next chunk's, in flight meanwhile (from here on fewer values are live: at
+    // the chunk's start it took 60 registers more, 175 against 154 us for 16,411
+    // ragged rows of 4 heads of 128)
+    fetch(t0 + kChunk);
 
     // S <- e^(G_last) S + k^T (e^(G_last - G) u)
     bf16x8 ws[2][3];

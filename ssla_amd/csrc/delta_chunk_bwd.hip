@@ -95,18 +95,20 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
   RowTile<DT, KP> kt, qt;
   f32x4 tmr[3], rvr;
   ET dr[16];
+  // (a chunk before the segment: resources of no bytes, zeros and no traffic)
   auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
-    const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
+    const int rows = t0 >= t_begin ? static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0)) : 0;
     const int64_t at = (t0 * a.Hk + hk) * a.K;
     const int stride = a.Hk * a.K;
     kt.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
     qt.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
-    const int64_t c = (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h);
-    const f32x4 *src = reinterpret_cast<const f32x4 *>(a.tm + c * a.tm_floats + kTriFloats);
-    tmr[0] = src[2 * tid];
-    tmr[1] = src[2 * tid + 1];
-    tmr[2] = src[512 + tid];
-    if (tid < kRowFloats / 4) rvr = reinterpret_cast<const f32x4 *>(a.rowv + c * kRowFloats)[tid];
+    const int64_t c = chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h;
+    const Rsrc rt = rsrc_of(a.tm + c * a.tm_floats + kTriFloats, rows > 0 ? kTriFloats * 4 : 0);
+    const Rsrc rr = rsrc_of(a.rowv + c * kRowFloats, rows > 0 ? kRowFloats * 4 : 0);
+    tmr[0] = load4(rt, tid * 32);
+    tmr[1] = load4(rt, tid * 32 + 16);
+    tmr[2] = load4(rt, 8192 + tid * 16);
+    rvr = load4(rr, tid * 16);   // (96 threads' worth)
     const Rsrc rd = rows_rsrc(ga.dout, (t0 * a.H + h) * a.V, rows, vrow, a.V, ES);
 #pragma unroll
     for (int i = 0; i < 16; ++i) dr[i] = load_one<ET>(rd, voff + idx_of(i >> 2, i & 3) * vrow * ES);
@@ -146,7 +148,6 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
     if constexpr (!SEG)
       cols.store(ga.chunk_grad + (chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h) * KV, D);
     __syncthreads();
-    if (c > 0) fetch(t0 - kChunk);   // the next chunk's, in flight meanwhile
 
     {   // P^T of this wavefront's row tile (rows j): q k^T has row i of P in the lanes that the operand needs
       const int j = idx_of(w, col);
@@ -252,6 +253,8 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
         }
       }
     }
+    fetch(t0 - kChunk);   // the next chunk's, in flight meanwhile (here: fewer values are live)
+
     // D <- e^(G_last) D + q^T (scale e^G do) - k^T (beta e^G dX)
     bf16x8 x1[2][3], x2[2][3];
 #pragma unroll
@@ -288,14 +291,17 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
 template <int DT, int KP>
 struct GradSmem {
   static constexpr int NP = Parts<DT>::n, KR = KP < 64 ? 64 : KP;
-  union {
-    struct {   // 32 value columns at a time
-      uint16_t dout[NP][kChunk * 32], u[3][kChunk * 32], dx[3][kChunk * 32], S[3][KR * 32], D[3][KR * 32];
-    } v;
-    struct {
-      uint16_t q[NP][kChunk * KP], k[NP][kChunk * KP];
-    } k;
+  struct Values {   // 32 value columns at a time
+    uint16_t dout[NP][kChunk * 32], u[3][kChunk * 32], dx[3][kChunk * 32], S[3][KR * 32], D[3][KR * 32];
   };
+  struct Keys {
+    uint16_t q[NP][kChunk * KP], k[NP][kChunk * KP];
+  };
+  // side by side where two workgroups a CU still fit: q and k then come with the first columns
+  static constexpr bool kApart = sizeof(Values) + sizeof(Keys) <= 76 * 1024;
+  struct Apart { Values v; Keys k; };
+  union Over { Values v; Keys k; };
+  std::conditional_t<kApart, Apart, Over> m;
   float rowv[kRowVecs][kChunk];
   float base[kChunk], to_next[kChunk], dxv[kChunk];
   float sd[4];
@@ -333,6 +339,19 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
   for (int i = 0; i < 4; ++i) C1[i] = C2[i] = C3[i] = C4[i] = zero;
   float dxv = 0.f, sd = 0.f;
   const int pair = w >> 1;
+  auto keys = [&]() __attribute__((always_inline)) {
+    RowTile<DT, KP> x;
+    const int64_t at = (t0 * a.Hk + hk) * a.K;
+    const int stride = a.Hk * a.K;
+    x.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
+    x.store(&sm.m.k.q[0][0], kChunk * KP);
+    x.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
+    x.store(&sm.m.k.k[0][0], kChunk * KP);
+  };
+  if (tid < kRowFloats / 4)
+    reinterpret_cast<f32x4 *>(&sm.rowv[0][0])[tid] =
+        reinterpret_cast<const f32x4 *>(a.rowv + (slot * a.H + h) * kRowFloats)[tid];
+  if (GradSmem<DT, KP>::kApart) keys();
   for (int c0 = 0; c0 < a.V; c0 += 32) {
     {
       const int nc = a.V - c0;
@@ -345,9 +364,9 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
       vt.fetch(slab(a.v, ES), vrow, nc, ga.dvec);
       ut.fetch(slab(a.u, 4), vrow, nc, ga.vvec);
       xt.fetch(slab(ga.dx, 4), vrow, nc, ga.vvec);
-      dt.store(&sm.v.dout[0][0], kChunk * 32);
-      ut.store(&sm.v.u[0][0], kChunk * 32);
-      xt.store(&sm.v.dx[0][0], kChunk * 32);
+      dt.store(&sm.m.v.dout[0][0], kChunk * 32);
+      ut.store(&sm.m.v.u[0][0], kChunk * 32);
+      xt.store(&sm.m.v.dx[0][0], kChunk * 32);
 #pragma unroll
       for (int j = 0; j < 8; ++j) dxv = fmaf(vt.value(0, j), xt.value(0, j), dxv);
 #pragma unroll
@@ -356,8 +375,8 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
         const int64_t at = static_cast<int64_t>(k0) * a.V + c0;
         st.fetch(rows_rsrc(Sp, at, a.K - k0, a.V, nc, 4), a.V, nc, ga.vvec);
         gt.fetch(rows_rsrc(Dp, at, a.K - k0, a.V, nc, 4), a.V, nc, ga.vvec);
-        st.store(&sm.v.S[0][k0 * 32], KR * 32);
-        gt.store(&sm.v.D[0][k0 * 32], KR * 32);
+        st.store(&sm.m.v.S[0][k0 * 32], KR * 32);
+        gt.store(&sm.m.v.D[0][k0 * 32], KR * 32);
 #pragma unroll
         for (int j = 0; j < 8; ++j) sd = fmaf(st.value(0, j), gt.value(0, j), sd);
       }
@@ -365,21 +384,21 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
     __syncthreads();
     bf16x8 od[NP], ou[3], ox[3];   // this wavefront's rows of do, u, dX
 #pragma unroll
-    for (int i = 0; i < NP; ++i) od[i] = op_rows<32>(sm.v.dout[i], w, 0, lane);
+    for (int i = 0; i < NP; ++i) od[i] = op_rows<32>(sm.m.v.dout[i], w, 0, lane);
 #pragma unroll
     for (int i = 0; i < 3; ++i) {
-      ou[i] = op_rows<32>(sm.v.u[i], w, 0, lane);
-      ox[i] = op_rows<32>(sm.v.dx[i], w, 0, lane);
+      ou[i] = op_rows<32>(sm.m.v.u[i], w, 0, lane);
+      ox[i] = op_rows<32>(sm.m.v.dx[i], w, 0, lane);
     }
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
       bf16x8 s[3];
 #pragma unroll
-      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.v.S[i], t, 0, lane);
+      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.m.v.S[i], t, 0, lane);
       Z[t] = mul<2>(od, s, Z[t]);
       Y[t] = mul<2>(ox, s, Y[t]);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.v.D[i], t, 0, lane);
+      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.m.v.D[i], t, 0, lane);
       W[t] = mul<2>(ou, s, W[t]);
     }
 #pragma unroll
@@ -387,17 +406,17 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
       if ((t >> 1) <= pair) {   // rows j <= i: u do^T, u dX^T
         bf16x8 x[3];
 #pragma unroll
-        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.v.u[i], t, 0, lane);
+        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.m.v.u[i], t, 0, lane);
         C1[t] = mul<2>(x, od, C1[t]);
         C2[t] = mul<2>(x, ox, C2[t]);
       }
       if ((t >> 1) >= pair) {   // rows i >= j: do u^T, dX u^T
         bf16x8 x[3], y[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) y[i] = op_rows<32>(sm.v.dout[i], t, 0, lane);
+        for (int i = 0; i < NP; ++i) y[i] = op_rows<32>(sm.m.v.dout[i], t, 0, lane);
         C3[t] = mul<2>(y, ou, C3[t]);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.v.dx[i], t, 0, lane);
+        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.m.v.dx[i], t, 0, lane);
         C4[t] = mul<2>(x, ou, C4[t]);
       }
     }
@@ -405,15 +424,7 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
   }
 
   {
-    RowTile<DT, KP> x;
-    const int64_t at = (t0 * a.Hk + hk) * a.K;
-    const int stride = a.Hk * a.K;
-    x.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
-    x.store(&sm.k.q[0][0], kChunk * KP);
-    x.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
-    x.store(&sm.k.k[0][0], kChunk * KP);
-    const float *src = a.rowv + (slot * a.H + h) * kRowFloats;
-    for (int e = tid; e < kRowFloats; e += 256) (&sm.rowv[0][0])[e] = src[e];
+    if (!GradSmem<DT, KP>::kApart) keys();
     dxv += __shfl_xor(dxv, 1);
     dxv += __shfl_xor(dxv, 2);
     if ((tid & 3) == 0) sm.dxv[tid >> 2] = dxv;
@@ -487,13 +498,13 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
         if (ks > pair) continue;
         bf16x8 x[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.k[i], t, ks, lane);
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.k[i], t, ks, lane);
         b = mul<2>(pA[ks], x, b);
         d = mul<2>(nA[ks], x, d);
         if (ks == pair) {
           kv = own(x);
 #pragma unroll
-          for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.q[i], t, ks, lane);
+          for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.q[i], t, ks, lane);
           qv = own(x);
         }
       }
@@ -533,10 +544,10 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
         if (ks < pair) continue;
         bf16x8 x[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.k[i], t, ks, lane);
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.k[i], t, ks, lane);
         e = mul<2>(nT[ks], x, e);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.k.q[i], t, ks, lane);
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.q[i], t, ks, lane);
         c = mul<2>(pT[ks], x, c);
       }
       kc += Z[t] * c;

@@ -137,6 +137,9 @@ __device__ __forceinline__ E load_one(const Rsrc &rs, uint32_t off) {
   if constexpr (sizeof(E) == 2) return static_cast<E>(__builtin_amdgcn_raw_buffer_load_b16(rs, off, 0, 0));
   else return __builtin_bit_cast(E, __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0));
 }
+__device__ __forceinline__ f32x4 load4(const Rsrc &rs, uint32_t off) {
+  return __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, off, 0, 0));
+}
 template <typename E>
 __device__ __forceinline__ void store_one(const Rsrc &rs, uint32_t off, E x) {
   if constexpr (sizeof(E) == 2) __builtin_amdgcn_raw_buffer_store_b16(x, rs, off, 0, 0);
@@ -222,15 +225,15 @@ inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255);
 inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
 
 // Chunks per segment: as many as leave about 512 workgroups (two a CU) of 64
-// value columns, and for a batch of few heads at least 4 and sqrt(chunks / 5),
-// where the two walks over a segment (3.5 us a chunk) take as long as the fold
-// over the segments (1.3 us each).  Measured: 8 x 4096 rows of 8 heads of 64 174
-// us at 8 chunks, 189-213 at 4, 6 and 16; one sequence of 16,384 rows and one
-// head 113 us at 7, 127 at 4, 195 at 2.
-inline int seg_chunks(int64_t T, int H, int V) {
+// value columns, and for a batch of few heads at least 4 and, with c chunks in an
+// average sequence, sqrt(c / 5), where the two walks over a segment (3.5 us a
+// chunk) take as long as the fold over the segments (1.3 us each).  Measured: 8 x
+// 4096 rows of 8 heads of 64 174 us at 8 chunks, 189-213 at 4, 6, 11 and 16; one
+// sequence of 16,384 rows and one head 113 us at 7, 127 at 4, 195 at 2.
+inline int seg_chunks(int n_seq, int64_t T, int H, int V) {
   const int64_t chunks = (T + kChunk - 1) / kChunk, work = chunks * H * ((V + 63) / 64);
   int64_t per = std::max<int64_t>(4, (work + 511) / 512);
-  while (per * per * 5 < chunks) ++per;
+  while (per * per * 5 * n_seq < chunks) ++per;
   return static_cast<int>(std::min<int64_t>(1 << 20, per));
 }
 
@@ -245,7 +248,7 @@ struct DeltaLayout {
 inline DeltaLayout delta_layout(int n_seq, int64_t T, int Hk, int H, int K, int V, bool grad) {
   DeltaLayout L{};
   L.KP = padded_keys(K);
-  L.per = seg_chunks(T, H, V);
+  L.per = seg_chunks(std::max(n_seq, 1), T, H, V);
   const int64_t unit = static_cast<int64_t>(L.per) * kChunk;
   L.chunk_slots = T / kChunk + n_seq + 1;
   L.seg_slots = T / unit + n_seq + 1;
