@@ -239,7 +239,7 @@ int ssla_seq_bounds_async(const int64_t *cu_seqlens, int n_seq, int64_t *host_ou
  * they were.
  * ------------------------------------------------------------------------ */
 
-/* Token by token, the state in registers: K <= 256, any V.  cu_seqlens NULL
+/* Token by token, the state in registers: K <= 256, any V up to 2^20.  cu_seqlens NULL
  * (with T == n_seq): sequence n is row n.  state_idx (int32 [n_seq] or NULL)
  * redirects the states as for ssla_gla_recurrent_fwd: h0 and ht may be the same
  * table of n_state_rows rows; an entry out of range or not above the one
@@ -252,9 +252,10 @@ int ssla_gated_delta_recurrent(const void *q, const void *k, const void *v, cons
                                int n_state_rows, int32_t *status, int dtype, void *stream);
 
 /* By chunks of 64 rows, all products on the matrix cores with the precision of
- * fp32 (fp32 values as sums of bf16): K <= 128, any V.  A row whose k, g or beta
- * is not finite (a g of -inf is) makes its head's o and state NaN from that
- * row on, one of v its column; earlier rows keep their values.  Workspace:
+ * fp32 (fp32 values as sums of bf16): K <= 128, any V up to 2^20.  A row whose g,
+ * beta or k . k is not finite (a g of -inf is) makes its head's o and state NaN
+ * from that row on, one of v its column; earlier rows keep their values.
+ * Workspace:
  * ssla_gated_delta_chunk_workspace_size bytes, 16-byte aligned, no
  * initialisation.  segments (NULL, or ssla_gated_delta_chunk_segments_size bytes,
  * 16-byte aligned) receives the states and maps of the segments that long

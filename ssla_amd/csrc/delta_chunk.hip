@@ -21,7 +21,7 @@
 // initial state, so it needs no M), a fold carries the states over the segments,
 // and the walk starts every segment from its state.
 //
-// Values that are not finite: a row whose k, beta or g is not finite makes all
+// Values that are not finite: a row whose beta, g or k . k is not finite makes all
 // columns of its head NaN from that row on, one in v or in a state its own
 // column; earlier rows are computed without them.
 #include "delta_tile.h"
@@ -30,7 +30,8 @@
 namespace ssla {
 namespace {
 
-__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
+// (what rounds to an infinity in bf16 counts as one)
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) < 3.38e38f; }
 
 // -------------------------------------------------- matrices of the chunks --
 // One workgroup per (chunk slot, head): the row factors and Tm.
@@ -99,7 +100,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
     // a row that is not finite (a gate of -inf is: it empties the state) and
     // those after it are left out of Tm; its beta becomes NaN, which the walk
     // turns into NaN for all that follows
-    const bool bad = lane < rows && !(finite(diag[lane]) && finite(bv) && gv < 3.402823466e38f);
+    const bool bad = lane < rows && !(finite(diag[lane]) && finite(bv) && gv < 3.38e38f);
     const unsigned long long any = __ballot(bad);
     const int r0 = any ? __ffsll(static_cast<long long>(any)) - 1 : kChunk;
     if (lane >= r0) {

@@ -352,35 +352,42 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
     reinterpret_cast<f32x4 *>(&sm.rowv[0][0])[tid] =
         reinterpret_cast<const f32x4 *>(a.rowv + (slot * a.H + h) * kRowFloats)[tid];
   if (GradSmem<DT, KP>::kApart) keys();
-  for (int c0 = 0; c0 < a.V; c0 += 32) {
-    {
-      const int nc = a.V - c0;
-      RowTile<DT, 32> dt, vt;
-      RowTile<SSLA_F32, 32> ut, xt, st, gt;
-      auto slab = [&](const void *p, int es) __attribute__((always_inline)) {   // the rows from column c0 on
-        return rows_rsrc(p, vat + c0, rows, vrow, nc, es);
-      };
-      dt.fetch(slab(ga.dout, ES), vrow, nc, ga.dvec);
-      vt.fetch(slab(a.v, ES), vrow, nc, ga.dvec);
-      ut.fetch(slab(a.u, 4), vrow, nc, ga.vvec);
-      xt.fetch(slab(ga.dx, 4), vrow, nc, ga.vvec);
-      dt.store(&sm.m.v.dout[0][0], kChunk * 32);
-      ut.store(&sm.m.v.u[0][0], kChunk * 32);
-      xt.store(&sm.m.v.dx[0][0], kChunk * 32);
+  // 32 value columns: the values' rows, and the states' (64 keys a tile)
+  constexpr int KH = (KP + 63) / 64, KR = GradSmem<DT, KP>::KR;
+  RowTile<DT, 32> dt, vt;
+  RowTile<SSLA_F32, 32> ut, xt, st[KH], gt[KH];
+  auto fetch = [&](int c0) __attribute__((always_inline)) {   // (columns past V: resources of no bytes)
+    const int nc = a.V - c0, nr = nc > 0 ? rows : 0;
+    dt.fetch(rows_rsrc(ga.dout, vat + c0, nr, vrow, nc, ES), vrow, nc, ga.dvec);
+    vt.fetch(rows_rsrc(a.v, vat + c0, nr, vrow, nc, ES), vrow, nc, ga.dvec);
+    ut.fetch(rows_rsrc(a.u, vat + c0, nr, vrow, nc, 4), vrow, nc, ga.vvec);
+    xt.fetch(rows_rsrc(ga.dx, vat + c0, nr, vrow, nc, 4), vrow, nc, ga.vvec);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) dxv = fmaf(vt.value(0, j), xt.value(0, j), dxv);
-#pragma unroll
-      for (int k0 = 0; k0 < KP; k0 += 64) {
-        constexpr int KR = GradSmem<DT, KP>::KR;
-        const int64_t at = static_cast<int64_t>(k0) * a.V + c0;
-        st.fetch(rows_rsrc(Sp, at, a.K - k0, a.V, nc, 4), a.V, nc, ga.vvec);
-        gt.fetch(rows_rsrc(Dp, at, a.K - k0, a.V, nc, 4), a.V, nc, ga.vvec);
-        st.store(&sm.m.v.S[0][k0 * 32], KR * 32);
-        gt.store(&sm.m.v.D[0][k0 * 32], KR * 32);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sd = fmaf(st.value(0, j), gt.value(0, j), sd);
-      }
+    for (int i = 0; i < KH; ++i) {
+      const int64_t at = static_cast<int64_t>(64 * i) * a.V + c0;
+      const int nk = nc > 0 ? a.K - 64 * i : 0;
+      st[i].fetch(rows_rsrc(Sp, at, nk, a.V, nc, 4), a.V, nc, ga.vvec);
+      gt[i].fetch(rows_rsrc(Dp, at, nk, a.V, nc, 4), a.V, nc, ga.vvec);
     }
+  };
+  // (the next columns in flight: where the parts of fp32 inputs leave registers for them)
+  constexpr bool kAhead = NP == 1 || KP == 128;
+  if (kAhead) fetch(0);
+  for (int c0 = 0; c0 < a.V; c0 += 32) {
+    if (!kAhead) fetch(c0);
+    dt.store(&sm.m.v.dout[0][0], kChunk * 32);
+    ut.store(&sm.m.v.u[0][0], kChunk * 32);
+    xt.store(&sm.m.v.dx[0][0], kChunk * 32);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) dxv = fmaf(vt.value(0, j), xt.value(0, j), dxv);
+#pragma unroll
+    for (int i = 0; i < KH; ++i) {
+      st[i].store(&sm.m.v.S[0][64 * i * 32], KR * 32);
+      gt[i].store(&sm.m.v.D[0][64 * i * 32], KR * 32);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sd = fmaf(st[i].value(0, j), gt[i].value(0, j), sd);
+    }
+    if (kAhead) fetch(c0 + 32);
     __syncthreads();
     bf16x8 od[NP], ou[3], ox[3];   // this wavefront's rows of do, u, dX
 #pragma unroll

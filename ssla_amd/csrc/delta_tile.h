@@ -350,10 +350,10 @@ inline WalkArgs walk_args(const DeltaLayout &L, char *ws, const void *q, const v
   return a;
 }
 
-// Offsets inside `rows` rows, or inside a state, are 32 bits.
+// Offsets inside `rows` rows, or inside a state (of up to 256 padded keys), are 32 bits.
 inline int check_widths(const char *what, int rows, int Hk, int H, int K, int V) {
   if (std::max(static_cast<int64_t>(Hk) * K, static_cast<int64_t>(H) * std::max(K, V)) * rows * 4 > 0x7fffffff ||
-      static_cast<int64_t>(K) * V * 4 > 0x3fffffff) {
+      V > 1 << 20) {
     set_error("%s: rows of %d x %d or %d x %d values are too wide", what, Hk, K, H, V);
     return SSLA_ERR_UNSUPPORTED;
   }

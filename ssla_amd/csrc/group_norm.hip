@@ -556,7 +556,7 @@ NormPlan plan_of(int64_t N, int64_t L, int C, int G, int W, bool bwd) {
   const int per = C / G;
   p.W = W;
   const int64_t nv = L * (per / W);
-  p.lanes = nv <= 64 * (kHold / W);
+  p.lanes = nv <= 64 * (kHold / W) && L * C <= 0x7fffffff;   // (offsets inside a sample are 32 bits there)
   if (p.lanes) {
     p.SG = 1;
     while (p.SG < 64 && p.SG < nv) p.SG *= 2;

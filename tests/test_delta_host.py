@@ -147,10 +147,11 @@ def test_chunk_backward_entry_refuses():
 def test_rows_too_wide_are_refused():
     """Offsets inside a block of rows, or inside a state, are 32 bits."""
     lib = _lib.load()
-    for H, K, V in ((1 << 17, 64, 128), (1, 128, 1 << 22)):
+    for H, K, V in ((1 << 17, 64, 128), (1, 128, 1 << 22), (1, 1, (1 << 20) + 1)):
         assert lib.ssla_gated_delta_chunk_fwd(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None,
                                               None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
         assert lib.ssla_gated_delta_chunk_bwd(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None, None,
                                               None, None, None, None, None, None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
-    assert lib.ssla_gated_delta_recurrent(None, None, None, None, None, 8, 1, 0, 1, 1 << 18, 64, 128, 1.0, None, None, None,
-                                          None, 0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
+    for H, K, V in ((1 << 18, 64, 128), (1, 1, (1 << 20) + 1)):
+        assert lib.ssla_gated_delta_recurrent(None, None, None, None, None, 8, 1, 0, 1, H, K, V, 1.0, None, None, None, None,
+                                              0, None, 0, None) == _lib.SSLA_ERR_UNSUPPORTED

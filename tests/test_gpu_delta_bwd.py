@@ -194,3 +194,37 @@ def test_same_bits_every_time(dev):
     first = gradients(dev, x, s0, cu, 0.125, do, dht)
     for _ in range(3):
         assert all(torch.equal(a, b) for a, b in zip(first, gradients(dev, x, s0, cu, 0.125, do, dht)))
+
+
+def test_training_step_in_a_graph(dev):
+    """Forward and backward of the rule and of the head-wise norm behind it,
+    captured once and replayed on changing inputs with eager steps in between:
+    every replay equals its eager step."""
+    from ssla_amd.delta import chunk_gated_delta
+    from ssla_amd.norm import group_norm_act
+    x, cu, s0 = inputs([500, 90], 1, 2, 64, 32, torch.bfloat16, seed=17)
+    cu, do = cu.to(dev), torch.randn(590, 64).bfloat16().to(dev)
+
+    def step(leaves):
+        o, ht = chunk_gated_delta(*leaves[:5], cu, initial_state=leaves[5], output_final_state=True)
+        y = group_norm_act(o.flatten(1), 2, activation="silu")
+        return y, *torch.autograd.grad((y, ht.sum()), leaves, (do, torch.ones((), device=dev)))
+
+    static = [t.to(dev).requires_grad_() for t in (*x, s0)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(static)
+    for i in range(4):
+        with torch.no_grad():
+            static[2].copy_(x[2] * (1 + i))
+            static[5].copy_(s0 * (1 - i))
+        graph.replay()
+        want = step([t.detach().clone().requires_grad_() for t in static])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
