@@ -60,10 +60,31 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
 
   RowTile<DT, KP> kt;
   kt.fetch(rows_rsrc(k, (t0 * Hk + hk) * K, rows, Hk * K, K, RowTile<DT, KP>::ES), Hk * K, K, vec);
+  // the row factors, while k is on its way: e^-150 is 0 in fp32; sums in 64 bits,
+  // kept as two floats, so that differences of far sums stay exact
   float gv = 0.f, bv = 0.f;
-  if (w == 0 && lane < rows) {
-    gv = g[(t0 + lane) * H + h];
-    bv = beta[(t0 + lane) * H + h];
+  auto factors = [&]() __attribute__((always_inline)) {
+    double G = static_cast<double>(fmaxf(gv, -150.f)) * 1.4426950408889634;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const double up = __shfl_up(G, d);
+      if (lane >= d) G += up;
+    }
+    const float hi = static_cast<float>(G), lo = static_cast<float>(G - static_cast<double>(hi));
+    const float eg = fast_exp2(hi) * fast_exp2(lo), last = __shfl(hi, 63), last_lo = __shfl(lo, 63);
+    sv[kBeta][lane] = bv;
+    sv[kBetaG][lane] = bv * eg;
+    sv[kScaleG][lane] = scale * eg;
+    sv[kToEnd][lane] = fast_exp2((last - hi) + (last_lo - lo));
+    sv[kGHi][lane] = hi;
+    sv[kGLo][lane] = lo;
+  };
+  if (w == 0) {
+    if (lane < rows) {
+      gv = g[(t0 + lane) * H + h];
+      bv = beta[(t0 + lane) * H + h];
+    }
+    factors();
   }
   kt.store(&sk[0][0], kChunk * KP);
   __syncthreads();
@@ -103,26 +124,13 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
     const bool bad = lane < rows && !(finite(diag[lane]) && finite(bv) && gv < 3.38e38f);
     const unsigned long long any = __ballot(bad);
     const int r0 = any ? __ffsll(static_cast<long long>(any)) - 1 : kChunk;
-    if (lane >= r0) {
-      gv = 0.f;
-      bv = lane == r0 ? __builtin_nanf("") : 0.f;
+    if (any) {
+      if (lane >= r0) {
+        gv = 0.f;
+        bv = lane == r0 ? __builtin_nanf("") : 0.f;
+      }
+      factors();
     }
-    // e^-150 is 0 in fp32; sums in 64 bits, kept as two floats, so that
-    // differences of far sums stay exact
-    double G = static_cast<double>(fmaxf(gv, -150.f)) * 1.4426950408889634;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const double up = __shfl_up(G, d);
-      if (lane >= d) G += up;
-    }
-    const float hi = static_cast<float>(G), lo = static_cast<float>(G - static_cast<double>(hi));
-    const float eg = fast_exp2(hi) * fast_exp2(lo), last = __shfl(hi, 63), last_lo = __shfl(lo, 63);
-    sv[kBeta][lane] = bv;
-    sv[kBetaG][lane] = bv * eg;
-    sv[kScaleG][lane] = scale * eg;
-    sv[kToEnd][lane] = fast_exp2((last - hi) + (last_lo - lo));
-    sv[kGHi][lane] = hi;
-    sv[kGLo][lane] = lo;
     diag[lane] = lane < r0 ? bv : 0.f;   // now: beta of the rows that Tm takes
   }
   __syncthreads();

@@ -6,9 +6,10 @@
 // (k . q) u) and S <- e^g S + k u^T, so a token waits on one reduction over
 // the keys, not on two.
 //
-// Sequences: one wavefront per (sequence, head, 16 value columns), lane = (key
-// group of four, column), each with KR state rows in fp32; the value columns of a
-// state are independent of each other.  Tokens are fetched BT at a time with
+// Sequences: one wavefront per (sequence, head, NC value columns), lane = (key
+// group of 64 / NC, column), each with KR state rows in fp32; the value columns of
+// a state are independent of each other.  NC is 16, and 8 (half the instructions
+// a token, twice the wavefronts) for batches that leave SIMDs without one.  Tokens are fetched BT at a time with
 // 16-byte loads while the block before runs, and parked in LDS of the wavefront's
 // own as fp32, with the decays and the products k . q, so a token's chain is the
 // sum S^T k, u and the update.  Bound by issue: about 65 instructions a token and
@@ -53,10 +54,13 @@ __device__ __forceinline__ void lds_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-// Sum over the lanes that share a lane's low four bits (the key groups): lane
-// swaps on the VALU, where a shuffle would be a trip through LDS in every token's
-// chain.  A value swapped with itself gives both partners' values to both.
+// Sum over the lanes of a column (the key groups): lane swaps on the VALU, where a
+// shuffle would be a trip through LDS in every token's chain.  A value swapped
+// with itself gives both partners' values to both.
+template <int NC>
 __device__ __forceinline__ float sum_groups(float x) {
+  if constexpr (NC == 8)
+    x += __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x128, 0xf, 0xf, false));
   const uint32_t b = __float_as_uint(x);
   const auto r = __builtin_amdgcn_permlane16_swap(b, b, false, false);
   const uint32_t y = __float_as_uint(__uint_as_float(r[0]) + __uint_as_float(r[1]));
@@ -119,25 +123,28 @@ struct Rows {
   }
 };
 
-template <int KR, int BT>
+template <int NC, int KR, int BT>
 struct BlockLds {   // one wavefront's
-  float k[BT][4 * KR], q[BT][4 * KR], v[BT][16], gb[BT][4];   // gb: decay, beta, k . q
+  static constexpr int KT = 64 / NC * KR;
+  float k[BT][KT], q[BT][KT], v[BT][NC], gb[BT][4];   // gb: decay, beta, k . q
 };
 
-template <int KR, int BT, int DT>
+template <int NC, int KR, int BT, int DT>
 __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a) {
   typedef typename Elem<DT>::T ET;
   constexpr int ES = sizeof(ET);
-  __shared__ __align__(16) BlockLds<KR, BT> sm[4];
+  typedef BlockLds<NC, KR, BT> Lds;
+  constexpr int KT = Lds::KT;
+  __shared__ __align__(16) Lds sm[4];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  BlockLds<KR, BT> &m = sm[w];
-  const int n_vt = (a.V + 15) >> 4;
+  Lds &m = sm[w];
+  const int n_vt = (a.V + NC - 1) / NC;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + w;
   if (item >= static_cast<int64_t>(a.n_seq) * a.H * n_vt) return;   // whole wavefront
   const int vt = static_cast<int>(item % n_vt), h = static_cast<int>((item / n_vt) % a.H);
   const int64_t n = item / (static_cast<int64_t>(n_vt) * a.H);
-  const int hk = h / (a.H / a.Hk), c0 = vt * 16, nc = min(16, a.V - c0);
-  const int col = lane & 15, kg = lane >> 4;
+  const int hk = h / (a.H / a.Hk), c0 = vt * NC, nc = min(NC, a.V - c0);
+  const int col = lane % NC, kg = lane / NC;
 
   // (clamped to [0, T): no offset addresses memory outside the tensors)
   int64_t bos = n, eos = n + 1;
@@ -163,8 +170,8 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
     for (int i = 0; i < KR; ++i) S[i] = load_one<float>(rs, soff + i * a.V * 4);
   }
 
-  Rows<DT, BT, 4 * KR, 4 * KR> kr, qr;
-  Rows<DT, BT, 16, 16> vr;
+  Rows<DT, BT, KT, KT> kr, qr;
+  Rows<DT, BT, NC, NC> vr;
   float gr = 0.f;
   auto fetch = [&](int64_t t0) __attribute__((always_inline)) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(BT), eos - t0));
@@ -185,11 +192,11 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
     lds_order();
     if (t0 + BT < eos) fetch(t0 + BT);   // the next block's, in flight meanwhile
     {   // k . q of all tokens: four lanes each
-      const int t = lane >> 2, j0 = (lane & 3) * KR;
+      const int t = lane >> 2, j0 = (lane & 3) * (KT / 4);
       float s = 0.f;
       if (t < BT)
 #pragma unroll
-        for (int i = 0; i < KR; ++i) s = fmaf(m.k[t][j0 + i], m.q[t][j0 + i], s);
+        for (int i = 0; i < KT / 4; ++i) s = fmaf(m.k[t][j0 + i], m.q[t][j0 + i], s);
       s += __shfl_xor(s, 1);
       s += __shfl_xor(s, 2);
       if (t < BT && (lane & 3) == 0) m.gb[t][2] = s;
@@ -216,7 +223,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
         p0 = fmaf(qx[i >> 2][i & 3], S[i], p0);
         p1 = fmaf(qx[i >> 2][(i & 3) + 1], S[i + 1], p1);
       }
-      const float eg = gb[0], r = sum_groups(r0 + r1), p = sum_groups(p0 + p1);
+      const float eg = gb[0], r = sum_groups<NC>(r0 + r1), p = sum_groups<NC>(p0 + p1);
       const float u = gb[1] * fmaf(-eg, r, vv);
 #pragma unroll
       for (int i = 0; i < KR; ++i) S[i] = fmaf(kx[i >> 2][i & 3], u, eg * S[i]);
@@ -225,7 +232,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
       if (kg == 0) m.v[t][col] = o;   // o in the place of v
     }
     lds_order();
-    Rows<DT, BT, 16, 16>::put(&m.v[0][0], rows_rsrc(a.o, (t0 * a.H + h) * a.V + c0, rows, vstride, nc, ES), vstride, nc,
+    Rows<DT, BT, NC, NC>::put(&m.v[0][0], rows_rsrc(a.o, (t0 * a.H + h) * a.V + c0, rows, vstride, nc, ES), vstride, nc,
                               a.vvec);
     lds_order();
   }
@@ -242,7 +249,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
 template <int VL, int RPL, int DT>
 __global__ __launch_bounds__(256) void delta_step_kernel(const DeltaArgs a) {
   typedef typename Elem<DT>::T ET;
-  constexpr int KG = 64 / VL, CW = 4 * VL;
+  constexpr int CW = 4 * VL;
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n_vt = (a.V + CW - 1) / CW;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + w;
@@ -347,8 +354,12 @@ int launch_delta(const DeltaArgs &a, hipStream_t st) {
   // single tokens: 16-byte pieces of the states' rows, at most 32 rows a lane
   const int vl = a.V <= 16 ? 4 : a.V <= 32 ? 8 : 16;
   const bool step = a.cu == nullptr && a.V % 4 == 0 && aligned(a.h0, 16) && aligned(a.ht, 16) && (a.K + 64 / vl - 1) / (64 / vl) <= 32;
-  const int64_t tiles = step ? (a.V + 4 * vl - 1) / (4 * vl) : (a.V + 15) / 16;
-  const int64_t blocks = (static_cast<int64_t>(a.n_seq) * a.H * tiles + 3) / 4;
+  // fewer wavefronts than the 1,024 SIMDs: 8 columns each (71 histories of 9,001
+  // tokens, 4 heads of 32: 568 wavefronts of 16 columns 157 us, twice as many of 8 125 us)
+  const int64_t seqs = static_cast<int64_t>(a.n_seq) * a.H;
+  const bool narrow = !step && seqs * ((a.V + 15) / 16) < 1024 && a.V > 8;
+  const int64_t tiles = step ? (a.V + 4 * vl - 1) / (4 * vl) : narrow ? (a.V + 7) / 8 : (a.V + 15) / 16;
+  const int64_t blocks = (seqs * tiles + 3) / 4;
   if (blocks > 0x7fffffff) {
     set_error("gated_delta_recurrent: too many (sequence, head, tile) items");
     return SSLA_ERR_UNSUPPORTED;
@@ -360,7 +371,11 @@ int launch_delta(const DeltaArgs &a, hipStream_t st) {
     else launch_step<16, DT>(a, grid, st);
     return launch_status("gated_delta_recurrent");
   }
-#define SSLA_DELTA(KR_, BT_) hipLaunchKernelGGL((delta_recurrent_kernel<KR_, BT_, DT>), grid, block, 0, st, a)
+#define SSLA_DELTA(KR_, BT_)                                                                                   \
+  do {                                                                                                         \
+    if (narrow) hipLaunchKernelGGL((delta_recurrent_kernel<8, (KR_ > 4 ? KR_ / 2 : 4), BT_, DT>), grid, block, 0, st, a); \
+    else hipLaunchKernelGGL((delta_recurrent_kernel<16, KR_, BT_, DT>), grid, block, 0, st, a);                \
+  } while (0)
   if (a.K <= 16) SSLA_DELTA(4, 16);
   else if (a.K <= 32) SSLA_DELTA(8, 16);
   else if (a.K <= 64) SSLA_DELTA(16, 16);

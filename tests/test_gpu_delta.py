@@ -52,6 +52,21 @@ def test_recurrent(dev, dtype, Hk, H, K, V):
         close(ht, rs, K, max(lens), torch.float32, "ht")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("Hk,H,K,V", [(2, 2, 16, 32), (1, 2, 32, 24), (2, 2, 64, 40), (1, 2, 100, 17), (2, 2, 256, 32)])
+def test_many_sequences(dev, dtype, Hk, H, K, V):
+    """Batches with more than a wavefront of 16 columns for each SIMD (the small
+    ones run 8 columns a wavefront)."""
+    from ssla_amd.delta import fused_recurrent_gated_delta
+    lens = [(7 * n) % 5 for n in range(300)]
+    x, cu, s0 = inputs(lens, Hk, H, K, V, dtype, seed=K)
+    o, ht = fused_recurrent_gated_delta(*(t.to(dev) for t in x), cu.to(dev), initial_state=s0.to(dev),
+                                        output_final_state=True)
+    ro, rs = gated_delta(*x, lens, K ** -0.5, s0)
+    close(o, ro, K, 4, dtype, "o")
+    close(ht, rs, K, 4, torch.float32, "ht")
+
+
 def test_recurrent_edges_of_the_gates(dev):
     """Gates of -inf and 0, writes of weight 0 and 1, 16-bit gates, strided
     inputs, offsets on the host and a scale of its own."""
