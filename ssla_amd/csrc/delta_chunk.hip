@@ -329,13 +329,10 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : MODE == kS
       for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4 *>(&sm.tm[i][tid * 8]) = to_bits(s[i]);
     }
     {   // sets 4, 5: half a lane's values of each thread
-      bf16x8 s[3];
-      split(join(tmr[2], f32x4{0.f, 0.f, 0.f, 0.f}), s);
+      uint2 s[3];
+      split(tmr[2], s);
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        const uint4 x = to_bits(s[i]);
-        *reinterpret_cast<uint2 *>(&sm.tm[i][2048 + tid * 4]) = make_uint2(x.x, x.y);
-      }
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2 *>(&sm.tm[i][2048 + tid * 4]) = s[i];
     }
     if (tid < kRowFloats / 4) reinterpret_cast<f32x4 *>(&sm.rowv[0][0])[tid] = rvr;
   };

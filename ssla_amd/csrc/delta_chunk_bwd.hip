@@ -120,12 +120,10 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
     split(join(tmr[0], tmr[1]), s);   // sets 0 .. 3: a lane's eight values of one thread
 #pragma unroll
     for (int i = 0; i < 3; ++i) *reinterpret_cast<uint4 *>(&sm.tm[i][tid * 8]) = to_bits(s[i]);
-    split(join(tmr[2], f32x4{0.f, 0.f, 0.f, 0.f}), s);   // sets 4, 5: half a lane's values
+    uint2 half[3];
+    split(tmr[2], half);   // sets 4, 5: half a lane's values
 #pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      const uint4 x = to_bits(s[i]);
-      *reinterpret_cast<uint2 *>(&sm.tm[i][2048 + tid * 4]) = make_uint2(x.x, x.y);
-    }
+    for (int i = 0; i < 3; ++i) *reinterpret_cast<uint2 *>(&sm.tm[i][2048 + tid * 4]) = half[i];
     if (tid < kRowFloats / 4) reinterpret_cast<f32x4 *>(&sm.rowv[0][0])[tid] = rvr;
   };
   auto row8 = [&](int vec, int p) __attribute__((always_inline)) {

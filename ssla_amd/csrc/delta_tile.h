@@ -38,11 +38,10 @@ template <int DT> struct Parts { static constexpr int n = DT == SSLA_BF16 ? 1 : 
 // a shift and a mask: the vector conversion back would convert each value anew.)
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
-template <int N>
-__device__ __forceinline__ void split(const f32x8 &x, bf16x8 (&p)[N]) {
-  uint32_t w[N][4];
+template <int N, int P>
+__device__ __forceinline__ void split_pairs(const float (&x)[2 * P], uint32_t (&w)[N][P]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < P; ++j) {
     float a = x[2 * j], b = x[2 * j + 1];
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -53,8 +52,22 @@ __device__ __forceinline__ void split(const f32x8 &x, bf16x8 (&p)[N]) {
       }
     }
   }
+}
+template <int N>
+__device__ __forceinline__ void split(const f32x8 &x, bf16x8 (&p)[N]) {
+  const float v[8] = {x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]};
+  uint32_t w[N][4];
+  split_pairs<N, 4>(v, w);
 #pragma unroll
   for (int i = 0; i < N; ++i) p[i] = from_bits<bf16x8>(make_uint4(w[i][0], w[i][1], w[i][2], w[i][3]));
+}
+template <int N>
+__device__ __forceinline__ void split(const f32x4 &x, uint2 (&p)[N]) {
+  const float v[4] = {x[0], x[1], x[2], x[3]};
+  uint32_t w[N][2];
+  split_pairs<N, 2>(v, w);
+#pragma unroll
+  for (int i = 0; i < N; ++i) p[i] = make_uint2(w[i][0], w[i][1]);
 }
 // Sum over the 16 lanes of a DPP row, in every lane of it.
 __device__ __forceinline__ float row_sum(float x) {
