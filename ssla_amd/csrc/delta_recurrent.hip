@@ -202,34 +202,52 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
       if (t < BT && (lane & 3) == 0) m.gb[t][2] = s;
     }
     lds_order();
-    f32x4 kx[KR / 4], qx[KR / 4], gb;
-    float vv;
-    auto token = [&](int t) __attribute__((always_inline)) {
-      gb = *reinterpret_cast<const f32x4 *>(&m.gb[t][0]);
-      vv = m.v[t][col];
+    struct Token {
+      f32x4 k[KR / 4], q[KR / 4], gb;
+      float v;
+    };
+    auto read = [&](Token &x, int t) __attribute__((always_inline)) {
+      t = min(t, BT - 1);
+      x.gb = *reinterpret_cast<const f32x4 *>(&m.gb[t][0]);
+      x.v = m.v[t][col];
 #pragma unroll
       for (int i = 0; i < KR / 4; ++i) {
-        kx[i] = *reinterpret_cast<const f32x4 *>(&m.k[t][kg * KR + 4 * i]);
-        qx[i] = *reinterpret_cast<const f32x4 *>(&m.q[t][kg * KR + 4 * i]);
+        x.k[i] = *reinterpret_cast<const f32x4 *>(&m.k[t][kg * KR + 4 * i]);
+        x.q[i] = *reinterpret_cast<const f32x4 *>(&m.q[t][kg * KR + 4 * i]);
       }
     };
-    token(0);
-    for (int t = 0; t < rows; ++t) {
+    auto write = [&](const Token &x, int t) __attribute__((always_inline)) {
       float r0 = 0.f, r1 = 0.f, p0 = 0.f, p1 = 0.f;
 #pragma unroll
       for (int i = 0; i < KR; i += 2) {
-        r0 = fmaf(kx[i >> 2][i & 3], S[i], r0);
-        r1 = fmaf(kx[i >> 2][(i & 3) + 1], S[i + 1], r1);
-        p0 = fmaf(qx[i >> 2][i & 3], S[i], p0);
-        p1 = fmaf(qx[i >> 2][(i & 3) + 1], S[i + 1], p1);
+        r0 = fmaf(x.k[i >> 2][i & 3], S[i], r0);
+        r1 = fmaf(x.k[i >> 2][(i & 3) + 1], S[i + 1], r1);
+        p0 = fmaf(x.q[i >> 2][i & 3], S[i], p0);
+        p1 = fmaf(x.q[i >> 2][(i & 3) + 1], S[i + 1], p1);
       }
-      const float eg = gb[0], r = sum_groups<NC>(r0 + r1), p = sum_groups<NC>(p0 + p1);
-      const float u = gb[1] * fmaf(-eg, r, vv);
+      const float eg = x.gb[0], r = sum_groups<NC>(r0 + r1), p = sum_groups<NC>(p0 + p1);
+      const float u = x.gb[1] * fmaf(-eg, r, x.v);
 #pragma unroll
-      for (int i = 0; i < KR; ++i) S[i] = fmaf(kx[i >> 2][i & 3], u, eg * S[i]);
-      const float o = a.scale * fmaf(gb[2], u, eg * p);
-      token(min(t + 1, BT - 1));   // on its way while the sums above finish
-      if (kg == 0) m.v[t][col] = o;   // o in the place of v
+      for (int i = 0; i < KR; ++i) S[i] = fmaf(x.k[i >> 2][i & 3], u, eg * S[i]);
+      if (kg == 0) m.v[t][col] = a.scale * fmaf(x.gb[2], u, eg * p);   // o in the place of v
+    };
+    // a token's values are read while the one before runs (two sets of registers,
+    // where the keys' leave room for them)
+    Token x, y;
+    read(x, 0);
+    if constexpr (KR <= 16) {
+      for (int t = 0; t < rows; t += 2) {
+        read(y, t + 1);
+        write(x, t);
+        if (t + 1 == rows) break;
+        read(x, t + 2);
+        write(y, t + 1);
+      }
+    } else {
+      for (int t = 0; t < rows; ++t) {
+        write(x, t);
+        read(x, t + 1);
+      }
     }
     lds_order();
     Rows<DT, BT, NC, NC>::put(&m.v[0][0], rows_rsrc(a.o, (t0 * a.H + h) * a.V + c0, rows, vstride, nc, ES), vstride, nc,
