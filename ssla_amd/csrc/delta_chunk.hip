@@ -21,6 +21,13 @@
 // initial state, so it needs no M), a fold carries the states over the segments,
 // and the walk starts every segment from its state.
 //
+// Measured at 8 sequences of 4096 rows, 8 heads of 64, bf16: matrices 31 us,
+// segments 63, fold 12, walk 57; 153 a pass among others, 0.9 TB/s of the inputs
+// and outputs.  Bound by latency: a SIMD has two (walk) or three (segments)
+// wavefronts, VALU busy 37 % and matrix cores 20 % of the time; more wavefronts
+// need fewer registers than the states, one operand's parts and the next chunk's
+// loads take.
+//
 // Values that are not finite: a row whose beta, g or k . k is not finite makes all
 // columns of its head NaN from that row on, one in v or in a state its own
 // column; earlier rows are computed without them.

@@ -19,6 +19,9 @@
 // rows i >= t, from rows j < t to the next state, and from state to state.  Row
 // and column sums of the first kind are dot products of the rows of q and k with
 // the pieces of dq and dk, so no second Gram matrix is formed.
+// Measured at 8 sequences of 4096 rows, 8 heads of 64, bf16: reverse segments 56
+// us, fold 15, reverse walk 80, chunk gradients 172 (465 MB, 2.7 TB/s: bound by
+// the loads of u, dX, S and D and their splits, at two wavefronts a SIMD).
 // Shared key heads: every value head's dq and dk in fp32, added in the order of
 // the heads.
 #include "delta_tile.h"

@@ -12,12 +12,13 @@
 // a token, twice the wavefronts) for batches that leave SIMDs without one.  Tokens are fetched BT at a time with
 // 16-byte loads while the block before runs, and parked in LDS of the wavefront's
 // own as fp32, with the decays and the products k . q, so a token's chain is the
-// sum S^T k, u and the update.  Bound by issue: about 65 instructions a token and
-// 16 columns.
+// sum S^T k, u and the update.  Bound by issue (4,510 histories of 13 tokens, 4
+// heads of 32, fp32: 87 us, 3.1 TB/s), long histories by the chain, 0.21 us a token.
 //
 // Single tokens: one wavefront per (row, head, 4 VL value columns), the whole of
 // a state's columns in registers as 16-byte pieces, every load in flight at once.
-// Bound by memory: a state is read and written.
+// Bound by memory: a state is read and written (1,024 rows, 8 heads of 128 x 128:
+// 210 us, 5.1 TB/s).
 #include "delta_tile.h"
 
 namespace ssla {
