@@ -254,8 +254,8 @@ int ssla_gated_delta_recurrent(const void *q, const void *k, const void *v, cons
 /* By chunks of 64 rows, all products on the matrix cores with the precision of
  * fp32 (fp32 values as sums of bf16): K <= 128, any V up to 2^20.  A row whose g,
  * beta or k . k is not finite (a g of -inf is) makes its head's o and state NaN
- * from that row on, one of v its column; earlier rows keep their values.
- * Workspace:
+ * from that row on, one of v its column; earlier rows keep their values.  ht must
+ * not overlap h0.  Workspace:
  * ssla_gated_delta_chunk_workspace_size bytes, 16-byte aligned, no
  * initialisation.  segments (NULL, or ssla_gated_delta_chunk_segments_size bytes,
  * 16-byte aligned) receives the states and maps of the segments that long

@@ -52,6 +52,10 @@ def _shapes(name, q, k, v, g, beta):
     return T, Hk, H, K, V
 
 
+def _f32(t):
+    return (t if t.dtype is torch.float32 else t.float()).contiguous()   # (a .to that does nothing costs as much as a check)
+
+
 def _offsets(name, cu_seqlens, dev):
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
         raise ValueError(f"{name}: cu_seqlens must be integers [N + 1], got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
@@ -67,7 +71,7 @@ def _recurrent(q, k, v, g, beta, cu, n_seq, scale, h0, ht, state_idx=None, statu
     T, Hk, K = q.shape
     H, V = v.shape[1:]
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    g, beta = g.to(torch.float32).contiguous(), beta.to(torch.float32).contiguous()
+    g, beta = _f32(g), _f32(beta)
     o = torch.empty(T, H, V, device=v.device, dtype=v.dtype)
     P = _lib.ptr
     with _lib.on_device_of(q):
@@ -175,7 +179,7 @@ def chunk_gated_delta(
     if initial_state is not None and initial_state.shape != (N, H, K, V):
         raise ValueError(f"{name}: initial_state must be {(N, H, K, V)}, got {tuple(initial_state.shape)}")
     scale = K ** -0.5 if scale is None else float(scale)
-    h0 = None if initial_state is None else initial_state.to(torch.float32).contiguous()
+    h0 = None if initial_state is None else _f32(initial_state)
     grad = torch.is_grad_enabled() and any(
         t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
     if grad and K > 128:
@@ -184,7 +188,7 @@ def chunk_gated_delta(
         ht = torch.empty(N, H, K, V, device=dev, dtype=torch.float32) if output_final_state else None
         return _recurrent(q, k, v, g, beta, cu, N, scale, h0, ht), ht
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
-    g, beta = g.to(torch.float32).contiguous(), beta.to(torch.float32).contiguous()
+    g, beta = _f32(g), _f32(beta)
     if grad:
         return ChunkGatedDeltaFunction.apply(q, k, v, g, beta, h0, cu, scale, output_final_state)
     return _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)[:2]
@@ -213,18 +217,18 @@ def fused_recurrent_gated_delta(
     N = cu.numel() - 1
     if initial_state is not None and initial_state.shape != (N, H, K, V):
         raise ValueError(f"{name}: initial_state must be {(N, H, K, V)}, got {tuple(initial_state.shape)}")
-    h0 = None if initial_state is None else initial_state.to(torch.float32).contiguous()
+    h0 = None if initial_state is None else _f32(initial_state)
     ht = torch.empty(N, H, K, V, device=dev, dtype=torch.float32) if output_final_state else None
     o = _recurrent(q, k, v, g, beta, cu, N, K ** -0.5 if scale is None else scale, h0, ht)
     return o, ht
 
 
-def _sites(name, idx, n, dev):
+def _sites(name, idx, n):
     if idx.shape != (n,) or idx.is_floating_point():
         raise ValueError(f"{name}: the site list must be integers [{n}], got {idx.dtype} {tuple(idx.shape)}")
-    if idx.dtype == torch.int64:   # (kept out of range where 32 bits do not hold it)
+    if idx.dtype is torch.int64:   # (kept out of range where 32 bits do not hold it)
         idx = idx.clamp(-1, 0x7fffffff)
-    return idx.to(device=dev, dtype=torch.int32).contiguous()
+    return (idx if idx.dtype is torch.int32 else idx.to(torch.int32)).contiguous()
 
 
 def sparse_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -245,7 +249,7 @@ def sparse_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     dev = _lib.require_cuda(q, k, v, g, beta, state, seq_site)
     _lib.require_no_grad(name, q, k, v, g, beta, state)
     cu = _offsets(name, cu_seqlens, dev)
-    idx = _sites(name, seq_site, cu.numel() - 1, dev)
+    idx = _sites(name, seq_site, cu.numel() - 1)
     status = _lib.new_status(dev) if check and idx.numel() else None
     o = _recurrent(q, k, v, g, beta, cu, idx.numel(), K ** -0.5 if scale is None else scale, state, state, idx, status)
     if status is not None and _lib.read_status(status) != _lib.SSLA_OK:
@@ -265,7 +269,7 @@ def sparse_delta_step(site_idx: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
     _table(name, state, H, K, V)
     dev = _lib.require_cuda(q, k, v, g, beta, state, site_idx)
     _lib.require_no_grad(name, q, k, v, g, beta, state)
-    idx = _sites(name, site_idx, n, dev)
+    idx = _sites(name, site_idx, n)
     status = _lib.new_status(dev) if check and n else None
     o = _recurrent(q, k, v, g, beta, None, n, K ** -0.5 if scale is None else scale, state, state, idx, status)
     if status is not None and _lib.read_status(status) != _lib.SSLA_OK:

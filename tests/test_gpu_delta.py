@@ -191,3 +191,20 @@ def test_step_in_a_graph_and_on_a_stream(dev):
         want = sparse_delta_step(at, *cur, eager)
         torch.cuda.synchronize()
         assert torch.equal(out, want) and torch.equal(state, eager)
+
+
+@pytest.mark.parametrize("dtype", [torch.int64, torch.int16, torch.uint8])
+def test_site_lists_of_other_integers(dev, dtype):
+    """Site lists of any integer type name the same sites as 32-bit ones."""
+    from ssla_amd.delta import sparse_delta_scan, sparse_delta_step
+    (q, k, v, g, beta), cu, _ = inputs([3, 0, 5], 1, 2, 16, 20, torch.float32, seed=21)
+    x = [t.to(dev) for t in (q, k, v, g, beta)]
+    state = torch.randn(6, 2, 16, 20, generator=torch.Generator().manual_seed(4)).to(dev)
+    at = torch.tensor([0, 2, 5], device=dev)
+    outs = []
+    for t in (torch.int32, dtype):
+        s = state.clone()
+        o = sparse_delta_scan(*x, cu.to(dev), at.to(t), s, check=True)
+        outs.append((o, sparse_delta_step(at.to(t), *(a[:3] for a in x), s, check=True), s))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+    assert not torch.equal(outs[0][2], state)
