@@ -289,6 +289,41 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : 2) void de
 }
 
 // ------------------------------------------------------ the chunks' gradients --
+// 64 rows of 32 columns, four columns for each of 512 threads.
+template <int DT>
+struct ColTile {
+  typedef typename Elem<DT>::T E;
+  static constexpr int ES = sizeof(E);
+  struct Piece { E e[4]; };
+  Piece p;
+
+  __device__ __forceinline__ void fetch(const Rsrc &rs, int thread, int stride, int n_cols, bool vec) {
+    const int row = thread >> 3, col = (thread & 7) * 4;
+    const uint32_t at = static_cast<uint32_t>(row * stride + col) * ES;
+    if (vec) {
+      const uint32_t off = col + 4 <= n_cols ? at : kOutside;
+      if constexpr (ES == 2) p = __builtin_bit_cast(Piece, __builtin_amdgcn_raw_buffer_load_b64(rs, off, 0, 0));
+      else p = __builtin_bit_cast(Piece, load4(rs, off));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p.e[j] = load_one<E>(rs, col + j < n_cols ? at + ES * j : kOutside);
+    }
+  }
+  __device__ __forceinline__ float value(int j) const { return of_elem<DT>(p.e[j]); }
+  // plane j at t + j * stride elements
+  __device__ __forceinline__ void store(uint16_t *t, int stride) const {
+    uint16_t *dst = t + sw<32>(threadIdx.x >> 3, (threadIdx.x & 7) * 4);
+    if constexpr (DT == SSLA_BF16) {
+      *reinterpret_cast<uint2 *>(dst) = __builtin_bit_cast(uint2, p);
+    } else {
+      uint2 w[Parts<DT>::n];
+      split(f32x4{value(0), value(1), value(2), value(3)}, w);
+#pragma unroll
+      for (int j = 0; j < Parts<DT>::n; ++j) *reinterpret_cast<uint2 *>(dst + j * stride) = w[j];
+    }
+  }
+};
+
 template <int DT, int KP>
 struct GradSmem {
   static constexpr int NP = Parts<DT>::n, KR = KP < 64 ? 64 : KP;
@@ -298,25 +333,49 @@ struct GradSmem {
   struct Keys {
     uint16_t q[NP][kChunk * KP], k[NP][kChunk * KP];
   };
+  struct Pass {   // what the rows' wavefronts add to dk
+    f32x4 dk[KP / 16][256];
+  };
   // side by side where two workgroups a CU still fit: q and k then come with the first columns
-  static constexpr bool kApart = sizeof(Values) + sizeof(Keys) <= 76 * 1024;
-  struct Apart { Values v; Keys k; };
-  union Over { Values v; Keys k; };
+  static constexpr bool kApart = std::max(sizeof(Values), sizeof(Pass)) + sizeof(Keys) <= 76 * 1024;
+  union Front { Values v; Pass x; };
+  struct Apart { Front f; Keys k; };
+  struct Behind { Pass x; Keys k; };
+  union Over { Values v; Behind b; };
   std::conditional_t<kApart, Apart, Over> m;
   float rowv[kRowVecs][kChunk];
-  float base[kChunk], to_next[kChunk], dxv[kChunk];
-  float sd[4];
+  float base[2][kChunk], to_next[kChunk], dxv[kChunk], db[kChunk], eg[kChunk];
+  float sd[8];
+  __device__ __forceinline__ Values &values() {
+    if constexpr (kApart) return m.f.v;
+    else return m.v;
+  }
+  __device__ __forceinline__ Keys &keys() {
+    if constexpr (kApart) return m.k;
+    else return m.b.k;
+  }
+  __device__ __forceinline__ Pass &pass() {
+    if constexpr (kApart) return m.f.x;
+    else return m.b.x;
+  }
 };
 
-// One workgroup per (chunk slot, head); wavefront w owns the rows of tile w.
+// One workgroup per (chunk slot, head), two wavefronts per row tile w: one has what
+// the rows i of the tile read (do, dX with S and the rows before: dq), one what the
+// rows j write (u with D and the rows behind: dk, to which the first adds its dN k
+// and dX S^T).
 template <int DT, int KP>
-__global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(const GradArgs ga) {
+__global__ __launch_bounds__(512, KP == 128 ? 2 : 4) void delta_grad_kernel(const GradArgs ga) {
   constexpr int NP = Parts<DT>::n, KT = KP / 16;
   typedef Elem<DT> E;
   typedef typename E::T ET;
   const WalkArgs &a = ga.w;
-  __shared__ __align__(16) GradSmem<DT, KP> sm;
-  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  typedef GradSmem<DT, KP> Smem;
+  __shared__ __align__(16) Smem sm;
+  typename Smem::Values &sv = sm.values();
+  typename Smem::Keys &sk = sm.keys();
+  const int tid = threadIdx.x, lane = tid & 63, w8 = __builtin_amdgcn_readfirstlane(tid >> 6), w = w8 & 3;
+  const bool reads = w8 < 4;
   const int col = lane & 15, G = lane >> 4;
   const int h = static_cast<int>(blockIdx.x % a.H), hk = h / (a.H / a.Hk);
   const int64_t slot = blockIdx.x / a.H;
@@ -332,116 +391,66 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
   const int vrow = a.H * a.V;
   constexpr int ES = sizeof(ET);
 
-  f32x4 Z[KT], Y[KT], W[KT], C1[4], C2[4], C3[4], C4[4];
   const f32x4 zero = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < KT; ++i) Z[i] = Y[i] = W[i] = zero;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) C1[i] = C2[i] = C3[i] = C4[i] = zero;
   float dxv = 0.f, sd = 0.f;
   const int pair = w >> 1;
-  auto keys = [&]() __attribute__((always_inline)) {
+  auto keys = [&]() __attribute__((always_inline)) {   // the first four wavefronts q, the others k
     RowTile<DT, KP> x;
     const int64_t at = (t0 * a.Hk + hk) * a.K;
     const int stride = a.Hk * a.K;
-    x.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
-    x.store(&sm.m.k.q[0][0], kChunk * KP);
-    x.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
-    x.store(&sm.m.k.k[0][0], kChunk * KP);
+    x.fetch(rows_rsrc(reads ? a.q : a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
+    x.store(reads ? &sk.q[0][0] : &sk.k[0][0], kChunk * KP);
   };
   if (tid < kRowFloats / 4)
     reinterpret_cast<f32x4 *>(&sm.rowv[0][0])[tid] =
         reinterpret_cast<const f32x4 *>(a.rowv + (slot * a.H + h) * kRowFloats)[tid];
-  if (GradSmem<DT, KP>::kApart) keys();
+  if (Smem::kApart) keys();
   // 32 value columns: the values' rows, and the states' (64 keys a tile)
-  constexpr int KH = (KP + 63) / 64, KR = GradSmem<DT, KP>::KR;
-  RowTile<DT, 32> dt, vt;
-  RowTile<SSLA_F32, 32> ut, xt, st[KH], gt[KH];
-  auto fetch = [&](int c0) __attribute__((always_inline)) {   // (columns past V: resources of no bytes)
-    const int nc = a.V - c0, nr = nc > 0 ? rows : 0;
-    dt.fetch(rows_rsrc(ga.dout, vat + c0, nr, vrow, nc, ES), vrow, nc, ga.dvec);
-    vt.fetch(rows_rsrc(a.v, vat + c0, nr, vrow, nc, ES), vrow, nc, ga.dvec);
-    ut.fetch(rows_rsrc(a.u, vat + c0, nr, vrow, nc, 4), vrow, nc, ga.vvec);
-    xt.fetch(rows_rsrc(ga.dx, vat + c0, nr, vrow, nc, 4), vrow, nc, ga.vvec);
+  constexpr int KH = (KP + 63) / 64, KR = Smem::KR;
+  auto columns = [&](int c0) __attribute__((always_inline)) {
+    const int nc = a.V - c0;
+    int thread = tid;   // (taken anew: offsets kept over the loop would cost a wavefront's registers)
+    asm volatile("" : "+v"(thread));
+    ColTile<DT> dt, vt;
+    ColTile<SSLA_F32> ut, xt, st[KH], gt[KH];
+    dt.fetch(rows_rsrc(ga.dout, vat + c0, rows, vrow, nc, ES), thread, vrow, nc, ga.dvec);
+    vt.fetch(rows_rsrc(a.v, vat + c0, rows, vrow, nc, ES), thread, vrow, nc, ga.dvec);
+    ut.fetch(rows_rsrc(a.u, vat + c0, rows, vrow, nc, 4), thread, vrow, nc, ga.vvec);
+    xt.fetch(rows_rsrc(ga.dx, vat + c0, rows, vrow, nc, 4), thread, vrow, nc, ga.vvec);
 #pragma unroll
     for (int i = 0; i < KH; ++i) {
       const int64_t at = static_cast<int64_t>(64 * i) * a.V + c0;
-      const int nk = nc > 0 ? a.K - 64 * i : 0;
-      st[i].fetch(rows_rsrc(Sp, at, nk, a.V, nc, 4), a.V, nc, ga.vvec);
-      gt[i].fetch(rows_rsrc(Dp, at, nk, a.V, nc, 4), a.V, nc, ga.vvec);
+      st[i].fetch(rows_rsrc(Sp, at, a.K - 64 * i, a.V, nc, 4), thread, a.V, nc, ga.vvec);
+      gt[i].fetch(rows_rsrc(Dp, at, a.K - 64 * i, a.V, nc, 4), thread, a.V, nc, ga.vvec);
     }
-  };
-  // (the next columns in flight: where the parts of fp32 inputs leave registers for them)
-  constexpr bool kAhead = NP == 1 || KP == 128;
-  if (kAhead) fetch(0);
-  for (int c0 = 0; c0 < a.V; c0 += 32) {
-    if (!kAhead) fetch(c0);
-    dt.store(&sm.m.v.dout[0][0], kChunk * 32);
-    ut.store(&sm.m.v.u[0][0], kChunk * 32);
-    xt.store(&sm.m.v.dx[0][0], kChunk * 32);
+    __syncthreads();   // the columns before are read
+    dt.store(&sv.dout[0][0], kChunk * 32);
+    ut.store(&sv.u[0][0], kChunk * 32);
+    xt.store(&sv.dx[0][0], kChunk * 32);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dxv = fmaf(vt.value(0, j), xt.value(0, j), dxv);
+    for (int j = 0; j < 4; ++j) dxv = fmaf(vt.value(j), xt.value(j), dxv);
 #pragma unroll
     for (int i = 0; i < KH; ++i) {
-      st[i].store(&sm.m.v.S[0][64 * i * 32], KR * 32);
-      gt[i].store(&sm.m.v.D[0][64 * i * 32], KR * 32);
+      st[i].store(&sv.S[0][64 * i * 32], KR * 32);
+      gt[i].store(&sv.D[0][64 * i * 32], KR * 32);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sd = fmaf(st[i].value(0, j), gt[i].value(0, j), sd);
-    }
-    if (kAhead) fetch(c0 + 32);
-    __syncthreads();
-    bf16x8 od[NP], ou[3], ox[3];   // this wavefront's rows of do, u, dX
-#pragma unroll
-    for (int i = 0; i < NP; ++i) od[i] = op_rows<32>(sm.m.v.dout[i], w, 0, lane);
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-      ou[i] = op_rows<32>(sm.m.v.u[i], w, 0, lane);
-      ox[i] = op_rows<32>(sm.m.v.dx[i], w, 0, lane);
-    }
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      bf16x8 s[3];
-#pragma unroll
-      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.m.v.S[i], t, 0, lane);
-      Z[t] = mul<2>(od, s, Z[t]);
-      Y[t] = mul<2>(ox, s, Y[t]);
-#pragma unroll
-      for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sm.m.v.D[i], t, 0, lane);
-      W[t] = mul<2>(ou, s, W[t]);
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      if ((t >> 1) <= pair) {   // rows j <= i: u do^T, u dX^T
-        bf16x8 x[3];
-#pragma unroll
-        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.m.v.u[i], t, 0, lane);
-        C1[t] = mul<2>(x, od, C1[t]);
-        C2[t] = mul<2>(x, ox, C2[t]);
-      }
-      if ((t >> 1) >= pair) {   // rows i >= j: do u^T, dX u^T
-        bf16x8 x[3], y[NP];
-#pragma unroll
-        for (int i = 0; i < NP; ++i) y[i] = op_rows<32>(sm.m.v.dout[i], t, 0, lane);
-        C3[t] = mul<2>(y, ou, C3[t]);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sm.m.v.dx[i], t, 0, lane);
-        C4[t] = mul<2>(x, ou, C4[t]);
-      }
+      for (int j = 0; j < 4; ++j) sd = fmaf(st[i].value(j), gt[i].value(j), sd);
     }
     __syncthreads();
-  }
-
-  {
-    if (!GradSmem<DT, KP>::kApart) keys();
+  };
+  auto behind_columns = [&]() __attribute__((always_inline)) {
+    __syncthreads();   // the last columns are read
+    if (!Smem::kApart) keys();
     dxv += __shfl_xor(dxv, 1);
     dxv += __shfl_xor(dxv, 2);
-    if ((tid & 3) == 0) sm.dxv[tid >> 2] = dxv;
+    dxv += __shfl_xor(dxv, 4);
+    if ((tid & 7) == 0) sm.dxv[tid >> 3] = dxv;
 #pragma unroll
     for (int d = 32; d; d >>= 1) sd += __shfl_xor(sd, d);
-    if (lane == 0) sm.sd[w] = sd;
-  }
-  __syncthreads();
-
+    if (lane == 0) sm.sd[w8] = sd;
+    if (w8 == 7) sm.eg[lane] = fast_exp2(sm.rowv[kGHi][lane]) * fast_exp2(sm.rowv[kGLo][lane]);
+    __syncthreads();
+  };
   auto row8 = [&](int vec, int p) __attribute__((always_inline)) {
     const f32x4 *s = reinterpret_cast<const f32x4 *>(&sm.rowv[vec][32 * p + 8 * G]);
     return join(s[0], s[1]);
@@ -449,10 +458,11 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
   const bool part = ga.dq_part != nullptr;   // every value head's in fp32
   const int krow = (part ? a.H : a.Hk) * a.K, GS = part ? 4 : ES;
   const int64_t kat = part ? (t0 * a.H + h) * a.K : (t0 * a.Hk + hk) * a.K;
-  const Rsrc rq = rows_rsrc(part ? static_cast<const void *>(ga.dq_part) : ga.dq, kat, rows, krow, a.K, GS);
-  const Rsrc rk = rows_rsrc(part ? static_cast<const void *>(ga.dk_part) : ga.dk, kat, rows, krow, a.K, GS);
+  const Rsrc rs = rows_rsrc(reads ? (part ? static_cast<const void *>(ga.dq_part) : ga.dq)
+                                  : (part ? static_cast<const void *>(ga.dk_part) : ga.dk),
+                            kat, rows, krow, a.K, GS);
   const int row0 = idx_of(w, 4 * G), me = idx_of(w, col);   // own rows row0 .. + 3 in accumulators, own row in operands
-  auto put = [&](const Rsrc &rs, int t, const f32x4 &x) __attribute__((always_inline)) {
+  auto put = [&](int t, const f32x4 &x) __attribute__((always_inline)) {
     const int key = idx_of(t, col);
     const uint32_t off = key < a.K ? static_cast<uint32_t>(row0 * krow + key) * GS : kOutside;
 #pragma unroll
@@ -473,67 +483,155 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
     }
     return y;
   };
-  const f32x4 sg = *reinterpret_cast<const f32x4 *>(&sm.rowv[kScaleG][row0]);
-  const f32x4 bt4 = *reinterpret_cast<const f32x4 *>(&sm.rowv[kBeta][row0]);
-  const f32x4 bg = *reinterpret_cast<const f32x4 *>(&sm.rowv[kBetaG][row0]);
-  const f32x4 te = *reinterpret_cast<const f32x4 *>(&sm.rowv[kToEnd][row0]);
-  const float mhi = sm.rowv[kGHi][me], mlo = sm.rowv[kGLo][me];
-  // per own row: q . (from the state), q . (dP k), k . (dP^T q), k . (dN k),
-  // k . ((beta dN)^T k), k . (dX S^T), k . (u D^T)
-  f32x4 qa = zero, qb = zero, kc = zero, kd = zero, ke = zero, ky = zero, kw = zero;
-  {
-    // dP, dN with this wavefront's rows i in the lanes (contraction j <= i)
-    bf16x8 pA[2][3], nA[2][3];
+  // (each kind of wavefronts runs its own loop, with as many barriers as the other's)
+  if (reads) {
+    f32x4 A1[KT], A2[KT], C1[4], C2[4];   // do S^T, dX S^T; u do^T, u dX^T of the row tiles up to the own one's pair
+#pragma unroll
+    for (int i = 0; i < KT; ++i) A1[i] = A2[i] = zero;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) C1[i] = C2[i] = zero;
+    for (int c0 = 0; c0 < a.V; c0 += 32) {
+      columns(c0);
+      bf16x8 od[NP], ox[3];   // this wavefront's rows of do, dX
+#pragma unroll
+      for (int i = 0; i < NP; ++i) od[i] = op_rows<32>(sv.dout[i], w, 0, lane);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) ox[i] = op_rows<32>(sv.dx[i], w, 0, lane);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        bf16x8 s[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sv.S[i], t, 0, lane);
+        A1[t] = mul<2>(od, s, A1[t]);
+        A2[t] = mul<2>(ox, s, A2[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if ((t >> 1) > pair) continue;
+        bf16x8 x[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sv.u[i], t, 0, lane);
+        C1[t] = mul<2>(x, od, C1[t]);
+        C2[t] = mul<2>(x, ox, C2[t]);
+      }
+    }
+    behind_columns();
+    const f32x4 bt4 = *reinterpret_cast<const f32x4 *>(&sm.rowv[kBeta][row0]);
+    const float mhi = sm.rowv[kGHi][me], mlo = sm.rowv[kGLo][me];
+    // dP, dN with this wavefront's rows i in the lanes (contraction j <= i), one
+    // after the other: parts of both would take more registers than there are
+    f32x8 n1[2];
+    bf16x8 p[2][3];
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
+      if (ks > pair) continue;
       const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks);
-      f32x8 p1 = join(C1[2 * ks], C1[2 * ks + 1]), n1 = join(C2[2 * ks], C2[2 * ks + 1]);
+      f32x8 p1 = join(C1[2 * ks], C1[2 * ks + 1]);
+      n1[ks] = join(C2[2 * ks], C2[2 * ks + 1]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = 32 * ks + 8 * G + j;
         const float e = fast_exp2((mhi - ghi[j]) + (mlo - glo[j]));
         p1[j] = keep(r <= me, a.scale * p1[j] * e);
-        n1[j] = keep(r < me, -n1[j] * e);
+        n1[ks][j] = keep(r < me, -n1[ks][j] * e);
       }
-      split(p1, pA[ks]);
-      split(n1, nA[ks]);
+      split(p1, p[ks]);
+    }
+    // per own row: q . dq, k . (dN k), k . (dX S^T)
+    f32x4 qa = zero, kd = zero, ky = zero;
+    {
+      const f32x4 sg = *reinterpret_cast<const f32x4 *>(&sm.rowv[kScaleG][row0]);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        f32x4 b = zero, qv = zero;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          if (ks > pair) continue;
+          bf16x8 x[NP];
+#pragma unroll
+          for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sk.k[i], t, ks, lane);
+          b = mul<2>(p[ks], x, b);
+          if (ks == pair) {
+#pragma unroll
+            for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sk.q[i], t, ks, lane);
+            qv = own(x);
+          }
+        }
+        b += sg * A1[t];
+        qa += qv * b;
+        put(t, b);
+      }
     }
 #pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+      if (ks <= pair) split(n1[ks], p[ks]);
+    const f32x4 bg = *reinterpret_cast<const f32x4 *>(&sm.rowv[kBetaG][row0]);
+#pragma unroll
     for (int t = 0; t < KT; ++t) {
-      f32x4 b = zero, d = zero, kv = zero, qv = zero;
+      f32x4 d = zero, kv = zero;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         if (ks > pair) continue;
         bf16x8 x[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.k[i], t, ks, lane);
-        b = mul<2>(pA[ks], x, b);
-        d = mul<2>(nA[ks], x, d);
-        if (ks == pair) {
-          kv = own(x);
-#pragma unroll
-          for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.q[i], t, ks, lane);
-          qv = own(x);
-        }
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sk.k[i], t, ks, lane);
+        d = mul<2>(p[ks], x, d);
+        if (ks == pair) kv = own(x);
       }
-      const f32x4 ia = sg * Z[t], hw = te * W[t];
-      qa += qv * ia;
-      qb += qv * b;
       kd += kv * d;
-      ky += kv * Y[t];
-      kw += kv * hw;
-      put(rq, t, ia + b);
-      Z[t] = kv;                             // (from here on: the own rows of k)
-      Y[t] = bt4 * d + (hw - bg * Y[t]);     // (from here on: what dk has so far)
+      ky += kv * A2[t];
+      sm.pass().dk[t][tid] = bt4 * d - bg * A2[t];
     }
-  }
-  {
-    // their transposes with the own rows j in the lanes (contraction i >= j)
-    bf16x8 pT[2][3], nT[2][3];
+    const f32x4 eg = *reinterpret_cast<const f32x4 *>(&sm.eg[row0]);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {   // the keys' sums, of what the row needs
+      const float base = row_sum((qa[r] - bg[r] * ky[r]) + bt4[r] * kd[r]);
+      const float db = row_sum(fmaf(-eg[r], ky[r], kd[r]));
+      if (col == 0) {
+        sm.base[0][row0 + r] = base;
+        sm.db[row0 + r] = db;
+      }
+    }
+    __syncthreads();
+  } else {
+    f32x4 A1[KT], C1[4], C2[4];   // u D^T; do u^T, dX u^T of the row tiles from the own one's pair on
+#pragma unroll
+    for (int i = 0; i < KT; ++i) A1[i] = zero;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) C1[i] = C2[i] = zero;
+    for (int c0 = 0; c0 < a.V; c0 += 32) {
+      columns(c0);
+      bf16x8 ou[3];   // this wavefront's rows of u
+#pragma unroll
+      for (int i = 0; i < 3; ++i) ou[i] = op_rows<32>(sv.u[i], w, 0, lane);
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        bf16x8 s[3];
+#pragma unroll
+        for (int i = 0; i < 3; ++i) s[i] = op_rows<32>(sv.D[i], t, 0, lane);
+        A1[t] = mul<2>(ou, s, A1[t]);
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        if ((t >> 1) < pair) continue;
+        bf16x8 x[3], y[NP];
+#pragma unroll
+        for (int i = 0; i < NP; ++i) y[i] = op_rows<32>(sv.dout[i], t, 0, lane);
+        C1[t] = mul<2>(y, ou, C1[t]);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) x[i] = op_rows<32>(sv.dx[i], t, 0, lane);
+        C2[t] = mul<2>(x, ou, C2[t]);
+      }
+    }
+    behind_columns();
+    const float mhi = sm.rowv[kGHi][me], mlo = sm.rowv[kGLo][me];
+    bf16x8 p[2][3], m[2][3];
+    // dP^T, dN^T with the own rows j in the lanes (contraction i >= j)
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
+      if (ks < pair) continue;
       const f32x8 ghi = row8(kGHi, ks), glo = row8(kGLo, ks), bt = row8(kBeta, ks);
-      f32x8 p2 = join(C3[2 * ks], C3[2 * ks + 1]), n2 = join(C4[2 * ks], C4[2 * ks + 1]);
+      f32x8 p2 = join(C1[2 * ks], C1[2 * ks + 1]), n2 = join(C2[2 * ks], C2[2 * ks + 1]);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int r = 32 * ks + 8 * G + j;
@@ -541,44 +639,48 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
         p2[j] = keep(r >= me, a.scale * p2[j] * e);
         n2[j] = keep(r > me, -bt[j] * n2[j] * e);
       }
-      split(p2, pT[ks]);
-      split(n2, nT[ks]);
+      split(p2, p[ks]);
+      split(n2, m[ks]);
     }
+    const f32x4 te = *reinterpret_cast<const f32x4 *>(&sm.rowv[kToEnd][row0]);
+    // per own row: k . (dP^T q + (beta dN)^T k), k . (u D^T)
+    f32x4 kc = zero, kw = zero;
 #pragma unroll
     for (int t = 0; t < KT; ++t) {
-      f32x4 c = zero, e = zero;
+      f32x4 c = zero, e = zero, kv = zero;
 #pragma unroll
       for (int ks = 0; ks < 2; ++ks) {
         if (ks < pair) continue;
         bf16x8 x[NP];
 #pragma unroll
-        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.k[i], t, ks, lane);
-        e = mul<2>(nT[ks], x, e);
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sk.k[i], t, ks, lane);
+        e = mul<2>(m[ks], x, e);
+        if (ks == pair) kv = own(x);
 #pragma unroll
-        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sm.m.k.q[i], t, ks, lane);
-        c = mul<2>(pT[ks], x, c);
+        for (int i = 0; i < NP; ++i) x[i] = op_cols<KP>(sk.q[i], t, ks, lane);
+        c = mul<2>(p[ks], x, c);
       }
-      kc += Z[t] * c;
-      ke += Z[t] * e;
-      put(rk, t, Y[t] + (c + e));
+      const f32x4 hw = te * A1[t];
+      c += e;
+      kc += kv * c;
+      kw += kv * hw;
+      A1[t] = hw + c;
     }
-  }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {   // the keys' sums, of what the row needs
-    const int i = row0 + r;
-    const float eg = fast_exp2(sm.rowv[kGHi][i]) * fast_exp2(sm.rowv[kGLo][i]);
-    const float base = row_sum((qa[r] - bg[r] * ky[r]) + ((qb[r] - kc[r]) + (bt4[r] * kd[r] - ke[r])));
-    const float next = row_sum(kw[r]), db = row_sum(fmaf(-eg, ky[r], kd[r]));
-    if (col == 0) {
-      sm.base[i] = base;
-      sm.to_next[i] = next;
-      if (i < rows) ga.dbeta[(t0 + i) * a.H + h] = sm.dxv[i] + db;
+    for (int r = 0; r < 4; ++r) {
+      const float base = row_sum(-kc[r]), next = row_sum(kw[r]);
+      if (col == 0) {
+        sm.base[1][row0 + r] = base;
+        sm.to_next[row0 + r] = next;
+      }
     }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < KT; ++t) put(t, sm.pass().dk[t][tid - 256] + A1[t]);
   }
-  __syncthreads();
-  if (w == 0) {
+  if (w8 == 0) {
     // dg_t = sum_(i >= t) base_i + sum_(j < t) to_next_j + e^(G_last) <S, D>
-    float s = sm.base[lane], p = sm.to_next[lane];
+    float s = sm.base[0][lane] + sm.base[1][lane], p = sm.to_next[lane];
     const float mine = p;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -586,9 +688,13 @@ __global__ __launch_bounds__(256, KP == 128 ? 1 : 2) void delta_grad_kernel(cons
       if (lane + d < 64) s += down;
       if (lane >= d) p += up;
     }
-    const float through = fast_exp2(sm.rowv[kGHi][kChunk - 1]) * fast_exp2(sm.rowv[kGLo][kChunk - 1]);
-    const float sdt = (sm.sd[0] + sm.sd[1]) + (sm.sd[2] + sm.sd[3]);
-    if (lane < rows) ga.dg[(t0 + lane) * a.H + h] = s + fmaf(through, sdt, p - mine);
+    float sdt = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sdt += sm.sd[i];
+    if (lane < rows) {
+      ga.dg[(t0 + lane) * a.H + h] = s + fmaf(sm.eg[kChunk - 1], sdt, p - mine);
+      ga.dbeta[(t0 + lane) * a.H + h] = sm.dxv[lane] + sm.db[lane];
+    }
   }
 }
 
@@ -646,7 +752,7 @@ int launch_bwd(const DeltaLayout &L, const GradArgs &ga, hipStream_t st) {
     if (const int e = delta_fold(L, a, ga.seg_grad, true, st)) return e;
   }
   hipLaunchKernelGGL((delta_reverse_kernel<DT, KP, false>), grid_of(L.seg_slots * a.H * vg), block, 0, st, ga);
-  hipLaunchKernelGGL((delta_grad_kernel<DT, KP>), grid_of(L.chunk_slots * a.H), block, 0, st, ga);
+  hipLaunchKernelGGL((delta_grad_kernel<DT, KP>), grid_of(L.chunk_slots * a.H), dim3(512), 0, st, ga);
   return launch_status("gated_delta_chunk_bwd");
 }
 

@@ -172,7 +172,7 @@ __device__ __forceinline__ float of_elem(typename Elem<DT>::T x) {
 }
 
 // 64 rows of a matrix with row stride `stride` (values), fetched into registers
-// by 256 threads and stored to LDS as Parts<DT>::n tiles of bf16; rows past the
+// by 256 threads (or once by each 256 of them) and stored to LDS as Parts<DT>::n tiles of bf16; rows past the
 // resource and columns from n_cols on are zero.  Where rows are whole 16-byte
 // pieces at aligned addresses (vec) they are read 16 bytes at a time.
 template <int DT, int KP>
@@ -186,7 +186,7 @@ struct RowTile {
   __device__ __forceinline__ void fetch(const Rsrc &rs, int stride, int n_cols, bool vec) {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = threadIdx.x + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
+      const int u = (threadIdx.x & 255) + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
       const uint32_t at = static_cast<uint32_t>(row * stride + col) * ES;
       if (vec) {
         struct Raw { uint4 w[W]; } raw;
@@ -206,7 +206,7 @@ struct RowTile {
   __device__ __forceinline__ void store(uint16_t *t, int stride) const {
 #pragma unroll
     for (int i = 0; i < U; ++i) {
-      const int u = threadIdx.x + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
+      const int u = (threadIdx.x & 255) + 256 * i, row = u / (KP / 8), col = (u % (KP / 8)) * 8;
       uint16_t *dst = t + sw<KP>(row, col);
       if constexpr (DT == SSLA_BF16) {
         *reinterpret_cast<uint4 *>(dst) = __builtin_bit_cast(uint4, p[i]);
