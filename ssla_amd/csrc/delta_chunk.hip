@@ -553,13 +553,151 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : MODE == kS
   }
 }
 
-// The fold (see delta_fold): one workgroup per (sequence, head, 64 columns), a
-// segment after the other.  A segment's M is staged in LDS for the four
-// wavefronts, read by rows or (REV: M^T) by columns; the next one is in flight.
-template <int KP, bool REV>
-__global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restrict__ cu, int64_t T, int H, int K, int V,
-                                                         int per, const uint16_t *__restrict__ seg_map,
-                                                         float *__restrict__ states) {
+// The fold (see delta_fold): one workgroup per (sequence, head, 16 columns), a
+// segment after the other, in lane order what the walk has: a wavefront owns one or
+// two of the state's key tiles, reads its rows of M as operands from memory, kept
+// kAhead segments in flight, and passes its keys' parts to the others through LDS
+// (two buffers: one barrier a segment).  The chain of a segment is then twelve
+// matrix instructions, a split and the pass.
+template <int KP>
+struct FoldSize {
+  static constexpr int NT = KP / 16, WAVES = NT < 4 ? NT : 4, TPW = NT / WAVES, KS = KP / 32;
+  static constexpr int kAhead = KP == 128 ? 2 : 4;
+};
+template <int KP>
+__global__ __launch_bounds__(64 * FoldSize<KP>::WAVES) void delta_fold_kernel(
+    const int64_t *__restrict__ cu, int n_seq, int64_t T, int H, int K, int V, int per,
+    const uint16_t *__restrict__ seg_map, float *__restrict__ states) {
+  typedef FoldSize<KP> F;
+  constexpr int PLANE = KP * KP, D = F::kAhead;
+  __shared__ __align__(16) uint2 parts[2][F::KS][3][64][2];
+  const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, G = lane >> 4;
+  // (a sequence and head's columns are a multiple of 8 workgroups apart: on one die,
+  // whose L2 then holds M for all of them)
+  const int units = n_seq * H, apart = (units + 7) & ~7, u = static_cast<int>(blockIdx.x % apart);
+  if (u >= units) return;
+  const int vcol = static_cast<int>(blockIdx.x / apart) * 16 + col, h = u % H, n = u / H;
+  const int64_t bos = min(max(cu[n], (int64_t)0), T), eos = min(max(cu[n + 1], bos), T);
+  const int64_t unit = static_cast<int64_t>(per) * kChunk, KV = static_cast<int64_t>(K) * V;
+  const int inner = static_cast<int>((eos - bos + unit - 1) / unit) - 1;   // segments but the last
+  if (inner < 2) return;   // the only state is there already
+  const StateCols<F::NT> cols(K, V, vcol, vcol < V, G);
+  struct Step {
+    bf16x8 m[F::TPW][F::KS][3];
+    f32x4 L[F::TPW];
+  };
+  Step ahead[D];
+  f32x4 S[F::TPW];
+  // pointers that move on by a segment: with one wavefront a SIMD, what a step costs
+  // is its instructions, of which addresses from a segment's number were a third
+  const int64_t first = (bos / unit) * H + h, ds = H * KV, dm = static_cast<int64_t>(H) * (3 * PLANE);
+  float *out = states + first * KV;
+  const float *in = out;
+  const uint16_t *map = seg_map + first * (3 * PLANE);
+  uint32_t moff[F::TPW], soff[F::TPW][4];
+#pragma unroll
+  for (int t = 0; t < F::TPW; ++t) {
+    moff[t] = (idx_of(w * F::TPW + t, col) * KP + 8 * G) * 2;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) soff[t][i] = cols.off + idx_of(w * F::TPW + t, i) * cols.V4;
+  }
+  auto state = [&](f32x4 (&x)[F::TPW]) __attribute__((always_inline)) {
+    const Rsrc r = cols.rs(in);
+#pragma unroll
+    for (int t = 0; t < F::TPW; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[t][i] = load_one<float>(r, soff[t][i]);
+  };
+  int next = 0;   // the segment that is fetched next
+  auto fetch = [&](Step &x) __attribute__((always_inline)) {
+    const bool on = ++next < inner;   // (past the end: the last one again)
+    map += on ? dm : 0;
+    in += on ? ds : 0;
+    const Rsrc r = rsrc_of(map, 3 * PLANE * 2);
+#pragma unroll
+    for (int t = 0; t < F::TPW; ++t)
+#pragma unroll
+      for (int p = 0; p < 3; ++p)
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ++ks)
+          x.m[t][ks][p] = from_bits<bf16x8>(__builtin_bit_cast(
+              uint4, __builtin_amdgcn_raw_buffer_load_b128(r, moff[t] + 64 * ks, p * PLANE * 2, 0)));
+    state(x.L);
+  };
+  state(S);
+#pragma unroll
+  for (int d = 0; d + 1 < D; ++d) fetch(ahead[d]);
+  // a segment; meanwhile a later one goes into the operands that the one before had
+  auto step = [&](int parity, const Step &x, auto ahead_of) __attribute__((always_inline)) {
+    auto &buf = parts[parity];
+#pragma unroll
+    for (int t = 0; t < F::TPW; ++t) {
+      const int tile = w * F::TPW + t;
+      uint2 s[3];
+      split(S[t], s);
+#pragma unroll
+      for (int p = 0; p < 3; ++p) buf[tile >> 1][p][lane][tile & 1] = s[p];
+    }
+    __syncthreads();
+    ahead_of();
+    // (a chain of products for each 32 keys, step by step side by side)
+    bf16x8 s[F::KS][3];
+    f32x4 c[F::TPW][F::KS];
+#pragma unroll
+    for (int ks = 0; ks < F::KS; ++ks) {
+#pragma unroll
+      for (int p = 0; p < 3; ++p) s[ks][p] = from_bits<bf16x8>(*reinterpret_cast<const uint4 *>(&buf[ks][p][lane][0]));
+#pragma unroll
+      for (int t = 0; t < F::TPW; ++t) c[t][ks] = ks ? f32x4{0.f, 0.f, 0.f, 0.f} : x.L[t];
+    }
+#pragma unroll
+    for (int o = 2; o >= 0; --o)
+#pragma unroll
+      for (int i = 0; i <= o; ++i)
+#pragma unroll
+        for (int ks = 0; ks < F::KS; ++ks)
+#pragma unroll
+          for (int t = 0; t < F::TPW; ++t)
+            c[t][ks] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.m[t][ks][i], s[ks][o - i], c[t][ks], 0, 0, 0);
+#pragma unroll
+    for (int t = 0; t < F::TPW; ++t) {
+      if constexpr (F::KS == 1) S[t] = c[t][0];
+      else if constexpr (F::KS == 2) S[t] = c[t][0] + c[t][1];
+      else S[t] = (c[t][0] + c[t][1]) + (c[t][2] + c[t][3]);
+    }
+    // (a load behind each product: in one piece they would hold up the chain)
+    __builtin_amdgcn_sched_group_barrier(0x100, 3 * F::KS, 0);
+#pragma unroll
+    for (int i = 0; i < 6 * F::KS * F::TPW; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    }
+    out += ds;
+    const Rsrc r = cols.rs(out);
+#pragma unroll
+    for (int t = 0; t < F::TPW; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) store_one<float>(r, soff[t][i], S[t][i]);
+  };
+  static_assert(D % 2 == 0, "a step's buffer is known");
+  int j = 1;
+  for (; j + D <= inner; j += D) {   // (no way out inside: the loads' order stays known)
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      step((d + 1) & 1, ahead[d], [&]() __attribute__((always_inline)) { fetch(ahead[(d + D - 1) % D]); });
+  }
+#pragma unroll
+  for (int d = 0; d + 1 < D; ++d)
+    if (j + d < inner) step((d + 1) & 1, ahead[d], []() {});
+}
+
+// The fold in reverse, with M^T: one workgroup per (sequence, head, 64 columns).  A
+// segment's M is staged in LDS for the four wavefronts, which read it by columns;
+// the next one is in flight.
+template <int KP>
+__global__ __launch_bounds__(256) void delta_fold_reverse_kernel(const int64_t *__restrict__ cu, int64_t T, int H, int K, int V,
+                                                                 int per, const uint16_t *__restrict__ seg_map,
+                                                                 float *__restrict__ states) {
   constexpr int NT = KP / 16, PLANE = KP * KP, N = (3 * PLANE / 8 + 255) / 256;
   __shared__ __align__(16) uint16_t sm[3 * PLANE];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, col = lane & 15, G = lane >> 4;
@@ -576,14 +714,14 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
   typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
   u32x4 pm[N];
   f32x4 S[NT], L[NT];
-  auto fetch = [&](int64_t i) __attribute__((always_inline)) {   // step i: M of segment i, or (REV) inner - i
-    const uint16_t *m = seg_map + slot(REV ? inner - i : i) * (3 * PLANE);
+  auto fetch = [&](int64_t i) __attribute__((always_inline)) {   // step i: M of segment inner - i
+    const uint16_t *m = seg_map + slot(inner - i) * (3 * PLANE);
 #pragma unroll
     for (int e = 0; e < N; ++e)
       if (tid + 256 * e < 3 * PLANE / 8) pm[e] = reinterpret_cast<const u32x4 *>(m)[tid + 256 * e];
-    cols.load(states + slot(REV ? inner - 1 - i : i) * KV, L);
+    cols.load(states + slot(inner - 1 - i) * KV, L);
   };
-  cols.load(states + slot(REV ? inner - 1 : 0) * KV, S);
+  cols.load(states + slot(inner - 1) * KV, S);
   fetch(1);
   for (int64_t i = 1; i < inner; ++i) {
 #pragma unroll
@@ -605,10 +743,10 @@ __global__ __launch_bounds__(256) void delta_fold_kernel(const int64_t *__restri
       for (int ks = 0; ks < NT / 2; ++ks) {
         bf16x8 x[3];
 #pragma unroll
-        for (int p = 0; p < 3; ++p) x[p] = REV ? op_cols<KP>(sm + p * PLANE, t, ks, lane) : op_rows<KP>(sm + p * PLANE, t, ks, lane);
+        for (int p = 0; p < 3; ++p) x[p] = op_cols<KP>(sm + p * PLANE, t, ks, lane);
         S[t] = mul<2>(x, s[ks], S[t]);
       }
-    cols.store(states + slot(REV ? inner - 1 - i : i) * KV, S);
+    cols.store(states + slot(inner - 1 - i) * KV, S);
     __syncthreads();   // M is read
   }
 }
@@ -620,7 +758,7 @@ inline int v_groups(int V) { return ((V + 15) / 16 + 3) / 4; }
 int check_grids(const char *what, const DeltaLayout &L, const WalkArgs &a) {
   const int64_t walk = L.seg_slots * a.H * v_groups(a.V), prep = L.chunk_slots * a.H;
   const int64_t inner = L.inner_slots * a.H * (v_groups(a.V) + L.KP / 64 + 1);
-  if (std::max({prep, walk, inner, static_cast<int64_t>(a.n_seq) * a.H * v_groups(a.V)}) > 0x7fffffff) {
+  if (std::max({prep, walk, inner, (static_cast<int64_t>(a.n_seq) * a.H + 7) * ((a.V + 15) / 16)}) > 0x7fffffff) {
     set_error("%s: too many workgroups", what);
     return SSLA_ERR_UNSUPPORTED;
   }
@@ -675,15 +813,16 @@ int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g
 }
 
 int delta_fold(const DeltaLayout &L, const WalkArgs &a, float *states, bool reverse, hipStream_t st) {
-  const dim3 grid = grid_of(static_cast<int64_t>(a.n_seq) * a.H * v_groups(a.V)), block(256);
+  const int64_t units = static_cast<int64_t>(a.n_seq) * a.H;
+  const dim3 ahead = grid_of((units + 7) / 8 * 8 * ((a.V + 15) / 16)), back = grid_of(units * v_groups(a.V));
 #define SSLA_FOLD(KP_)                                                                                               \
   do {                                                                                                               \
     if (reverse)                                                                                                     \
-      hipLaunchKernelGGL((delta_fold_kernel<KP_, true>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per,         \
+      hipLaunchKernelGGL((delta_fold_reverse_kernel<KP_>), back, dim3(256), 0, st, a.cu, a.T, a.H, a.K, a.V, a.per,  \
                          a.seg_map, states);                                                                         \
     else                                                                                                             \
-      hipLaunchKernelGGL((delta_fold_kernel<KP_, false>), grid, block, 0, st, a.cu, a.T, a.H, a.K, a.V, a.per,        \
-                         a.seg_map, states);                                                                         \
+      hipLaunchKernelGGL((delta_fold_kernel<KP_>), ahead, dim3(64 * FoldSize<KP_>::WAVES), 0, st, a.cu, a.n_seq, a.T, \
+                         a.H, a.K, a.V, a.per, a.seg_map, states);                                                   \
   } while (0)
   if (L.KP == 32) SSLA_FOLD(32);
   else if (L.KP == 64) SSLA_FOLD(64);
