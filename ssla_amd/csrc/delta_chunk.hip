@@ -22,7 +22,7 @@
 // and the walk starts every segment from its state.
 //
 // Measured at 8 sequences of 4096 rows, 8 heads of 64, bf16: matrices 31 us,
-// segments 63, fold 12, walk 57; 153 a pass among others, 0.9 TB/s of the inputs
+// segments 66, fold 9, walk 60; 151 a pass among others, 0.9 TB/s of the inputs
 // and outputs.  Bound by latency: a SIMD has two (walk) or three (segments)
 // wavefronts, VALU busy 37 % and matrix cores 20 % of the time; more wavefronts
 // need fewer registers than the states, one operand's parts and the next chunk's
@@ -554,11 +554,13 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : MODE == kS
 }
 
 // The fold (see delta_fold): one workgroup per (sequence, head, 16 columns), a
-// segment after the other, in lane order what the walk has: a wavefront owns one or
-// two of the state's key tiles, reads its rows of M as operands from memory, kept
-// kAhead segments in flight, and passes its keys' parts to the others through LDS
-// (two buffers: one barrier a segment).  The chain of a segment is then twelve
-// matrix instructions, a split and the pass.
+// segment after the other.  A wavefront owns one or two of the state's key tiles,
+// reads its rows of M from memory as operands, kAhead segments in flight, and passes
+// its keys' parts to the other wavefronts through LDS (two buffers: one barrier a
+// segment).  Bound by what one CU can read past its L2, 28 KB a segment of K = 64:
+// 62 segments of 65,536 rows take 51 us, 58 where the columns of a head read M
+// through different L2s, and the same with 2 to 8 segments in flight or half the
+// instructions; 86 with M staged in LDS for 64 columns by one CU.
 template <int KP>
 struct FoldSize {
   static constexpr int NT = KP / 16, WAVES = NT < 4 ? NT : 4, TPW = NT / WAVES, KS = KP / 32;

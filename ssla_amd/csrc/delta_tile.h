@@ -239,10 +239,11 @@ inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
 
 // Chunks per segment: as many as leave about 512 workgroups (two a CU) of 64
 // value columns, and for a batch of few heads at least 4 and, with c chunks in an
-// average sequence, sqrt(c / 5), where the two walks over a segment (3.5 us a
-// chunk) take as long as the fold over the segments (1.3 us each).  Measured: 8 x
-// 4096 rows of 8 heads of 64 174 us at 8 chunks, 189-213 at 4, 6, 11 and 16; one
-// sequence of 16,384 rows and one head 113 us at 7, 127 at 4, 195 at 2.
+// average sequence, sqrt(c / 5), where the walks over a segment (3.5 us a chunk)
+// take as long as the folds over the segments (0.8 us each, 1.3 in reverse).
+// Measured: 8 x 4096 rows of 8 heads of 64 161 us at 8 chunks, 177 at 6; 32,768 rows
+// of 4 heads of 128 348 us at 11, 379 at 8; one head of 16,384 rows 95 us at 8, 92 at
+// 6 and 5.
 inline int seg_chunks(int n_seq, int64_t T, int H, int V) {
   const int64_t chunks = (T + kChunk - 1) / kChunk, work = chunks * H * ((V + 63) / 64);
   int64_t per = std::max<int64_t>(4, (work + 511) / 512);
