@@ -561,6 +561,20 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : MODE == kS
 // 62 segments of 65,536 rows take 51 us, 58 where the columns of a head read M
 // through different L2s, and the same with 2 to 8 segments in flight or half the
 // instructions; 86 with M staged in LDS for 64 columns by one CU.
+// Of many short sequences few are cut: a workgroup then takes an inner segment's slot
+// (n_slots of them) and serves the sequence whose first one it is; otherwise sequence i.
+__device__ __forceinline__ bool fold_rows(const int64_t *cu, int n_seq, int64_t T, int64_t unit, int n_slots, int i,
+                                          int64_t &bos, int64_t &eos) {
+  if (n_slots < n_seq) {
+    int n;
+    int64_t first;
+    return seq_of_slot<false>(cu, n_seq, T, unit, i, n, bos, eos, first) && first == i;
+  }
+  bos = min(max(cu[i], (int64_t)0), T);
+  eos = min(max(cu[i + 1], bos), T);
+  return true;
+}
+
 template <int KP>
 struct FoldSize {
   static constexpr int NT = KP / 16, WAVES = NT < 4 ? NT : 4, TPW = NT / WAVES, KS = KP / 32;
@@ -568,7 +582,7 @@ struct FoldSize {
 };
 template <int KP>
 __global__ __launch_bounds__(64 * FoldSize<KP>::WAVES) void delta_fold_kernel(
-    const int64_t *__restrict__ cu, int n_seq, int64_t T, int H, int K, int V, int per,
+    const int64_t *__restrict__ cu, int n_seq, int n_slots, int64_t T, int H, int K, int V, int per,
     const uint16_t *__restrict__ seg_map, float *__restrict__ states) {
   typedef FoldSize<KP> F;
   constexpr int PLANE = KP * KP, D = F::kAhead;
@@ -576,11 +590,12 @@ __global__ __launch_bounds__(64 * FoldSize<KP>::WAVES) void delta_fold_kernel(
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, G = lane >> 4;
   // (a sequence and head's columns are a multiple of 8 workgroups apart: on one die,
   // whose L2 then holds M for all of them)
-  const int units = n_seq * H, apart = (units + 7) & ~7, u = static_cast<int>(blockIdx.x % apart);
+  const int units = min(n_seq, n_slots) * H, apart = (units + 7) & ~7, u = static_cast<int>(blockIdx.x % apart);
   if (u >= units) return;
-  const int vcol = static_cast<int>(blockIdx.x / apart) * 16 + col, h = u % H, n = u / H;
-  const int64_t bos = min(max(cu[n], (int64_t)0), T), eos = min(max(cu[n + 1], bos), T);
+  const int vcol = static_cast<int>(blockIdx.x / apart) * 16 + col, h = u % H;
   const int64_t unit = static_cast<int64_t>(per) * kChunk, KV = static_cast<int64_t>(K) * V;
+  int64_t bos, eos;
+  if (!fold_rows(cu, n_seq, T, unit, n_slots, u / H, bos, eos)) return;   // workgroup-uniform
   const int inner = static_cast<int>((eos - bos + unit - 1) / unit) - 1;   // segments but the last
   if (inner < 2) return;   // the only state is there already
   const StateCols<F::NT> cols(K, V, vcol, vcol < V, G);
@@ -697,7 +712,8 @@ __global__ __launch_bounds__(64 * FoldSize<KP>::WAVES) void delta_fold_kernel(
 // segment's M is staged in LDS for the four wavefronts, which read it by columns;
 // the next one is in flight.
 template <int KP>
-__global__ __launch_bounds__(256) void delta_fold_reverse_kernel(const int64_t *__restrict__ cu, int64_t T, int H, int K, int V,
+__global__ __launch_bounds__(256) void delta_fold_reverse_kernel(const int64_t *__restrict__ cu, int n_seq, int n_slots,
+                                                                 int64_t T, int H, int K, int V,
                                                                  int per, const uint16_t *__restrict__ seg_map,
                                                                  float *__restrict__ states) {
   constexpr int NT = KP / 16, PLANE = KP * KP, N = (3 * PLANE / 8 + 255) / 256;
@@ -706,9 +722,9 @@ __global__ __launch_bounds__(256) void delta_fold_reverse_kernel(const int64_t *
   const int n_groups = (((V + 15) >> 4) + 3) >> 2;
   const int vcol = ((blockIdx.x % n_groups) * 4 + w) * 16 + col;
   const int h = static_cast<int>((blockIdx.x / n_groups) % H);
-  const int64_t n = blockIdx.x / n_groups / H;
-  const int64_t bos = min(max(cu[n], (int64_t)0), T), eos = min(max(cu[n + 1], bos), T);
   const int64_t unit = static_cast<int64_t>(per) * kChunk, KV = static_cast<int64_t>(K) * V;
+  int64_t bos, eos;
+  if (!fold_rows(cu, n_seq, T, unit, n_slots, static_cast<int>(blockIdx.x / n_groups / H), bos, eos)) return;   // workgroup-uniform
   const int64_t inner = (eos - bos + unit - 1) / unit - 1;   // segments but the last
   if (inner < 2) return;   // the only state is there already
   const StateCols<NT> cols(K, V, vcol, vcol < V, G);
@@ -815,16 +831,18 @@ int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g
 }
 
 int delta_fold(const DeltaLayout &L, const WalkArgs &a, float *states, bool reverse, hipStream_t st) {
-  const int64_t units = static_cast<int64_t>(a.n_seq) * a.H;
+  if (L.inner_slots < 2) return launch_status("gated_delta_chunk");   // no sequence of three segments
+  const int n_slots = static_cast<int>(std::min<int64_t>(L.inner_slots, 0x7fffffff));
+  const int64_t units = static_cast<int64_t>(std::min(a.n_seq, n_slots)) * a.H;
   const dim3 ahead = grid_of((units + 7) / 8 * 8 * ((a.V + 15) / 16)), back = grid_of(units * v_groups(a.V));
 #define SSLA_FOLD(KP_)                                                                                               \
   do {                                                                                                               \
     if (reverse)                                                                                                     \
-      hipLaunchKernelGGL((delta_fold_reverse_kernel<KP_>), back, dim3(256), 0, st, a.cu, a.T, a.H, a.K, a.V, a.per,  \
-                         a.seg_map, states);                                                                         \
+      hipLaunchKernelGGL((delta_fold_reverse_kernel<KP_>), back, dim3(256), 0, st, a.cu, a.n_seq, n_slots, a.T, a.H, \
+                         a.K, a.V, a.per, a.seg_map, states);                                                        \
     else                                                                                                             \
-      hipLaunchKernelGGL((delta_fold_kernel<KP_>), ahead, dim3(64 * FoldSize<KP_>::WAVES), 0, st, a.cu, a.n_seq, a.T, \
-                         a.H, a.K, a.V, a.per, a.seg_map, states);                                                   \
+      hipLaunchKernelGGL((delta_fold_kernel<KP_>), ahead, dim3(64 * FoldSize<KP_>::WAVES), 0, st, a.cu, a.n_seq,     \
+                         n_slots, a.T, a.H, a.K, a.V, a.per, a.seg_map, states);                                     \
   } while (0)
   if (L.KP == 32) SSLA_FOLD(32);
   else if (L.KP == 64) SSLA_FOLD(64);

@@ -228,3 +228,10 @@ def test_training_step_in_a_graph(dev):
         want = step([t.detach().clone().requires_grad_() for t in static])
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+
+
+@pytest.mark.parametrize("dtype,K,V", [(torch.bfloat16, 64, 64), (torch.float32, 24, 40)])
+def test_long_among_many_short(dev, dtype, K, V):
+    def slow(q, k, v, g, beta):
+        g.div_(8)
+    both(dev, [5, 0, 3, 800, 2, 1, 0, 7, 1100] + [1, 0, 2] * 8 + [513, 9, 300], 1, 2, K, V, dtype, seed=K, change=slow)

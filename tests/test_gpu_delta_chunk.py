@@ -242,3 +242,20 @@ def test_chunk_kernels_on_short_sequences(dev, dtype, Hk, H, K, V):
         ro, rs = gated_delta(*few, [T], 0.5, s0[:1])
         close(o, ro, K, T, dtype, "o")
         close(ht, rs, K, T, torch.float32, "ht")
+
+
+MANY = [5, 0, 3, 800, 2, 1, 0, 7, 1100] + [1, 0, 2] * 8 + [513, 9, 300]   # more sequences than inner segments
+
+
+@pytest.mark.parametrize("dtype,K,V", [(torch.bfloat16, 64, 64), (torch.float32, 24, 40)])
+def test_long_among_many_short(dev, dtype, K, V):
+    """Long sequences that start in a unit of rows where short ones lie too, with
+    a gradient recorded (the chunk kernels whatever the average length is)."""
+    x, cu, s0 = inputs(MANY, 1, 2, K, V, dtype, seed=K)
+    x[3] = x[3] / 8
+    x[4].requires_grad_()
+    o, ht = run(dev, x, cu, s0)
+    assert o.requires_grad
+    ro, rs = gated_delta(*(t.detach() for t in x), MANY, K ** -0.5, s0)
+    close(o.detach(), ro, K, max(MANY), dtype, "o")
+    close(ht.detach(), rs, K, max(MANY), torch.float32, "ht")
