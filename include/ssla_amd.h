@@ -267,6 +267,18 @@ int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, cons
                                float scale, const float *h0, void *o, float *ht, void *segments, int dtype,
                                void *workspace, size_t workspace_bytes, void *stream);
 
+/* The same sequences, each by the kernel for its length: up to 64 rows as
+ * ssla_gated_delta_recurrent, longer ones as ssla_gated_delta_chunk_fwd (K <= 128).
+ * For batches of many short sequences that may hold long ones; the lengths are
+ * read on the device.  Workspace:
+ * ssla_gated_delta_mixed_workspace_size bytes, 16-byte aligned, no
+ * initialisation. */
+size_t ssla_gated_delta_mixed_workspace_size(int64_t T, int H, int K, int V);
+int ssla_gated_delta_mixed_fwd(const void *q, const void *k, const void *v, const float *g, const float *beta,
+                               const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,
+                               float scale, const float *h0, void *o, float *ht, int dtype, void *workspace,
+                               size_t workspace_bytes, void *stream);
+
 /* Gradients of ssla_gated_delta_chunk_fwd: dout [T, H, V] in `dtype`, dht fp32
  * [n_seq, H, K, V] or NULL; dq, dk, dv in `dtype` and the inputs' shapes (dq and
  * dk of a shared key head are the sums over its value heads), dg, dbeta fp32

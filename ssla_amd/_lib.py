@@ -80,6 +80,9 @@ SIGNATURES = {
     "ssla_gated_delta_chunk_segments_size": (_sz, [_i32, _i64, _i32, _i32, _i32]),
     "ssla_gated_delta_chunk_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
                                           _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
+    "ssla_gated_delta_mixed_workspace_size": (_sz, [_i64, _i32, _i32, _i32]),
+    "ssla_gated_delta_mixed_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
+                                          _vp, _vp, _i32, _vp, _sz, _vp]),
     "ssla_gated_delta_chunk_bwd_workspace_size": (_sz, [_i32, _i64, _i32, _i32, _i32, _i32]),
     "ssla_gated_delta_chunk_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
                                           _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),

@@ -46,8 +46,9 @@ template <int DT, int KP>
 __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict__ k, const float *__restrict__ g,
                                                          const float *__restrict__ beta,
                                                          const int64_t *__restrict__ cu, int n_seq, int64_t T, int Hk,
-                                                         int H, int K, int vec, float scale, float *__restrict__ tm,
-                                                         int tm_floats, float *__restrict__ rowv) {
+                                                         int H, int K, int vec, int mixed, float scale,
+                                                         float *__restrict__ tm, int tm_floats,
+                                                         float *__restrict__ rowv) {
   constexpr int NP = Parts<DT>::n, LD = 68;
   constexpr int SK = NP * kChunk * KP * 2, SA = kChunk * LD * 4;
   __shared__ __align__(16) char buf[SK > SA ? SK : SA];
@@ -60,7 +61,9 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(const void *__restrict_
   const int64_t slot = blockIdx.x / H;
   int n;
   int64_t bos, eos, first;
-  if (!seq_of_slot(cu, n_seq, T, kChunk, slot, n, bos, eos, first)) return;   // workgroup-uniform
+  auto slot_of = [&](int64_t row, int i) __attribute__((always_inline)) { return chunk_slot(row, i, 0, mixed); };
+  if (!seq_of_slot_by(cu, n_seq, T, slot, slot_of, n, bos, eos, first)) return;   // workgroup-uniform
+  if (mixed && eos - bos <= kChunk) return;
   const int64_t t0 = bos + (slot - first) * kChunk;
   if (t0 >= eos) return;
   const int rows = static_cast<int>(min(static_cast<int64_t>(kChunk), eos - t0));
@@ -280,7 +283,12 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : MODE == kS
   const int64_t unit = static_cast<int64_t>(a.per) * kChunk;
   int n;
   int64_t bos, eos, first;
-  if (!seq_of_slot<!SEG>(a.cu, a.n_seq, a.T, unit, slot, n, bos, eos, first)) return;   // workgroup-uniform
+  // (segments have at least 4 chunks: in a mixed batch 64 rows a slot do)
+  auto slot_of = [&](int64_t row, int i) __attribute__((always_inline)) {
+    return MODE == kOutput && a.mixed ? row / kChunk : pieces_before(row, unit, a.T) + (SEG ? 0 : i);
+  };
+  if (!seq_of_slot_by(a.cu, a.n_seq, a.T, slot, slot_of, n, bos, eos, first)) return;   // workgroup-uniform
+  if (MODE == kOutput && a.mixed && eos - bos <= kChunk) return;
   const int64_t seg = slot - first, t_begin = bos + seg * unit;
   if (SEG ? t_begin + unit >= eos : (t_begin >= eos && seg > 0)) return;
   if (SEG && seg == 0 && grp * 4 >= n_vt) return;   // (a first segment's M)
@@ -315,7 +323,7 @@ __global__ __launch_bounds__(256, (DT == SSLA_F32 && KP == 128) ? 1 : MODE == kS
     const int stride = a.Hk * a.K;
     kt.fetch(rows_rsrc(a.k, at, rows, stride, a.K, ES), stride, a.K, a.vec);
     if constexpr (OUT) qt.fetch(rows_rsrc(a.q, at, rows, stride, a.K, ES), stride, a.K, a.vec);
-    const int64_t c = chunk_slot(bos, n, (t0 - bos) / kChunk) * a.H + h;
+    const int64_t c = chunk_slot(bos, n, (t0 - bos) / kChunk, MODE != kStates && a.mixed) * a.H + h;
     const Rsrc rt = rsrc_of(a.tm + c * a.tm_floats, rows > 0 ? kTriFloats * 4 : 0);
     const Rsrc rr = rsrc_of(a.rowv + c * kRowFloats, rows > 0 ? kRowFloats * 4 : 0);
     tmr[0] = load4(rt, tid * 32);
@@ -788,7 +796,7 @@ void launch_chunk(const DeltaLayout &L, const WalkArgs &a, const float *g, const
                   bool have_segs, hipStream_t st) {
   const dim3 block(256);
   hipLaunchKernelGGL((delta_prep_kernel<DT, KP>), grid_of(L.chunk_slots * a.H), block, 0, st, a.k, g, beta, a.cu, a.n_seq,
-                     a.T, a.Hk, a.H, a.K, a.vec, a.scale, const_cast<float *>(a.tm), a.tm_floats,
+                     a.T, a.Hk, a.H, a.K, a.vec, a.mixed, a.scale, const_cast<float *>(a.tm), a.tm_floats,
                      const_cast<float *>(a.rowv));
   if (L.inner_slots > 0 && !have_segs) {
     const int groups = ((a.V + 15) / 16 + KP / 16 + 3) / 4;
@@ -863,32 +871,71 @@ extern "C" size_t ssla_gated_delta_chunk_segments_size(int n_seq, int64_t T, int
   return ssla::delta_layout(n_seq, T, H, H, K, V, false).seg_bytes;
 }
 
-extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, const float *g,
-                                          const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk,
-                                          int H, int K, int V, float scale, const float *h0, void *o, float *ht,
-                                          void *segments, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
-  using namespace ssla;
+extern "C" size_t ssla_gated_delta_mixed_workspace_size(int64_t T, int H, int K, int V) {
+  if (T < 0 || H <= 0 || K <= 0 || K > 128 || V <= 0) return 0;
+  return ssla::delta_layout(1, T, H, H, K, V, false, true).total;
+}
+
+namespace ssla {
+namespace {
+
+// mixed: up to kChunk rows token by token, longer sequences by chunks, both kinds of
+// kernels over the whole batch (a workgroup whose sequence is the other kind's
+// ends after its search).  Measured, 4 heads, bf16: a prompt of 15,900 rows among 512
+// single rows 84 us at K = 32, 149 at 64 and 466 at 128 (all token by token 3,684,
+// 5,002 and 10,675, all by chunks 104, 235 and 457); without a long one the empty
+// launches are added to the tokens' time: 4,096 sequences of 16 rows 68 -> 98 us at K =
+// 32 and 274 -> 296 at 64 (by chunks 347 and 415), 32 of 20 rows 13 -> 25 (20).
+int chunk_fwd(const char *what, bool mixed, const void *q, const void *k, const void *v, const float *g, const float *beta,
+              const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V, float scale, const float *h0,
+              void *o, float *ht, void *segments, int dtype, void *workspace, size_t workspace_bytes, hipStream_t st) {
   clear_error();
   SSLA_CHECK_ARG(n_seq >= 0 && T >= 0 && Hk > 0 && H > 0 && H % Hk == 0 && K > 0 && V > 0,
-                 "gated_delta_chunk_fwd: bad sizes n_seq=%d T=%lld Hk=%d H=%d K=%d V=%d", n_seq, (long long)T, Hk, H, K,
-                 V);
+                 "%s: bad sizes n_seq=%d T=%lld Hk=%d H=%d K=%d V=%d", what, n_seq, (long long)T, Hk, H, K, V);
   if (K > 128) {
-    set_error("gated_delta_chunk_fwd: K=%d exceeds 128", K);
+    set_error("%s: K=%d exceeds 128", what, K);
     return SSLA_ERR_UNSUPPORTED;
   }
   if (n_seq == 0) return SSLA_OK;
-  SSLA_CHECK_ARG(cu_seqlens != nullptr, "gated_delta_chunk_fwd: cu_seqlens is NULL");
-  SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "gated_delta_chunk_fwd: null tensor pointer");
-  if (const int e = check_widths("gated_delta_chunk_fwd", kChunk, Hk, H, K, V)) return e;
-  const DeltaLayout L = delta_layout(n_seq, T, Hk, H, K, V, false);
+  SSLA_CHECK_ARG(cu_seqlens != nullptr, "%s: cu_seqlens is NULL", what);
+  SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "%s: null tensor pointer", what);
+  if (const int e = check_widths(what, kChunk, Hk, H, K, V)) return e;
+  const DeltaLayout L = delta_layout(n_seq, T, Hk, H, K, V, false, mixed);
   if (!workspace || workspace_bytes < L.total || !aligned(workspace, 16)) {
-    set_error("gated_delta_chunk_fwd: needs %zu bytes of workspace, got %zu", L.total, workspace_bytes);
+    set_error("%s: needs %zu bytes of workspace, got %zu", what, L.total, workspace_bytes);
     return SSLA_ERR_WORKSPACE;
   }
-  SSLA_CHECK_ARG(aligned(segments, 16), "gated_delta_chunk_fwd: segments must be 16-byte aligned");
+  SSLA_CHECK_ARG(aligned(segments, 16), "%s: segments must be 16-byte aligned", what);
   WalkArgs a = walk_args(L, static_cast<char *>(workspace), q, k, v, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, dtype,
                          false, segments);
   a.o = o;
   a.ht = ht;
-  return launch_dtype("gated_delta_chunk_fwd", L, a, g, beta, false, false, dtype, static_cast<hipStream_t>(stream));
+  a.mixed = mixed;
+  if (mixed) {
+    if (const int e = check_grids(what, L, a)) return e;
+    if (const int e = delta_recurrent_up_to(what, kChunk, q, k, v, g, beta, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, o,
+                                            ht, nullptr, 0, nullptr, dtype, st))
+      return e;
+    if (T <= kChunk) return SSLA_OK;   // no longer sequence
+  }
+  return launch_dtype(what, L, a, g, beta, false, false, dtype, st);
+}
+
+}  // namespace
+}  // namespace ssla
+
+extern "C" int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, const float *g,
+                                          const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk,
+                                          int H, int K, int V, float scale, const float *h0, void *o, float *ht,
+                                          void *segments, int dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  return ssla::chunk_fwd("gated_delta_chunk_fwd", false, q, k, v, g, beta, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, o,
+                         ht, segments, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
+}
+
+extern "C" int ssla_gated_delta_mixed_fwd(const void *q, const void *k, const void *v, const float *g,
+                                          const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk,
+                                          int H, int K, int V, float scale, const float *h0, void *o, float *ht, int dtype,
+                                          void *workspace, size_t workspace_bytes, void *stream) {
+  return ssla::chunk_fwd("gated_delta_mixed_fwd", true, q, k, v, g, beta, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, o,
+                         ht, nullptr, dtype, workspace, workspace_bytes, static_cast<hipStream_t>(stream));
 }

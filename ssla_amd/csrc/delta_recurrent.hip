@@ -33,7 +33,7 @@ struct DeltaArgs {
   float *ht;
   void *o;
   int32_t *status;
-  int64_t T;
+  int64_t T, longest;     // sequences of more rows are left to another kernel
   int n_seq, Hk, H, K, V, n_rows, kvec, vvec;   // k and q, v and o: rows of whole 16-byte pieces
   float scale;
 };
@@ -153,6 +153,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(const DeltaArgs a)
     bos = min(max(a.cu[n], (int64_t)0), a.T);
     eos = min(max(a.cu[n + 1], bos), a.T);
   }
+  if (eos - bos > a.longest) return;   // whole wavefront
   const int64_t row = state_row(a, n), vstride = static_cast<int64_t>(a.H) * a.V, kstride = static_cast<int64_t>(a.Hk) * a.K;
   if (row < 0) {
     report(a);
@@ -369,7 +370,7 @@ bool launch_step(const DeltaArgs &a, dim3 grid, hipStream_t st) {
 }
 
 template <int DT>
-int launch_delta(const DeltaArgs &a, hipStream_t st) {
+int launch_delta(const char *what, const DeltaArgs &a, hipStream_t st) {
   // single tokens: 16-byte pieces of the states' rows, at most 32 rows a lane
   const int vl = a.V <= 16 ? 4 : a.V <= 32 ? 8 : 16;
   const bool step = a.cu == nullptr && a.V % 4 == 0 && aligned(a.h0, 16) && aligned(a.ht, 16) && (a.K + 64 / vl - 1) / (64 / vl) <= 32;
@@ -380,7 +381,7 @@ int launch_delta(const DeltaArgs &a, hipStream_t st) {
   const int64_t tiles = step ? (a.V + 4 * vl - 1) / (4 * vl) : narrow ? (a.V + 7) / 8 : (a.V + 15) / 16;
   const int64_t blocks = (seqs * tiles + 3) / 4;
   if (blocks > 0x7fffffff) {
-    set_error("gated_delta_recurrent: too many (sequence, head, tile) items");
+    set_error("%s: too many (sequence, head, tile) items", what);
     return SSLA_ERR_UNSUPPORTED;
   }
   const dim3 grid(static_cast<unsigned>(blocks)), block(256);
@@ -388,7 +389,7 @@ int launch_delta(const DeltaArgs &a, hipStream_t st) {
     if (vl == 4) launch_step<4, DT>(a, grid, st);
     else if (vl == 8) launch_step<8, DT>(a, grid, st);
     else launch_step<16, DT>(a, grid, st);
-    return launch_status("gated_delta_recurrent");
+    return launch_status(what);
   }
 #define SSLA_DELTA(KR_, BT_)                                                                                   \
   do {                                                                                                         \
@@ -401,10 +402,29 @@ int launch_delta(const DeltaArgs &a, hipStream_t st) {
   else if (a.K <= 128) SSLA_DELTA(32, 8);
   else SSLA_DELTA(64, 4);
 #undef SSLA_DELTA
-  return launch_status("gated_delta_recurrent");
+  return launch_status(what);
 }
 
 }  // namespace
+
+int delta_recurrent_up_to(const char *what, int64_t longest, const void *q, const void *k, const void *v, const float *g,
+                          const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,
+                          float scale, const float *h0, void *o, float *ht, const int32_t *state_idx, int n_state_rows,
+                          int32_t *status, int dtype, hipStream_t st) {
+  const int64_t es = dtype == SSLA_F32 ? 4 : 2;
+  const int kvec = K * es % 16 == 0 && aligned(q, 16) && aligned(k, 16);
+  const int vvec = V * es % 16 == 0 && aligned(v, 16) && aligned(o, 16);
+  const DeltaArgs a{q, k, v, g, beta, cu_seqlens, state_idx, h0, ht, o, status, T, longest, n_seq, Hk, H, K, V,
+                    n_state_rows, kvec, vvec, scale};
+  switch (dtype) {
+    case SSLA_F32: return launch_delta<SSLA_F32>(what, a, st);
+    case SSLA_BF16: return launch_delta<SSLA_BF16>(what, a, st);
+    case SSLA_F16: return launch_delta<SSLA_F16>(what, a, st);
+  }
+  set_error("%s: unsupported dtype %d", what, dtype);
+  return SSLA_ERR_DTYPE;
+}
+
 }  // namespace ssla
 
 extern "C" int ssla_gated_delta_recurrent(const void *q, const void *k, const void *v, const float *g,
@@ -427,17 +447,6 @@ extern "C" int ssla_gated_delta_recurrent(const void *q, const void *k, const vo
   SSLA_CHECK_ARG(state_idx == nullptr || (n_state_rows >= 0 && h0 && ht),
                  "gated_delta_recurrent: state_idx without a state table");
   if (const int e = check_widths("gated_delta_recurrent", 16, Hk, H, K, V)) return e;
-  const int64_t es = dtype == SSLA_F32 ? 4 : 2;
-  const int kvec = K * es % 16 == 0 && aligned(q, 16) && aligned(k, 16);
-  const int vvec = V * es % 16 == 0 && aligned(v, 16) && aligned(o, 16);
-  const DeltaArgs a{q, k, v, g, beta, cu_seqlens, state_idx, h0, ht, o, status, T, n_seq, Hk, H, K, V, n_state_rows, kvec,
-                    vvec, scale};
-  const hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case SSLA_F32: return launch_delta<SSLA_F32>(a, st);
-    case SSLA_BF16: return launch_delta<SSLA_BF16>(a, st);
-    case SSLA_F16: return launch_delta<SSLA_F16>(a, st);
-  }
-  set_error("gated_delta_recurrent: unsupported dtype %d", dtype);
-  return SSLA_ERR_DTYPE;
+  return delta_recurrent_up_to("gated_delta_recurrent", INT64_MAX, q, k, v, g, beta, cu_seqlens, n_seq, T, Hk, H, K, V,
+                               scale, h0, o, ht, state_idx, n_state_rows, status, dtype, static_cast<hipStream_t>(stream));
 }

@@ -231,8 +231,11 @@ enum { kBeta = 0, kBetaG, kScaleG, kToEnd, kGHi, kGLo, kRowVecs };
 constexpr int kRowFloats = kRowVecs * kChunk;
 
 // Chunk c (of 64 rows) of sequence n that starts at row bos has slot
-// bos / 64 + n + c; see seq_of_slot.
-__device__ __forceinline__ int64_t chunk_slot(int64_t bos, int n, int64_t c) { return bos / kChunk + n + c; }
+// bos / 64 + n + c; see seq_of_slot.  In a mixed batch (sequences of up to kChunk
+// rows run token by token) it has bos / 32 + c.
+__device__ __forceinline__ int64_t chunk_slot(int64_t bos, int n, int64_t c, bool mixed = false) {
+  return (bos >> (mixed ? 5 : 6)) + (mixed ? 0 : n) + c;
+}
 
 inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
@@ -259,13 +262,14 @@ struct DeltaLayout {
   int64_t chunk_slots, seg_slots, inner_slots;
   int per, KP;
 };
-inline DeltaLayout delta_layout(int n_seq, int64_t T, int Hk, int H, int K, int V, bool grad) {
+inline DeltaLayout delta_layout(int n_seq, int64_t T, int Hk, int H, int K, int V, bool grad, bool mixed = false) {
   DeltaLayout L{};
   L.KP = padded_keys(K);
-  L.per = seg_chunks(std::max(n_seq, 1), T, H, V);
+  // (a mixed batch may be one long sequence and nothing else)
+  L.per = seg_chunks(mixed ? 1 : std::max(n_seq, 1), T, H, V);
   const int64_t unit = static_cast<int64_t>(L.per) * kChunk;
-  L.chunk_slots = T / kChunk + n_seq + 1;
-  L.seg_slots = T / unit + n_seq + 1;
+  L.chunk_slots = mixed ? T / (kChunk / 2) + 1 : T / kChunk + n_seq + 1;
+  L.seg_slots = mixed ? T / kChunk + 1 : T / unit + n_seq + 1;
   L.inner_slots = T > 0 ? (T - 1) / unit : 0;   // 0: no sequence is cut
   size_t p = 0;
   auto take = [&](size_t bytes) {
@@ -340,7 +344,7 @@ struct WalkArgs {
   float *chunk_state;     // per chunk: the state entering it
   float *u;               // [T, H, V]
   int64_t T;
-  int n_seq, Hk, H, K, V, per, vec, tm_floats;
+  int n_seq, Hk, H, K, V, per, vec, tm_floats, mixed;
   float scale;
 };
 
@@ -378,6 +382,12 @@ inline int check_widths(const char *what, int rows, int Hk, int H, int K, int V)
 // maps, and every chunk's entering state and u (delta_chunk.hip), for the backward.
 int delta_forward_states(const DeltaLayout &L, const WalkArgs &a, const float *g, const float *beta, bool have_segs,
                          int dtype, hipStream_t st);
+
+// Token by token, the sequences of up to `longest` rows (delta_recurrent.hip).
+int delta_recurrent_up_to(const char *what, int64_t longest, const void *q, const void *k, const void *v, const float *g,
+                          const float *beta, const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,
+                          float scale, const float *h0, void *o, float *ht, const int32_t *state_idx, int n_state_rows,
+                          int32_t *status, int dtype, hipStream_t st);
 
 // Carries states over a sequence's segments (delta_chunk.hip).  Forward: with M and
 // L of segments 1 .., and L of segment 0 the state behind it, L of segment j

@@ -20,14 +20,16 @@ __device__ __forceinline__ int64_t readlane64(int64_t x, int from) {
 // for up to 64 sequences, two for 4,096.  OWN false leaves n out of first(n):
 // slots that only pieces with a successor in their sequence own (at most
 // (T - 1) / unit of them).
-template <bool OWN = true>
-__device__ __forceinline__ bool seq_of_slot(const int64_t *cu, int n_seq, int64_t T, int64_t unit, int64_t slot, int &n,
-                                            int64_t &bos, int64_t &eos, int64_t &first) {
-  // (32-bit division where it holds: the 64-bit one is dozens of instructions)
-  auto slot_of = [&](int64_t row, int i) __attribute__((always_inline)) {
-    return (T < 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(row) / static_cast<uint32_t>(unit))
-                           : row / unit) + (OWN ? i : 0);
-  };
+//
+// Where only sequences of more than m rows matter (m >= 1) and a piece has at
+// least 2 m, they own floor(bos_n / m) + j without n: at most T / m + 1 slots
+// however many short sequences lie between.  (With R > m rows a sequence has
+// ceil(R / 2 m) <= floor(R / m) pieces, so the next start is past them, and a short
+// one that starts in the same m rows comes before it.)  slot_of(row, i): the
+// first slot of sequence i that starts at `row`.
+template <typename SlotOf>
+__device__ __forceinline__ bool seq_of_slot_by(const int64_t *cu, int n_seq, int64_t T, int64_t slot, SlotOf slot_of, int &n,
+                                               int64_t &bos, int64_t &eos, int64_t &first) {
   const int lane = threadIdx.x & 63;
   int lo = 0, hi = n_seq;
   do {
@@ -47,6 +49,18 @@ __device__ __forceinline__ bool seq_of_slot(const int64_t *cu, int n_seq, int64_
   } while (hi - lo > 1);
   n = lo;
   return first <= slot;   // (always, unless the starts decrease: then no row before the sequence's is touched)
+}
+
+// row / unit (32-bit division where it holds: the 64-bit one is dozens of instructions)
+__device__ __forceinline__ int64_t pieces_before(int64_t row, int64_t unit, int64_t T) {
+  return T < 0x7fffffff ? static_cast<int64_t>(static_cast<uint32_t>(row) / static_cast<uint32_t>(unit)) : row / unit;
+}
+template <bool OWN = true>
+__device__ __forceinline__ bool seq_of_slot(const int64_t *cu, int n_seq, int64_t T, int64_t unit, int64_t slot, int &n,
+                                            int64_t &bos, int64_t &eos, int64_t &first) {
+  auto slot_of = [&](int64_t row, int i)
+      __attribute__((always_inline)) { return pieces_before(row, unit, T) + (OWN ? i : 0); };
+  return seq_of_slot_by(cu, n_seq, T, slot, slot_of, n, bos, eos, first);
 }
 
 }  // namespace ssla

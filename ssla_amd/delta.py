@@ -106,13 +106,36 @@ def _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state, keep=False):
     return o, ht, segments
 
 
+_SHORT = 64   # rows of a sequence that ssla_gated_delta_mixed_fwd runs token by token
+
+
 def _token_rows(K: int) -> int:
-    """Rows of an average sequence up to which the token-by-token kernel is
-    faster: its time grows with K, the chunk kernels' hardly.  Measured at 32,768
-    rows and 4 heads, chunks against tokens: K = 32 fp32 80 / 36 us at 64 rows and
-    68 / 41 at 128, K = 64 bf16 118 / 103 at 32 and 80 / 101 at 64, K = 128 bf16 890 /
-    495 at 16 and 268 / 414 at 64."""
+    """Rows of an average sequence up to which a batch runs short sequences
+    token by token: that kernel's time grows with K, the chunk kernels' hardly.
+    Measured on sequences of one length, 4 heads, bf16, chunks against tokens, us:
+    32,768 rows, K = 32 68 / 34 at 64 rows and 65 / 38 at 96, K = 64 115 / 119 at 32
+    and 84 / 118 at 48, K = 128 807 / 671 at 16 and 556 / 627 at 24; 2,048 rows, where
+    the length counts too (a token waits 0.20 to 0.41 us for the one before), K =
+    32 20 / 17 at 64 and 23 / 24 at 96, K = 64 23 / 15 at 32, K = 128 64 / 48 at 16."""
     return max(16, min(64, 2048 // K))
+
+
+def _mixed_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state):
+    """One ssla_gated_delta_mixed_fwd call on contiguous tensors: o and the final
+    states."""
+    T, Hk, K = q.shape
+    H, V = v.shape[1:]
+    N = cu.numel() - 1
+    o = torch.empty_like(v)
+    ht = torch.empty(N, H, K, V, device=v.device, dtype=torch.float32) if output_final_state else None
+    lib, P = _lib.load(), _lib.ptr
+    with _lib.on_device_of(q):
+        nbytes = lib.ssla_gated_delta_mixed_workspace_size(T, H, K, V)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        st = lib.ssla_gated_delta_mixed_fwd(P(q), P(k), P(v), P(g), P(beta), P(cu), N, T, Hk, H, K, V, float(scale), P(h0),
+                                            P(o), P(ht), _lib.DTYPE_CODE[q.dtype], P(ws), nbytes, _lib.stream_of(q))
+    _lib.check(st, "ssla_gated_delta_mixed_fwd")
+    return o, ht
 
 
 class ChunkGatedDeltaFunction(torch.autograd.Function):
@@ -169,8 +192,10 @@ def chunk_gated_delta(
     K up to 128 runs the chunk kernels (chunks of 64 tokens), whose products keep
     the precision of fp32 for every dtype, and is differentiable in q, k, v, g, beta and the
     initial state (once; rows in no sequence get zeros).  Without a
-    gradient, sequences so short on average that chunks stay mostly empty run
-    the token-by-token kernel; so do wider keys (K up to 256), forward only."""
+    gradient, where sequences are so short on average that chunks would stay
+    mostly empty, those of up to 64 rows run the token-by-token kernel, longer ones
+    the chunk kernels (told on the device); wider keys (K up to 256) run token by
+    token, forward only."""
     name = "chunk_gated_delta"
     T, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
     dev = _lib.require_cuda(q, k, v, g, beta, initial_state)
@@ -184,11 +209,16 @@ def chunk_gated_delta(
         t is not None and t.requires_grad for t in (q, k, v, g, beta, initial_state))
     if grad and K > 128:
         raise NotImplementedError(f"{name}: the backward takes K up to 128 (got {K}; call it under torch.no_grad())")
-    if not grad and (K > 128 or T <= N * _token_rows(K)):
+    # short on average says nothing of the longest: unless no sequence can be far
+    # longer (tokens wait for one another), each is told by its own length
+    short = not grad and T <= N * _token_rows(K)
+    if not grad and (K > 128 or short and T <= 2 * _SHORT):
         ht = torch.empty(N, H, K, V, device=dev, dtype=torch.float32) if output_final_state else None
         return _recurrent(q, k, v, g, beta, cu, N, scale, h0, ht), ht
     q, k, v = q.contiguous(), k.contiguous(), v.contiguous()
     g, beta = _f32(g), _f32(beta)
+    if short:
+        return _mixed_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)
     if grad:
         return ChunkGatedDeltaFunction.apply(q, k, v, g, beta, h0, cu, scale, output_final_state)
     return _chunk_fwd(q, k, v, g, beta, cu, scale, h0, output_final_state)[:2]
