@@ -596,11 +596,13 @@ __global__ __launch_bounds__(64 * FoldSize<KP>::WAVES) void delta_fold_kernel(
   constexpr int PLANE = KP * KP, D = F::kAhead;
   __shared__ __align__(16) uint2 parts[2][F::KS][3][64][2];
   const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, G = lane >> 4;
-  // (a sequence and head's columns are a multiple of 8 workgroups apart: on one die,
-  // whose L2 then holds M for all of them)
-  const int units = min(n_seq, n_slots) * H, apart = (units + 7) & ~7, u = static_cast<int>(blockIdx.x % apart);
+  // (a sequence and head's columns are 8 workgroups apart: on one die, whose L2 then
+  // holds M for all of them, and next to each other there, on CUs of their own,
+  // however many sequences without a fold lie between)
+  const int units = min(n_seq, n_slots) * H, n_cols = (V + 15) >> 4, b = static_cast<int>(blockIdx.x >> 3);
+  const int u = b / n_cols * 8 + static_cast<int>(blockIdx.x & 7);
   if (u >= units) return;
-  const int vcol = static_cast<int>(blockIdx.x / apart) * 16 + col, h = u % H;
+  const int vcol = (b % n_cols) * 16 + col, h = u % H;
   const int64_t unit = static_cast<int64_t>(per) * kChunk, KV = static_cast<int64_t>(K) * V;
   int64_t bos, eos;
   if (!fold_rows(cu, n_seq, T, unit, n_slots, u / H, bos, eos)) return;   // workgroup-uniform
