@@ -240,17 +240,24 @@ __device__ __forceinline__ int64_t chunk_slot(int64_t bos, int n, int64_t c, boo
 inline size_t align256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 inline int padded_keys(int K) { return K <= 32 ? 32 : K <= 64 ? 64 : 128; }
 
-// Chunks per segment: as many as leave about 512 workgroups (two a CU) of 64
-// value columns, and for a batch of few heads at least 4 and, with c chunks in an
-// average sequence, sqrt(c / 5), where the walks over a segment (3.5 us a chunk)
-// take as long as the folds over the segments (0.8 us each, 1.3 in reverse).
-// Measured: 8 x 4096 rows of 8 heads of 64 161 us at 8 chunks, 177 at 6; 32,768 rows
-// of 4 heads of 128 348 us at 11, 379 at 8; one head of 16,384 rows 95 us at 8, 92 at
-// 6 and 5.
+// Chunks per segment: as many as leave about 512 workgroups of 64 value columns (two
+// a CU, where the kernel's LDS admits two), and at least 4; where heads are few, with
+// c chunks in an average sequence at least sqrt(c / 5), where the walks over a
+// segment (3.5 us a chunk) take about as long as the folds over the segments (0.8 us
+// each, 1.3 in reverse).  Measured: 8 x 4096 rows of 8 heads of 64 143 us at 8 chunks,
+// 172 at 4; 65,536 rows of one head of 128 384 us at 15, 420 at 11, 496 at 8; of one
+// head of 64 172 at 15, 165 at 11, 170 at 8; 16,384 of one head of 64 96 at 8, 90 at 5 and
+// 6 (c / 8 instead of c / 5 took 379 us instead of 348 for 32,768 rows of 4 heads of 128).
+// The average may come of sequences that are hardly there, beside a long one: no
+// batch is cut into more than 128 segments unless one sequence of all rows would be.
+// Measured for 65,536 rows of one head, 4 and 8 chunks: one sequence beside 63 single
+// rows 241 and 171 us at 64 columns, 872 and 496 at 128; 64 equal sequences 69 and 77,
+// 164 and 131.  (8 at least for fewer rows too: 12 sequences in 8,209 rows, a training
+// step, 222 and 299.)
 inline int seg_chunks(int n_seq, int64_t T, int H, int V) {
   const int64_t chunks = (T + kChunk - 1) / kChunk, work = chunks * H * ((V + 63) / 64);
   int64_t per = std::max<int64_t>(4, (work + 511) / 512);
-  while (per * per * 5 * n_seq < chunks) ++per;
+  while (per * per * 5 < chunks && (per * per * 5 * n_seq < chunks || per * 128 < chunks)) ++per;
   return static_cast<int>(std::min<int64_t>(1 << 20, per));
 }
 
