@@ -13,6 +13,7 @@ import threading
 from pathlib import Path
 
 import torch
+from torch.autograd import forward_ad
 
 LIB_PATH = Path(__file__).resolve().parent / "libssla_amd.so"
 
@@ -351,3 +352,10 @@ def require_no_grad(name: str, *tensors: torch.Tensor) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise NotImplementedError(f"{name}: only the forward pass is implemented "
                                   "(call it under torch.no_grad())")
+
+
+def require_no_tangent(name: str, *tensors: torch.Tensor) -> None:
+    """Refuses dual tensors: a kernel sees their primals only."""
+    if forward_ad._current_level >= 0 and any(   # (the level first: unpacking costs as much as the other checks)
+            t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name}: forward-mode derivatives are not implemented")

@@ -19,7 +19,8 @@ layouts, same state tables) and has no counterpart in the reference.
 Layouts: q, k ``[T, Hk, K]``, v ``[T, H, V]`` (one dtype of fp32, bf16, fp16),
 g (log-gates) and beta ``[T, H]`` floating point, ``cu_seqlens`` ``[N + 1]``,
 states fp32 ``[N, H, K, V]``.  ``H`` is a multiple of ``Hk``: value head h reads
-key head ``h // (H // Hk)``.  A gate of -inf empties the state.
+key head ``h // (H // Hk)``.  A gate of -inf empties the state.  Tensors with
+forward-mode tangents are refused.
 """
 from __future__ import annotations
 
@@ -198,6 +199,7 @@ def chunk_gated_delta(
     token, forward only."""
     name = "chunk_gated_delta"
     T, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
+    _lib.require_no_tangent(name, q, k, v, g, beta, initial_state)
     dev = _lib.require_cuda(q, k, v, g, beta, initial_state)
     cu = _offsets(name, cu_seqlens, dev)
     N = cu.numel() - 1
@@ -241,6 +243,7 @@ def fused_recurrent_gated_delta(
     cu_seqlens[-1])`` are unspecified.  Makes no host sync; forward only."""
     name = "fused_recurrent_gated_delta"
     T, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
+    _lib.require_no_tangent(name, q, k, v, g, beta, initial_state)
     dev = _lib.require_cuda(q, k, v, g, beta, initial_state)
     _lib.require_no_grad(name, q, k, v, g, beta, initial_state)
     cu = _offsets(name, cu_seqlens, dev)
@@ -276,6 +279,7 @@ def sparse_delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torc
     name = "sparse_delta_scan"
     T, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
     _table(name, state, H, K, V)
+    _lib.require_no_tangent(name, q, k, v, g, beta, state)
     dev = _lib.require_cuda(q, k, v, g, beta, state, seq_site)
     _lib.require_no_grad(name, q, k, v, g, beta, state)
     cu = _offsets(name, cu_seqlens, dev)
@@ -297,6 +301,7 @@ def sparse_delta_step(site_idx: torch.Tensor, q: torch.Tensor, k: torch.Tensor, 
     name = "sparse_delta_step"
     n, Hk, H, K, V = _shapes(name, q, k, v, g, beta)
     _table(name, state, H, K, V)
+    _lib.require_no_tangent(name, q, k, v, g, beta, state)
     dev = _lib.require_cuda(q, k, v, g, beta, state, site_idx)
     _lib.require_no_grad(name, q, k, v, g, beta, state)
     idx = _sites(name, site_idx, n)

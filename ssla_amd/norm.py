@@ -95,7 +95,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     (``x.shape[1:-1]``; none for ``[N, C]``, where every row is a sample) and
     ``C / num_groups`` neighbouring channels, in fp32.  weight, bias: ``[C]`` or
     None; activation: None, "relu" or "silu".  Differentiable in x, weight and
-    bias (once)."""
+    bias (once, in reverse mode: forward-mode tangents are refused)."""
     if x.dim() < 2:
         raise ValueError(f"group_norm_act: x must be [N, ..., C], got shape {tuple(x.shape)}")
     C = x.shape[-1]
@@ -110,6 +110,7 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     for t, nm in ((weight, "weight"), (bias, "bias")):
         if t is not None and (t.shape != (C,) or not t.is_floating_point()):
             raise ValueError(f"group_norm_act: {nm} must be [{C}] floating point, got {tuple(t.shape)} {t.dtype}")
+    _lib.require_no_tangent("group_norm_act", x, weight, bias)
     _lib.require_cuda(x, weight, bias)
     x = _whole(x)
     w, b = (None if t is None else _whole(t.to(torch.float32)) for t in (weight, bias))
