@@ -58,7 +58,7 @@ def _f32(t):
 
 
 def _offsets(name, cu_seqlens, dev):
-    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point():
+    if cu_seqlens.dim() != 1 or cu_seqlens.numel() < 1 or cu_seqlens.is_floating_point() or cu_seqlens.is_complex():
         raise ValueError(f"{name}: cu_seqlens must be integers [N + 1], got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
     return cu_seqlens.to(device=dev, dtype=torch.int64).contiguous()
 
@@ -78,7 +78,7 @@ def _recurrent(q, k, v, g, beta, cu, n_seq, scale, h0, ht, state_idx=None, statu
     with _lib.on_device_of(q):
         st = _lib.load().ssla_gated_delta_recurrent(
             P(q), P(k), P(v), P(g), P(beta), P(cu), n_seq, T, Hk, H, K, V, float(scale), P(h0), P(o), P(ht),
-            P(state_idx), 0 if state_idx is None else h0.shape[0], P(status), _lib.DTYPE_CODE[q.dtype],
+            P(state_idx), 0 if state_idx is None else min(h0.shape[0], 0x7fffffff), P(status), _lib.DTYPE_CODE[q.dtype],
             _lib.stream_of(q))
     _lib.check(st, "ssla_gated_delta_recurrent")
     return o
@@ -257,10 +257,10 @@ def fused_recurrent_gated_delta(
 
 
 def _sites(name, idx, n):
-    if idx.shape != (n,) or idx.is_floating_point():
+    if idx.shape != (n,) or idx.is_floating_point() or idx.is_complex():
         raise ValueError(f"{name}: the site list must be integers [{n}], got {idx.dtype} {tuple(idx.shape)}")
-    if idx.dtype is torch.int64:   # (kept out of range where 32 bits do not hold it)
-        idx = idx.clamp(-1, 0x7fffffff)
+    if idx.dtype.itemsize == 8:   # (kept out of range where 32 bits do not hold it)
+        idx = idx.to(torch.int64).clamp(-1, 0x7fffffff)
     return (idx if idx.dtype is torch.int32 else idx.to(torch.int32)).contiguous()
 
 
