@@ -190,9 +190,12 @@ def chunk_gated_delta(
     final state ``[N, H, K, V]`` or None.  ``scale`` defaults to ``K ** -0.5``.
     Rows of o outside ``[cu_seqlens[0], cu_seqlens[-1])`` are unspecified.
 
-    K up to 128 runs the chunk kernels (chunks of 64 tokens), whose products keep
-    the precision of fp32 for every dtype, and is differentiable in q, k, v, g, beta and the
-    initial state (once; rows in no sequence get zeros).  Without a
+    K up to 128 runs the chunk kernels (chunks of 64 tokens) and is differentiable
+    in q, k, v, g, beta and the initial state (once; rows in no sequence get zeros).
+    Their products keep the precision of fp32 for states, gradients and the o of
+    fp32 inputs; o of 16-bit inputs leaves out up to 2^-15 of its terms (2^-18 in the
+    mean) before its own rounding.  Gates may be positive, but no more than 88 in sum from a
+    chunk's first token on (e^88 is the end of fp32).  Without a
     gradient, where sequences are so short on average that chunks would stay
     mostly empty, those of up to 64 rows run the token-by-token kernel, longer ones
     the chunk kernels (told on the device); wider keys (K up to 256) run token by
