@@ -273,9 +273,10 @@ int ssla_gated_delta_chunk_fwd(const void *q, const void *k, const void *v, cons
 /* The same sequences, each by the kernel for its length: up to 64 rows as
  * ssla_gated_delta_recurrent, longer ones as ssla_gated_delta_chunk_fwd (K <= 128).
  * For batches of many short sequences that may hold long ones; the lengths are
- * read on the device.  Workspace:
- * ssla_gated_delta_mixed_workspace_size bytes, 16-byte aligned, no
- * initialisation. */
+ * read on the device.  Rows too wide for the chunk kernels' 32-bit offsets run
+ * token by token whatever their sequence's length.  Workspace:
+ * ssla_gated_delta_mixed_workspace_size bytes (0: none; else mostly 430 a row and
+ * head), 16-byte aligned, no initialisation. */
 size_t ssla_gated_delta_mixed_workspace_size(int64_t T, int H, int K, int V);
 int ssla_gated_delta_mixed_fwd(const void *q, const void *k, const void *v, const float *g, const float *beta,
                                const int64_t *cu_seqlens, int n_seq, int64_t T, int Hk, int H, int K, int V,

@@ -873,8 +873,17 @@ extern "C" size_t ssla_gated_delta_chunk_segments_size(int n_seq, int64_t T, int
   return ssla::delta_layout(n_seq, T, H, H, K, V, false).seg_bytes;
 }
 
+namespace ssla {
+namespace {
+
+// Rows too wide for the chunk kernels' offsets, but not for a token's.
+bool tokens_alone(int H, int K, int V) { return check_widths("gated_delta_mixed_fwd", kChunk, 1, H, K, V) != SSLA_OK; }
+
+}  // namespace
+}  // namespace ssla
+
 extern "C" size_t ssla_gated_delta_mixed_workspace_size(int64_t T, int H, int K, int V) {
-  if (T < 0 || H <= 0 || K <= 0 || K > 128 || V <= 0) return 0;
+  if (T < 0 || H <= 0 || K <= 0 || K > 128 || V <= 0 || ssla::tokens_alone(H, K, V)) return 0;
   return ssla::delta_layout(1, T, H, H, K, V, false, true).total;
 }
 
@@ -901,6 +910,12 @@ int chunk_fwd(const char *what, bool mixed, const void *q, const void *k, const 
   if (n_seq == 0) return SSLA_OK;
   SSLA_CHECK_ARG(cu_seqlens != nullptr, "%s: cu_seqlens is NULL", what);
   SSLA_CHECK_ARG(T == 0 || (q && k && v && g && beta && o), "%s: null tensor pointer", what);
+  if (mixed && tokens_alone(H, K, V)) {
+    clear_error();
+    if (const int e = check_widths(what, 16, Hk, H, K, V)) return e;
+    return delta_recurrent_up_to(what, INT64_MAX, q, k, v, g, beta, cu_seqlens, n_seq, T, Hk, H, K, V, scale, h0, o, ht,
+                                 nullptr, 0, nullptr, dtype, st);
+  }
   if (const int e = check_widths(what, kChunk, Hk, H, K, V)) return e;
   const DeltaLayout L = delta_layout(n_seq, T, Hk, H, K, V, false, mixed);
   if (!workspace || workspace_bytes < L.total || !aligned(workspace, 16)) {

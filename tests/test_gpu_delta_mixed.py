@@ -112,3 +112,25 @@ def test_captured_with_offsets_that_change(dev):
         eo, eh = chunk_gated_delta(*d, offsets(lens), initial_state=s0, output_final_state=True)
         torch.cuda.synchronize()
         assert torch.equal(o, eo) and torch.equal(ht, eh), lens[:3]
+
+
+def test_rows_too_wide_for_chunks(dev):
+    """Rows that only the token kernel's offsets reach run token by token, whatever
+    their lengths (ssla_gated_delta_mixed_fwd takes no workspace then)."""
+    from ssla_amd import _lib
+    from ssla_amd.delta import chunk_gated_delta, fused_recurrent_gated_delta
+    H, K, V, lens = 1 << 17, 64, 1, [1, 120, 1, 2, 9]
+    assert _lib.load().ssla_gated_delta_mixed_workspace_size(sum(lens), H, K, V) == 0
+    gen = torch.Generator(device=dev).manual_seed(1)
+    T = sum(lens)
+    q, k = (torch.nn.functional.normalize(torch.randn(T, 1, K, generator=gen, device=dev), dim=-1) for _ in range(2))
+    v = torch.randn(T, H, V, generator=gen, device=dev)
+    g, beta = -torch.rand(T, H, generator=gen, device=dev), torch.rand(T, H, generator=gen, device=dev)
+    cu = torch.tensor([0] + lens, device=dev).cumsum(0)
+    o, ht = chunk_gated_delta(q, k, v, g, beta, cu, output_final_state=True)
+    to, ts = fused_recurrent_gated_delta(q, k, v, g, beta, cu, output_final_state=True)
+    assert torch.equal(o, to) and torch.equal(ht, ts)
+    at = [0, 77, H - 1]
+    ro, _ = gated_delta(*(t.cpu() for t in (q.expand(-1, 3, -1), k.expand(-1, 3, -1), v[:, at], g[:, at], beta[:, at])), lens,
+                        K ** -0.5)
+    close(o[:, at], ro, K, max(lens), torch.float32, "o")
