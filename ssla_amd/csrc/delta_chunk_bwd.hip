@@ -20,7 +20,7 @@
 // and column sums of the first kind are dot products of the rows of q and k with
 // the pieces of dq and dk, so no second Gram matrix is formed.
 // Measured at 8 sequences of 4096 rows, 8 heads of 64, bf16: reverse segments 59
-// us, fold 16, reverse walk 81, chunk gradients 160 (465 MB, 2.9 TB/s: bound by the
+// us, fold 16, reverse walk 81, chunk gradients 158 (495 MB, 3.1 TB/s: bound by the
 // loads of u, dX, S and D between barriers, VALU busy 51 % and matrix cores 22 % of
 // the time at four wavefronts a SIMD; 167 at two, where every wavefront had both
 // sides of its rows and the next loads in flight).

@@ -12,8 +12,11 @@
 // a token, twice the wavefronts) for batches that leave SIMDs without one.  Tokens are fetched BT at a time with
 // 16-byte loads while the block before runs, and parked in LDS of the wavefront's
 // own as fp32, with the decays and the products k . q, so a token's chain is the
-// sum S^T k, u and the update.  Bound by issue (4,510 histories of 13 tokens, 4
-// heads of 32, fp32: 87 us, 3.1 TB/s), long histories by the chain, 0.21 us a token.
+// sum S^T k, u and the update.  Bound by vector instructions (4,510 histories of 13
+// tokens, 4 heads of 32, fp32: 87 us, 3.1 TB/s; VALU busy 66 % of the time, 69
+// instructions a token and 16 columns where its formula takes about 50: blocks are
+// staged and dotted for 16 tokens), long histories by the chain, 0.20 us a token of
+// 32 keys, 0.27 of 64 and 0.41 of 128.
 //
 // Single tokens: one wavefront per (row, head, 4 VL value columns), the whole of
 // a state's columns in registers as 16-byte pieces, every load in flight at once.
