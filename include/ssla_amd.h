@@ -255,10 +255,12 @@ int ssla_gated_delta_recurrent(const void *q, const void *k, const void *v, cons
  * bf16: three for states, u, gradients and the o of fp32 inputs, which keeps the
  * precision of fp32; two where only a 16-bit o follows (up to 2^-15 of its
  * terms, 2^-18 in the mean, before its rounding).  K <= 128, any V up to 2^20.
- * Gates may be positive, at most 88 in sum from a chunk's first row on.  A row
- * whose g, beta or k . k is not finite (a g of -inf is) makes its head's o and
- * state NaN from that row on, one of v its column; earlier rows keep their
- * values.  ht must not overlap h0.  Workspace:
+ * Gates may be positive; the precision holds while consecutive ones inside a chunk
+ * are at most 64 in sum, and past 88 values are not finite; values smaller than
+ * 2^-110 keep fewer bits (their parts are not normal).  A row whose g, beta or
+ * k . k is not finite (a g of -inf is) makes its head's o and state NaN from that
+ * row on, one of v its column; earlier rows keep their values.  ht must not
+ * overlap h0.  Workspace:
  * ssla_gated_delta_chunk_workspace_size bytes, 16-byte aligned, no
  * initialisation.  segments (NULL, or ssla_gated_delta_chunk_segments_size bytes,
  * 16-byte aligned) receives the states and maps of the segments that long

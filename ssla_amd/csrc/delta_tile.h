@@ -7,7 +7,8 @@
 // up to 2^-24 of the operands' product, 2^-27 in the mean (computed for random
 // values).  Where only an o of 16 bits follows: two parts an operand and orders up to
 // one, which leaves out up to 2^-15, 2^-18 in the mean; o's own rounding is up to 2^-8
-// (bf16) or 2^-11 (fp16).  States, sums and the values that are carried on keep the precision of fp32 that way, at a sixth of the bf16
+// (bf16) or 2^-11 (fp16).  Parts below 2^-126 count as 0 in the products, so values
+// below 2^-110 have less than three.  States, sums and the values that are carried on keep the precision of fp32 that way, at a sixth of the bf16
 // rate for two fp32 operands and a third where one is a bf16 input; the fp32
 // matrix instructions run at a sixteenth.
 //

@@ -194,8 +194,11 @@ def chunk_gated_delta(
     in q, k, v, g, beta and the initial state (once; rows in no sequence get zeros).
     Their products keep the precision of fp32 for states, gradients and the o of
     fp32 inputs; o of 16-bit inputs leaves out up to 2^-15 of its terms (2^-18 in the
-    mean) before its own rounding.  Gates may be positive, but no more than 88 in sum from a
-    chunk's first token on (e^88 is the end of fp32).  Without a
+    mean) before its own rounding.  Gates may be positive; the precision holds while no
+    consecutive ones inside a chunk are more than 64 in sum (a state that grew by
+    more and fades again meets decays whose parts fp32's normal numbers do not
+    hold), and past 88 (the end of fp32) values are not finite.  Values smaller than
+    2^-110 keep fewer bits for the same reason.  Without a
     gradient, where sequences are so short on average that chunks would stay
     mostly empty, those of up to 64 rows run the token-by-token kernel, longer ones
     the chunk kernels (told on the device); wider keys (K up to 256) run token by

@@ -90,3 +90,54 @@ def compare(dev, dtype, x, s0, do, dht, scale):
             t = t + HALF[dtype] * rms(r) + (2.0 ** -15 * rms(r) if name == "o" else 0.0)
         off = rms(a.double().cpu() - r)
         assert off <= t, f"{name}: {off:.3g}, bound {t:.3g}, of {rms(r):.3g}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("total", [63.0, 87.0])
+def test_gates_up_to_the_stated_sum(dev, total):
+    """Consecutive positive gates from a state of zeros, and back again.  Up to 64 in
+    sum every token is as near as its state's size allows (its o is scale S^T q: off
+    by at most the bound of test_gpu_delta_chunk, (K + 256) T half steps, of scale sum
+    |q| max |S|); up to 88 values are finite.  (A decay of e^-64 = 2^-92.3 has a third
+    part of 2^-108 or more, of e^-87 = 2^-125.5 one below 2^-126, the smallest normal
+    number, which counts as 0 in the products.)"""
+    from ssla_amd.delta import _chunk_fwd, fused_recurrent_gated_delta
+    K = V = 32
+    x, _, _, _, scale = case("fading", torch.float32, K, V, T=90)
+    q, k, v, g, beta = x
+    g[:] = -0.01
+    g[2:8], g[20:26] = total / 6, -total / 6
+    g[64:70], g[75:81] = total / 6, -total / 6
+    S, ref, tol = torch.zeros(H, K, V, dtype=torch.float64), [], []
+    for t in range(90):
+        o, S, _ = form.forward(*(a[t:t + 1] for a in x), scale, S)
+        ref.append(o)
+        tol.append((K + 256) * 90 * 2.0 ** -24 * scale * q[t].double().abs().sum(-1) * S.abs().amax((1, 2)))
+    ref, tol = torch.cat(ref), torch.stack(tol)[..., None]
+    d, cu = [t.to(dev) for t in x], torch.tensor([0, 90], device=dev)
+    chunks, tokens = _chunk_fwd(*d, cu, scale, None, False)[0], fused_recurrent_gated_delta(*d, cu, scale=scale)[0]
+    assert torch.isfinite(chunks).all()
+    for o in (tokens, chunks) if total <= 64 else (tokens,):
+        err = (o.double().cpu() - ref).abs()
+        assert bool((err <= tol).all()), float((err / tol).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("power", [-90, 90])
+@pytest.mark.parametrize("K,V", [(64, 64), (32, 20)])
+def test_small_and_large_values(dev, power, K, V):
+    """The rule is linear in v: values 2^power times as large give results that are,
+    bit for bit (dv apart, which v does not enter)."""
+    from ssla_amd.delta import chunk_gated_delta
+    x, _, do, _, scale = case("long memory", torch.float32, K, V, T=600)
+
+    def run(v):
+        leaves = [t.to(dev).requires_grad_() for t in (x[0], x[1], v, x[3], x[4])]
+        o, ht = chunk_gated_delta(*leaves, torch.tensor([0, 600], device=dev), scale=scale, output_final_state=True)
+        dq, dk, dv, dg, db = torch.autograd.grad(o, leaves, do.to(dev))
+        return [t.detach() for t in (o, ht, dq, dk, dg, db)], dv
+
+    (one, dv1), (other, dv2) = run(x[2]), run(x[2] * 2.0 ** power)
+    assert torch.equal(dv1, dv2)
+    for name, a, b in zip(("o", "ht", "dq", "dk", "dg", "dbeta"), one, other):
+        assert torch.equal(a * 2.0 ** power, b), name
