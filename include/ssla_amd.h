@@ -344,6 +344,42 @@ int ssla_diag_scan_bwd(const float *dout, const float *g, const float *h,
                        const int64_t *cu_seqlens, int n_seq, int64_t T,
                        int C, float *du, float *dg, void *stream);
 
+/* Gated linear recurrence over packed sequences (no reference counterpart; the
+ * diagonal scan above with states, gates and a read-out of its own):
+ *   h_t = a_t h_{t-1} + u_t,   o_t = q_t h_t  (q NULL: o_t = h_t)
+ * with a_t = g_t, e^(g_t) or sigmoid(g_t) (SSLA_GATE_*), from h0 (fp32
+ * [n_seq, C]; NULL: zeros) to ht (fp32 [n_seq, C], may be NULL; an empty
+ * sequence's is its h0).  u, q: [T, C] of dtype `dtype`, g of `dtype` or fp32,
+ * rows ldu, ldq, ldg elements apart; o [T, C] contiguous.  Rows in no sequence
+ * are written with zeros.  keep: NULL, or ssla_gated_scan_keep_size bytes that
+ * the forward fills for the backward.  The backward takes dout [T, C] and dht
+ * (fp32 [n_seq, C] or NULL) and writes du, dq (dtype; dq only with q), dg
+ * (g_dtype), all [T, C], and dh0 (fp32 [n_seq, C], may be NULL).
+ * Workspace: ssla_gated_scan_workspace_size bytes, 16-byte aligned, no
+ * initialisation, one for each call in flight; 0: none. */
+enum { SSLA_GATE_VALUE = 0, SSLA_GATE_LOG = 1, SSLA_GATE_SIGMOID = 2 };
+size_t ssla_gated_scan_workspace_size(int64_t T, int C);
+size_t ssla_gated_scan_keep_size(int64_t T, int C);
+int ssla_gated_scan_fwd(const void *u, int64_t ldu, const void *g, int64_t ldg, const void *q, int64_t ldq,
+                        const int64_t *cu_seqlens, int n_seq, int64_t T, int C, int gate, const float *h0,
+                        void *o, float *ht, void *keep, int dtype, int g_dtype, void *workspace,
+                        size_t workspace_bytes, void *stream);
+int ssla_gated_scan_bwd(const void *u, int64_t ldu, const void *g, int64_t ldg, const void *q, int64_t ldq,
+                        const int64_t *cu_seqlens, int n_seq, int64_t T, int C, int gate, const float *h0,
+                        const void *keep, const void *dout, const float *dht, void *du, void *dg, void *dq,
+                        float *dh0, int dtype, int g_dtype, void *workspace, size_t workspace_bytes,
+                        void *stream);
+
+/* One token of each active row of a state table (fp32 [n_rows, C], updated in
+ * place): the recurrence above on a sequence of one row per entry of row_idx
+ * (strictly increasing, inside [0, n_rows)), whose state is state[row_idx[i]].
+ * u, g, q, o: n_active rows.  An entry that is out of range or not above the one
+ * before it is skipped: its o row is zeros, no state changes, and SSLA_ERR_ARG is
+ * stored in *status (device int32, may be NULL; see ssla_status_read). */
+int ssla_sparse_gated_step(const int32_t *row_idx, int n_active, const void *u, int64_t ldu, const void *g,
+                           int64_t ldg, const void *q, int64_t ldq, float *state, int n_rows, int C, int gate,
+                           void *o, int32_t *status, int dtype, int g_dtype, void *stream);
+
 /* One time bin of the per-site matrix-state GLA update.  For active site
  * i (site = site_idx[i], strictly increasing, inside [0, n_sites)):
  *   S[site] <- diag(exp(g_i)) S[site] + k_i v_i^T ;  o_i = (scale q_i)^T S[site]

@@ -73,6 +73,14 @@ SIGNATURES = {
                                       _f32, _vp, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _sz, _vp]),
     "ssla_diag_scan_fwd": (_i32, [_vp, _vp, _vp, _i32, _i64, _i32, _vp, _vp]),
     "ssla_diag_scan_bwd": (_i32, [_vp, _vp, _vp, _vp, _i32, _i64, _i32, _vp, _vp, _vp]),
+    "ssla_gated_scan_workspace_size": (_sz, [_i64, _i32]),
+    "ssla_gated_scan_keep_size": (_sz, [_i64, _i32]),
+    "ssla_gated_scan_fwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32,
+                                   _i32, _vp, _sz, _vp]),
+    "ssla_gated_scan_bwd": (_i32, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp,
+                                   _vp, _vp, _vp, _i32, _i32, _vp, _sz, _vp]),
+    "ssla_sparse_gated_step": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i32, _i32, _vp, _vp, _i32,
+                                      _i32, _vp]),
     "ssla_sparse_gla_step": (_i32, [_vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i32,
                                     _f32, _vp, _vp, _vp]),
     "ssla_gated_delta_recurrent": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
