@@ -18,10 +18,12 @@
 // were known.  A tile with a sequence's start publishes its leaving state at once.
 // Tiles are handed out in order by a ticket and publish before they wait, so every
 // tile waited for has started and the wait ends.  A word says by itself whether it
-// is there (an all-ones word is not): no fences.
+// is there, a map or a state: no fences.
 // The backward does the same from the last tile on; the states it needs come from
 // the forward, which leaves one every 64 rows, and are computed again in between.
 #include "vec.h"
+
+#include <type_traits>
 
 namespace ssla {
 namespace {
@@ -31,28 +33,38 @@ constexpr int kValue = SSLA_GATE_VALUE, kLog = SSLA_GATE_LOG, kSigmoid = SSLA_GA
 // e^x with the product x log2(e) in two parts: off by 4 2^-24 at any x whose e^x is a
 // normal number (e^x of one product by up to 100 2^-24).
 __device__ __forceinline__ float exp_of(float x) {
-  const float y = x * kLog2e;
-  const float e = fast_exp2(y);
-  return fabsf(y) < 126.f ? fmaf(e * 0.6931472f, fmaf(x, 1.925963e-8f, fmaf(x, kLog2e, -y)), e) : e;   // (past that 0, infinite or near it)
+  const float y = x * kLog2e, e = fast_exp2(y);
+  const float lo = fmaf(x, 1.925963e-8f, fmaf(x, kLog2e, -y));
+  return fabsf(y) < 126.f ? fmaf(e, lo * 0.6931472f, e) : e;   // (past that 0, infinite or near it)
 }
 
-// The gate and its derivative.  sigmoid from e^-|g|: both it and 1 - it keep their
-// relative precision on either side.
+// The gate; and with its derivative, sigmoid's from e^-|g|: both it and 1 - it keep
+// their relative precision on either side.
 struct Gate { float a, slope; };
-__device__ __forceinline__ Gate gate_of(int kind, float g) {
-  if (kind == kValue) return {g, 1.f};
-  if (kind == kLog) {
-    const float a = exp_of(g);
-    return {a, a};
+template <int KIND>
+__device__ __forceinline__ float gate_value(float g) {
+  if constexpr (KIND == kValue) return g;
+  if constexpr (KIND == kLog) return exp_of(g);
+  return __builtin_amdgcn_rcpf(1.f + exp_of(-g));   // (e^-g infinite: 0)
+}
+template <int KIND>
+__device__ __forceinline__ Gate gate_of(float g) {
+  if constexpr (KIND == kSigmoid) {
+    const float t = exp_of(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + t), s = t * r;
+    return {g >= 0.f ? r : s, r * s};
   }
-  const float t = exp_of(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + t), s = t * r;
-  return {g >= 0.f ? r : s, r * s};
+  const float a = gate_value<KIND>(g);
+  return {a, KIND == kLog ? a : 1.f};
 }
 
-constexpr int R = 8;             // rows of a lane
+constexpr int kFwdRows = 8, kBwdRows = 4;   // rows of a lane
+constexpr int kMostRows = 8;
 constexpr int kBlock = 256;
 constexpr int kKeepRows = 64;    // rows between the states left for the backward
-constexpr int kMostValues = kBlock * 8;   // (row group, channel) pairs of a tile
+constexpr int kMostLanes = 16;   // lanes of a row
+constexpr int kMostGroups = 64;  // row groups of a tile
+constexpr int kMostValues = kBlock * 4;   // (row group, channel) pairs of a tile
+constexpr int kMostWidth = 1 << 20;       // elements from row to row: offsets in a tile are 32 bits
 
 struct ScanArgs {
   const void *u, *g, *q, *dout;   // q may be NULL
@@ -65,10 +77,10 @@ struct ScanArgs {
   void *o, *du, *dg, *dq;
   float *ht, *dh0, *keep;         // may be NULL (keep: not in the backward)
   int CT, RG, cblocks;            // lanes of a row, row groups, channel blocks
-  int64_t tiles;
+  int tiles;                      // of rows
   uint32_t *ticket;               // NULL: one tile of rows
-  uint64_t *maps;                 // [tiles][cblocks CT W]: A and U
-  uint32_t *states;               // the state that leaves a tile
+  uint64_t *words;                // [tiles][cblocks CT W]: what a tile says of itself
+  uint32_t *hints;                // [cblocks][tiles]
 };
 
 // ------------------------------------------------------- tiles and sequences --
@@ -76,67 +88,76 @@ struct ScanArgs {
 // kOutside of all sequences; fin[row] the sequence that ends with the row, or -1.
 constexpr int kInside = -1, kOutside = -2;
 
+struct Span { int64_t b, e; };   // a sequence's rows
+__device__ __forceinline__ Span span_of(const ScanArgs &a, int n) {
+  Span s;
+  s.b = min(max(a.cu[n], (int64_t)0), a.T);
+  s.e = min(max(a.cu[n + 1], s.b), a.T);
+  return s;
+}
+
 // Fills mark and fin of the rows r0 .. r0 + rows; false where all rows are kInside
-// and none ends a sequence.  Two rounds of 256 probes for up to 65,536 sequences.
-__device__ bool mark_rows(const ScanArgs &a, int64_t r0, int rows, int *mark, int *fin) {
+// and none ends a sequence.  `mine`: sequence threadIdx.x, `all` the rows of any.  More
+// than kBlock sequences are searched, two rounds of probes for up to 65,536.
+__device__ __forceinline__ bool mark_rows(const ScanArgs &a, const Span &mine, const Span &all, int64_t r0, int rows, int *mark,
+                                          int *fin) {
   const int tid = threadIdx.x;
-  for (int i = tid; i < rows; i += kBlock) {
-    mark[i] = kInside;
-    fin[i] = -1;
-  }
-  if (a.n_seq == 0) {
-    __syncthreads();
-    for (int i = tid; i < rows; i += kBlock) mark[i] = kOutside;
-    __syncthreads();
-    return true;
-  }
-  int lo = 0, hi = a.n_seq;   // the last sequence that begins at r0 or before is in [lo, hi)
-  while (hi - lo > kBlock) {  // (the same for all threads)
-    const int step = (hi - lo + kBlock - 1) / kBlock;
-    const int64_t i = lo + static_cast<int64_t>(tid) * step;
-    const int cnt = __syncthreads_count(i < hi && a.cu[i] <= r0);
-    lo += max(cnt - 1, 0) * step;
-    hi = min(hi, lo + step);
-  }
-  const int64_t first = min(max(a.cu[0], (int64_t)0), a.T), last = min(max(a.cu[a.n_seq], first), a.T);
-  __syncthreads();
   bool some = false;
-  for (int n0 = lo; n0 < a.n_seq; n0 += kBlock) {
-    const int n = n0 + tid;
-    bool past = true;
-    if (n < a.n_seq) {
-      const int64_t b = min(max(a.cu[n], (int64_t)0), a.T), e = min(max(a.cu[n + 1], b), a.T);
-      past = b >= r0 + rows;
-      if (e > b) {
-        if (b >= r0 && b < r0 + rows) {
-          mark[b - r0] = n;
-          some = true;
-        }
-        if (e > r0 && e <= r0 + rows) {
-          fin[e - 1 - r0] = n;
-          some = true;
-        }
+  for (int i = tid; i < rows; i += kBlock) {
+    const bool out = r0 + i < all.b || r0 + i >= all.e;
+    mark[i] = out ? kOutside : kInside;
+    fin[i] = -1;
+    some |= out;
+  }
+  auto put = [&](const Span &s, int n) {
+    if (s.e > s.b) {
+      if (s.b >= r0 && s.b < r0 + rows) {
+        mark[s.b - r0] = n;
+        some = true;
+      }
+      if (s.e > r0 && s.e <= r0 + rows) {
+        fin[s.e - 1 - r0] = n;
+        some = true;
       }
     }
-    if (__syncthreads_or(past)) break;
-  }
-  for (int i = tid; i < rows; i += kBlock)
-    if (r0 + i < first || r0 + i >= last) {
-      mark[i] = kOutside;
-      some = true;
+  };
+  if (a.n_seq <= kBlock) {   // (the same for all threads)
+    __syncthreads();
+    if (tid < a.n_seq) put(mine, tid);
+  } else {
+    int lo = 0, hi = a.n_seq;   // the last sequence that begins at r0 or before is in [lo, hi)
+    while (hi - lo > kBlock) {
+      const int step = (hi - lo + kBlock - 1) / kBlock;
+      const int64_t i = lo + static_cast<int64_t>(tid) * step;
+      const int cnt = __syncthreads_count(i < hi && a.cu[i] <= r0);
+      lo += max(cnt - 1, 0) * step;
+      hi = min(hi, lo + step);
     }
+    for (bool past = false; lo < a.n_seq && !past; lo += kBlock) {
+      const int n = lo + tid;
+      Span s{r0 + rows, 0};
+      if (n < a.n_seq) s = span_of(a, n);
+      past = __syncthreads_or(s.b >= r0 + rows);
+      put(s, n);
+    }
+  }
   return __syncthreads_or(some);
 }
 
 // --------------------------------------------------- states between the tiles --
-constexpr uint32_t kNone32 = 0xffffffffu;
-constexpr uint64_t kNone64 = ~0ull;
+// A tile's word in a channel: nothing yet (all ones), its map (A low, U high), or the
+// state that leaves it (kState low, the state high).
+constexpr uint64_t kNone = ~0ull;
+constexpr uint32_t kState = 0xfffffffeu;
 
-// A value's bits as a word that can be told from one that is not there.
-__device__ __forceinline__ uint32_t word_of(float x) {
-  const uint32_t b = __float_as_uint(x);
-  return b == kNone32 ? 0x7fc00000u : b;
+__device__ __forceinline__ uint64_t state_word(float x) {
+  return static_cast<uint64_t>(__float_as_uint(x)) << 32 | kState;
 }
+__device__ __forceinline__ uint64_t map_word(float A, float U) {   // (a NaN of A's like the marks is made the usual one)
+  const uint32_t b = __float_as_uint(A);
+  return static_cast<uint64_t>(__float_as_uint(U)) << 32 | (b >= kState ? 0x7fc00000u : b);
+}
+__device__ __forceinline__ bool is_state(uint64_t w) { return static_cast<uint32_t>(w) == kState; }
 template <typename T>
 __device__ __forceinline__ T look(const T *p) {
   return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -147,53 +168,28 @@ __device__ __forceinline__ void show(T *p, T x) {
 }
 // (a factor that overflowed must not meet a state of zero)
 __device__ __forceinline__ float apply(float A, float x, float U) { return x == 0.f ? U : fmaf(A, x, U); }
-__device__ __forceinline__ float apply(uint64_t m, float x) {
-  return apply(__uint_as_float(static_cast<uint32_t>(m)), x, __uint_as_float(static_cast<uint32_t>(m >> 32)));
+// The state behind a tile that x enters: the same bits whichever of its words was there.
+__device__ __forceinline__ float apply(uint64_t w, float x) {
+  const float U = __uint_as_float(static_cast<uint32_t>(w >> 32));
+  return is_state(w) ? U : apply(__uint_as_float(static_cast<uint32_t>(w)), x, U);
 }
 
-// The state that enters tile k > 0 in column c of `wide`.
-__device__ float entering_state(const ScanArgs &a, int64_t k, int64_t c, int64_t wide) {
-  constexpr int NW = 8;   // tiles of a round trip
-  const uint64_t *maps = a.maps + c;
-  const uint32_t *states = a.states + c;
-  int64_t near = k - 1;
-  for (;;) {
-    uint64_t m[NW];
-    uint32_t s[NW];
-#pragma unroll
-    for (int i = 0; i < NW; ++i) {
-      const int64_t at = max(near - i, (int64_t)0) * wide;
-      s[i] = look(states + at);
-      m[i] = look(maps + at);
-    }
-    int found = -1, ready = NW;
-#pragma unroll
-    for (int i = NW - 1; i >= 0; --i) {
-      if (s[i] != kNone32) found = i;
-      else if (m[i] == kNone64) {
-        ready = i;
-        found = -1;
-      }
-    }
-    // (found: the nearest known state, with every map this side of it)
-    if (found >= 0) {
-      float x = 0.f;
-#pragma unroll
-      for (int i = NW - 1; i >= 0; --i) {
-        if (i == found) x = __uint_as_float(s[i]);
-        else if (i < found) x = apply(m[i], x);
-      }
-      // the maps of the rounds before this one
-      for (int64_t at = near + 1; at < k; at += NW) {
-#pragma unroll
-        for (int i = 0; i < NW; ++i) m[i] = look(maps + min(at + i, k - 1) * wide);
-#pragma unroll
-        for (int i = 0; i < NW; ++i)
-          if (at + i < k) x = apply(m[i], x);
-      }
-      return x;
-    }
-    if (ready == NW) near -= NW;
+// What a tile has published in a channel block, told by a word of its own next to its
+// neighbours': a wavefront sees 64 tiles at one read.  Only a hint where to look:
+// the words say by themselves whether they are there.
+constexpr uint32_t kNoHint = ~0u, kMapHint = 1, kStateHint = 2;
+
+// The nearest tile before k > 0 whose state is known, with maps from there on; for a
+// whole wavefront.
+__device__ __forceinline__ int known_tile(const uint32_t *hints, int k) {
+  const int lane = threadIdx.x & 63;
+  for (int near = k - 1;;) {
+    const int t = near - lane;
+    const uint32_t h = t >= 0 ? look(hints + t) : kMapHint;
+    const uint64_t states = __ballot(h == kStateHint), nothing = __ballot(h == kNoHint);
+    const int s = states ? __builtin_ctzll(states) : 64, n = nothing ? __builtin_ctzll(nothing) : 64;
+    if (s < n) return near - s;
+    if (n == 64) near -= 64;   // (tile 0 is known or not there: it stays at 0 or above)
     else __builtin_amdgcn_s_sleep(1);
   }
 }
@@ -201,23 +197,23 @@ __device__ float entering_state(const ScanArgs &a, int64_t k, int64_t c, int64_t
 __global__ __launch_bounds__(256) void scan_clear_kernel(uint32_t *ticket, uint64_t *words, int64_t n) {
   if (blockIdx.x == 0 && threadIdx.x == 0) *ticket = 0;
   for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256)
-    words[i] = kNone64;
+    words[i] = kNone;
 }
 
 // Which tile and channel block a workgroup has.
-__device__ __forceinline__ int64_t take_tile(const ScanArgs &a, uint32_t *slot) {
+__device__ __forceinline__ int take_tile(const ScanArgs &a, uint32_t *slot) {
   if (!a.ticket) return blockIdx.x;
   if (threadIdx.x == 0) *slot = atomicAdd(a.ticket, 1u);
   __syncthreads();
-  return *slot;
+  return __builtin_amdgcn_readfirstlane(*slot);
 }
 
 // Joins the maps of the RG row groups of channel c (LDS, `cw` channels a row group)
 // from the first or the last on; cut[k]: the state leaving group k is U, whatever enters.
-struct Joined { float A, U; bool cut; };
+struct Joined { float A, U; };
 template <bool BACK>
 __device__ __forceinline__ Joined join_groups(const float *A, const float *U, const int *cut, int RG, int cw, int c) {
-  Joined j{1.f, 0.f, false};
+  Joined j{1.f, 0.f};
 #pragma unroll 8
   for (int i = 0; i < RG; ++i) {
     const int k = BACK ? RG - 1 - i : i;
@@ -225,7 +221,6 @@ __device__ __forceinline__ Joined join_groups(const float *A, const float *U, co
     const bool r = cut[k];
     j.U = r ? y : apply(x, j.U, y);
     j.A *= x;
-    j.cut |= r;
   }
   return j;
 }
@@ -240,221 +235,334 @@ __device__ __forceinline__ void enter_groups(const float *A, float *U, const int
     x = cut[k] ? y : apply(f, x, y);
   }
 }
-// A channel's part between its maps: publishes, finds the entering state (`closed`:
-// the tile's first row takes none) and fills U.
+// What the threads share between a tile's maps.
+constexpr int kWords = 16;   // tiles of a round trip
+struct TileSmem {
+  float A[kMostValues], U[kMostValues];
+  uint64_t words[kWords * kMostLanes * 4];
+  int mark[kMostGroups * kMostRows], fin[kMostGroups * kMostRows], cut[kMostGroups];
+  int from;
+  uint32_t slot;
+};
+
+// Between a tile's maps, for the whole workgroup: publishes, finds the entering states
+// (`closed`: the tile's first row takes none) and fills U.  The threads from `first` on
+// have a channel each; all of them fetch the words.
 template <bool BACK>
-__device__ __forceinline__ void enter_tile(const ScanArgs &a, int64_t k, int64_t col, int64_t wide, const float *A, float *U,
-                                           const int *cut, bool closed, int cw, int c) {
+__device__ __forceinline__ void enter_tile(const ScanArgs &a, TileSmem &sm, float *U, int k, int cb, bool closed, int cw,
+                                           int first) {
+  const int tid = threadIdx.x, c = tid - first, mine = a.C - cb * cw;   // (channels that exist)
+  const bool on = c >= 0 && c < cw && c < mine;
   float x = 0.f;
   if (a.ticket) {
-    const Joined j = join_groups<BACK>(A, U, cut, a.RG, cw, c);
-    const int64_t at = k * wide + col;
-    const bool known = k == 0 || j.cut;
-    if (known) show(a.states + at, word_of(j.U));
-    else show(a.maps + at, static_cast<uint64_t>(word_of(j.A)) | static_cast<uint64_t>(__float_as_uint(j.U)) << 32);
+    const int64_t wide = static_cast<int64_t>(a.cblocks) * cw;
+    uint64_t *words = a.words + static_cast<int64_t>(cb) * cw;
+    uint32_t *hints = a.hints + static_cast<int64_t>(cb) * a.tiles;
+    bool known = k == 0;
+    Joined j{0.f, 0.f};
+    if (c >= 0 && c < 64) {   // (a whole wavefront)
+      known |= __any(c < a.RG && sm.cut[c] != 0);
+      if (on) {
+        j = join_groups<BACK>(sm.A, U, sm.cut, a.RG, cw, c);
+        show(words + k * wide + c, known ? state_word(j.U) : map_word(j.A, j.U));
+      }
+      if (c == 0) show(hints + k, known ? kStateHint : kMapHint);
+    }
     asm volatile("" ::: "memory");   // (published before anything is waited for)
-    if (k > 0 && !closed) x = entering_state(a, k, col, wide);
-    if (!known) show(a.states + at, word_of(apply(j.A, x, j.U)));
+    if (k > 0 && !closed) {
+      if (c >= 0 && c < 64) {
+        const int from = known_tile(hints, k);
+        if (c == 0) sm.from = from;
+      }
+      __syncthreads();
+      const int per = kBlock / cw, i0 = tid / cw, cc = tid - i0 * cw, from = __builtin_amdgcn_readfirstlane(sm.from);
+      for (int at = from; at < k; at += kWords) {
+        const int n = min(k - at, kWords);
+        if (i0 < per && cc < mine)
+          for (int i = i0; i < n; i += 4 * per) {
+            uint64_t w[4];
+            bool there;
+            do {   // (a word may come after its hint)
+              there = true;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int t = i + e * per;
+                w[e] = t < n ? look(words + (at + t) * wide + cc) : 0;
+                there = there && w[e] != kNone && (t > 0 || at > from || is_state(w[e]));
+              }
+            } while (!there);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (i + e * per < n) sm.words[(i + e * per) * cw + cc] = w[e];
+          }
+        __syncthreads();
+        if (on)
+          for (int i = 0; i < n; ++i) x = apply(sm.words[i * cw + c], x);
+        __syncthreads();
+      }
+    }
+    if (!known) {
+      if (on) show(words + k * wide + c, state_word(apply(j.A, x, j.U)));
+      if (c == 0) show(hints + k, kStateHint);
+    }
   }
-  enter_groups<BACK>(A, U, cut, a.RG, cw, c, x);
+  if (on) enter_groups<BACK>(sm.A, U, sm.cut, a.RG, cw, c, x);
 }
 
-template <int DT, int W>
-__device__ __forceinline__ void load_rows(Vec<DT, W> (&x)[R], const void *p, int64_t ld, int64_t row0, int64_t T, int c) {
+// R rows of W values from channel c of row `row` of a tile that begins at `first`, ld
+// apart; behind the last row that exists, that one again.
+template <int DT, int W, int R>
+__device__ __forceinline__ void load_rows(Vec<DT, W> (&x)[R], const void *p, int64_t first, int64_t ld, int row, int last, int c) {
+  const typename Elem<DT>::T *base = static_cast<const typename Elem<DT>::T *>(p) + first * ld;
 #pragma unroll
   for (int i = 0; i < R; ++i)
-    if (row0 + i < T) x[i] = load_vec<DT, W>(p, (row0 + i) * ld + c);
+    x[i] = load_vec<DT, W>(base, static_cast<uint32_t>(min(row + i, last)) * static_cast<uint32_t>(ld) + c);
+}
+
+// Keeps the values as they were read: without this their 32-bit forms are kept over
+// the wait, twice the registers.
+template <typename V, int R>
+__device__ __forceinline__ void as_read(V (&x)[R]) {
+  struct Raw { uint32_t w[(sizeof(V) + 3) / 4]; };
+  if constexpr (sizeof(V) % 4 == 0)
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      Raw r = __builtin_bit_cast(Raw, x[i]);
+#pragma unroll
+      for (uint32_t &w : r.w) asm volatile("" : "+v"(w));
+      x[i] = __builtin_bit_cast(V, r);
+    }
+}
+
+// f(i, e) of all values held.
+template <int R, int W, typename F>
+__device__ __forceinline__ void each(F f) {
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int e = 0; e < W; ++e) f(i, e);
+}
+// f(KIND as a constant) of a call's kind of gate: decided once for all values held.
+template <typename F>
+__device__ __forceinline__ void by_kind(int kind, F f) {
+  if (kind == kSigmoid) f(std::integral_constant<int, kSigmoid>());
+  else if (kind == kLog) f(std::integral_constant<int, kLog>());
+  else f(std::integral_constant<int, kValue>());
+}
+
+// The states of empty sequences, dealt over the tiles: what enters leaves.
+__device__ __forceinline__ void empty_states(const ScanArgs &a, const float *from, float *to, int k, int cb, int cw) {
+  const int c = cb * cw + threadIdx.x;
+  for (int64_t n = k; n < a.n_seq; n += a.tiles) {
+    const Span s = span_of(a, static_cast<int>(n));
+    if (s.e == s.b && static_cast<int>(threadIdx.x) < cw && c < a.C) to[n * a.C + c] = from ? from[n * a.C + c] : 0.f;
+  }
 }
 
 // ------------------------------------------------------------------ forward --
-template <int DT, int DTG, int W>
+template <int DT, int DTG, int W, bool READ>
 __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(const ScanArgs a) {
-  __shared__ float sA[kMostValues], sU[kMostValues];
-  __shared__ int mark[kBlock * R], fin[kBlock * R], cut[kBlock];
-  __shared__ uint32_t slot;
-  const int64_t id = take_tile(a, &slot);
-  const int64_t k = id / a.cblocks;
-  const int cb = static_cast<int>(id - k * a.cblocks), cw = a.CT * W, tid = threadIdx.x;
-  const int rg = tid / a.CT, cl = tid - rg * a.CT, rows = a.RG * R;
-  const int64_t r0 = k * rows, row0 = r0 + rg * R;
-  const int c = (cb * a.CT + cl) * W;
-  const bool on = rg < a.RG && c < a.C;
-  Vec<DT, W> u[R], q[R];
-  Vec<DTG, W> g[R];
-  if (on) {
-    load_rows<DT, W>(u, a.u, a.ldu, row0, a.T, c);
-    load_rows<DTG, W>(g, a.g, a.ldg, row0, a.T, c);
-    if (a.q) load_rows<DT, W>(q, a.q, a.ldq, row0, a.T, c);
+  constexpr int R = kFwdRows;
+  __shared__ TileSmem sm;
+  const int tid = threadIdx.x, cw = a.CT * W, rows = a.RG * R;
+  const int rg = tid / a.CT, cl = tid - rg * a.CT;
+  const Span all = a.n_seq ? Span{span_of(a, 0).b, span_of(a, a.n_seq - 1).e} : Span{0, 0};
+  const Span mine = tid < a.n_seq ? span_of(a, tid) : Span{0, 0};
+  const int id = take_tile(a, &sm.slot);
+  const int k = id / a.cblocks, cb = id - k * a.cblocks;
+  if (a.T == 0) {   // (one tile without rows)
+    if (a.ht) empty_states(a, a.h0, a.ht, k, cb, cw);
+    return;
   }
-  const bool some = mark_rows(a, r0, rows, mark, fin);
+  const int64_t r0 = static_cast<int64_t>(k) * rows;
+  const int row = rg * R;
+  const int exist = static_cast<int>(min(a.T - r0, static_cast<int64_t>(rows))), left = exist - row;
+  const bool on = rg < a.RG && (cb * a.CT + cl) * W < a.C;
+  const int c = on ? (cb * a.CT + cl) * W : 0;   // (lanes without a channel read the first)
+  Vec<DT, W> u[R], q[READ ? R : 1];
+  Vec<DTG, W> g[R];
+  load_rows<DT, W, R>(u, a.u, r0, a.ldu, row, exist - 1, c);
+  load_rows<DTG, W, R>(g, a.g, r0, a.ldg, row, exist - 1, c);
+  if constexpr (READ) load_rows<DT, W, R>(q, a.q, r0, a.ldq, row, exist - 1, c);
+  const bool some = mark_rows(a, mine, all, r0, rows, sm.mark, sm.fin);
   float f[R][W];
+  auto state0 = [&](int m, int e) { return a.h0 ? a.h0[static_cast<int64_t>(m) * a.C + c + e] : 0.f; };
+  by_kind(a.gate, [&](auto kind) { each<R, W>([&](int i, int e) { f[i][e] = gate_value<kind()>(g[i][e]); }); });
   if (on) {
-#pragma unroll
-    for (int i = 0; i < R; ++i)
-#pragma unroll
-      for (int e = 0; e < W; ++e) f[i][e] = gate_of(a.gate, g[i][e]).a;
     float A[W], U[W];
-    bool reset = false;
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       A[e] = 1.f;
       U[e] = 0.f;
     }
+    bool reset = false;
+    if (!some) {
+      each<R, W>([&](int i, int e) {
+        U[e] = fmaf(f[i][e], U[e], u[i][e]);
+        A[e] *= f[i][e];
+      });
+    } else {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int m = some ? mark[rg * R + i] : kInside;
-      if (m == kInside) {
+      for (int i = 0; i < R; ++i) {
+        const int m = sm.mark[row + i];
+        reset |= m != kInside;
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          U[e] = fmaf(f[i][e], U[e], u[i][e]);
+          U[e] = m == kOutside ? 0.f : fmaf(f[i][e], m >= 0 ? state0(m, e) : U[e], u[i][e]);
           A[e] *= f[i][e];
         }
-      } else {
-        reset = true;
-#pragma unroll
-        for (int e = 0; e < W; ++e)
-          U[e] = m < 0 ? 0.f : fmaf(f[i][e], a.h0 ? a.h0[static_cast<int64_t>(m) * a.C + c + e] : 0.f, u[i][e]);
       }
     }
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      sA[rg * cw + cl * W + e] = A[e];
-      sU[rg * cw + cl * W + e] = U[e];
+      sm.A[rg * cw + cl * W + e] = A[e];
+      sm.U[rg * cw + cl * W + e] = U[e];
     }
-    if (cl == 0) cut[rg] = reset;
+    if (cl == 0) sm.cut[rg] = reset;
   }
   __syncthreads();
-  const int64_t wide = static_cast<int64_t>(a.cblocks) * cw;
-  if (tid < cw && cb * cw + tid < a.C)
-    enter_tile<false>(a, k, static_cast<int64_t>(cb) * cw + tid, wide, sA, sU, cut, some && mark[0] != kInside, cw, tid);
+  enter_tile<false>(a, sm, sm.U, k, cb, some && sm.mark[0] != kInside, cw, 0);
   __syncthreads();
+  as_read(u);
+  if constexpr (READ) as_read(q);
   if (on) {
     float h[W];
 #pragma unroll
-    for (int e = 0; e < W; ++e) h[e] = sU[rg * cw + cl * W + e];
-    if (a.keep && row0 % kKeepRows == 0 && row0 < a.T)
+    for (int e = 0; e < W; ++e) h[e] = sm.U[rg * cw + cl * W + e];
+    if (a.keep && (r0 + row) % kKeepRows == 0 && left > 0)
 #pragma unroll
-      for (int e = 0; e < W; ++e) a.keep[row0 / kKeepRows * a.C + c + e] = h[e];
+      for (int e = 0; e < W; ++e) a.keep[(r0 + row) / kKeepRows * a.C + c + e] = h[e];
+    typename Elem<DT>::T *out = static_cast<typename Elem<DT>::T *>(a.o) + r0 * a.C;
+    const uint32_t at = row * a.C + c;
+    if (!some) {
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (row0 + i >= a.T) break;
-      const int m = some ? mark[rg * R + i] : kInside;
-      Vec<DT, W> o;
-      if (m == kOutside) {
-#pragma unroll
-        for (int e = 0; e < W; ++e) o.set(e, 0.f);
-      } else {
-        if (m >= 0)
-#pragma unroll
-          for (int e = 0; e < W; ++e) h[e] = a.h0 ? a.h0[static_cast<int64_t>(m) * a.C + c + e] : 0.f;
+      for (int i = 0; i < R; ++i) {
+        Vec<DT, W> o;
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           h[e] = fmaf(f[i][e], h[e], u[i][e]);
-          o.set(e, a.q ? h[e] * q[i][e] : h[e]);
+          o.set(e, READ ? h[e] * q[READ ? i : 0][e] : h[e]);
         }
-        const int n = some ? fin[rg * R + i] : -1;
-        if (a.ht && n >= 0)
-#pragma unroll
-          for (int e = 0; e < W; ++e) a.ht[static_cast<int64_t>(n) * a.C + c + e] = h[e];
+        store_vec<DT, W>(out, at + static_cast<uint32_t>(i) * a.C, o);
       }
-      store_vec<DT, W>(a.o, (row0 + i) * a.C + c, o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const int m = sm.mark[row + i], n = sm.fin[row + i];
+        Vec<DT, W> o;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          h[e] = fmaf(f[i][e], m >= 0 ? state0(m, e) : h[e], u[i][e]);
+          o.set(e, m == kOutside ? 0.f : READ ? h[e] * q[READ ? i : 0][e] : h[e]);
+          if (a.ht && n >= 0) a.ht[static_cast<int64_t>(n) * a.C + c + e] = h[e];
+        }
+        if (i < left) store_vec<DT, W>(out, at + static_cast<uint32_t>(i) * a.C, o);
+      }
     }
   }
-  if (a.ht)   // empty sequences, dealt over the tiles
-    for (int64_t n = k; n < a.n_seq; n += a.tiles) {
-      const int64_t b = min(max(a.cu[n], (int64_t)0), a.T);
-      if (a.cu[n + 1] <= b && tid < cw && cb * cw + tid < a.C)
-        a.ht[n * a.C + cb * cw + tid] = a.h0 ? a.h0[n * a.C + cb * cw + tid] : 0.f;
-    }
+  if (a.ht) empty_states(a, a.h0, a.ht, k, cb, cw);
 }
 
 // ----------------------------------------------------------------- backward --
-template <int DT, int DTG, int W>
+template <int DT, int DTG, int W, bool READ>
 __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(const ScanArgs a) {
-  __shared__ float sA[kMostValues], sU[kMostValues], sE[kMostValues];
-  __shared__ int mark[kBlock * R], fin[kBlock * R], cut[kBlock];
-  __shared__ uint32_t slot;
-  const int64_t id = take_tile(a, &slot);
-  const int64_t back = id / a.cblocks, k = a.tiles - 1 - back;
-  const int cb = static_cast<int>(id - back * a.cblocks), cw = a.CT * W, tid = threadIdx.x;
-  const int rg = tid / a.CT, cl = tid - rg * a.CT, rows = a.RG * R;
-  const int64_t r0 = k * rows, row0 = r0 + rg * R;
-  const int c = (cb * a.CT + cl) * W;
-  const bool on = rg < a.RG && c < a.C;
-  Vec<DT, W> u[R], q[R], d[R];
-  Vec<DTG, W> g[R];
-  if (on) {
-    load_rows<DT, W>(u, a.u, a.ldu, row0, a.T, c);
-    load_rows<DTG, W>(g, a.g, a.ldg, row0, a.T, c);
-    load_rows<DT, W>(d, a.dout, a.C, row0, a.T, c);
-    if (a.q) load_rows<DT, W>(q, a.q, a.ldq, row0, a.T, c);
+  constexpr int R = kBwdRows;
+  __shared__ TileSmem sm;
+  __shared__ float sE[kMostValues];
+  const int tid = threadIdx.x, cw = a.CT * W, rows = a.RG * R;
+  const int rg = tid / a.CT, cl = tid - rg * a.CT;
+  const Span all = a.n_seq ? Span{span_of(a, 0).b, span_of(a, a.n_seq - 1).e} : Span{0, 0};
+  const Span mine = tid < a.n_seq ? span_of(a, tid) : Span{0, 0};
+  const int id = take_tile(a, &sm.slot);
+  const int back = id / a.cblocks, k = a.tiles - 1 - back, cb = id - back * a.cblocks;
+  if (a.T == 0) {
+    if (a.dh0) empty_states(a, a.dht, a.dh0, k, cb, cw);
+    return;
   }
-  const bool some = mark_rows(a, r0, rows, mark, fin);
+  const int64_t r0 = static_cast<int64_t>(k) * rows;
+  const int row = rg * R;
+  const int exist = static_cast<int>(min(a.T - r0, static_cast<int64_t>(rows))), left = exist - row;
+  const bool on = rg < a.RG && (cb * a.CT + cl) * W < a.C;
+  const int c = on ? (cb * a.CT + cl) * W : 0;   // (lanes without a channel read the first)
+  Vec<DT, W> u[R], q[READ ? R : 1], d[R];
+  Vec<DTG, W> g[R];
+  load_rows<DT, W, R>(u, a.u, r0, a.ldu, row, exist - 1, c);
+  load_rows<DTG, W, R>(g, a.g, r0, a.ldg, row, exist - 1, c);
+  load_rows<DT, W, R>(d, a.dout, r0, a.C, row, exist - 1, c);
+  if constexpr (READ) load_rows<DT, W, R>(q, a.q, r0, a.ldq, row, exist - 1, c);
+  // (the forward left the state that enters the tile)
+  const float entering = tid < cw && cb * cw + tid < a.C ? a.keep[r0 / kKeepRows * a.C + cb * cw + tid] : 0.f;
+  const bool some = mark_rows(a, mine, all, r0, rows, sm.mark, sm.fin);
   Gate f[R][W];
-  auto state0 = [&](int m, int e) __attribute__((always_inline)) {
-    return a.h0 ? a.h0[static_cast<int64_t>(m) * a.C + c + e] : 0.f;
-  };
-  auto grad_of = [&](int i, int e) __attribute__((always_inline)) { return a.q ? d[i][e] * q[i][e] : d[i][e]; };
+  auto state0 = [&](int m, int e) { return a.h0 ? a.h0[static_cast<int64_t>(m) * a.C + c + e] : 0.f; };
+  auto grad0 = [&](int n, int e) { return a.dht ? a.dht[static_cast<int64_t>(n) * a.C + c + e] : 0.f; };
+  auto grad_of = [&](int i, int e) { return READ ? d[i][e] * q[READ ? i : 0][e] : d[i][e]; };
+  by_kind(a.gate, [&](auto kind) { each<R, W>([&](int i, int e) { f[i][e] = gate_of<kind()>(g[i][e]); }); });
   if (on) {
     float A[W], U[W], E[W];
-    bool reset = false;
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       A[e] = 1.f;
       U[e] = E[e] = 0.f;
     }
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int m = some ? mark[rg * R + i] : kInside;
-      reset |= m != kInside;
-#pragma unroll
-      for (int e = 0; e < W; ++e) {
-        f[i][e] = gate_of(a.gate, g[i][e]);
-        U[e] = m == kOutside ? 0.f : fmaf(f[i][e].a, m >= 0 ? state0(m, e) : U[e], u[i][e]);
+    bool reset = false;
+    if (!some) {
+      each<R, W>([&](int i, int e) {
+        U[e] = fmaf(f[i][e].a, U[e], u[i][e]);
         A[e] *= f[i][e].a;
-      }
-    }
+      });
+      each<R, W>([&](int i, int e) { E[e] = f[R - 1 - i][e].a * (grad_of(R - 1 - i, e) + E[e]); });
+    } else {
 #pragma unroll
-    for (int i = R - 1; i >= 0; --i) {
-      const int m = some ? mark[rg * R + i] : kInside, n = some ? fin[rg * R + i] : -1;
+      for (int i = 0; i < R; ++i) {
+        const int m = sm.mark[row + i];
+        reset |= m != kInside || sm.fin[row + i] >= 0;   // (nothing goes past a beginning or an end)
 #pragma unroll
-      for (int e = 0; e < W; ++e) {
-        if (n >= 0) E[e] = a.dht ? a.dht[static_cast<int64_t>(n) * a.C + c + e] : 0.f;
-        E[e] = m == kInside ? f[i][e].a * (grad_of(i, e) + E[e]) : 0.f;   // (nothing goes past a beginning)
+        for (int e = 0; e < W; ++e) {
+          U[e] = m == kOutside ? 0.f : fmaf(f[i][e].a, m >= 0 ? state0(m, e) : U[e], u[i][e]);
+          A[e] *= f[i][e].a;
+        }
       }
-      // a sequence's end takes nothing from the rows behind it
-      reset |= n >= 0;
+#pragma unroll
+      for (int i = R - 1; i >= 0; --i) {
+        const int m = sm.mark[row + i], n = sm.fin[row + i];
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float x = n >= 0 ? grad0(n, e) : E[e];
+          E[e] = m == kInside ? f[i][e].a * (grad_of(i, e) + x) : 0.f;
+        }
+      }
     }
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      sA[rg * cw + cl * W + e] = A[e];
-      sU[rg * cw + cl * W + e] = U[e];
+      sm.A[rg * cw + cl * W + e] = A[e];
+      sm.U[rg * cw + cl * W + e] = U[e];
       sE[rg * cw + cl * W + e] = E[e];
     }
-    if (cl == 0) cut[rg] = reset;
+    if (cl == 0) sm.cut[rg] = reset;
   }
   __syncthreads();
-  const int64_t wide = static_cast<int64_t>(a.cblocks) * cw;
-  // one half of the threads takes the states forward, the other the gradients back
-  const int half = tid < kBlock / 2 ? tid : tid - kBlock / 2;
-  if (half < cw && cb * cw + half < a.C) {
-    if (tid < kBlock / 2)
-      enter_groups<false>(sA, sU, cut, a.RG, cw, half, r0 < a.T ? a.keep[r0 / kKeepRows * a.C + cb * cw + half] : 0.f);
-    else
-      enter_tile<true>(a, back, static_cast<int64_t>(cb) * cw + half, wide, sA, sE, cut,
-                       some && (mark[rows - 1] == kOutside || fin[rows - 1] >= 0), cw, half);
-  }
+  // the first threads take the states forward, those from half on the gradients back
+  if (tid < cw && cb * cw + tid < a.C) enter_groups<false>(sm.A, sm.U, sm.cut, a.RG, cw, tid, entering);
+  enter_tile<true>(a, sm, sE, back, cb, some && (sm.mark[rows - 1] == kOutside || sm.fin[rows - 1] >= 0), cw, kBlock / 2);
   __syncthreads();
+  as_read(u);
+  as_read(d);
+  if constexpr (READ) as_read(q);
   if (on) {
     float h[W], x[W], before[R][W];
 #pragma unroll
     for (int e = 0; e < W; ++e) {
-      h[e] = sU[rg * cw + cl * W + e];
+      h[e] = sm.U[rg * cw + cl * W + e];
       x[e] = sE[rg * cw + cl * W + e];
     }
+    const int64_t first = r0 * a.C;
+    const uint32_t at = row * a.C + c;
+    typedef typename Elem<DT>::T TU;
+    typedef typename Elem<DTG>::T TG;
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int m = some ? mark[rg * R + i] : kInside;
+      const int m = some ? sm.mark[row + i] : kInside;
       Vec<DT, W> dq;
 #pragma unroll
       for (int e = 0; e < W; ++e) {
@@ -463,34 +571,29 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(const ScanArgs a) {
         h[e] = fmaf(f[i][e].a, h[e], u[i][e]);
         dq.set(e, m == kOutside ? 0.f : d[i][e] * h[e]);
       }
-      if (a.q && row0 + i < a.T) store_vec<DT, W>(a.dq, (row0 + i) * a.C + c, dq);
+      if (READ && i < left) store_vec<DT, W>(static_cast<TU *>(a.dq) + first, at + static_cast<uint32_t>(i) * a.C, dq);
     }
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
-      const int m = some ? mark[rg * R + i] : kInside, n = some ? fin[rg * R + i] : -1;
+      const int m = some ? sm.mark[row + i] : kInside, n = some ? sm.fin[row + i] : -1;
       Vec<DT, W> du;
       Vec<DTG, W> dg;
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        if (n >= 0) x[e] = a.dht ? a.dht[static_cast<int64_t>(n) * a.C + c + e] : 0.f;
+        if (n >= 0) x[e] = grad0(n, e);
         const float s = grad_of(i, e) + x[e];
         du.set(e, m == kOutside ? 0.f : s);
         dg.set(e, m == kOutside ? 0.f : s * before[i][e] * f[i][e].slope);
         x[e] = f[i][e].a * s;
         if (m >= 0 && a.dh0) a.dh0[static_cast<int64_t>(m) * a.C + c + e] = x[e];
       }
-      if (row0 + i < a.T) {
-        store_vec<DT, W>(a.du, (row0 + i) * a.C + c, du);
-        store_vec<DTG, W>(a.dg, (row0 + i) * a.C + c, dg);
+      if (i < left) {
+        store_vec<DT, W>(static_cast<TU *>(a.du) + first, at + static_cast<uint32_t>(i) * a.C, du);
+        store_vec<DTG, W>(static_cast<TG *>(a.dg) + first, at + static_cast<uint32_t>(i) * a.C, dg);
       }
     }
   }
-  if (a.dh0)   // empty sequences
-    for (int64_t n = k; n < a.n_seq; n += a.tiles) {
-      const int64_t b = min(max(a.cu[n], (int64_t)0), a.T);
-      if (a.cu[n + 1] <= b && tid < cw && cb * cw + tid < a.C)
-        a.dh0[n * a.C + cb * cw + tid] = a.dht ? a.dht[n * a.C + cb * cw + tid] : 0.f;
-    }
+  if (a.dh0) empty_states(a, a.dht, a.dh0, k, cb, cw);
 }
 
 // --------------------------------------------------------- single tokens --
@@ -515,7 +618,9 @@ __global__ __launch_bounds__(256) void scan_step_kernel(const StepArgs a) {
     return;
   }
   float &s = a.state[static_cast<int64_t>(row) * a.C + c];
-  s = fmaf(gate_of(a.gate, Elem<DTG>::load(a.g, i * a.ldg + c)).a, s, Elem<DT>::load(a.u, i * a.ldu + c));
+  const float g = Elem<DTG>::load(a.g, i * a.ldg + c);
+  const float f = a.gate == kSigmoid ? gate_value<kSigmoid>(g) : a.gate == kLog ? gate_value<kLog>(g) : g;
+  s = fmaf(f, s, Elem<DT>::load(a.u, i * a.ldu + c));
   Elem<DT>::store(a.o, x, a.q ? s * Elem<DT>::load(a.q, i * a.ldq + c) : s);
 }
 
@@ -531,6 +636,10 @@ int check_sizes(const char *what, int n_seq, int64_t T, int C, int gate, int dty
     set_error("%s: unsupported dtypes %d, gates %d", what, dtype, g_dtype);
     return SSLA_ERR_DTYPE;
   }
+  if (C > kMostWidth || (T > 1 && (ldu > kMostWidth || ldg > kMostWidth || ldq > kMostWidth))) {
+    set_error("%s: rows of more than %d values, or that far apart", what, kMostWidth);
+    return SSLA_ERR_UNSUPPORTED;
+  }
   if (T > (1ll << 40) / C || static_cast<int64_t>(n_seq) * C > (1ll << 38)) {
     set_error("%s: too many values", what);
     return SSLA_ERR_UNSUPPORTED;
@@ -545,35 +654,35 @@ int check_sizes(const char *what, int n_seq, int64_t T, int C, int gate, int dty
     else { if (g_dtype == SSLA_F32) { CALL(SSLA_F16, SSLA_F32); } else { CALL(SSLA_F16, SSLA_F16); } } \
   } while (0)
 
-// How the rows and channels are cut for vectors of W values: up to kLanes lanes a
+// How the rows and channels are cut for vectors of W values and R rows a lane: up to kMostLanes lanes a
 // row, as many row groups as a workgroup has room for (a power of two, so that a
 // tile is a multiple of kKeepRows rows).
-constexpr int kLanes = 16;
 struct ScanPlan {
   int CT, RG, cblocks;
   int64_t tiles;
 };
-ScanPlan plan_of(int64_t T, int C, int W, int lanes) {
+ScanPlan plan_of(int64_t T, int C, int W, int R) {
   ScanPlan p;
   const int cv = C / W;
-  p.CT = (cv + (cv + lanes - 1) / lanes - 1) / ((cv + lanes - 1) / lanes);
+  p.CT = (cv + (cv + kMostLanes - 1) / kMostLanes - 1) / ((cv + kMostLanes - 1) / kMostLanes);
   p.cblocks = (cv + p.CT - 1) / p.CT;
   p.RG = kKeepRows / R;
-  while (2 * p.RG * p.CT <= kBlock) p.RG *= 2;
+  while (2 * p.RG * p.CT <= kBlock && p.RG < kMostGroups) p.RG *= 2;
   p.tiles = std::max<int64_t>(1, (T + p.RG * R - 1) / (p.RG * R));
   return p;
 }
 constexpr size_t kHead = 256;   // the ticket's line
-int64_t word_count(const ScanPlan &p, int W) {   // 64-bit words of maps and states
-  return (p.tiles * p.cblocks * p.CT * W * 3 + 1) / 2;
+int64_t word_count(const ScanPlan &p, int W) {   // words and hints
+  return p.tiles * p.cblocks * p.CT * W + (p.tiles * p.cblocks + 1) / 2;
 }
 size_t ws_bytes(int64_t T, int C) {   // whatever vectors the addresses allow
   int64_t most = 0;
-  for (int W = 1; W <= 8; W *= 2)
-    if (W != 2 && C % W == 0) {
-      const ScanPlan p = plan_of(T, C, W, kLanes);
-      if (p.tiles > 1) most = std::max(most, word_count(p, W));
-    }
+  for (int W = 1; W <= 4; W *= 4)
+    if (C % W == 0)
+      for (int R : {kFwdRows, kBwdRows}) {
+        const ScanPlan p = plan_of(T, C, W, R);
+        if (p.tiles > 1) most = std::max(most, word_count(p, W));
+      }
   return most ? kHead + static_cast<size_t>(most) * 8 : 0;
 }
 
@@ -595,8 +704,8 @@ int widest(int C, int most, std::initializer_list<Rows> all) {
 
 // Sets the plan, clears the words and launches `kernel`.
 template <typename Kernel>
-int launch_scan(const char *what, ScanArgs &a, int W, Kernel kernel, void *workspace, size_t workspace_bytes, hipStream_t st) {
-  const ScanPlan p = plan_of(a.T, a.C, W, kLanes);
+int launch_scan(const char *what, ScanArgs &a, int W, int R, Kernel kernel, void *workspace, size_t workspace_bytes, hipStream_t st) {
+  const ScanPlan p = plan_of(a.T, a.C, W, R);
   const size_t need = p.tiles > 1 ? kHead + static_cast<size_t>(word_count(p, W)) * 8 : 0;
   if (need && !(workspace && workspace_bytes >= need && aligned(workspace, 16))) {
     set_error("%s: needs %zu bytes of workspace, got %zu", what, ws_bytes(a.T, a.C), workspace_bytes);
@@ -606,14 +715,14 @@ int launch_scan(const char *what, ScanArgs &a, int W, Kernel kernel, void *works
     set_error("%s: too many workgroups", what);
     return SSLA_ERR_UNSUPPORTED;
   }
-  a.CT = p.CT; a.RG = p.RG; a.cblocks = p.cblocks; a.tiles = p.tiles;
+  a.CT = p.CT; a.RG = p.RG; a.cblocks = p.cblocks; a.tiles = static_cast<int>(p.tiles);
   if (need) {
     const int64_t n = word_count(p, W);
     a.ticket = static_cast<uint32_t *>(workspace);
-    a.maps = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + kHead);
-    a.states = reinterpret_cast<uint32_t *>(a.maps + p.tiles * p.cblocks * p.CT * W);
+    a.words = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + kHead);
+    a.hints = reinterpret_cast<uint32_t *>(a.words + p.tiles * p.cblocks * p.CT * W);
     hipLaunchKernelGGL(scan_clear_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((n + 1023) / 1024, 2048))), dim3(256), 0,
-                       st, a.ticket, a.maps, n);
+                       st, a.ticket, a.words, n);
   }
   hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.tiles * p.cblocks)), dim3(kBlock), 0, st, a);
   return SSLA_OK;
@@ -642,13 +751,14 @@ extern "C" int ssla_gated_scan_fwd(const void *u, int64_t ldu, const void *g, in
   a.u = u; a.g = g; a.q = q; a.ldu = ldu; a.ldg = ldg; a.ldq = ldq;
   a.cu = cu_seqlens; a.n_seq = n_seq; a.T = T; a.C = C; a.gate = gate;
   a.h0 = h0; a.o = o; a.ht = ht; a.keep = static_cast<float *>(keep);
-  const int W = widest(C, dtype == SSLA_F32 ? 4 : 8, {{u, ldu, dtype}, {g, ldg, g_dtype}, {q, q ? ldq : 0, dtype}, {o, C, dtype}});
+  const int W = widest(C, 4, {{u, ldu, dtype}, {g, ldg, g_dtype}, {q, q ? ldq : 0, dtype}, {o, C, dtype}});
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   int status = SSLA_OK;
 #define SSLA_LAUNCH(D, G, W_) \
-  status = launch_scan("gated_scan_fwd", a, W_, scan_fwd_kernel<D, G, W_>, workspace, workspace_bytes, static_cast<hipStream_t>(stream))
-#define SSLA_CALL(D, G)                                              \
-  if (W == 8) { if constexpr (D != SSLA_F32) SSLA_LAUNCH(D, G, 8); } \
-  else if (W == 4) SSLA_LAUNCH(D, G, 4);                             \
+  status = q ? launch_scan("gated_scan_fwd", a, W_, kFwdRows, scan_fwd_kernel<D, G, W_, true>, workspace, workspace_bytes, st) \
+             : launch_scan("gated_scan_fwd", a, W_, kFwdRows, scan_fwd_kernel<D, G, W_, false>, workspace, workspace_bytes, st)
+#define SSLA_CALL(D, G)             \
+  if (W == 4) SSLA_LAUNCH(D, G, 4); \
   else SSLA_LAUNCH(D, G, 1)
   SSLA_SCAN_TYPES(SSLA_CALL);
 #undef SSLA_CALL
@@ -674,9 +784,11 @@ extern "C" int ssla_gated_scan_bwd(const void *u, int64_t ldu, const void *g, in
   a.keep = static_cast<float *>(const_cast<void *>(keep));
   const int W = widest(C, 4, {{u, ldu, dtype}, {g, ldg, g_dtype}, {q, q ? ldq : 0, dtype}, {dout, C, dtype}, {du, C, dtype},
                               {dg, C, g_dtype}, {dq, C, dtype}});
+  const hipStream_t st = static_cast<hipStream_t>(stream);
   int status = SSLA_OK;
 #define SSLA_LAUNCH(D, G, W_) \
-  status = launch_scan("gated_scan_bwd", a, W_, scan_bwd_kernel<D, G, W_>, workspace, workspace_bytes, static_cast<hipStream_t>(stream))
+  status = q ? launch_scan("gated_scan_bwd", a, W_, kBwdRows, scan_bwd_kernel<D, G, W_, true>, workspace, workspace_bytes, st) \
+             : launch_scan("gated_scan_bwd", a, W_, kBwdRows, scan_bwd_kernel<D, G, W_, false>, workspace, workspace_bytes, st)
 #define SSLA_CALL(D, G)             \
   if (W == 4) SSLA_LAUNCH(D, G, 4); \
   else SSLA_LAUNCH(D, G, 1)

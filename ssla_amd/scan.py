@@ -181,7 +181,7 @@ def gated_scan(
 
     States are fp32; a long sequence is cut along time and the pieces' states are
     joined in their order, so results do not vary from call to call.  Over a piece
-    (up to 2,048 rows) the gates are multiplied: factors larger than 1 in magnitude
+    (up to 512 rows) the gates are multiplied: factors larger than 1 in magnitude
     hold while such a product stays inside fp32.  Differentiable in u, g, q and the
     initial state (once, in reverse mode: forward-mode tangents are refused).  Makes
     no host sync."""
