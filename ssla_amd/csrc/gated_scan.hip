@@ -57,9 +57,13 @@ __device__ __forceinline__ Gate gate_of(float g) {
   return {a, KIND == kLog ? a : 1.f};
 }
 
-constexpr int kFwdRows = 8, kBwdRows = 4;   // rows of a lane
+// Rows of a lane, and threads: large tiles are few steps between them, small ones leave
+// registers for more workgroups.  65,536 rows of 1,024 channels (us): 8 rows 145 with
+// 256 threads, 137 with 512, 172 with 1,024; 4 rows 230.  Training step of 8 x 4,096
+// rows, forward with 8: backward with 4 rows 231, with 8 263 (512 threads).
+constexpr int kFwdRows = 8, kBwdRows = 4;
 constexpr int kMostRows = 8;
-constexpr int kBlock = 256;
+constexpr int kBlock = 512;
 constexpr int kKeepRows = 64;    // rows between the states left for the backward
 constexpr int kMostLanes = 16;   // lanes of a row
 constexpr int kMostGroups = 64;  // row groups of a tile
