@@ -310,7 +310,7 @@ int ssla_gated_delta_chunk_bwd(const void *q, const void *k, const void *v, cons
  * dtype), dweight and dbias (fp32 [C], summed in a fixed order) may be NULL.
  * Workspaces: the queried bytes, 16-byte aligned, no initialisation; 0: none.
  * ------------------------------------------------------------------------ */
-enum { SSLA_ACT_NONE = 0, SSLA_ACT_RELU = 1, SSLA_ACT_SILU = 2 };
+enum { SSLA_ACT_NONE = 0, SSLA_ACT_RELU = 1, SSLA_ACT_SILU = 2, SSLA_ACT_SIGMOID = 3 };
 size_t ssla_group_norm_workspace_size(int64_t N, int64_t L, int C, int G);
 int ssla_group_norm_fwd(const void *x, int64_t N, int64_t L, int C, int G, const float *weight, const float *bias,
                         float eps, int act, void *y, float *stats, int dtype, void *workspace,
@@ -319,6 +319,58 @@ size_t ssla_group_norm_bwd_workspace_size(int64_t N, int64_t L, int C, int G);
 int ssla_group_norm_bwd(const void *dy, const void *x, const float *stats, int64_t N, int64_t L, int C, int G,
                         const float *weight, const float *bias, int act, void *dx, float *dweight, float *dbias,
                         int dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Norms around a block, by rows (no reference counterpart).
+ * Gated: y = norm(x) act(z) over N rows of C channels in G groups,
+ *   norm(x) = x / sqrt(mean(x^2) + eps) * weight + bias   (SSLA_NORM_RMS)
+ * or of x less its mean (SSLA_NORM_LAYER), mean over a group's C / G channels
+ * (at most 8,192); act: SSLA_ACT_SILU or SSLA_ACT_SIGMOID.  x, z: rows ldx, ldz
+ * elements apart; y, dy, dx, dz contiguous; all of dtype `dtype`.  weight, bias:
+ * fp32 [C] or NULL.
+ * Residual: sum = residual + alpha gamma drop(branch), y = norm(sum) (G = 1), with
+ * branch = norm(x) by post_weight where `post` is not 0, else x, and drop as
+ * ssla_counter_dropout with p (0: none), seed and subsequence, elements counted
+ * from x's start.  x, y of dtype `dtype`, residual and sum of r_dtype (that or
+ * fp32), all [N, C]; y is the norm of the sum before its rounding.  weight, bias,
+ * gamma, post_weight: fp32 [C] or NULL.
+ * The backwards take the forward's inputs again (nothing else is kept) and the
+ * gradients of y and sum (one of these may be NULL); the gradients of tensors
+ * and weights that are NULL are not written; those of weights are fp32 [C],
+ * summed in a fixed order.  Workspaces: the queried bytes, 16-byte aligned, no
+ * initialisation; needed where a weight's gradient is.
+ * ------------------------------------------------------------------------ */
+enum { SSLA_NORM_RMS = 0, SSLA_NORM_LAYER = 1 };
+int ssla_gated_norm_fwd(const void *x, int64_t ldx, const void *z, int64_t ldz, int64_t N, int C, int G, int kind,
+                        const float *weight, const float *bias, float eps, int act, void *y, int dtype,
+                        void *stream);
+size_t ssla_gated_norm_bwd_workspace_size(int64_t N, int C, int G);
+int ssla_gated_norm_bwd(const void *dy, const void *x, int64_t ldx, const void *z, int64_t ldz, int64_t N, int C,
+                        int G, int kind, const float *weight, const float *bias, float eps, int act, void *dx,
+                        void *dz, float *dweight, float *dbias, int dtype, void *workspace,
+                        size_t workspace_bytes, void *stream);
+int ssla_residual_norm_fwd(const void *x, const void *residual, int64_t N, int C, int kind, const float *weight,
+                           const float *bias, float eps, float alpha, const float *gamma, int post,
+                           const float *post_weight, float p, const int64_t *seed, uint32_t subsequence, void *y,
+                           void *sum, int dtype, int r_dtype, void *stream);
+size_t ssla_residual_norm_bwd_workspace_size(int64_t N, int C);
+int ssla_residual_norm_bwd(const void *dy, const void *dsum, const void *x, const void *residual, int64_t N, int C,
+                           int kind, const float *weight, float eps, float alpha, const float *gamma, int post,
+                           const float *post_weight, float p, const int64_t *seed, uint32_t subsequence, void *dx,
+                           void *dresidual, float *dweight, float *dbias, float *dgamma, float *dpost_weight,
+                           int dtype, int r_dtype, void *workspace, size_t workspace_bytes, void *stream);
+
+/* ------------------------------------------------------------------------
+ * Dropout by a counter-based generator (no reference counterpart):
+ *   y_i = keep_i x_i 2^16 / (2^16 - t),  t = round(p 2^16)
+ * keep_i: 16 bits of Philox4x32-10 reach t.  Element i has word (i % 8) / 2 of
+ * the block with counter (i / 8 low, i / 8 high, subsequence, 0) and key *seed (low,
+ * high; on the device), its low half for even i.  What is dropped is 0 whatever x
+ * holds; t = 2^16 drops all.  The backward is the same call on dy: no mask is
+ * stored.  x, y: n elements of dtype `dtype`.
+ * ------------------------------------------------------------------------ */
+int ssla_counter_dropout(const void *x, int64_t n, float p, const int64_t *seed, uint32_t subsequence, void *y,
+                         int dtype, void *stream);
 
 /* ------------------------------------------------------------------------
  * G2 -- sparse sequential scans.

@@ -4,6 +4,7 @@ with the kernels.  The recurrence comes with how far a computation may be off
 whose every step is off by a relative `eps`."""
 from __future__ import annotations
 
+import numpy as np
 import torch
 
 
@@ -74,3 +75,59 @@ def gated_scan(u, g, lens, q=None, gate="value", h0=None, do=None, dht=None, eps
     out.update(du=(E, offE), dg=(dA * slope, offA * slope.abs() + 2 * eps * (dA * slope).abs()),
                dq=(do * H, do.abs() * O + eps * (do * H).abs()), dh0=(c, off))
     return out
+
+
+def _norm(x, groups, weight, bias, eps, kind):
+    v = x.reshape(x.shape[0], groups, -1)
+    if kind == "layer":
+        v = v - v.mean(2, keepdim=True)
+    v = (v / torch.sqrt((v * v).mean(2, keepdim=True) + eps)).reshape(x.shape)
+    v = v if weight is None else v * weight.double()
+    return v if bias is None else v + bias.double()
+
+
+def gated_norm(x, z, num_groups=1, weight=None, bias=None, eps=1e-5, activation="silu", kind="rms"):
+    """Rows [N, C]; differentiable."""
+    z = z.double()
+    s = 1 / (1 + torch.exp(-z))
+    return _norm(x.double(), num_groups, weight, bias, eps, kind) * (z * s if activation == "silu" else s)
+
+
+def residual_norm(x, residual, weight=None, bias=None, eps=1e-5, kind="rms", scale=None, post_norm=False, post_weight=None,
+                  keep=None, p=0.0):
+    """(y, sum) of rows [N, C]; keep: the dropout's mask, or None."""
+    v = _norm(x.double(), 1, post_weight, None, eps, kind) if post_norm else x.double()
+    if keep is not None:
+        v = torch.where(keep, v * dropout_scale(p), torch.zeros_like(v))
+    if scale is not None:
+        v = v * (scale.double() if torch.is_tensor(scale) else scale)
+    s = residual.double() + v
+    return _norm(s, 1, weight, bias, eps, kind), s
+
+
+def philox(counter, key):
+    """Philox4x32-10: counter [n, 4] and key of two 32-bit words -> [n, 4]."""
+    c = [np.asarray(counter[:, i], dtype=np.uint64) for i in range(4)]
+    k = [int(key[0]), int(key[1])]
+    low = np.uint64(0xffffffff)
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> np.uint64(32)) ^ c[1] ^ np.uint64(k[0]), b & low, (a >> np.uint64(32)) ^ c[3] ^ np.uint64(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & 0xffffffff, (k[1] + 0xBB67AE85) & 0xffffffff]
+    return np.stack(c, 1).astype(np.uint32)
+
+
+def dropout_scale(p):
+    t = round(p * 65536)
+    return 65536 / (65536 - t) if t < 65536 else 0.0
+
+
+def dropout_keep(n, p, seed, subsequence=0, first=0):
+    """Which of the elements first .. first + n of a tensor stay."""
+    blocks = np.arange(first // 8, (first + n + 7) // 8, dtype=np.uint64)
+    counter = np.stack([blocks & np.uint64(0xffffffff), blocks >> np.uint64(32), np.full_like(blocks, subsequence),
+                        np.zeros_like(blocks)], 1)
+    seed &= (1 << 64) - 1
+    words = philox(counter, (seed & 0xffffffff, seed >> 32))
+    bits = np.stack([words & 0xffff, words >> 16], 2).reshape(-1)[first % 8:][:n]
+    return torch.from_numpy(bits >= round(p * 65536))

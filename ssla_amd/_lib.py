@@ -27,7 +27,7 @@ SSLA_ERR_UNSUPPORTED = -5
 SSLA_F32, SSLA_BF16, SSLA_F16 = 0, 1, 2
 DTYPE_CODE = {torch.float32: SSLA_F32, torch.bfloat16: SSLA_BF16, torch.float16: SSLA_F16}
 
-_vp, _i32, _i64, _f32, _sz = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t
+_vp, _i32, _i64, _f32, _sz, _u32 = C.c_void_p, C.c_int, C.c_int64, C.c_float, C.c_size_t, C.c_uint32
 
 
 class HeadLevel(C.Structure):
@@ -100,6 +100,16 @@ SIGNATURES = {
     "ssla_group_norm_bwd_workspace_size": (_sz, [_i64, _i64, _i32, _i32]),
     "ssla_group_norm_bwd": (_i32, [_vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _sz,
                                    _vp]),
+    "ssla_gated_norm_fwd": (_i32, [_vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _i32, _vp, _i32, _vp]),
+    "ssla_gated_norm_bwd_workspace_size": (_sz, [_i64, _i32, _i32]),
+    "ssla_gated_norm_bwd": (_i32, [_vp, _vp, _i64, _vp, _i64, _i64, _i32, _i32, _i32, _vp, _vp, _f32, _i32, _vp, _vp, _vp,
+                                   _vp, _i32, _vp, _sz, _vp]),
+    "ssla_residual_norm_fwd": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _f32, _f32, _vp, _i32, _vp, _f32, _vp, _u32, _vp,
+                                      _vp, _i32, _i32, _vp]),
+    "ssla_residual_norm_bwd_workspace_size": (_sz, [_i64, _i32]),
+    "ssla_residual_norm_bwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _f32, _f32, _vp, _i32, _vp, _f32, _vp, _u32,
+                                      _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _sz, _vp]),
+    "ssla_counter_dropout": (_i32, [_vp, _i64, _f32, _vp, _u32, _vp, _i32, _vp]),
     "ssla_status_read": (_i32, [_vp, C.POINTER(_i32), _vp]),
     "ssla_site_project": (_i32, [_vp, _i64, _i32, _vp, _i32, _f32, _vp, _vp, _vp, _vp, _vp]),
     "ssla_site_finish": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _vp, _vp, _vp, _f32, _i32, _vp, _vp]),

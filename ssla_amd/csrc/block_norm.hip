@@ -1,0 +1,737 @@
+// Norms around a block, by rows, with their backward passes.
+//
+// Gated: the norm of an attention's output by groups of channels, times its gate,
+//   y = (n w + b) act(z),  n = (x - mean) rstd  (or x rstd),
+//   dz = dy (n w + b) act'(z),  dv = dy act(z),  dw = sum dv n,  db = sum dv,
+//   dx = rstd (h - mean(h) - n mean(h n)),  h = dv w   (no mean(h) without a mean)
+// Residual: a stream's step from one block to the next,
+//   p = norm2(x) w2 (or x),  s = r + c keep p,  y = norm(s) w + b
+// with c = alpha gamma / (1 - p) and keep a mask that is drawn again in the backward:
+//   ds = ds' + norm'(dy),  dr = ds,  dgamma = sum ds keep p,  dp = c keep ds,
+//   dw2 = sum dp n2,  dx = norm2'(dp).
+//
+// Bound by memory: each tensor is read or written once in either direction.  A row
+// (a group of one) lies in the registers of S lanes, S a power of two: up to 64
+// lanes of a wavefront with up to 8 values each, whose sums are shuffles, or more
+// than one wavefront, whose sums are joined in LDS.  Nothing of a norm is kept for the backward: with x (and r)
+// at hand again its sums cost shuffles, not memory.  Lane groups step over the rows
+// with the next one on its way.  Sums over rows stay with their lanes, are added up
+// in the workgroup and then down the workgroups, in a fixed order.
+#include "philox.h"
+#include "vec.h"
+
+#include <math.h>
+
+namespace ssla {
+namespace {
+
+constexpr int kHold = 8;        // values that a lane holds of a row
+constexpr int kMostLanes = 1024;
+constexpr int kFwdThreads = 256, kBwdThreads = 512;   // of a workgroup, unless a row needs more
+
+struct RowArgs {
+  const void *x, *r, *z, *dy, *ds;   // ds, and dy of the residual's backward, may be NULL
+  int64_t ldx, ldz;                  // elements from row to row of x and z (gated)
+  const float *w, *b, *w2, *gamma;   // may be NULL
+  void *y, *s;                       // y and the stream, or dx and dr (the backward's may be NULL)
+  void *dz;
+  float *part;                       // [workgroups][kinds][C] sums over rows; NULL: not wanted
+  int64_t N;                         // rows
+  int C, G, per, S, layer, post, silu;
+  int64_t slots;                     // rows at once, of each group
+  float eps, alpha;
+  Draw draw;
+};
+
+// ------------------------------------------------------------- a row's lanes --
+// The sums of x and y over a row's lanes, in the same order on every lane.  WIDE: over
+// several wavefronts, all threads of the workgroup at once.
+template <int WIDE>
+__device__ __forceinline__ void row_sums(float &x, float &y, int S, float *sm, int &turn) {
+  if constexpr (WIDE == 0) {
+    for (int d = 1; d < S; d <<= 1) {
+      x += __shfl_xor(x, d);
+      y += __shfl_xor(y, d);
+    }
+  } else {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      x += __shfl_xor(x, d);
+      y += __shfl_xor(y, d);
+    }
+    float *at = sm + (turn ^= 32);   // (two places in turn: one barrier a sum)
+    if ((threadIdx.x & 63) == 0) {
+      at[threadIdx.x >> 6] = x;
+      at[16 + (threadIdx.x >> 6)] = y;
+    }
+    __syncthreads();
+    const int waves = S >> 6, first = threadIdx.x / S * waves;
+    x = y = 0.f;
+    for (int i = 0; i < waves; ++i) {
+      x += at[first + i];
+      y += at[16 + first + i];
+    }
+  }
+}
+template <int WIDE>
+__device__ __forceinline__ float row_sum(float x, int S, float *sm, int &turn) {
+  float y = 0.f;
+  row_sums<WIDE>(x, y, S, sm, turn);
+  return x;
+}
+
+// f(i, e) of all values held.  Lanes without a value hold zeros that their sums take in.
+template <int W, int NV, typename F>
+__device__ __forceinline__ void each(F f) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < W; ++e) f(i, e);
+}
+
+// x becomes its normalised values; returns 1 / deviation.
+template <int WIDE, int W, int NV>
+__device__ __forceinline__ float normalise(float (&x)[NV][W], const bool (&ok)[NV], const RowArgs &a, float *sm, int &turn) {
+  const float inv = 1.f / static_cast<float>(a.per);
+  if (a.layer) {
+    float t = 0.f;
+    each<W, NV>([&](int i, int e) { t += x[i][e]; });
+    const float mean = row_sum<WIDE>(t, a.S, sm, turn) * inv;
+    each<W, NV>([&](int i, int e) { x[i][e] = ok[i] ? x[i][e] - mean : 0.f; });
+  }
+  float t = 0.f;
+  each<W, NV>([&](int i, int e) { t = fmaf(x[i][e], x[i][e], t); });
+  const float rstd = 1.f / sqrtf(row_sum<WIDE>(t, a.S, sm, turn) * inv + a.eps);
+  each<W, NV>([&](int i, int e) { x[i][e] *= rstd; });
+  return rstd;
+}
+// h, the gradient of normalised values n, becomes that of what they were made of.
+template <int WIDE, int W, int NV>
+__device__ __forceinline__ void normalise_back(float (&h)[NV][W], const float (&n)[NV][W], float rstd, const bool (&ok)[NV],
+                                               const RowArgs &a, float *sm, int &turn) {
+  const float inv = 1.f / static_cast<float>(a.per);
+  float t = 0.f, v = 0.f;
+  each<W, NV>([&](int i, int e) {
+    t += h[i][e];
+    v = fmaf(h[i][e], n[i][e], v);
+  });
+  row_sums<WIDE>(t, v, a.S, sm, turn);
+  const float m = a.layer ? t * inv : 0.f;
+  v *= inv;
+  each<W, NV>([&](int i, int e) { h[i][e] = ok[i] ? rstd * (h[i][e] - m - n[i][e] * v) : 0.f; });
+}
+
+// W values of a vector over the channels, or of its default.
+template <int W>
+__device__ __forceinline__ void load_weights(const float *p, int c, float other, float (&x)[W]) {
+#pragma unroll
+  for (int e = 0; e < W; ++e) x[e] = other;
+  if (!p) return;
+  if constexpr (W >= 4) {
+#pragma unroll
+    for (int e = 0; e < W; e += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(p + c + e);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[e + i] = v[i];
+    }
+  } else {
+    x[0] = p[c];
+  }
+}
+
+// Where a lane works: its place j among the S lanes of a row, the group of channels g
+// and the first row; lane groups that have none (`on` false) idle along.
+template <int W, int NV>
+struct Place {
+  int j, g, c[NV];
+  int64_t row, first;   // its first row, and the workgroup's
+  bool on, col[NV], has[NV], ok[NV];   // the vector's channels exist; with a row at all; with the row worked on
+  __device__ __forceinline__ explicit Place(const RowArgs &a) {
+    const int64_t sub = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / a.S;
+    j = threadIdx.x & (a.S - 1);
+    g = static_cast<int>(sub % a.G);
+    row = sub / a.G;
+    first = static_cast<int64_t>(blockIdx.x) * blockDim.x / a.S / a.G;
+    on = row < a.slots;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      c[i] = (j + a.S * i) * W;
+      col[i] = c[i] < a.per;
+      has[i] = on && col[i];
+      ok[i] = has[i] && row < a.N;
+      c[i] = (col[i] ? c[i] : 0) + g * a.per;
+    }
+  }
+  // Row n is the one worked on: lanes behind the last row idle along.
+  __device__ __forceinline__ void at(int64_t n, int64_t N) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) ok[i] = has[i] && n < N;
+  }
+};
+
+template <int DT, int W, int NV>
+__device__ __forceinline__ void load_row(Vec<DT, W> (&x)[NV], const void *p, int64_t at, const Place<W, NV> &l, bool on) {
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    x[i] = Vec<DT, W>{};
+    if (l.has[i] && on) x[i] = load_vec<DT, W>(p, at + l.c[i]);
+  }
+}
+
+// Adds the workgroup's sums over rows and leaves them in rows of a.part ([rows][KINDS][C]):
+// a row a workgroup, or a row a slot where a workgroup has not all groups of channels.
+template <int W, int NV, int KINDS>
+__device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV> &l, const float (&sum)[KINDS][NV][W], float *sm) {
+  const int lanes = blockDim.x, groups = lanes / a.S, mine = threadIdx.x / a.S;   // lane groups
+  const bool all = a.G <= groups;
+  const int64_t to = all ? static_cast<int64_t>(blockIdx.x) : l.row;
+#pragma unroll
+  for (int k = 0; k < KINDS; ++k) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int e = 0; e < W; ++e) sm[(e * NV + i) * lanes + threadIdx.x] = l.has[i] ? sum[k][i][e] : 0.f;
+    __syncthreads();
+    // lane groups of one group of channels are G apart: the first adds them up
+    if (mine < a.G && (all || l.on))
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (l.col[i])
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            float t = 0.f;
+            for (int q = mine; q < groups; q += a.G) t += sm[(e * NV + i) * lanes + q * a.S + l.j];
+            a.part[(to * KINDS + k) * a.C + l.c[i] + e] = t;
+          }
+  }
+}
+
+__device__ __forceinline__ float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z)); }
+
+// -------------------------------------------------------------------- gated --
+template <int DT, int W, int NV, int WIDE>
+__global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void gated_fwd_kernel(const RowArgs a) {
+  __shared__ float sm[64];
+  int turn = 0;
+  Place<W, NV> l(a);
+  Vec<DT, W> x[NV], z[NV], nx[NV], nz[NV];
+  load_row<DT, W, NV>(nx, a.x, l.row * a.ldx, l, l.row < a.N);
+  load_row<DT, W, NV>(nz, a.z, l.row * a.ldz, l, l.row < a.N);
+  for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
+    l.at(n, a.N);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = nx[i];
+      z[i] = nz[i];
+    }
+    if (n + a.slots < a.N) {
+      load_row<DT, W, NV>(nx, a.x, (n + a.slots) * a.ldx, l, true);
+      load_row<DT, W, NV>(nz, a.z, (n + a.slots) * a.ldz, l, true);
+    }
+    float v[NV][W];
+    each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
+    normalise<WIDE, W, NV>(v, l.ok, a, sm, turn);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (l.ok[i]) {
+        float w[W], b[W];
+        load_weights<W>(a.w, l.c[i], 1.f, w);
+        load_weights<W>(a.b, l.c[i], 0.f, b);
+        Vec<DT, W> y;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float g = z[i][e], s = sigmoid_of(g);
+          y.set(e, fmaf(v[i][e], w[e], b[e]) * (a.silu ? g * s : s));
+        }
+        store_vec<DT, W>(a.y, n * a.C + l.c[i], y);
+      }
+  }
+}
+
+template <int DT, int W, int NV, int WIDE>
+__global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(const RowArgs a) {
+  __shared__ float sm[(WIDE ? WIDE : kBwdThreads) * kHold];
+  int turn = 0;
+  Place<W, NV> l(a);
+  float sum[2][NV][W];   // of w and b
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < W; ++e) sum[0][i][e] = sum[1][i][e] = 0.f;
+  Vec<DT, W> x[NV], z[NV], dy[NV], nx[NV], nz[NV], ndy[NV];
+  auto fetch = [&](int64_t n, bool on) {
+    load_row<DT, W, NV>(nx, a.x, n * a.ldx, l, on);
+    load_row<DT, W, NV>(nz, a.z, n * a.ldz, l, on);
+    load_row<DT, W, NV>(ndy, a.dy, n * a.C, l, on);
+  };
+  fetch(l.row, l.row < a.N);
+  for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
+    l.at(n, a.N);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = nx[i];
+      z[i] = nz[i];
+      dy[i] = ndy[i];
+    }
+    if (n + a.slots < a.N) fetch(n + a.slots, true);
+    float v[NV][W], h[NV][W];
+    each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
+    const float rstd = normalise<WIDE, W, NV>(v, l.ok, a, sm, turn);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        float w[W], b[W];
+        load_weights<W>(a.w, l.c[i], 1.f, w);
+        load_weights<W>(a.b, l.c[i], 0.f, b);
+        Vec<DT, W> dz;
+#pragma unroll
+        for (int e = 0; e < W; ++e) {
+          const float g = z[i][e], s = sigmoid_of(g), o = sigmoid_of(-g);
+          const float act = a.silu ? g * s : s, slope = a.silu ? fmaf(g * s, o, s) : s * o;
+          const float d = dy[i][e], dv = d * act;
+          dz.set(e, d * fmaf(v[i][e], w[e], b[e]) * slope);
+          sum[0][i][e] = fmaf(dv, v[i][e], sum[0][i][e]);
+          sum[1][i][e] += dv;
+          h[i][e] = dv * w[e];
+        }
+        if (a.dz && l.ok[i]) store_vec<DT, W>(a.dz, n * a.C + l.c[i], dz);
+      }
+    if (a.y) {
+      normalise_back<WIDE, W, NV>(h, v, rstd, l.ok, a, sm, turn);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (l.ok[i]) {
+          Vec<DT, W> dx;
+#pragma unroll
+          for (int e = 0; e < W; ++e) dx.set(e, h[i][e]);
+          store_vec<DT, W>(a.y, n * a.C + l.c[i], dx);
+        }
+    }
+  }
+  if (a.part) leave_sums<W, NV, 2>(a, l, sum, sm);
+}
+
+// ----------------------------------------------------------------- residual --
+// The stream's value before its norm and, for the backward, what is kept of the way
+// there: the branch's normalised values, their 1 / deviation and the mask.
+template <int DT, int DTR, int W, int NV, int WIDE>
+struct Stream {
+  float s[NV][W], n2[NV][W], rstd2;
+  uint32_t keep[NV];
+  __device__ __forceinline__ void run(const RowArgs &a, const Place<W, NV> &l, const Vec<DT, W> (&x)[NV], const Vec<DTR, W> (&r)[NV],
+                                      float scale, uint64_t seed, int64_t n, float *sm, int &turn) {
+    each<W, NV>([&](int i, int e) { n2[i][e] = x[i][e]; });
+    rstd2 = a.post ? normalise<WIDE, W, NV>(n2, l.ok, a, sm, turn) : 1.f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      keep[i] = ~0u;
+      if (a.draw.threshold) keep[i] = kept<W>(a.draw, seed, static_cast<uint64_t>(n) * a.C + l.c[i]);
+      float w2[W], c[W];
+      load_weights<W>(a.w2, l.c[i], 1.f, w2);
+      load_weights<W>(a.gamma, l.c[i], 1.f, c);
+#pragma unroll
+      for (int e = 0; e < W; ++e) s[i][e] = r[i][e] + (keep[i] >> e & 1 ? c[e] * scale * (n2[i][e] * w2[e]) : 0.f);
+    }
+  }
+};
+
+template <int DT, int DTR, int W, int NV, int WIDE>
+__global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void residual_fwd_kernel(const RowArgs a) {
+  __shared__ float sm[64];
+  int turn = 0;
+  Place<W, NV> l(a);
+  const float scale = a.alpha * (a.draw.threshold ? a.draw.scale : 1.f);
+  const uint64_t seed = a.draw.threshold ? static_cast<uint64_t>(*a.draw.seed) : 0;
+  Vec<DT, W> x[NV], nx[NV];
+  Vec<DTR, W> r[NV], nr[NV];
+  load_row<DT, W, NV>(nx, a.x, l.row * a.C, l, l.row < a.N);
+  load_row<DTR, W, NV>(nr, a.r, l.row * a.C, l, l.row < a.N);
+  for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
+    l.at(n, a.N);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = nx[i];
+      r[i] = nr[i];
+    }
+    if (n + a.slots < a.N) {
+      load_row<DT, W, NV>(nx, a.x, (n + a.slots) * a.C, l, true);
+      load_row<DTR, W, NV>(nr, a.r, (n + a.slots) * a.C, l, true);
+    }
+    Stream<DT, DTR, W, NV, WIDE> t;
+    t.run(a, l, x, r, scale, seed, n, sm, turn);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (l.ok[i]) {
+        Vec<DTR, W> s;
+#pragma unroll
+        for (int e = 0; e < W; ++e) s.set(e, t.s[i][e]);
+        store_vec<DTR, W>(a.s, n * a.C + l.c[i], s);
+      }
+    normalise<WIDE, W, NV>(t.s, l.ok, a, sm, turn);
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      if (l.ok[i]) {
+        float w[W], b[W];
+        load_weights<W>(a.w, l.c[i], 1.f, w);
+        load_weights<W>(a.b, l.c[i], 0.f, b);
+        Vec<DT, W> y;
+#pragma unroll
+        for (int e = 0; e < W; ++e) y.set(e, fmaf(t.s[i][e], w[e], b[e]));
+        store_vec<DT, W>(a.y, n * a.C + l.c[i], y);
+      }
+  }
+}
+
+template <int DT, int DTR, int W, int NV, int WIDE>
+__global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel(const RowArgs a) {
+  __shared__ float sm[(WIDE ? WIDE : kBwdThreads) * kHold];
+  int turn = 0;
+  Place<W, NV> l(a);
+  float sum[4][NV][W];   // of w, b, gamma, w2
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+#pragma unroll
+    for (int e = 0; e < W; ++e) sum[0][i][e] = sum[1][i][e] = sum[2][i][e] = sum[3][i][e] = 0.f;
+  const float scale = a.alpha * (a.draw.threshold ? a.draw.scale : 1.f);
+  const uint64_t seed = a.draw.threshold ? static_cast<uint64_t>(*a.draw.seed) : 0;
+  Vec<DT, W> x[NV], nx[NV], dy[NV], ndy[NV];
+  Vec<DTR, W> r[NV], nr[NV], ds[NV], nds[NV];
+  auto fetch = [&](int64_t n, bool on) {
+    load_row<DT, W, NV>(nx, a.x, n * a.C, l, on);
+    load_row<DTR, W, NV>(nr, a.r, n * a.C, l, on);
+    load_row<DT, W, NV>(ndy, a.dy, n * a.C, l, on && a.dy);
+    load_row<DTR, W, NV>(nds, a.ds, n * a.C, l, on && a.ds);
+  };
+  fetch(l.row, l.row < a.N);
+  for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
+    l.at(n, a.N);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      x[i] = nx[i];
+      r[i] = nr[i];
+      dy[i] = ndy[i];
+      ds[i] = nds[i];
+    }
+    if (n + a.slots < a.N) fetch(n + a.slots, true);
+    Stream<DT, DTR, W, NV, WIDE> t;
+    t.run(a, l, x, r, scale, seed, n, sm, turn);
+    float d[NV][W];
+    if (a.dy) {
+      const float rstd = normalise<WIDE, W, NV>(t.s, l.ok, a, sm, turn);
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+          float w[W];
+          load_weights<W>(a.w, l.c[i], 1.f, w);
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const float g = dy[i][e];
+            sum[0][i][e] = fmaf(g, t.s[i][e], sum[0][i][e]);
+            sum[1][i][e] += g;
+            d[i][e] = g * w[e];
+          }
+        }
+      normalise_back<WIDE, W, NV>(d, t.s, rstd, l.ok, a, sm, turn);
+      each<W, NV>([&](int i, int e) { d[i][e] += ds[i][e]; });   // (zeros without one)
+    } else {
+      each<W, NV>([&](int i, int e) { d[i][e] = ds[i][e]; });
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        if (a.s && l.ok[i]) {
+          Vec<DTR, W> dr;
+#pragma unroll
+          for (int e = 0; e < W; ++e) dr.set(e, d[i][e]);
+          store_vec<DTR, W>(a.s, n * a.C + l.c[i], dr);
+        }
+        float w2[W], c[W];
+        load_weights<W>(a.w2, l.c[i], 1.f, w2);
+        load_weights<W>(a.gamma, l.c[i], 1.f, c);
+#pragma unroll
+        for (int e = 0; e < W; ++e) {   // (what was dropped is 0 whatever it was)
+          const bool on = t.keep[i] >> e & 1;
+          const float g = on ? d[i][e] * scale : 0.f, v = on ? t.n2[i][e] : 0.f, dp = g * c[e];
+          sum[2][i][e] = fmaf(g, v * w2[e], sum[2][i][e]);
+          sum[3][i][e] = fmaf(dp, v, sum[3][i][e]);
+          d[i][e] = dp * w2[e];
+        }
+      }
+    if (a.y) {
+      if (a.post) normalise_back<WIDE, W, NV>(d, t.n2, t.rstd2, l.ok, a, sm, turn);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+        if (l.ok[i]) {
+          Vec<DT, W> dx;
+#pragma unroll
+          for (int e = 0; e < W; ++e) dx.set(e, d[i][e]);
+          store_vec<DT, W>(a.y, n * a.C + l.c[i], dx);
+        }
+    }
+  }
+  if (a.part) leave_sums<W, NV, 4>(a, l, sum, sm);
+}
+
+// Sums down R rows of [R][KINDS C]: 64 columns a workgroup, 16 wavefronts with every
+// 16th row each.
+struct Sums { float *to[4]; };
+__global__ __launch_bounds__(1024) void row_cols_kernel(const float *__restrict__ src, int64_t R, int64_t cols, int C, Sums out) {
+  __shared__ float sm[16][64];
+  const int w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+  float t = 0.f;
+  if (c < cols) {
+#pragma unroll 8
+    for (int64_t r = w; r < R; r += 16) t += src[r * cols + c];
+  }
+  sm[w][lane] = t;
+  __syncthreads();
+  if (w == 0 && c < cols) {
+    t = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) t += sm[i][lane];
+    float *to = out.to[c / C];
+    if (to) to[c % C] = t;
+  }
+}
+
+// ----------------------------------------------------------------- launches --
+// How the rows are dealt, from the sizes and the widest vector the addresses allow.
+struct RowPlan {
+  int W, NV, S, threads;
+  bool wide;
+  int64_t slots, blocks, rows;   // rows: of sums
+};
+// Wavefronts: the forward's lane groups have a few rows each, the backward's as many as
+// leave two workgroups a CU: their sums over rows go through memory once a workgroup.
+constexpr int64_t kFwdWaves = 8192, kBwdWaves = 4096;
+
+RowPlan plan_of(int64_t N, int per, int G, int W, bool bwd) {
+  RowPlan p{};
+  p.W = W;
+  const int nv = per / W, most = kHold / W;
+  p.S = 1;
+  while (p.S < nv && (p.S < 64 || static_cast<int64_t>(p.S) * most < nv)) p.S *= 2;
+  p.wide = p.S > 64;
+  p.threads = std::max(bwd ? kBwdThreads : kFwdThreads, p.S);
+  p.NV = 1;
+  while (p.NV < most && (p.wide || static_cast<int64_t>(p.S) * p.NV < nv)) p.NV *= W == 1 ? kHold : 2;
+  const int64_t groups = p.threads / p.S;   // lane groups of a workgroup
+  const int64_t need = (N * G + groups - 1) / groups;
+  p.blocks = std::min(need, (bwd ? kBwdWaves : kFwdWaves) * 64 / p.threads);
+  // a lane group keeps its group of channels, so all groups have as many (one row at a time at least)
+  p.slots = std::min(N, std::max<int64_t>(1, p.blocks * groups / G));
+  p.blocks = (p.slots * G + groups - 1) / groups;
+  p.rows = G <= groups ? p.blocks : p.slots;
+  return p;
+}
+
+struct Tensor { const void *p; int64_t ld; int dtype; };
+int widest(int per, int dtype, std::initializer_list<Tensor> tensors, std::initializer_list<const float *> weights) {
+  for (const float *w : weights)
+    if (!aligned(w, 16)) return 1;   // (NULL is aligned)
+  for (int W = dtype == SSLA_F32 ? 4 : 8; W >= 4; W /= 2) {
+    bool ok = per % W == 0;
+    for (const Tensor &t : tensors) {
+      const int bytes = std::min(16, W * (t.dtype == SSLA_F32 ? 4 : 2));
+      ok = ok && aligned(t.p, bytes) && t.ld * (t.dtype == SSLA_F32 ? 4 : 2) % bytes == 0;
+    }
+    if (ok) return W;
+  }
+  return 1;
+}
+
+size_t sums_bytes(int64_t N, int per, int G, int kinds) {   // whatever vectors the addresses allow
+  int64_t most = 0;
+  for (int W = 1; W <= 8; W *= 2)
+    if (W != 2 && per % W == 0) most = std::max(most, plan_of(N, per, G, W, true).rows);
+  return static_cast<size_t>(most) * kinds * per * G * sizeof(float);
+}
+
+int check_sizes(const char *what, int64_t N, int C, int G, int kind, int dtype, int r_dtype) {
+  SSLA_CHECK_ARG(N >= 0 && C > 0 && G > 0 && C % G == 0 && (kind == SSLA_NORM_RMS || kind == SSLA_NORM_LAYER),
+                 "%s: bad sizes N=%lld C=%d G=%d kind=%d", what, (long long)N, C, G, kind);
+  const bool known = dtype == SSLA_F32 || dtype == SSLA_BF16 || dtype == SSLA_F16;
+  if (!known || (r_dtype != dtype && r_dtype != SSLA_F32)) {
+    set_error("%s: unsupported dtypes %d, %d", what, dtype, r_dtype);
+    return SSLA_ERR_DTYPE;
+  }
+  if (C / G > kHold * kMostLanes || C > 1 << 24 || N > (1ll << 40) / C) {
+    set_error("%s: at most %d channels in a group and 2^40 values", what, kHold * kMostLanes);
+    return SSLA_ERR_UNSUPPORTED;
+  }
+  return SSLA_OK;
+}
+int check_ws(const char *what, const void *ws, size_t have, size_t need) {
+  if (need == 0 || (ws && have >= need && aligned(ws, 16))) return SSLA_OK;
+  set_error("%s: needs %zu bytes of workspace, got %zu", what, need, have);
+  return SSLA_ERR_WORKSPACE;
+}
+int check_draw(const char *what, float p, const int64_t *seed, Draw &d) {
+  SSLA_CHECK_ARG(p >= 0.f && p <= 1.f, "%s: p must lie in [0, 1], got %g", what, static_cast<double>(p));
+  d.threshold = static_cast<uint32_t>(lrint(static_cast<double>(p) * 65536.0));
+  SSLA_CHECK_ARG(d.threshold == 0 || seed, "%s: seed is NULL", what);
+  d.seed = seed;
+  d.scale = d.threshold < 65536 ? static_cast<float>(65536.0 / (65536.0 - d.threshold)) : 0.f;
+  return SSLA_OK;
+}
+
+// Launches K<..., W, NV, WIDE> by the plan (WIDE: the threads whose registers a row of
+// several wavefronts has to do with; 0: rows of one wavefront).
+#define SSLA_ROWS_NV(K, W_, NV_, ...)                                                                        \
+  if (p.W == W_ && p.NV == NV_) {                                                                            \
+    if (p.wide) {                                                                                            \
+      if constexpr (W_ * NV_ == kHold) {                                                                     \
+        if (p.threads <= 512) hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, 512>), grid, block, 0, st, a);     \
+        else hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, kMostLanes>), grid, block, 0, st, a);               \
+      }                                                                                                      \
+    } else {                                                                                                 \
+      hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, 0>), grid, block, 0, st, a);                               \
+    }                                                                                                        \
+  }
+#define SSLA_ROWS(K, D, ...)                                  \
+  do {                                                        \
+    const dim3 grid(static_cast<unsigned>(p.blocks)), block(p.threads); \
+    if constexpr (D != SSLA_F32) {                            \
+      SSLA_ROWS_NV(K, 8, 1, __VA_ARGS__)                      \
+    }                                                         \
+    SSLA_ROWS_NV(K, 4, 1, __VA_ARGS__)                        \
+    SSLA_ROWS_NV(K, 4, 2, __VA_ARGS__)                        \
+    SSLA_ROWS_NV(K, 1, 1, __VA_ARGS__)                        \
+    SSLA_ROWS_NV(K, 1, 8, __VA_ARGS__)                        \
+  } while (0)
+#define SSLA_GATED(K)                                             \
+  if (dtype == SSLA_F32) SSLA_ROWS(K, SSLA_F32, SSLA_F32);        \
+  else if (dtype == SSLA_BF16) SSLA_ROWS(K, SSLA_BF16, SSLA_BF16); \
+  else SSLA_ROWS(K, SSLA_F16, SSLA_F16)
+#define SSLA_RESIDUAL(K)                                                                 \
+  if (dtype == SSLA_F32) SSLA_ROWS(K, SSLA_F32, SSLA_F32, SSLA_F32);                     \
+  else if (dtype == SSLA_BF16 && r_dtype == SSLA_F32) SSLA_ROWS(K, SSLA_BF16, SSLA_BF16, SSLA_F32); \
+  else if (dtype == SSLA_BF16) SSLA_ROWS(K, SSLA_BF16, SSLA_BF16, SSLA_BF16);            \
+  else if (r_dtype == SSLA_F32) SSLA_ROWS(K, SSLA_F16, SSLA_F16, SSLA_F32);              \
+  else SSLA_ROWS(K, SSLA_F16, SSLA_F16, SSLA_F16)
+
+void set_plan(RowArgs &a, const RowPlan &p) {
+  a.S = p.S;
+  a.slots = p.slots;
+}
+void add_columns(const float *part, int64_t rows, int kinds, int C, Sums out, hipStream_t st) {
+  const int64_t cols = static_cast<int64_t>(kinds) * C;
+  hipLaunchKernelGGL(row_cols_kernel, dim3(static_cast<unsigned>((cols + 63) / 64)), dim3(1024), 0, st, part, rows, cols, C, out);
+}
+
+}  // namespace
+}  // namespace ssla
+
+extern "C" int ssla_gated_norm_fwd(const void *x, int64_t ldx, const void *z, int64_t ldz, int64_t N, int C, int G, int kind,
+                                   const float *weight, const float *bias, float eps, int act, void *y, int dtype,
+                                   void *stream) {
+  using namespace ssla;
+  clear_error();
+  if (const int e = check_sizes("gated_norm_fwd", N, C, G, kind, dtype, dtype)) return e;
+  SSLA_CHECK_ARG((act == SSLA_ACT_SILU || act == SSLA_ACT_SIGMOID) && (N <= 1 || (ldx >= C && ldz >= C)),
+                 "gated_norm_fwd: bad activation %d or row strides %lld, %lld", act, (long long)ldx, (long long)ldz);
+  if (N == 0) return SSLA_OK;
+  SSLA_CHECK_ARG(x && z && y, "gated_norm_fwd: null pointer");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  RowArgs a{};
+  a.x = x; a.z = z; a.ldx = ldx; a.ldz = ldz; a.w = weight; a.b = bias; a.y = y;
+  a.N = N; a.C = C; a.G = G; a.per = C / G; a.layer = kind == SSLA_NORM_LAYER; a.silu = act == SSLA_ACT_SILU; a.eps = eps;
+  const RowPlan p = plan_of(N, C / G, G, widest(C / G, dtype, {{x, ldx, dtype}, {z, ldz, dtype}, {y, C, dtype}}, {weight, bias}), false);
+  set_plan(a, p);
+  SSLA_GATED(gated_fwd_kernel);
+  return launch_status("gated_norm_fwd");
+}
+
+extern "C" size_t ssla_gated_norm_bwd_workspace_size(int64_t N, int C, int G) {
+  return N > 0 && C > 0 && G > 0 && C % G == 0 ? ssla::sums_bytes(N, C / G, G, 2) : 0;
+}
+
+extern "C" int ssla_gated_norm_bwd(const void *dy, const void *x, int64_t ldx, const void *z, int64_t ldz, int64_t N, int C,
+                                   int G, int kind, const float *weight, const float *bias, float eps, int act, void *dx,
+                                   void *dz, float *dweight, float *dbias, int dtype, void *workspace,
+                                   size_t workspace_bytes, void *stream) {
+  using namespace ssla;
+  clear_error();
+  if (const int e = check_sizes("gated_norm_bwd", N, C, G, kind, dtype, dtype)) return e;
+  SSLA_CHECK_ARG((act == SSLA_ACT_SILU || act == SSLA_ACT_SIGMOID) && (N <= 1 || (ldx >= C && ldz >= C)),
+                 "gated_norm_bwd: bad activation %d or row strides %lld, %lld", act, (long long)ldx, (long long)ldz);
+  SSLA_CHECK_ARG(N == 0 || (dy && x && z), "gated_norm_bwd: null pointer");
+  const bool sums = dweight || dbias;
+  if (const int e = check_ws("gated_norm_bwd", workspace, workspace_bytes,
+                             sums ? ssla_gated_norm_bwd_workspace_size(N, C, G) : 0)) return e;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  RowPlan p{};
+  if (N > 0) {
+    RowArgs a{};
+    a.x = x; a.z = z; a.dy = dy; a.ldx = ldx; a.ldz = ldz; a.w = weight; a.b = bias; a.y = dx; a.dz = dz;
+    a.part = sums ? static_cast<float *>(workspace) : nullptr;
+    a.N = N; a.C = C; a.G = G; a.per = C / G; a.layer = kind == SSLA_NORM_LAYER; a.silu = act == SSLA_ACT_SILU; a.eps = eps;
+    p = plan_of(N, C / G, G, widest(C / G, dtype, {{x, ldx, dtype}, {z, ldz, dtype}, {dy, C, dtype}, {dx, C, dtype}, {dz, C, dtype}},
+                                    {weight, bias}), true);
+    set_plan(a, p);
+    SSLA_GATED(gated_bwd_kernel);
+  }
+  if (sums) add_columns(static_cast<const float *>(workspace), p.rows, 2, C, {{dweight, dbias, nullptr, nullptr}}, st);
+  return launch_status("gated_norm_bwd");
+}
+
+extern "C" int ssla_residual_norm_fwd(const void *x, const void *residual, int64_t N, int C, int kind, const float *weight,
+                                      const float *bias, float eps, float alpha, const float *gamma, int post,
+                                      const float *post_weight, float p, const int64_t *seed, uint32_t subsequence, void *y,
+                                      void *sum, int dtype, int r_dtype, void *stream) {
+  using namespace ssla;
+  clear_error();
+  if (const int e = check_sizes("residual_norm_fwd", N, C, 1, kind, dtype, r_dtype)) return e;
+  RowArgs a{};
+  if (const int e = check_draw("residual_norm_fwd", p, seed, a.draw)) return e;
+  SSLA_CHECK_ARG(post || !post_weight, "residual_norm_fwd: a weight of a norm that is not asked for");
+  if (N == 0) return SSLA_OK;
+  SSLA_CHECK_ARG(x && residual && y && sum, "residual_norm_fwd: null pointer");
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  a.draw.subsequence = subsequence;
+  a.x = x; a.r = residual; a.w = weight; a.b = bias; a.w2 = post_weight; a.gamma = gamma; a.y = y; a.s = sum;
+  a.N = N; a.C = a.per = C; a.G = 1; a.layer = kind == SSLA_NORM_LAYER; a.post = post != 0; a.eps = eps; a.alpha = alpha;
+  const RowPlan pl = plan_of(N, C, 1, widest(C, dtype, {{x, C, dtype}, {residual, C, r_dtype}, {y, C, dtype}, {sum, C, r_dtype}},
+                                             {weight, bias, post_weight, gamma}), false);
+  {
+    const RowPlan &p = pl;
+    set_plan(a, p);
+    SSLA_RESIDUAL(residual_fwd_kernel);
+  }
+  return launch_status("residual_norm_fwd");
+}
+
+extern "C" size_t ssla_residual_norm_bwd_workspace_size(int64_t N, int C) {
+  return N > 0 && C > 0 ? ssla::sums_bytes(N, C, 1, 4) : 0;
+}
+
+extern "C" int ssla_residual_norm_bwd(const void *dy, const void *dsum, const void *x, const void *residual, int64_t N, int C,
+                                      int kind, const float *weight, float eps, float alpha, const float *gamma, int post,
+                                      const float *post_weight, float p, const int64_t *seed, uint32_t subsequence, void *dx,
+                                      void *dresidual, float *dweight, float *dbias, float *dgamma, float *dpost_weight,
+                                      int dtype, int r_dtype, void *workspace, size_t workspace_bytes, void *stream) {
+  using namespace ssla;
+  clear_error();
+  if (const int e = check_sizes("residual_norm_bwd", N, C, 1, kind, dtype, r_dtype)) return e;
+  RowArgs a{};
+  if (const int e = check_draw("residual_norm_bwd", p, seed, a.draw)) return e;
+  SSLA_CHECK_ARG(post || (!post_weight && !dpost_weight), "residual_norm_bwd: a weight of a norm that is not asked for");
+  SSLA_CHECK_ARG(N == 0 || ((dy || dsum) && x && residual), "residual_norm_bwd: null pointer");
+  const bool sums = dweight || dbias || dgamma || dpost_weight;
+  if (const int e = check_ws("residual_norm_bwd", workspace, workspace_bytes,
+                             sums ? ssla_residual_norm_bwd_workspace_size(N, C) : 0)) return e;
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+  int64_t rows = 0;
+  if (N > 0) {
+    a.draw.subsequence = subsequence;
+    a.x = x; a.r = residual; a.dy = dy; a.ds = dsum; a.w = weight; a.w2 = post_weight; a.gamma = gamma; a.y = dx; a.s = dresidual;
+    a.part = sums ? static_cast<float *>(workspace) : nullptr;
+    a.N = N; a.C = a.per = C; a.G = 1; a.layer = kind == SSLA_NORM_LAYER; a.post = post != 0; a.eps = eps; a.alpha = alpha;
+    const RowPlan p = plan_of(N, C, 1, widest(C, dtype, {{x, C, dtype}, {residual, C, r_dtype}, {dy, C, dtype}, {dsum, C, r_dtype},
+                                                         {dx, C, dtype}, {dresidual, C, r_dtype}}, {weight, post_weight, gamma}), true);
+    rows = p.rows;
+    set_plan(a, p);
+    SSLA_RESIDUAL(residual_bwd_kernel);
+  }
+  if (sums) add_columns(static_cast<const float *>(workspace), rows, 4, C, {{dweight, dbias, dgamma, dpost_weight}}, st);
+  return launch_status("residual_norm_bwd");
+}
