@@ -27,7 +27,7 @@ namespace {
 
 constexpr int kHold = 8;        // values that a lane holds of a row
 constexpr int kMostLanes = 1024;
-constexpr int kFwdThreads = 256, kBwdThreads = 512;   // of a workgroup, unless a row needs more
+constexpr int kFwdThreads = 256, kBwdThreads = 256;   // of a workgroup, unless a row needs more
 
 struct RowArgs {
   const void *x, *r, *z, *dy, *ds;   // ds, and dy of the residual's backward, may be NULL
@@ -44,40 +44,48 @@ struct RowArgs {
 };
 
 // ------------------------------------------------------------- a row's lanes --
-// The sums of x and y over a row's lanes, in the same order on every lane.  WIDE: over
+template <int CTRL>
+__device__ __forceinline__ float dpp_of(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, false));
+}
+// The sum over S neighbouring lanes (a power of two up to 64), the same on each, by lane
+// swaps on the VALU: neighbours, pairs, mirrored fours and eights (equal inside them by
+// then), rows of 16 and halves.
+__device__ __forceinline__ float lane_sum(float x, int S) {
+  if (S > 1) x += dpp_of<0xB1>(x);
+  if (S > 2) x += dpp_of<0x4E>(x);
+  if (S > 4) x += dpp_of<0x141>(x);
+  if (S > 8) x += dpp_of<0x140>(x);
+  if (S > 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if (S > 32) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  return x;
+}
+
+// The sums of M values over a row's lanes, in the same order on every lane.  WIDE: over
 // several wavefronts, all threads of the workgroup at once.
-template <int WIDE>
-__device__ __forceinline__ void row_sums(float &x, float &y, int S, float *sm, int &turn) {
-  if constexpr (WIDE == 0) {
-    for (int d = 1; d < S; d <<= 1) {
-      x += __shfl_xor(x, d);
-      y += __shfl_xor(y, d);
-    }
-  } else {
+template <int WIDE, int M>
+__device__ __forceinline__ void row_sums(float (&x)[M], int S, float *sm, int &turn) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      x += __shfl_xor(x, d);
-      y += __shfl_xor(y, d);
-    }
+  for (int k = 0; k < M; ++k) x[k] = lane_sum(x[k], WIDE ? 64 : S);
+  if constexpr (WIDE != 0) {
     float *at = sm + (turn ^= 32);   // (two places in turn: one barrier a sum)
-    if ((threadIdx.x & 63) == 0) {
-      at[threadIdx.x >> 6] = x;
-      at[16 + (threadIdx.x >> 6)] = y;
-    }
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int k = 0; k < M; ++k) at[16 * k + (threadIdx.x >> 6)] = x[k];
     __syncthreads();
     const int waves = S >> 6, first = threadIdx.x / S * waves;
-    x = y = 0.f;
-    for (int i = 0; i < waves; ++i) {
-      x += at[first + i];
-      y += at[16 + first + i];
+#pragma unroll
+    for (int k = 0; k < M; ++k) {
+      x[k] = 0.f;
+      for (int i = 0; i < waves; ++i) x[k] += at[16 * k + first + i];
     }
   }
-}
-template <int WIDE>
-__device__ __forceinline__ float row_sum(float x, int S, float *sm, int &turn) {
-  float y = 0.f;
-  row_sums<WIDE>(x, y, S, sm, turn);
-  return x;
 }
 
 // f(i, e) of all values held.  Lanes without a value hold zeros that their sums take in.
@@ -94,14 +102,16 @@ template <int WIDE, int W, int NV>
 __device__ __forceinline__ float normalise(float (&x)[NV][W], const bool (&ok)[NV], const RowArgs &a, float *sm, int &turn) {
   const float inv = 1.f / static_cast<float>(a.per);
   if (a.layer) {
-    float t = 0.f;
-    each<W, NV>([&](int i, int e) { t += x[i][e]; });
-    const float mean = row_sum<WIDE>(t, a.S, sm, turn) * inv;
+    float t[1] = {0.f};
+    each<W, NV>([&](int i, int e) { t[0] += x[i][e]; });
+    row_sums<WIDE>(t, a.S, sm, turn);
+    const float mean = t[0] * inv;
     each<W, NV>([&](int i, int e) { x[i][e] = ok[i] ? x[i][e] - mean : 0.f; });
   }
-  float t = 0.f;
-  each<W, NV>([&](int i, int e) { t = fmaf(x[i][e], x[i][e], t); });
-  const float rstd = 1.f / sqrtf(row_sum<WIDE>(t, a.S, sm, turn) * inv + a.eps);
+  float t[1] = {0.f};
+  each<W, NV>([&](int i, int e) { t[0] = fmaf(x[i][e], x[i][e], t[0]); });
+  row_sums<WIDE>(t, a.S, sm, turn);
+  const float rstd = 1.f / sqrtf(t[0] * inv + a.eps);
   each<W, NV>([&](int i, int e) { x[i][e] *= rstd; });
   return rstd;
 }
@@ -110,14 +120,13 @@ template <int WIDE, int W, int NV>
 __device__ __forceinline__ void normalise_back(float (&h)[NV][W], const float (&n)[NV][W], float rstd, const bool (&ok)[NV],
                                                const RowArgs &a, float *sm, int &turn) {
   const float inv = 1.f / static_cast<float>(a.per);
-  float t = 0.f, v = 0.f;
+  float t[2] = {0.f, 0.f};
   each<W, NV>([&](int i, int e) {
-    t += h[i][e];
-    v = fmaf(h[i][e], n[i][e], v);
+    t[0] += h[i][e];
+    t[1] = fmaf(h[i][e], n[i][e], t[1]);
   });
-  row_sums<WIDE>(t, v, a.S, sm, turn);
-  const float m = a.layer ? t * inv : 0.f;
-  v *= inv;
+  row_sums<WIDE>(t, a.S, sm, turn);
+  const float m = a.layer ? t[0] * inv : 0.f, v = t[1] * inv;
   each<W, NV>([&](int i, int e) { h[i][e] = ok[i] ? rstd * (h[i][e] - m - n[i][e] * v) : 0.f; });
 }
 
@@ -501,8 +510,8 @@ struct RowPlan {
   int64_t slots, blocks, rows;   // rows: of sums
 };
 // Wavefronts: the forward's lane groups have a few rows each, the backward's as many as
-// leave two workgroups a CU: their sums over rows go through memory once a workgroup.
-constexpr int64_t kFwdWaves = 8192, kBwdWaves = 4096;
+// leave three workgroups a CU: their sums over rows go through memory once a workgroup.
+constexpr int64_t kFwdWaves = 8192, kBwdWaves = 3072;
 
 RowPlan plan_of(int64_t N, int per, int G, int W, bool bwd) {
   RowPlan p{};
@@ -519,6 +528,7 @@ RowPlan plan_of(int64_t N, int per, int G, int W, bool bwd) {
   p.blocks = std::min(need, (bwd ? kBwdWaves : kFwdWaves) * 64 / p.threads);
   // a lane group keeps its group of channels, so all groups have as many (one row at a time at least)
   p.slots = std::min(N, std::max<int64_t>(1, p.blocks * groups / G));
+  p.slots = (N + (N + p.slots - 1) / p.slots - 1) / ((N + p.slots - 1) / p.slots);   // all as many rows as the busiest, or one less
   p.blocks = (p.slots * G + groups - 1) / groups;
   p.rows = G <= groups ? p.blocks : p.slots;
   return p;

@@ -228,9 +228,9 @@ def gated_norm(x: torch.Tensor, gate: torch.Tensor, num_groups: int = 1, weight:
     _lib.require_cuda(x, gate, weight, bias)
     rows, z = _flat(x), _flat(gate)
     options = num_groups, float(eps), GATE_ACTIVATIONS[activation], KINDS[kind]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, weight, bias)):
-        return GatedNormFunction.apply(rows, z, w, b, *options).view(x.shape)
-    return _gated_forward(rows, z, w, b, *options).view(x.shape)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, gate, weight, bias))
+    y = (GatedNormFunction.apply if grad else _gated_forward)(rows, z, w, b, *options)
+    return y if x.dim() == 2 else y.view(x.shape)   # (a view that changes nothing is a node of its own)
 
 
 class ResidualNormFunction(torch.autograd.Function):
@@ -328,10 +328,9 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
     if p > 0 and seed is None:
         raise ValueError(f"{name}: dropout needs a seed")
     seed = _seed(name, seed, subsequence, dev) if p > 0 else None
-    rows, r = _whole(x).view(-1, C), _whole(residual).view(-1, C)
+    flat = x.dim() == 2
+    rows, r = (_whole(t) if flat else _whole(t).view(-1, C) for t in (x, residual))
     options = float(eps), KINDS[kind], alpha, int(bool(post_norm)), p, subsequence
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        y, s = ResidualNormFunction.apply(rows, r, w, b, gamma, w2, seed, options)
-    else:
-        y, s = _residual_forward(rows, r, w, b, gamma, w2, seed, options)
-    return y.view(x.shape), s.view(x.shape)
+    grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    y, s = (ResidualNormFunction.apply if grad else _residual_forward)(rows, r, w, b, gamma, w2, seed, options)
+    return (y, s) if flat else (y.view(x.shape), s.view(x.shape))
