@@ -240,7 +240,7 @@ __device__ __forceinline__ void enter_groups(const float *A, float *U, const int
   }
 }
 // What the threads share between a tile's maps.
-constexpr int kWords = 16;   // tiles of a round trip
+constexpr int kWords = 64;   // tiles of a round trip
 struct TileSmem {
   float A[kMostValues], U[kMostValues];
   uint64_t words[kWords * kMostLanes * 4];
@@ -301,7 +301,14 @@ __device__ __forceinline__ void enter_tile(const ScanArgs &a, TileSmem &sm, floa
           }
         __syncthreads();
         if (on)
-          for (int i = 0; i < n; ++i) x = apply(sm.words[i * cw + c], x);
+          for (int i = 0; i < n; i += 8) {   // (eight reads on their way at once)
+            uint64_t w[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) w[e] = sm.words[min(i + e, n - 1) * cw + c];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (i + e < n) x = apply(w[e], x);
+          }
         __syncthreads();
       }
     }
