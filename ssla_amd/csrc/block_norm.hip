@@ -179,11 +179,11 @@ struct Place {
 };
 
 template <int DT, int W, int NV>
-__device__ __forceinline__ void load_row(Vec<DT, W> (&x)[NV], const void *p, int64_t at, const Place<W, NV> &l, bool on) {
+__device__ __forceinline__ void load_row(Held<DT, W> (&x)[NV], const void *p, int64_t at, const Place<W, NV> &l, bool on) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    x[i] = Vec<DT, W>{};
-    if (l.has[i] && on) x[i] = load_vec<DT, W>(p, at + l.c[i]);
+    x[i] = Held<DT, W>{};
+    if (l.has[i] && on) x[i] = load_held<DT, W>(p, at + l.c[i]);
   }
 }
 
@@ -224,7 +224,7 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void gated_fwd_kernel(co
   __shared__ float sm[64];
   int turn = 0;
   Place<W, NV> l(a);
-  Vec<DT, W> x[NV], z[NV], nx[NV], nz[NV];
+  Held<DT, W> x[NV], z[NV], nx[NV], nz[NV];
   load_row<DT, W, NV>(nx, a.x, l.row * a.ldx, l, l.row < a.N);
   load_row<DT, W, NV>(nz, a.z, l.row * a.ldz, l, l.row < a.N);
   for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(co
   for (int i = 0; i < NV; ++i)
 #pragma unroll
     for (int e = 0; e < W; ++e) sum[0][i][e] = sum[1][i][e] = 0.f;
-  Vec<DT, W> x[NV], z[NV], dy[NV], nx[NV], nz[NV], ndy[NV];
+  Held<DT, W> x[NV], z[NV], dy[NV], nx[NV], nz[NV], ndy[NV];
   auto fetch = [&](int64_t n, bool on) {
     load_row<DT, W, NV>(nx, a.x, n * a.ldx, l, on);
     load_row<DT, W, NV>(nz, a.z, n * a.ldz, l, on);
@@ -327,7 +327,7 @@ template <int DT, int DTR, int W, int NV, int WIDE>
 struct Stream {
   float s[NV][W], n2[NV][W], rstd2;
   uint32_t keep[NV];
-  __device__ __forceinline__ void run(const RowArgs &a, const Place<W, NV> &l, const Vec<DT, W> (&x)[NV], const Vec<DTR, W> (&r)[NV],
+  __device__ __forceinline__ void run(const RowArgs &a, const Place<W, NV> &l, const Held<DT, W> (&x)[NV], const Held<DTR, W> (&r)[NV],
                                       float scale, uint64_t seed, int64_t n, float *sm, int &turn) {
     each<W, NV>([&](int i, int e) { n2[i][e] = x[i][e]; });
     rstd2 = a.post ? normalise<WIDE, W, NV>(n2, l.ok, a, sm, turn) : 1.f;
@@ -351,8 +351,8 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void residual_fwd_kernel
   Place<W, NV> l(a);
   const float scale = a.alpha * (a.draw.threshold ? a.draw.scale : 1.f);
   const uint64_t seed = a.draw.threshold ? static_cast<uint64_t>(*a.draw.seed) : 0;
-  Vec<DT, W> x[NV], nx[NV];
-  Vec<DTR, W> r[NV], nr[NV];
+  Held<DT, W> x[NV], nx[NV];
+  Held<DTR, W> r[NV], nr[NV];
   load_row<DT, W, NV>(nx, a.x, l.row * a.C, l, l.row < a.N);
   load_row<DTR, W, NV>(nr, a.r, l.row * a.C, l, l.row < a.N);
   for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
@@ -403,8 +403,8 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
     for (int e = 0; e < W; ++e) sum[0][i][e] = sum[1][i][e] = sum[2][i][e] = sum[3][i][e] = 0.f;
   const float scale = a.alpha * (a.draw.threshold ? a.draw.scale : 1.f);
   const uint64_t seed = a.draw.threshold ? static_cast<uint64_t>(*a.draw.seed) : 0;
-  Vec<DT, W> x[NV], nx[NV], dy[NV], ndy[NV];
-  Vec<DTR, W> r[NV], nr[NV], ds[NV], nds[NV];
+  Held<DT, W> x[NV], nx[NV], dy[NV], ndy[NV];
+  Held<DTR, W> r[NV], nr[NV], ds[NV], nds[NV];
   auto fetch = [&](int64_t n, bool on) {
     load_row<DT, W, NV>(nx, a.x, n * a.C, l, on);
     load_row<DTR, W, NV>(nr, a.r, n * a.C, l, on);

@@ -24,4 +24,39 @@ __device__ __forceinline__ void store_vec(void *p, int64_t i, const Vec<DT, W> &
   reinterpret_cast<A *>(static_cast<typename Elem<DT>::T *>(p) + i)->v = x;
 }
 
+// The same to be held for a while: as the words they came in.  (16-bit values of a Vec
+// that are chosen or kept over a branch take a register each.)
+template <int DT, int W>
+struct Held {
+  static constexpr int kBytes = static_cast<int>(sizeof(typename Elem<DT>::T)) * W, kWords = (kBytes + 3) / 4;
+  uint32_t w[kWords];
+  __device__ __forceinline__ float operator[](int e) const {
+    if constexpr (DT == SSLA_F32) return __uint_as_float(w[e]);
+    else if constexpr (DT == SSLA_BF16) return __uint_as_float(e & 1 ? w[e >> 1] & 0xffff0000u : w[e >> 1] << 16);
+    else return f16_bits_to_f32(static_cast<uint16_t>(e & 1 ? w[e >> 1] >> 16 : w[e >> 1]));
+  }
+};
+template <int DT, int W>
+__device__ __forceinline__ Held<DT, W> load_held(const void *p, int64_t i) {
+  const typename Elem<DT>::T *at = static_cast<const typename Elem<DT>::T *>(p) + i;
+  Held<DT, W> h;
+  if constexpr (Held<DT, W>::kBytes < 4) {
+    h.w[0] = *at;
+  } else {
+    typedef uint32_t V __attribute__((ext_vector_type(Held<DT, W>::kWords > 4 ? 4 : Held<DT, W>::kWords)));
+    constexpr int n = Held<DT, W>::kWords > 4 ? 4 : Held<DT, W>::kWords;
+#pragma unroll
+    for (int k = 0; k < Held<DT, W>::kWords; k += n) {
+      if constexpr (n == 1) {
+        h.w[k] = *reinterpret_cast<const uint32_t *>(at);
+      } else {
+        const V v = *(reinterpret_cast<const V *>(at) + k / n);
+#pragma unroll
+        for (int e = 0; e < n; ++e) h.w[k + e] = v[e];
+      }
+    }
+  }
+  return h;
+}
+
 }  // namespace ssla
