@@ -245,6 +245,7 @@ struct TileSmem {
   float A[kMostValues], U[kMostValues];
   uint64_t words[kWords * kMostLanes * 4];
   int mark[kMostGroups * kMostRows], fin[kMostGroups * kMostRows], cut[kMostGroups];
+  int flags[kBlock];
   int from;
   uint32_t slot;
 };
@@ -353,6 +354,24 @@ __device__ __forceinline__ void each(F f) {
 #pragma unroll
     for (int e = 0; e < W; ++e) f(i, e);
 }
+// W values of a row of states (fp32, at any 4-byte border).
+template <int W>
+struct __attribute__((aligned(4))) States { float x[W]; };
+template <int W>
+__device__ __forceinline__ const States<W> &states_at(const float *p, int64_t i) {
+  return *reinterpret_cast<const States<W> *>(p + i);
+}
+// The rows n[0 .. B - 1] of p where they are rows and p is there: zeros otherwise.  All on
+// their way at once (a wait for each of many short sequences' is most of their time).
+template <int W, int B>
+__device__ __forceinline__ void load_states(States<W> (&s)[B], const float *p, const int (&n)[B], int C, int c) {
+#pragma unroll
+  for (int i = 0; i < B; ++i) {
+    s[i] = States<W>{};
+    if (p && n[i] >= 0) s[i] = states_at<W>(p, static_cast<int64_t>(n[i]) * C + c);
+  }
+}
+
 // f(KIND as a constant) of a call's kind of gate: decided once for all values held.
 template <typename F>
 __device__ __forceinline__ void by_kind(int kind, F f) {
@@ -361,19 +380,31 @@ __device__ __forceinline__ void by_kind(int kind, F f) {
   else f(std::integral_constant<int, kValue>());
 }
 
-// The states of empty sequences, dealt over the tiles: what enters leaves.
-__device__ __forceinline__ void empty_states(const ScanArgs &a, const float *from, float *to, int k, int cb, int cw) {
-  const int c = cb * cw + threadIdx.x;
-  for (int64_t n = k; n < a.n_seq; n += a.tiles) {
-    const Span s = span_of(a, static_cast<int>(n));
-    if (s.e == s.b && static_cast<int>(threadIdx.x) < cw && c < a.C) to[n * a.C + c] = from ? from[n * a.C + c] : 0.f;
+// The states of empty sequences, dealt over the tiles in blocks: what enters leaves.  For
+// the whole workgroup, flags: kBlock integers of its own.
+__device__ __forceinline__ void empty_states(const ScanArgs &a, const float *from, float *to, int k, int cb, int cw, int *flags) {
+  const int tid = threadIdx.x, c = cb * cw + tid, per = (a.n_seq + a.tiles - 1) / a.tiles;
+  const int last = static_cast<int>(min(static_cast<int64_t>(k + 1) * per, static_cast<int64_t>(a.n_seq)));
+  for (int64_t n0 = static_cast<int64_t>(k) * per; n0 < last; n0 += kBlock) {
+    const int64_t n = n0 + tid;
+    bool none = false;
+    if (n < last) {
+      const Span s = span_of(a, static_cast<int>(n));
+      none = s.e == s.b;
+    }
+    if (!__syncthreads_or(none)) continue;
+    flags[tid] = none;
+    __syncthreads();
+    for (int i = 0; i < kBlock && n0 + i < last; ++i)
+      if (flags[i] && tid < cw && c < a.C) to[(n0 + i) * a.C + c] = from ? from[(n0 + i) * a.C + c] : 0.f;
+    __syncthreads();
   }
 }
 
 // ------------------------------------------------------------------ forward --
 template <int DT, int DTG, int W, bool READ>
-__global__ __launch_bounds__(kBlock) void scan_fwd_kernel(const ScanArgs a) {
-  constexpr int R = kFwdRows;
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(DT == SSLA_F32 ? 2 : 4))) void scan_fwd_kernel(const ScanArgs a) {
+  constexpr int R = kFwdRows, B = 4;   // B: rows whose states are read at once
   __shared__ TileSmem sm;
   const int tid = threadIdx.x, cw = a.CT * W, rows = a.RG * R;
   const int rg = tid / a.CT, cl = tid - rg * a.CT;
@@ -382,7 +413,7 @@ __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(const ScanArgs a) {
   const int id = take_tile(a, &sm.slot);
   const int k = id / a.cblocks, cb = id - k * a.cblocks;
   if (a.T == 0) {   // (one tile without rows)
-    if (a.ht) empty_states(a, a.h0, a.ht, k, cb, cw);
+    if (a.ht) empty_states(a, a.h0, a.ht, k, cb, cw, sm.flags);
     return;
   }
   const int64_t r0 = static_cast<int64_t>(k) * rows;
@@ -397,7 +428,6 @@ __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(const ScanArgs a) {
   if constexpr (READ) load_rows<DT, W, R>(q, a.q, r0, a.ldq, row, exist - 1, c);
   const bool some = mark_rows(a, mine, all, r0, rows, sm.mark, sm.fin);
   float f[R][W];
-  auto state0 = [&](int m, int e) { return a.h0 ? a.h0[static_cast<int64_t>(m) * a.C + c + e] : 0.f; };
   by_kind(a.gate, [&](auto kind) { each<R, W>([&](int i, int e) { f[i][e] = gate_value<kind()>(g[i][e]); }); });
   if (on) {
     float A[W], U[W];
@@ -414,13 +444,20 @@ __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(const ScanArgs a) {
       });
     } else {
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const int m = sm.mark[row + i];
-        reset |= m != kInside;
+      for (int i0 = 0; i0 < R; i0 += B) {
+        int m[B];
+        States<W> s0[B];
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          U[e] = m == kOutside ? 0.f : fmaf(f[i][e], m >= 0 ? state0(m, e) : U[e], u[i][e]);
-          A[e] *= f[i][e];
+        for (int i = 0; i < B; ++i) m[i] = sm.mark[row + i0 + i];
+        load_states(s0, a.h0, m, a.C, c);
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          reset |= m[i] != kInside;
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            U[e] = m[i] == kOutside ? 0.f : fmaf(f[i0 + i][e], m[i] >= 0 ? s0[i].x[e] : U[e], u[i0 + i][e]);
+            A[e] *= f[i0 + i][e];
+          }
         }
       }
     }
@@ -458,26 +495,40 @@ __global__ __launch_bounds__(kBlock) void scan_fwd_kernel(const ScanArgs a) {
       }
     } else {
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        const int m = sm.mark[row + i], n = sm.fin[row + i];
-        Vec<DT, W> o;
+      for (int i0 = 0; i0 < R; i0 += B) {
+        int m[B];
+        States<W> s0[B];
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          h[e] = fmaf(f[i][e], m >= 0 ? state0(m, e) : h[e], u[i][e]);
-          o.set(e, m == kOutside ? 0.f : READ ? h[e] * q[READ ? i : 0][e] : h[e]);
-          if (a.ht && n >= 0) a.ht[static_cast<int64_t>(n) * a.C + c + e] = h[e];
+        for (int i = 0; i < B; ++i) m[i] = sm.mark[row + i0 + i];
+        load_states(s0, a.h0, m, a.C, c);
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          const int n = sm.fin[row + i0 + i];
+          Vec<DT, W> o;
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            h[e] = fmaf(f[i0 + i][e], m[i] >= 0 ? s0[i].x[e] : h[e], u[i0 + i][e]);
+            o.set(e, m[i] == kOutside ? 0.f : READ ? h[e] * q[READ ? i0 + i : 0][e] : h[e]);
+          }
+          if (a.ht && n >= 0) {
+            States<W> out_state;
+#pragma unroll
+            for (int e = 0; e < W; ++e) out_state.x[e] = h[e];
+            *reinterpret_cast<States<W> *>(a.ht + static_cast<int64_t>(n) * a.C + c) = out_state;
+          }
+          if (i0 + i < left) store_vec<DT, W>(out, at + static_cast<uint32_t>(i0 + i) * a.C, o);
         }
-        if (i < left) store_vec<DT, W>(out, at + static_cast<uint32_t>(i) * a.C, o);
       }
     }
   }
-  if (a.ht) empty_states(a, a.h0, a.ht, k, cb, cw);
+  if (a.ht) empty_states(a, a.h0, a.ht, k, cb, cw, sm.flags);
 }
 
 // ----------------------------------------------------------------- backward --
 template <int DT, int DTG, int W, bool READ>
-__global__ __launch_bounds__(kBlock) void scan_bwd_kernel(const ScanArgs a) {
+__global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) void scan_bwd_kernel(const ScanArgs a) {
   constexpr int R = kBwdRows;
+  static_assert(R == 4, "rows whose states are read at once");
   __shared__ TileSmem sm;
   __shared__ float sE[kMostValues];
   const int tid = threadIdx.x, cw = a.CT * W, rows = a.RG * R;
@@ -487,7 +538,7 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(const ScanArgs a) {
   const int id = take_tile(a, &sm.slot);
   const int back = id / a.cblocks, k = a.tiles - 1 - back, cb = id - back * a.cblocks;
   if (a.T == 0) {
-    if (a.dh0) empty_states(a, a.dht, a.dh0, k, cb, cw);
+    if (a.dh0) empty_states(a, a.dht, a.dh0, k, cb, cw, sm.flags);
     return;
   }
   const int64_t r0 = static_cast<int64_t>(k) * rows;
@@ -505,8 +556,6 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(const ScanArgs a) {
   const float entering = tid < cw && cb * cw + tid < a.C ? a.keep[r0 / kKeepRows * a.C + cb * cw + tid] : 0.f;
   const bool some = mark_rows(a, mine, all, r0, rows, sm.mark, sm.fin);
   Gate f[R][W];
-  auto state0 = [&](int m, int e) { return a.h0 ? a.h0[static_cast<int64_t>(m) * a.C + c + e] : 0.f; };
-  auto grad0 = [&](int n, int e) { return a.dht ? a.dht[static_cast<int64_t>(n) * a.C + c + e] : 0.f; };
   auto grad_of = [&](int i, int e) { return READ ? d[i][e] * q[READ ? i : 0][e] : d[i][e]; };
   by_kind(a.gate, [&](auto kind) { each<R, W>([&](int i, int e) { f[i][e] = gate_of<kind()>(g[i][e]); }); });
   if (on) {
@@ -524,23 +573,30 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(const ScanArgs a) {
       });
       each<R, W>([&](int i, int e) { E[e] = f[R - 1 - i][e].a * (grad_of(R - 1 - i, e) + E[e]); });
     } else {
+      int m[R], n[R];
+      States<W> s0[R];   // (states, then gradients of final ones)
 #pragma unroll
       for (int i = 0; i < R; ++i) {
-        const int m = sm.mark[row + i];
-        reset |= m != kInside || sm.fin[row + i] >= 0;   // (nothing goes past a beginning or an end)
+        m[i] = sm.mark[row + i];
+        n[i] = sm.fin[row + i];
+      }
+      load_states(s0, a.h0, m, a.C, c);
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        reset |= m[i] != kInside || n[i] >= 0;   // (nothing goes past a beginning or an end)
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          U[e] = m == kOutside ? 0.f : fmaf(f[i][e].a, m >= 0 ? state0(m, e) : U[e], u[i][e]);
+          U[e] = m[i] == kOutside ? 0.f : fmaf(f[i][e].a, m[i] >= 0 ? s0[i].x[e] : U[e], u[i][e]);
           A[e] *= f[i][e].a;
         }
       }
+      load_states(s0, a.dht, n, a.C, c);
 #pragma unroll
       for (int i = R - 1; i >= 0; --i) {
-        const int m = sm.mark[row + i], n = sm.fin[row + i];
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          const float x = n >= 0 ? grad0(n, e) : E[e];
-          E[e] = m == kInside ? f[i][e].a * (grad_of(i, e) + x) : 0.f;
+          const float x = n[i] >= 0 ? s0[i].x[e] : E[e];
+          E[e] = m[i] == kInside ? f[i][e].a * (grad_of(i, e) + x) : 0.f;
         }
       }
     }
@@ -571,40 +627,51 @@ __global__ __launch_bounds__(kBlock) void scan_bwd_kernel(const ScanArgs a) {
     const uint32_t at = row * a.C + c;
     typedef typename Elem<DT>::T TU;
     typedef typename Elem<DTG>::T TG;
+    int mark[R], fin[R];
+    States<W> s0[R];   // (states, then gradients of final ones)
 #pragma unroll
     for (int i = 0; i < R; ++i) {
-      const int m = some ? sm.mark[row + i] : kInside;
+      mark[i] = some ? sm.mark[row + i] : kInside;
+      fin[i] = some ? sm.fin[row + i] : -1;
+    }
+    if (some) load_states(s0, a.h0, mark, a.C, c);
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      const int m = mark[i];
       Vec<DT, W> dq;
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        if (m >= 0) h[e] = state0(m, e);
+        if (m >= 0) h[e] = s0[i].x[e];
         before[i][e] = h[e];
         h[e] = fmaf(f[i][e].a, h[e], u[i][e]);
         dq.set(e, m == kOutside ? 0.f : d[i][e] * h[e]);
       }
       if (READ && i < left) store_vec<DT, W>(static_cast<TU *>(a.dq) + first, at + static_cast<uint32_t>(i) * a.C, dq);
     }
+    if (some) load_states(s0, a.dht, fin, a.C, c);
 #pragma unroll
     for (int i = R - 1; i >= 0; --i) {
-      const int m = some ? sm.mark[row + i] : kInside, n = some ? sm.fin[row + i] : -1;
+      const int m = mark[i], n = fin[i];
       Vec<DT, W> du;
       Vec<DTG, W> dg;
+      States<W> first_grad;
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        if (n >= 0) x[e] = grad0(n, e);
+        if (n >= 0) x[e] = s0[i].x[e];
         const float s = grad_of(i, e) + x[e];
         du.set(e, m == kOutside ? 0.f : s);
         dg.set(e, m == kOutside ? 0.f : s * before[i][e] * f[i][e].slope);
         x[e] = f[i][e].a * s;
-        if (m >= 0 && a.dh0) a.dh0[static_cast<int64_t>(m) * a.C + c + e] = x[e];
+        first_grad.x[e] = x[e];
       }
+      if (m >= 0 && a.dh0) *reinterpret_cast<States<W> *>(a.dh0 + static_cast<int64_t>(m) * a.C + c) = first_grad;
       if (i < left) {
         store_vec<DT, W>(static_cast<TU *>(a.du) + first, at + static_cast<uint32_t>(i) * a.C, du);
         store_vec<DTG, W>(static_cast<TG *>(a.dg) + first, at + static_cast<uint32_t>(i) * a.C, dg);
       }
     }
   }
-  if (a.dh0) empty_states(a, a.dht, a.dh0, k, cb, cw);
+  if (a.dh0) empty_states(a, a.dht, a.dh0, k, cb, cw, sm.flags);
 }
 
 // --------------------------------------------------------- single tokens --
