@@ -666,6 +666,7 @@ extern "C" int ssla_gated_norm_bwd(const void *dy, const void *x, int64_t ldx, c
                  "gated_norm_bwd: bad activation %d or row strides %lld, %lld", act, (long long)ldx, (long long)ldz);
   SSLA_CHECK_ARG(N == 0 || (dy && x && z), "gated_norm_bwd: null pointer");
   const bool sums = dweight || dbias;
+  if (N == 0 && !sums) return SSLA_OK;
   if (const int e = check_ws("gated_norm_bwd", workspace, workspace_bytes,
                              sums ? ssla_gated_norm_bwd_workspace_size(N, C, G) : 0)) return e;
   const hipStream_t st = static_cast<hipStream_t>(stream);
@@ -727,6 +728,7 @@ extern "C" int ssla_residual_norm_bwd(const void *dy, const void *dsum, const vo
   SSLA_CHECK_ARG(post || (!post_weight && !dpost_weight), "residual_norm_bwd: a weight of a norm that is not asked for");
   SSLA_CHECK_ARG(N == 0 || ((dy || dsum) && x && residual), "residual_norm_bwd: null pointer");
   const bool sums = dweight || dbias || dgamma || dpost_weight;
+  if (N == 0 && !sums) return SSLA_OK;
   if (const int e = check_ws("residual_norm_bwd", workspace, workspace_bytes,
                              sums ? ssla_residual_norm_bwd_workspace_size(N, C) : 0)) return e;
   const hipStream_t st = static_cast<hipStream_t>(stream);

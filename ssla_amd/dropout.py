@@ -12,6 +12,7 @@ CPU fallback.
 """
 from __future__ import annotations
 
+import numbers
 from typing import Union
 
 import torch
@@ -22,8 +23,8 @@ __all__ = ["counter_dropout", "CounterDropoutFunction"]
 
 
 def _seed(name, seed, subsequence, device):
-    """The seed as one int64 on `device`."""
-    if not isinstance(subsequence, int) or not 0 <= subsequence < 1 << 32:
+    """The seed as one int64 on `device` (a number's by a fill, which a graph may hold)."""
+    if not isinstance(subsequence, numbers.Integral) or not 0 <= subsequence < 1 << 32:
         raise ValueError(f"{name}: subsequence must be an integer in [0, 2^32), got {subsequence!r}")
     if torch.is_tensor(seed):
         if seed.dtype != torch.int64 or seed.numel() != 1:
@@ -31,13 +32,13 @@ def _seed(name, seed, subsequence, device):
         if seed.device != device:
             raise ValueError(f"{name}: seed must lie on {device}, got {seed.device}")
         return seed
-    if not isinstance(seed, int) or not -(1 << 63) <= seed < 1 << 63:
+    if not isinstance(seed, numbers.Integral) or not -(1 << 63) <= seed < 1 << 63:
         raise ValueError(f"{name}: seed must be a 64-bit integer or a tensor of one, got {seed!r}")
-    return torch.full((1,), seed, dtype=torch.int64, device=device)
+    return torch.full((1,), int(seed), dtype=torch.int64, device=device)
 
 
 def _p(name, p):
-    if not isinstance(p, (int, float)) or not 0 <= p <= 1:
+    if not isinstance(p, numbers.Real) or not 0 <= p <= 1:
         raise ValueError(f"{name}: p must lie in [0, 1], got {p!r}")
     return float(p)
 

@@ -31,6 +31,7 @@ __all__ = ["scan", "SequentialScan", "gated_scan", "GatedScanFunction", "GATES",
            "sparse_gla_scan"]
 
 GATES = {"value": 0, "log": 1, "sigmoid": 2}
+_WIDEST = 1 << 20   # elements from row to row: offsets inside a tile of rows are 32 bits
 
 
 def _scan_fwd(u: torch.Tensor, g: torch.Tensor, cu: torch.Tensor) -> torch.Tensor:
@@ -89,8 +90,8 @@ def _gated_args(name, u, g, q, gate):
     if u.dim() != 2 or g.shape != u.shape or (q is not None and q.shape != u.shape) or u.shape[1] == 0:
         raise ValueError(f"{name}: u, g and q must all be [T, C], got {tuple(u.shape)}, {tuple(g.shape)}, "
                          f"{None if q is None else tuple(q.shape)}")
-    if u.shape[1] > 1 << 30:
-        raise NotImplementedError(f"{name}: at most 2^30 channels, got {u.shape[1]}")
+    if u.shape[1] > _WIDEST:
+        raise NotImplementedError(f"{name}: at most {_WIDEST} channels, got {u.shape[1]}")
     if gate not in GATES:
         raise ValueError(f"{name}: gate must be one of {list(GATES)}, got {gate!r}")
     if u.dtype not in _lib.DTYPE_CODE or (q is not None and q.dtype != u.dtype):
@@ -102,7 +103,7 @@ def _gated_args(name, u, g, q, gate):
 def _rows(t):
     """t with neighbouring channels side by side (the rows may lie apart, as those
     of a slice of a wider projection do)."""
-    return t if t is None or t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+    return t if t is None or t.stride(1) == 1 and t.shape[1] <= t.stride(0) <= _WIDEST else t.contiguous()
 
 
 def _gated_forward(u, g, q, cu, gate, h0, output_final_state, save=False):
@@ -191,6 +192,8 @@ def gated_scan(
     dev = _lib.require_cuda(u, g, q, initial_state)
     cu = _offsets(name, cu_seqlens, dev)
     N, C = cu.numel() - 1, u.shape[1]
+    if N > 0x7fffffff:
+        raise NotImplementedError(f"{name}: too many sequences ({N})")
     if initial_state is not None and (initial_state.shape != (N, C) or not initial_state.is_floating_point()):
         raise ValueError(f"{name}: initial_state must be floating point {(N, C)}, got {tuple(initial_state.shape)} "
                          f"{initial_state.dtype}")
@@ -216,6 +219,8 @@ def sparse_gated_step(site_idx: torch.Tensor, u: torch.Tensor, g: torch.Tensor, 
     name = "sparse_gated_step"
     _gated_args(name, u, g, q, gate)
     n, C = u.shape
+    if n > 0x7fffffff:
+        raise NotImplementedError(f"{name}: too many rows ({n})")
     if state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"{name}: state must be contiguous fp32 [n_sites, {C}]")
     _lib.require_no_tangent(name, u, g, q, state)

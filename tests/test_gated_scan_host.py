@@ -31,6 +31,16 @@ def test_scan_entries_refuse():
     for f in (fwd, bwd):
         assert f(cu=None) == _lib.SSLA_ERR_ARG
         assert f(T=1 << 34, C=1 << 10, ld=1 << 10) == _lib.SSLA_ERR_UNSUPPORTED
+        assert f(ld=(1 << 20) + 1) == _lib.SSLA_ERR_UNSUPPORTED      # (offsets in a tile of rows are 32 bits)
+        assert f(C=(1 << 20) + 1, ld=1 << 21) == _lib.SSLA_ERR_UNSUPPORTED
+    size = lib.ssla_gated_scan_workspace_size(100000, 64)
+    for f in (lib.ssla_gated_scan_fwd, lib.ssla_gated_scan_bwd):      # a long sequence needs its workspace (checked before any launch)
+        for ws, n in ((None, size), (16, 1000), (8, size)):
+            if f is lib.ssla_gated_scan_fwd:
+                st = f(16, 64, 16, 64, None, 0, 16, 1, 100000, 64, 0, None, 16, None, None, 0, 0, ws, n, None)
+            else:
+                st = f(16, 64, 16, 64, None, 0, 16, 1, 100000, 64, 0, None, 16, 16, None, 16, 16, None, None, 0, 0, ws, n, None)
+            assert st == _lib.SSLA_ERR_WORKSPACE, (ws, n)
     assert step(T=0) == _lib.SSLA_OK
     assert lib.ssla_sparse_gated_step(8, 1, None, 8, None, 8, None, 0, None, -1, 8, 0, None, None, 0, 0, None) == _lib.SSLA_ERR_ARG
     for size in (lib.ssla_gated_scan_workspace_size, lib.ssla_gated_scan_keep_size):
@@ -58,7 +68,7 @@ def test_functions_refuse(form):
     for u, g, q in ((x.double(), x, None), (x, x.int(), None), (x, x, x.half())):
         with pytest.raises(TypeError):
             f(u, g, q=q)
-    wide = torch.zeros(1, 1).expand(4, (1 << 30) + 1)
+    wide = torch.zeros(1, 1).expand(4, (1 << 20) + 1)
     with pytest.raises(NotImplementedError, match="channels"):
         f(wide, wide)
     for i in range(3):

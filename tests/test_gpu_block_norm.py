@@ -178,7 +178,7 @@ def check_residual(dev, case, kind, post, scale, affine, p, seed=77, sub=3, grad
     c = (alpha or 1.0) * big(gamma) * (block.dropout_scale(p) if p else 1.0)
     w2m = big(w2)
     branch, branch_off = c * n2 * w2m, c * w2m * (off2 + 5 * U * n2)
-    s = float(ref[1].abs().max())
+    s = float(ref[1].detach().abs().max())
     s_off = branch_off + U * (s + branch)
     near("sum", out[1].detach(), ref[1].detach(), s_off, r.dtype)
     off, n, rstd = norm_sizes(ref[1].detach(), 1, kind)

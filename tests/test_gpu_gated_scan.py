@@ -364,3 +364,81 @@ def test_step_skips_bad_entries(dev):
             sparse_gated_step(idx.to(dev), x["u"], x["g"], table.clone(), check=True)
     e = torch.zeros(0, C, device=dev)
     assert sparse_gated_step(torch.zeros(0, dtype=torch.int32, device=dev), e, e, table).shape == (0, C)
+
+
+def test_past_32_bits(dev):
+    """2^31 values a tensor: the last rows are those of a short call on the end alone
+    (gates of about a half forget 200 rows to nothing), in both directions."""
+    from ssla_amd.scan import gated_scan
+    T, C = (1 << 21) + 1000, 1024
+    gen = torch.Generator(device=dev).manual_seed(0)
+    u, g, do = (torch.randn(T, C, generator=gen, device=dev, dtype=B16) for _ in range(3))
+    u.requires_grad_(), g.requires_grad_()
+    o, ht = gated_scan(u, g, torch.tensor([0, T], device=dev), gate="sigmoid", output_final_state=True)
+    du, dg = torch.autograd.grad(o, (u, g), do)
+    for rows in (slice(T - 2000, T), slice(0, 2000)):
+        a, b = (t.detach()[rows].clone().requires_grad_() for t in (u, g))
+        p, pt = gated_scan(a, b, torch.tensor([0, 2000], device=dev), gate="sigmoid", output_final_state=True)
+        da, db = torch.autograd.grad(p, (a, b), do[rows])
+        mid = slice(1000, 1500)   # (1,000 rows from one end, 500 from the other)
+        for whole, part in ((o, p), (du, da), (dg, db)):
+            w, q = whole[rows][mid].detach().double(), part[mid].detach().double()
+            assert bool(((w - q).abs() <= 2.0 ** -7 * q.abs() + 1e-4).all())   # (one rounding either side of a border)
+        if rows.start:
+            assert torch.allclose(ht, pt, rtol=0, atol=64 * EPS)
+
+
+def test_offsets_that_decrease_end(dev):
+    """Offsets that are not in order leave their rows unspecified; the call ends, and a good
+    one after it is right."""
+    from ssla_amd.scan import gated_scan
+    x = {n: t.to(dev) for n, t in inputs([900], 40, F32, F32, "sigmoid", seed=1).items()}
+    good = torch.tensor([0, 900], device=dev)
+    want = gated_scan(x["u"], x["g"], good, gate="sigmoid")[0]
+    for cu in ([0, 500, 200, 900], [900, 0, 900], [-5, 2000, 3], [700, 700, 100]):
+        u = x["u"].clone().requires_grad_()
+        n = len(cu) - 1
+        o, ht = gated_scan(u, x["g"], torch.tensor(cu, device=dev), gate="sigmoid",
+                           initial_state=torch.zeros(n, 40, device=dev), output_final_state=True)
+        torch.autograd.grad((o, ht), u, (torch.ones_like(o), torch.ones_like(ht)))
+        torch.cuda.synchronize()
+        assert torch.equal(gated_scan(x["u"], x["g"], good, gate="sigmoid")[0], want)
+
+
+def test_two_graphs_of_one_pool(dev):
+    """Two captured calls whose workspaces may share memory, replayed in turn."""
+    from ssla_amd.scan import gated_scan
+    sets = [{n: t.to(dev) for n, t in inputs([6000, 50], C, B16, B16, "sigmoid", seed=C).items()} for C in (64, 136)]
+    cu = offsets([6000, 50]).to(dev)
+
+    def call(x):
+        return gated_scan(x["u"], x["g"], cu, q=x["q"], gate="sigmoid", initial_state=x["h0"], output_final_state=True)
+
+    want = [call(x) for x in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        [call(x) for x in sets]
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs, pool = [], [], None
+    for x in sets:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, pool=pool):
+            outs.append(call(x))
+        pool = graph.pool()
+        graphs.append(graph)
+    for i in range(4):
+        for graph, out, w in zip(graphs, outs, want):
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, w)), i
+
+
+def test_many_sequences(dev):
+    """More sequences than a workgroup has threads, of one row and of none."""
+    gen = torch.Generator().manual_seed(0)
+    lens = torch.randint(0, 3, (3000,), generator=gen).tolist()
+    check(dev, lens, inputs(lens, 12, F32, F32, "sigmoid", seed=0), "sigmoid")
+    check(dev, [1] * 1500, inputs([1] * 1500, 8, B16, F32, "log", seed=1), "log")
+    lens = [0] * 2000 + [700] + [0] * 2000
+    check(dev, lens, inputs(lens, 8, F32, F32, "value", seed=2), "value")
