@@ -97,64 +97,16 @@ __device__ __forceinline__ void each(F f) {
     for (int e = 0; e < W; ++e) f(i, e);
 }
 
-// x becomes its normalised values; returns 1 / deviation.
-template <int WIDE, int W, int NV>
-__device__ __forceinline__ float normalise(float (&x)[NV][W], const bool (&ok)[NV], const RowArgs &a, float *sm, int &turn) {
-  const float inv = 1.f / static_cast<float>(a.per);
-  if (a.layer) {
-    float t[1] = {0.f};
-    each<W, NV>([&](int i, int e) { t[0] += x[i][e]; });
-    row_sums<WIDE>(t, a.S, sm, turn);
-    const float mean = t[0] * inv;
-    each<W, NV>([&](int i, int e) { x[i][e] = ok[i] ? x[i][e] - mean : 0.f; });
-  }
-  float t[1] = {0.f};
-  each<W, NV>([&](int i, int e) { t[0] = fmaf(x[i][e], x[i][e], t[0]); });
-  row_sums<WIDE>(t, a.S, sm, turn);
-  const float rstd = 1.f / sqrtf(t[0] * inv + a.eps);
-  each<W, NV>([&](int i, int e) { x[i][e] *= rstd; });
-  return rstd;
-}
-// h, the gradient of normalised values n, becomes that of what they were made of.
-template <int WIDE, int W, int NV>
-__device__ __forceinline__ void normalise_back(float (&h)[NV][W], const float (&n)[NV][W], float rstd, const bool (&ok)[NV],
-                                               const RowArgs &a, float *sm, int &turn) {
-  const float inv = 1.f / static_cast<float>(a.per);
-  float t[2] = {0.f, 0.f};
-  each<W, NV>([&](int i, int e) {
-    t[0] += h[i][e];
-    t[1] = fmaf(h[i][e], n[i][e], t[1]);
-  });
-  row_sums<WIDE>(t, a.S, sm, turn);
-  const float m = a.layer ? t[0] * inv : 0.f, v = t[1] * inv;
-  each<W, NV>([&](int i, int e) { h[i][e] = ok[i] ? rstd * (h[i][e] - m - n[i][e] * v) : 0.f; });
-}
-
-// W values of a vector over the channels, or of its default.
-template <int W>
-__device__ __forceinline__ void load_weights(const float *p, int c, float other, float (&x)[W]) {
-#pragma unroll
-  for (int e = 0; e < W; ++e) x[e] = other;
-  if (!p) return;
-  if constexpr (W >= 4) {
-#pragma unroll
-    for (int e = 0; e < W; e += 4) {
-      const f32x4 v = *reinterpret_cast<const f32x4 *>(p + c + e);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[e + i] = v[i];
-    }
-  } else {
-    x[0] = p[c];
-  }
-}
-
 // Where a lane works: its place j among the S lanes of a row, the group of channels g
-// and the first row; lane groups that have none (`on` false) idle along.
-template <int W, int NV>
+// and the first row; lane groups that have none (`on` false) idle along.  A lane's values
+// are NV vectors of W neighbouring channels.  FULL: whole ones at their borders, else as
+// many of them as the group has channels, read one by one.
+template <int W, int NV, bool FULL>
 struct Place {
   int j, g, c[NV];
-  int64_t row, first;   // its first row, and the workgroup's
-  bool on, col[NV], has[NV], ok[NV];   // the vector's channels exist; with a row at all; with the row worked on
+  int64_t row, first;               // its first row, and the workgroup's
+  bool on;
+  int cols[NV], has[NV], now[NV];   // values that exist; with a row at all; with the row worked on
   __device__ __forceinline__ explicit Place(const RowArgs &a) {
     const int64_t sub = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / a.S;
     j = threadIdx.x & (a.S - 1);
@@ -165,32 +117,107 @@ struct Place {
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       c[i] = (j + a.S * i) * W;
-      col[i] = c[i] < a.per;
-      has[i] = on && col[i];
-      ok[i] = has[i] && row < a.N;
-      c[i] = (col[i] ? c[i] : 0) + g * a.per;
+      cols[i] = min(max(a.per - c[i], 0), W);
+      has[i] = on ? cols[i] : 0;
+      now[i] = row < a.N ? has[i] : 0;
+      c[i] = (cols[i] ? c[i] : 0) + g * a.per;
     }
   }
   // Row n is the one worked on: lanes behind the last row idle along.
   __device__ __forceinline__ void at(int64_t n, int64_t N) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) ok[i] = has[i] && n < N;
+    for (int i = 0; i < NV; ++i) now[i] = n < N ? has[i] : 0;
   }
+  __device__ __forceinline__ bool is(int i, int e) const { return FULL ? now[i] != 0 : e < now[i]; }
 };
 
-template <int DT, int W, int NV>
-__device__ __forceinline__ void load_row(Held<DT, W> (&x)[NV], const void *p, int64_t at, const Place<W, NV> &l, bool on) {
+// W values of a vector over the channels, or of its default.
+template <int W, int NV, bool FULL>
+__device__ __forceinline__ void load_weights(const float *p, const Place<W, NV, FULL> &l, int i, float other, float (&x)[W]) {
+#pragma unroll
+  for (int e = 0; e < W; ++e) x[e] = other;
+  if (!p) return;
+  if constexpr (FULL) {
+#pragma unroll
+    for (int e = 0; e < W; e += 4) {
+      const f32x4 v = *reinterpret_cast<const f32x4 *>(p + l.c[i] + e);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[e + k] = v[k];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      if (e < l.cols[i]) x[e] = p[l.c[i] + e];
+  }
+}
+
+// A row's values, zeros where there are none.
+template <int DT, int W, int NV, bool FULL>
+__device__ __forceinline__ void load_row(Held<DT, W> (&x)[NV], const void *p, int64_t at, const Place<W, NV, FULL> &l, bool on) {
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     x[i] = Held<DT, W>{};
-    if (l.has[i] && on) x[i] = load_held<DT, W>(p, at + l.c[i]);
+    if constexpr (FULL) {
+      if (l.has[i] && on) x[i] = load_held<DT, W>(p, at + l.c[i]);
+    } else if (on) {
+      const typename Elem<DT>::T *from = static_cast<const typename Elem<DT>::T *>(p) + at + l.c[i];
+#pragma unroll
+      for (int e = 0; e < W; ++e)
+        if (e < l.has[i]) {
+          if constexpr (DT == SSLA_F32) x[i].w[e] = __float_as_uint(from[e]);
+          else x[i].w[e >> 1] |= static_cast<uint32_t>(from[e]) << (e & 1 ? 16 : 0);
+        }
+    }
   }
+}
+template <int DT, int W, int NV, bool FULL>
+__device__ __forceinline__ void store_row(void *p, int64_t at, const Place<W, NV, FULL> &l, int i, const Vec<DT, W> &x) {
+  if constexpr (FULL) {
+    if (l.now[i]) store_vec<DT, W>(p, at + l.c[i], x);
+  } else {
+#pragma unroll
+    for (int e = 0; e < W; ++e)
+      if (e < l.now[i]) static_cast<typename Elem<DT>::T *>(p)[at + l.c[i] + e] = x.e[e];
+  }
+}
+
+// x becomes its normalised values; returns 1 / deviation.
+template <int WIDE, bool FULL, int W, int NV>
+__device__ __forceinline__ float normalise(float (&x)[NV][W], const Place<W, NV, FULL> &l, const RowArgs &a, float *sm, int &turn) {
+  const float inv = 1.f / static_cast<float>(a.per);
+  if (a.layer) {
+    float t[1] = {0.f};
+    each<W, NV>([&](int i, int e) { t[0] += x[i][e]; });
+    row_sums<WIDE>(t, a.S, sm, turn);
+    const float mean = t[0] * inv;
+    each<W, NV>([&](int i, int e) { x[i][e] = l.is(i, e) ? x[i][e] - mean : 0.f; });
+  }
+  float t[1] = {0.f};
+  each<W, NV>([&](int i, int e) { t[0] = fmaf(x[i][e], x[i][e], t[0]); });
+  row_sums<WIDE>(t, a.S, sm, turn);
+  const float rstd = 1.f / sqrtf(t[0] * inv + a.eps);
+  each<W, NV>([&](int i, int e) { x[i][e] *= rstd; });
+  return rstd;
+}
+// h, the gradient of normalised values n, becomes that of what they were made of.
+template <int WIDE, bool FULL, int W, int NV>
+__device__ __forceinline__ void normalise_back(float (&h)[NV][W], const float (&n)[NV][W], float rstd,
+                                               const Place<W, NV, FULL> &l, const RowArgs &a, float *sm, int &turn) {
+  const float inv = 1.f / static_cast<float>(a.per);
+  float t[2] = {0.f, 0.f};
+  each<W, NV>([&](int i, int e) {
+    t[0] += h[i][e];
+    t[1] = fmaf(h[i][e], n[i][e], t[1]);
+  });
+  row_sums<WIDE>(t, a.S, sm, turn);
+  const float m = a.layer ? t[0] * inv : 0.f, v = t[1] * inv;
+  each<W, NV>([&](int i, int e) { h[i][e] = l.is(i, e) ? rstd * (h[i][e] - m - n[i][e] * v) : 0.f; });
 }
 
 // Adds the workgroup's sums over rows and leaves them in rows of a.part ([rows][KINDS][C]):
 // a row a workgroup, or a row a slot where a workgroup has not all groups of channels.
-template <int W, int NV, int KINDS>
-__device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV> &l, const float (&sum)[KINDS][NV][W], float *sm) {
+template <int W, int NV, bool FULL, int KINDS>
+__device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV, FULL> &l, const float (&sum)[KINDS][NV][W], float *sm) {
   const int lanes = blockDim.x, groups = lanes / a.S, mine = threadIdx.x / a.S;   // lane groups
   const bool all = a.G <= groups;
   const int64_t to = all ? static_cast<int64_t>(blockIdx.x) : l.row;
@@ -206,9 +233,9 @@ __device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV> 
     if (mine < a.G && (all || l.on))
 #pragma unroll
       for (int i = 0; i < NV; ++i)
-        if (l.col[i])
 #pragma unroll
-          for (int e = 0; e < W; ++e) {
+        for (int e = 0; e < W; ++e)
+          if (e < l.cols[i]) {
             float t = 0.f;
             for (int q = mine; q < groups; q += a.G) t += sm[(e * NV + i) * lanes + q * a.S + l.j];
             a.part[(to * KINDS + k) * a.C + l.c[i] + e] = t;
@@ -219,14 +246,14 @@ __device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV> 
 __device__ __forceinline__ float sigmoid_of(float z) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z)); }
 
 // -------------------------------------------------------------------- gated --
-template <int DT, int W, int NV, int WIDE>
+template <int DT, int W, int NV, bool FULL, int WIDE>
 __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void gated_fwd_kernel(const RowArgs a) {
   __shared__ float sm[64];
   int turn = 0;
-  Place<W, NV> l(a);
+  Place<W, NV, FULL> l(a);
   Held<DT, W> x[NV], z[NV], nx[NV], nz[NV];
-  load_row<DT, W, NV>(nx, a.x, l.row * a.ldx, l, l.row < a.N);
-  load_row<DT, W, NV>(nz, a.z, l.row * a.ldz, l, l.row < a.N);
+  load_row<DT, W, NV, FULL>(nx, a.x, l.row * a.ldx, l, l.row < a.N);
+  load_row<DT, W, NV, FULL>(nz, a.z, l.row * a.ldz, l, l.row < a.N);
   for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
     l.at(n, a.N);
 #pragma unroll
@@ -235,34 +262,33 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void gated_fwd_kernel(co
       z[i] = nz[i];
     }
     if (n + a.slots < a.N) {
-      load_row<DT, W, NV>(nx, a.x, (n + a.slots) * a.ldx, l, true);
-      load_row<DT, W, NV>(nz, a.z, (n + a.slots) * a.ldz, l, true);
+      load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.ldx, l, true);
+      load_row<DT, W, NV, FULL>(nz, a.z, (n + a.slots) * a.ldz, l, true);
     }
     float v[NV][W];
     each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
-    normalise<WIDE, W, NV>(v, l.ok, a, sm, turn);
+    normalise<WIDE, FULL, W, NV>(v, l, a, sm, turn);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (l.ok[i]) {
+    for (int i = 0; i < NV; ++i) {
         float w[W], b[W];
-        load_weights<W>(a.w, l.c[i], 1.f, w);
-        load_weights<W>(a.b, l.c[i], 0.f, b);
+        load_weights(a.w, l, i, 1.f, w);
+        load_weights(a.b, l, i, 0.f, b);
         Vec<DT, W> y;
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           const float g = z[i][e], s = sigmoid_of(g);
           y.set(e, fmaf(v[i][e], w[e], b[e]) * (a.silu ? g * s : s));
         }
-        store_vec<DT, W>(a.y, n * a.C + l.c[i], y);
+        store_row<DT>(a.y, n * a.C, l, i, y);
       }
   }
 }
 
-template <int DT, int W, int NV, int WIDE>
+template <int DT, int W, int NV, bool FULL, int WIDE>
 __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(const RowArgs a) {
   __shared__ float sm[(WIDE ? WIDE : kBwdThreads) * kHold];
   int turn = 0;
-  Place<W, NV> l(a);
+  Place<W, NV, FULL> l(a);
   float sum[2][NV][W];   // of w and b
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -270,9 +296,9 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(co
     for (int e = 0; e < W; ++e) sum[0][i][e] = sum[1][i][e] = 0.f;
   Held<DT, W> x[NV], z[NV], dy[NV], nx[NV], nz[NV], ndy[NV];
   auto fetch = [&](int64_t n, bool on) {
-    load_row<DT, W, NV>(nx, a.x, n * a.ldx, l, on);
-    load_row<DT, W, NV>(nz, a.z, n * a.ldz, l, on);
-    load_row<DT, W, NV>(ndy, a.dy, n * a.C, l, on);
+    load_row<DT, W, NV, FULL>(nx, a.x, n * a.ldx, l, on);
+    load_row<DT, W, NV, FULL>(nz, a.z, n * a.ldz, l, on);
+    load_row<DT, W, NV, FULL>(ndy, a.dy, n * a.C, l, on);
   };
   fetch(l.row, l.row < a.N);
   for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
@@ -286,12 +312,12 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(co
     if (n + a.slots < a.N) fetch(n + a.slots, true);
     float v[NV][W], h[NV][W];
     each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
-    const float rstd = normalise<WIDE, W, NV>(v, l.ok, a, sm, turn);
+    const float rstd = normalise<WIDE, FULL, W, NV>(v, l, a, sm, turn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         float w[W], b[W];
-        load_weights<W>(a.w, l.c[i], 1.f, w);
-        load_weights<W>(a.b, l.c[i], 0.f, b);
+        load_weights(a.w, l, i, 1.f, w);
+        load_weights(a.b, l, i, 0.f, b);
         Vec<DT, W> dz;
 #pragma unroll
         for (int e = 0; e < W; ++e) {
@@ -303,58 +329,57 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(co
           sum[1][i][e] += dv;
           h[i][e] = dv * w[e];
         }
-        if (a.dz && l.ok[i]) store_vec<DT, W>(a.dz, n * a.C + l.c[i], dz);
+        if (a.dz) store_row<DT>(a.dz, n * a.C, l, i, dz);
       }
     if (a.y) {
-      normalise_back<WIDE, W, NV>(h, v, rstd, l.ok, a, sm, turn);
+      normalise_back<WIDE, FULL, W, NV>(h, v, rstd, l, a, sm, turn);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (l.ok[i]) {
+      for (int i = 0; i < NV; ++i) {
           Vec<DT, W> dx;
 #pragma unroll
           for (int e = 0; e < W; ++e) dx.set(e, h[i][e]);
-          store_vec<DT, W>(a.y, n * a.C + l.c[i], dx);
+          store_row<DT>(a.y, n * a.C, l, i, dx);
         }
     }
   }
-  if (a.part) leave_sums<W, NV, 2>(a, l, sum, sm);
+  if (a.part) leave_sums<W, NV, FULL, 2>(a, l, sum, sm);
 }
 
 // ----------------------------------------------------------------- residual --
 // The stream's value before its norm and, for the backward, what is kept of the way
 // there: the branch's normalised values, their 1 / deviation and the mask.
-template <int DT, int DTR, int W, int NV, int WIDE>
+template <int DT, int DTR, int W, int NV, bool FULL, int WIDE>
 struct Stream {
   float s[NV][W], n2[NV][W], rstd2;
   uint32_t keep[NV];
-  __device__ __forceinline__ void run(const RowArgs &a, const Place<W, NV> &l, const Held<DT, W> (&x)[NV], const Held<DTR, W> (&r)[NV],
+  __device__ __forceinline__ void run(const RowArgs &a, const Place<W, NV, FULL> &l, const Held<DT, W> (&x)[NV], const Held<DTR, W> (&r)[NV],
                                       float scale, uint64_t seed, int64_t n, float *sm, int &turn) {
     each<W, NV>([&](int i, int e) { n2[i][e] = x[i][e]; });
-    rstd2 = a.post ? normalise<WIDE, W, NV>(n2, l.ok, a, sm, turn) : 1.f;
+    rstd2 = a.post ? normalise<WIDE, FULL, W, NV>(n2, l, a, sm, turn) : 1.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       keep[i] = ~0u;
-      if (a.draw.threshold) keep[i] = kept<W>(a.draw, seed, static_cast<uint64_t>(n) * a.C + l.c[i]);
+      if (a.draw.threshold) keep[i] = kept<W, FULL>(a.draw, seed, static_cast<uint64_t>(n) * a.C + l.c[i]);
       float w2[W], c[W];
-      load_weights<W>(a.w2, l.c[i], 1.f, w2);
-      load_weights<W>(a.gamma, l.c[i], 1.f, c);
+      load_weights(a.w2, l, i, 1.f, w2);
+      load_weights(a.gamma, l, i, 1.f, c);
 #pragma unroll
       for (int e = 0; e < W; ++e) s[i][e] = r[i][e] + (keep[i] >> e & 1 ? c[e] * scale * (n2[i][e] * w2[e]) : 0.f);
     }
   }
 };
 
-template <int DT, int DTR, int W, int NV, int WIDE>
+template <int DT, int DTR, int W, int NV, bool FULL, int WIDE>
 __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void residual_fwd_kernel(const RowArgs a) {
   __shared__ float sm[64];
   int turn = 0;
-  Place<W, NV> l(a);
+  Place<W, NV, FULL> l(a);
   const float scale = a.alpha * (a.draw.threshold ? a.draw.scale : 1.f);
   const uint64_t seed = a.draw.threshold ? static_cast<uint64_t>(*a.draw.seed) : 0;
   Held<DT, W> x[NV], nx[NV];
   Held<DTR, W> r[NV], nr[NV];
-  load_row<DT, W, NV>(nx, a.x, l.row * a.C, l, l.row < a.N);
-  load_row<DTR, W, NV>(nr, a.r, l.row * a.C, l, l.row < a.N);
+  load_row<DT, W, NV, FULL>(nx, a.x, l.row * a.C, l, l.row < a.N);
+  load_row<DTR, W, NV, FULL>(nr, a.r, l.row * a.C, l, l.row < a.N);
   for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
     l.at(n, a.N);
 #pragma unroll
@@ -363,39 +388,37 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void residual_fwd_kernel
       r[i] = nr[i];
     }
     if (n + a.slots < a.N) {
-      load_row<DT, W, NV>(nx, a.x, (n + a.slots) * a.C, l, true);
-      load_row<DTR, W, NV>(nr, a.r, (n + a.slots) * a.C, l, true);
+      load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.C, l, true);
+      load_row<DTR, W, NV, FULL>(nr, a.r, (n + a.slots) * a.C, l, true);
     }
-    Stream<DT, DTR, W, NV, WIDE> t;
+    Stream<DT, DTR, W, NV, FULL, WIDE> t;
     t.run(a, l, x, r, scale, seed, n, sm, turn);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (l.ok[i]) {
+    for (int i = 0; i < NV; ++i) {
         Vec<DTR, W> s;
 #pragma unroll
         for (int e = 0; e < W; ++e) s.set(e, t.s[i][e]);
-        store_vec<DTR, W>(a.s, n * a.C + l.c[i], s);
+        store_row<DTR>(a.s, n * a.C, l, i, s);
       }
-    normalise<WIDE, W, NV>(t.s, l.ok, a, sm, turn);
+    normalise<WIDE, FULL, W, NV>(t.s, l, a, sm, turn);
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
-      if (l.ok[i]) {
+    for (int i = 0; i < NV; ++i) {
         float w[W], b[W];
-        load_weights<W>(a.w, l.c[i], 1.f, w);
-        load_weights<W>(a.b, l.c[i], 0.f, b);
+        load_weights(a.w, l, i, 1.f, w);
+        load_weights(a.b, l, i, 0.f, b);
         Vec<DT, W> y;
 #pragma unroll
         for (int e = 0; e < W; ++e) y.set(e, fmaf(t.s[i][e], w[e], b[e]));
-        store_vec<DT, W>(a.y, n * a.C + l.c[i], y);
+        store_row<DT>(a.y, n * a.C, l, i, y);
       }
   }
 }
 
-template <int DT, int DTR, int W, int NV, int WIDE>
+template <int DT, int DTR, int W, int NV, bool FULL, int WIDE>
 __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel(const RowArgs a) {
   __shared__ float sm[(WIDE ? WIDE : kBwdThreads) * kHold];
   int turn = 0;
-  Place<W, NV> l(a);
+  Place<W, NV, FULL> l(a);
   float sum[4][NV][W];   // of w, b, gamma, w2
 #pragma unroll
   for (int i = 0; i < NV; ++i)
@@ -406,10 +429,10 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
   Held<DT, W> x[NV], nx[NV], dy[NV], ndy[NV];
   Held<DTR, W> r[NV], nr[NV], ds[NV], nds[NV];
   auto fetch = [&](int64_t n, bool on) {
-    load_row<DT, W, NV>(nx, a.x, n * a.C, l, on);
-    load_row<DTR, W, NV>(nr, a.r, n * a.C, l, on);
-    load_row<DT, W, NV>(ndy, a.dy, n * a.C, l, on && a.dy);
-    load_row<DTR, W, NV>(nds, a.ds, n * a.C, l, on && a.ds);
+    load_row<DT, W, NV, FULL>(nx, a.x, n * a.C, l, on);
+    load_row<DTR, W, NV, FULL>(nr, a.r, n * a.C, l, on);
+    load_row<DT, W, NV, FULL>(ndy, a.dy, n * a.C, l, on && a.dy);
+    load_row<DTR, W, NV, FULL>(nds, a.ds, n * a.C, l, on && a.ds);
   };
   fetch(l.row, l.row < a.N);
   for (int64_t n = l.row; n - l.row + l.first < a.N; n += a.slots) {   // (as often in the whole workgroup)
@@ -422,15 +445,15 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
       ds[i] = nds[i];
     }
     if (n + a.slots < a.N) fetch(n + a.slots, true);
-    Stream<DT, DTR, W, NV, WIDE> t;
+    Stream<DT, DTR, W, NV, FULL, WIDE> t;
     t.run(a, l, x, r, scale, seed, n, sm, turn);
     float d[NV][W];
     if (a.dy) {
-      const float rstd = normalise<WIDE, W, NV>(t.s, l.ok, a, sm, turn);
+      const float rstd = normalise<WIDE, FULL, W, NV>(t.s, l, a, sm, turn);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
           float w[W];
-          load_weights<W>(a.w, l.c[i], 1.f, w);
+          load_weights(a.w, l, i, 1.f, w);
 #pragma unroll
           for (int e = 0; e < W; ++e) {
             const float g = dy[i][e];
@@ -439,22 +462,22 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
             d[i][e] = g * w[e];
           }
         }
-      normalise_back<WIDE, W, NV>(d, t.s, rstd, l.ok, a, sm, turn);
+      normalise_back<WIDE, FULL, W, NV>(d, t.s, rstd, l, a, sm, turn);
       each<W, NV>([&](int i, int e) { d[i][e] += ds[i][e]; });   // (zeros without one)
     } else {
       each<W, NV>([&](int i, int e) { d[i][e] = ds[i][e]; });
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (a.s && l.ok[i]) {
+        if (a.s) {
           Vec<DTR, W> dr;
 #pragma unroll
           for (int e = 0; e < W; ++e) dr.set(e, d[i][e]);
-          store_vec<DTR, W>(a.s, n * a.C + l.c[i], dr);
+          store_row<DTR>(a.s, n * a.C, l, i, dr);
         }
         float w2[W], c[W];
-        load_weights<W>(a.w2, l.c[i], 1.f, w2);
-        load_weights<W>(a.gamma, l.c[i], 1.f, c);
+        load_weights(a.w2, l, i, 1.f, w2);
+        load_weights(a.gamma, l, i, 1.f, c);
 #pragma unroll
         for (int e = 0; e < W; ++e) {   // (what was dropped is 0 whatever it was)
           const bool on = t.keep[i] >> e & 1;
@@ -465,18 +488,17 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
         }
       }
     if (a.y) {
-      if (a.post) normalise_back<WIDE, W, NV>(d, t.n2, t.rstd2, l.ok, a, sm, turn);
+      if (a.post) normalise_back<WIDE, FULL, W, NV>(d, t.n2, t.rstd2, l, a, sm, turn);
 #pragma unroll
-      for (int i = 0; i < NV; ++i)
-        if (l.ok[i]) {
+      for (int i = 0; i < NV; ++i) {
           Vec<DT, W> dx;
 #pragma unroll
           for (int e = 0; e < W; ++e) dx.set(e, d[i][e]);
-          store_vec<DT, W>(a.y, n * a.C + l.c[i], dx);
+          store_row<DT>(a.y, n * a.C, l, i, dx);
         }
     }
   }
-  if (a.part) leave_sums<W, NV, 4>(a, l, sum, sm);
+  if (a.part) leave_sums<W, NV, FULL, 4>(a, l, sum, sm);
 }
 
 // Sums down R rows of [R][KINDS C]: 64 columns a workgroup, 16 wavefronts with every
@@ -506,23 +528,25 @@ __global__ __launch_bounds__(1024) void row_cols_kernel(const float *__restrict_
 // How the rows are dealt, from the sizes and the widest vector the addresses allow.
 struct RowPlan {
   int W, NV, S, threads;
-  bool wide;
+  bool full, wide;
   int64_t slots, blocks, rows;   // rows: of sums
 };
 // Wavefronts: the forward's lane groups have a few rows each, the backward's as many as
 // leave three workgroups a CU: their sums over rows go through memory once a workgroup.
 constexpr int64_t kFwdWaves = 8192, kBwdWaves = 3072;
 
-RowPlan plan_of(int64_t N, int per, int G, int W, bool bwd) {
+RowPlan plan_of(int64_t N, int per, int G, int W, int dtype, bool bwd) {   // W 0: no vectors
   RowPlan p{};
+  p.full = W != 0;
+  if (!W) W = dtype == SSLA_F32 ? 4 : 8;
   p.W = W;
-  const int nv = per / W, most = kHold / W;
+  const int nv = (per + W - 1) / W, most = kHold / W;
   p.S = 1;
   while (p.S < nv && (p.S < 64 || static_cast<int64_t>(p.S) * most < nv)) p.S *= 2;
   p.wide = p.S > 64;
   p.threads = std::max(bwd ? kBwdThreads : kFwdThreads, p.S);
   p.NV = 1;
-  while (p.NV < most && (p.wide || static_cast<int64_t>(p.S) * p.NV < nv)) p.NV *= W == 1 ? kHold : 2;
+  while (p.NV < most && (p.wide || !p.full || static_cast<int64_t>(p.S) * p.NV < nv)) p.NV *= 2;
   const int64_t groups = p.threads / p.S;   // lane groups of a workgroup
   const int64_t need = (N * G + groups - 1) / groups;
   p.blocks = std::min(need, (bwd ? kBwdWaves : kFwdWaves) * 64 / p.threads);
@@ -537,7 +561,7 @@ RowPlan plan_of(int64_t N, int per, int G, int W, bool bwd) {
 struct Tensor { const void *p; int64_t ld; int dtype; };
 int widest(int per, int dtype, std::initializer_list<Tensor> tensors, std::initializer_list<const float *> weights) {
   for (const float *w : weights)
-    if (!aligned(w, 16)) return 1;   // (NULL is aligned)
+    if (!aligned(w, 16)) return 0;   // (NULL is aligned)
   for (int W = dtype == SSLA_F32 ? 4 : 8; W >= 4; W /= 2) {
     bool ok = per % W == 0;
     for (const Tensor &t : tensors) {
@@ -546,13 +570,14 @@ int widest(int per, int dtype, std::initializer_list<Tensor> tensors, std::initi
     }
     if (ok) return W;
   }
-  return 1;
+  return 0;
 }
 
-size_t sums_bytes(int64_t N, int per, int G, int kinds) {   // whatever vectors the addresses allow
+size_t sums_bytes(int64_t N, int per, int G, int kinds) {   // whatever type and vectors the call has
   int64_t most = 0;
-  for (int W = 1; W <= 8; W *= 2)
-    if (W != 2 && per % W == 0) most = std::max(most, plan_of(N, per, G, W, true).rows);
+  for (int dtype : {SSLA_F32, SSLA_BF16})
+    for (int W : {0, 4, 8})
+      if (!W || per % W == 0) most = std::max(most, plan_of(N, per, G, W, dtype, true).rows);
   return static_cast<size_t>(most) * kinds * per * G * sizeof(float);
 }
 
@@ -584,29 +609,30 @@ int check_draw(const char *what, float p, const int64_t *seed, Draw &d) {
   return SSLA_OK;
 }
 
-// Launches K<..., W, NV, WIDE> by the plan (WIDE: the threads whose registers a row of
+// Launches K<..., W, NV, FULL, WIDE> by the plan (WIDE: the threads whose registers a row of
 // several wavefronts has to do with; 0: rows of one wavefront).
-#define SSLA_ROWS_NV(K, W_, NV_, ...)                                                                        \
-  if (p.W == W_ && p.NV == NV_) {                                                                            \
+#define SSLA_ROWS_NV(K, W_, NV_, FULL_, ...)                                                                 \
+  if (p.W == W_ && p.NV == NV_ && p.full == FULL_) {                                                         \
     if (p.wide) {                                                                                            \
       if constexpr (W_ * NV_ == kHold) {                                                                     \
-        if (p.threads <= 512) hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, 512>), grid, block, 0, st, a);     \
-        else hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, kMostLanes>), grid, block, 0, st, a);               \
+        if (p.threads <= 512) hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, FULL_, 512>), grid, block, 0, st, a); \
+        else hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, FULL_, kMostLanes>), grid, block, 0, st, a);        \
       }                                                                                                      \
     } else {                                                                                                 \
-      hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, 0>), grid, block, 0, st, a);                               \
+      hipLaunchKernelGGL((K<__VA_ARGS__, W_, NV_, FULL_, 0>), grid, block, 0, st, a);                        \
     }                                                                                                        \
   }
 #define SSLA_ROWS(K, D, ...)                                  \
   do {                                                        \
     const dim3 grid(static_cast<unsigned>(p.blocks)), block(p.threads); \
     if constexpr (D != SSLA_F32) {                            \
-      SSLA_ROWS_NV(K, 8, 1, __VA_ARGS__)                      \
+      SSLA_ROWS_NV(K, 8, 1, true, __VA_ARGS__)                \
+      SSLA_ROWS_NV(K, 8, 1, false, __VA_ARGS__)               \
+    } else {                                                  \
+      SSLA_ROWS_NV(K, 4, 2, false, __VA_ARGS__)               \
     }                                                         \
-    SSLA_ROWS_NV(K, 4, 1, __VA_ARGS__)                        \
-    SSLA_ROWS_NV(K, 4, 2, __VA_ARGS__)                        \
-    SSLA_ROWS_NV(K, 1, 1, __VA_ARGS__)                        \
-    SSLA_ROWS_NV(K, 1, 8, __VA_ARGS__)                        \
+    SSLA_ROWS_NV(K, 4, 1, true, __VA_ARGS__)                  \
+    SSLA_ROWS_NV(K, 4, 2, true, __VA_ARGS__)                  \
   } while (0)
 #define SSLA_GATED(K)                                             \
   if (dtype == SSLA_F32) SSLA_ROWS(K, SSLA_F32, SSLA_F32);        \
@@ -645,7 +671,7 @@ extern "C" int ssla_gated_norm_fwd(const void *x, int64_t ldx, const void *z, in
   RowArgs a{};
   a.x = x; a.z = z; a.ldx = ldx; a.ldz = ldz; a.w = weight; a.b = bias; a.y = y;
   a.N = N; a.C = C; a.G = G; a.per = C / G; a.layer = kind == SSLA_NORM_LAYER; a.silu = act == SSLA_ACT_SILU; a.eps = eps;
-  const RowPlan p = plan_of(N, C / G, G, widest(C / G, dtype, {{x, ldx, dtype}, {z, ldz, dtype}, {y, C, dtype}}, {weight, bias}), false);
+  const RowPlan p = plan_of(N, C / G, G, widest(C / G, dtype, {{x, ldx, dtype}, {z, ldz, dtype}, {y, C, dtype}}, {weight, bias}), dtype, false);
   set_plan(a, p);
   SSLA_GATED(gated_fwd_kernel);
   return launch_status("gated_norm_fwd");
@@ -677,7 +703,7 @@ extern "C" int ssla_gated_norm_bwd(const void *dy, const void *x, int64_t ldx, c
     a.part = sums ? static_cast<float *>(workspace) : nullptr;
     a.N = N; a.C = C; a.G = G; a.per = C / G; a.layer = kind == SSLA_NORM_LAYER; a.silu = act == SSLA_ACT_SILU; a.eps = eps;
     p = plan_of(N, C / G, G, widest(C / G, dtype, {{x, ldx, dtype}, {z, ldz, dtype}, {dy, C, dtype}, {dx, C, dtype}, {dz, C, dtype}},
-                                    {weight, bias}), true);
+                                    {weight, bias}), dtype, true);
     set_plan(a, p);
     SSLA_GATED(gated_bwd_kernel);
   }
@@ -702,7 +728,7 @@ extern "C" int ssla_residual_norm_fwd(const void *x, const void *residual, int64
   a.x = x; a.r = residual; a.w = weight; a.b = bias; a.w2 = post_weight; a.gamma = gamma; a.y = y; a.s = sum;
   a.N = N; a.C = a.per = C; a.G = 1; a.layer = kind == SSLA_NORM_LAYER; a.post = post != 0; a.eps = eps; a.alpha = alpha;
   const RowPlan pl = plan_of(N, C, 1, widest(C, dtype, {{x, C, dtype}, {residual, C, r_dtype}, {y, C, dtype}, {sum, C, r_dtype}},
-                                             {weight, bias, post_weight, gamma}), false);
+                                             {weight, bias, post_weight, gamma}), dtype, false);
   {
     const RowPlan &p = pl;
     set_plan(a, p);
@@ -739,7 +765,7 @@ extern "C" int ssla_residual_norm_bwd(const void *dy, const void *dsum, const vo
     a.part = sums ? static_cast<float *>(workspace) : nullptr;
     a.N = N; a.C = a.per = C; a.G = 1; a.layer = kind == SSLA_NORM_LAYER; a.post = post != 0; a.eps = eps; a.alpha = alpha;
     const RowPlan p = plan_of(N, C, 1, widest(C, dtype, {{x, C, dtype}, {residual, C, r_dtype}, {dy, C, dtype}, {dsum, C, r_dtype},
-                                                         {dx, C, dtype}, {dresidual, C, r_dtype}}, {weight, post_weight, gamma}), true);
+                                                         {dx, C, dtype}, {dresidual, C, r_dtype}}, {weight, post_weight, gamma}), dtype, true);
     rows = p.rows;
     set_plan(a, p);
     SSLA_RESIDUAL(residual_bwd_kernel);

@@ -21,7 +21,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const void *x, int64_t n, 
       Vec<DT, W> v[8 / W];
 #pragma unroll
       for (int k = 0; k < 8 / W; ++k) v[k] = load_vec<DT, W>(x, 8 * i + k * W);
-      const uint32_t keep = kept<8>(d, seed, 8 * i);
+      const uint32_t keep = kept_of(d, seed, i);
 #pragma unroll
       for (int k = 0; k < 8 / W; ++k) {
 #pragma unroll
@@ -29,7 +29,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const void *x, int64_t n, 
         store_vec<DT, W>(y, 8 * i + k * W, v[k]);
       }
     } else {
-      const uint32_t keep = kept<8>(d, seed, 8 * i);
+      const uint32_t keep = kept_of(d, seed, i);
       for (int e = 0; e < 8 && 8 * i + e < n; ++e)
         Elem<DT>::store(y, 8 * i + e, keep >> e & 1 ? Elem<DT>::load(x, 8 * i + e) * d.scale : 0.f);
     }

@@ -31,16 +31,22 @@ __device__ __forceinline__ Bits bits_of(uint64_t i, uint64_t seed, uint32_t subs
   return {{c0, c1, c2, c3}};
 }
 
-// Which of the W elements from `at` on are kept, a bit each.  W of 4 or 8 starts at a
-// multiple of W.
-template <int W>
-__device__ __forceinline__ uint32_t kept(const Draw &d, uint64_t seed, uint64_t at) {
-  const Bits b = bits_of(at >> 3, seed, d.subsequence);
-  const uint32_t off = static_cast<uint32_t>(at) & 7;
+// Which of the eight elements of a block are kept, a bit each.
+__device__ __forceinline__ uint32_t kept_of(const Draw &d, uint64_t seed, uint64_t block) {
+  const Bits b = bits_of(block, seed, d.subsequence);
   uint32_t keep = 0;
 #pragma unroll
   for (int e = 0; e < 8; ++e) keep |= static_cast<uint32_t>((e & 1 ? b.w[e >> 1] >> 16 : b.w[e >> 1] & 0xffffu) >= d.threshold) << e;
-  return W == 8 ? keep : keep >> off;
+  return keep;
+}
+// Which of the W elements from `at` on are kept: W of 4 or 8.  FULL: `at` is a multiple of W;
+// else they may lie in two blocks.
+template <int W, bool FULL>
+__device__ __forceinline__ uint32_t kept(const Draw &d, uint64_t seed, uint64_t at) {
+  const uint32_t off = static_cast<uint32_t>(at) & 7;
+  uint32_t keep = kept_of(d, seed, at >> 3) >> off;
+  if (!FULL && off + W > 8) keep |= kept_of(d, seed, (at >> 3) + 1) << (8 - off);
+  return keep;
 }
 
 }  // namespace ssla
