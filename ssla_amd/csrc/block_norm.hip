@@ -532,8 +532,9 @@ struct RowPlan {
   int64_t slots, blocks, rows;   // rows: of sums
 };
 // Wavefronts: the forward's lane groups have a few rows each, the backward's as many as
-// leave three workgroups a CU: their sums over rows go through memory once a workgroup.
-constexpr int64_t kFwdWaves = 8192, kBwdWaves = 3072;
+// run at once (three workgroups a CU, of wide rows one): their sums over rows go through
+// memory once a workgroup.
+constexpr int64_t kFwdWaves = 8192, kBwdWaves[3] = {3072, 2048, 4096};   // (of 256, 512, 1,024 threads)
 
 RowPlan plan_of(int64_t N, int per, int G, int W, int dtype, bool bwd) {   // W 0: no vectors
   RowPlan p{};
@@ -549,7 +550,7 @@ RowPlan plan_of(int64_t N, int per, int G, int W, int dtype, bool bwd) {   // W 
   while (p.NV < most && (p.wide || !p.full || static_cast<int64_t>(p.S) * p.NV < nv)) p.NV *= 2;
   const int64_t groups = p.threads / p.S;   // lane groups of a workgroup
   const int64_t need = (N * G + groups - 1) / groups;
-  p.blocks = std::min(need, (bwd ? kBwdWaves : kFwdWaves) * 64 / p.threads);
+  p.blocks = std::min(need, (bwd ? kBwdWaves[p.threads / 512] : kFwdWaves) * 64 / p.threads);
   // a lane group keeps its group of channels, so all groups have as many (one row at a time at least)
   p.slots = std::min(N, std::max<int64_t>(1, p.blocks * groups / G));
   p.slots = (N + (N + p.slots - 1) / p.slots - 1) / ((N + p.slots - 1) / p.slots);   // all as many rows as the busiest, or one less
