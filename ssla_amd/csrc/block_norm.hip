@@ -105,7 +105,7 @@ template <int W, int NV, bool FULL>
 struct Place {
   int j, g, c[NV];
   int64_t row, first;               // its first row, and the workgroup's
-  bool on;
+  bool on, live;                    // has rows; has one to work on now
   int cols[NV], has[NV], now[NV];   // values that exist; with a row at all; with the row worked on
   __device__ __forceinline__ explicit Place(const RowArgs &a) {
     const int64_t sub = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) / a.S;
@@ -114,19 +114,21 @@ struct Place {
     row = sub / a.G;
     first = static_cast<int64_t>(blockIdx.x) * blockDim.x / a.S / a.G;
     on = row < a.slots;
+    live = on && row < a.N;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       c[i] = (j + a.S * i) * W;
       cols[i] = min(max(a.per - c[i], 0), W);
       has[i] = on ? cols[i] : 0;
-      now[i] = row < a.N ? has[i] : 0;
+      now[i] = live ? has[i] : 0;
       c[i] = (cols[i] ? c[i] : 0) + g * a.per;
     }
   }
   // Row n is the one worked on: lanes behind the last row idle along.
   __device__ __forceinline__ void at(int64_t n, int64_t N) {
+    live = on && n < N;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) now[i] = n < N ? has[i] : 0;
+    for (int i = 0; i < NV; ++i) now[i] = live ? has[i] : 0;
   }
   __device__ __forceinline__ bool is(int i, int e) const { return FULL ? now[i] != 0 : e < now[i]; }
 };
@@ -195,7 +197,7 @@ __device__ __forceinline__ float normalise(float (&x)[NV][W], const Place<W, NV,
   float t[1] = {0.f};
   each<W, NV>([&](int i, int e) { t[0] = fmaf(x[i][e], x[i][e], t[0]); });
   row_sums<WIDE>(t, a.S, sm, turn);
-  const float rstd = 1.f / sqrtf(t[0] * inv + a.eps);
+  const float rstd = l.live ? 1.f / sqrtf(t[0] * inv + a.eps) : 0.f;   // (idle lanes stay at zeros)
   each<W, NV>([&](int i, int e) { x[i][e] *= rstd; });
   return rstd;
 }
@@ -261,26 +263,25 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void gated_fwd_kernel(co
       x[i] = nx[i];
       z[i] = nz[i];
     }
-    if (n + a.slots < a.N) {
-      load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.ldx, l, true);
-      load_row<DT, W, NV, FULL>(nz, a.z, (n + a.slots) * a.ldz, l, true);
-    }
+    const bool more = n + a.slots < a.N;
+    load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.ldx, l, more);
+    load_row<DT, W, NV, FULL>(nz, a.z, (n + a.slots) * a.ldz, l, more);
     float v[NV][W];
     each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
     normalise<WIDE, FULL, W, NV>(v, l, a, sm, turn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        float w[W], b[W];
-        load_weights(a.w, l, i, 1.f, w);
-        load_weights(a.b, l, i, 0.f, b);
-        Vec<DT, W> y;
+      float w[W], b[W];
+      load_weights(a.w, l, i, 1.f, w);
+      load_weights(a.b, l, i, 0.f, b);
+      Vec<DT, W> y;
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const float g = z[i][e], s = sigmoid_of(g);
-          y.set(e, fmaf(v[i][e], w[e], b[e]) * (a.silu ? g * s : s));
-        }
-        store_row<DT>(a.y, n * a.C, l, i, y);
+      for (int e = 0; e < W; ++e) {
+        const float g = z[i][e], s = sigmoid_of(g);
+        y.set(e, fmaf(v[i][e], w[e], b[e]) * (a.silu ? g * s : s));
       }
+      store_row<DT>(a.y, n * a.C, l, i, y);
+    }
   }
 }
 
@@ -309,37 +310,37 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(co
       z[i] = nz[i];
       dy[i] = ndy[i];
     }
-    if (n + a.slots < a.N) fetch(n + a.slots, true);
+    fetch(n + a.slots, n + a.slots < a.N);   // (zeros behind the last row: those lanes add nothing)
     float v[NV][W], h[NV][W];
     each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
     const float rstd = normalise<WIDE, FULL, W, NV>(v, l, a, sm, turn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        float w[W], b[W];
-        load_weights(a.w, l, i, 1.f, w);
-        load_weights(a.b, l, i, 0.f, b);
-        Vec<DT, W> dz;
+      float w[W], b[W];
+      load_weights(a.w, l, i, 1.f, w);
+      load_weights(a.b, l, i, 0.f, b);
+      Vec<DT, W> dz;
 #pragma unroll
-        for (int e = 0; e < W; ++e) {
-          const float g = z[i][e], s = sigmoid_of(g), o = sigmoid_of(-g);
-          const float act = a.silu ? g * s : s, slope = a.silu ? fmaf(g * s, o, s) : s * o;
-          const float d = dy[i][e], dv = d * act;
-          dz.set(e, d * fmaf(v[i][e], w[e], b[e]) * slope);
-          sum[0][i][e] = fmaf(dv, v[i][e], sum[0][i][e]);
-          sum[1][i][e] += dv;
-          h[i][e] = dv * w[e];
-        }
-        if (a.dz) store_row<DT>(a.dz, n * a.C, l, i, dz);
+      for (int e = 0; e < W; ++e) {
+        const float g = z[i][e], s = sigmoid_of(g), o = sigmoid_of(-g);
+        const float act = a.silu ? g * s : s, slope = a.silu ? fmaf(g * s, o, s) : s * o;
+        const float d = dy[i][e], dv = d * act;
+        dz.set(e, d * fmaf(v[i][e], w[e], b[e]) * slope);
+        sum[0][i][e] = fmaf(dv, v[i][e], sum[0][i][e]);
+        sum[1][i][e] += dv;
+        h[i][e] = dv * w[e];
       }
+      if (a.dz) store_row<DT>(a.dz, n * a.C, l, i, dz);
+    }
     if (a.y) {
       normalise_back<WIDE, FULL, W, NV>(h, v, rstd, l, a, sm, turn);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-          Vec<DT, W> dx;
+        Vec<DT, W> dx;
 #pragma unroll
-          for (int e = 0; e < W; ++e) dx.set(e, h[i][e]);
-          store_row<DT>(a.y, n * a.C, l, i, dx);
-        }
+        for (int e = 0; e < W; ++e) dx.set(e, h[i][e]);
+        store_row<DT>(a.y, n * a.C, l, i, dx);
+      }
     }
   }
   if (a.part) leave_sums<W, NV, FULL, 2>(a, l, sum, sm);
@@ -387,30 +388,29 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void residual_fwd_kernel
       x[i] = nx[i];
       r[i] = nr[i];
     }
-    if (n + a.slots < a.N) {
-      load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.C, l, true);
-      load_row<DTR, W, NV, FULL>(nr, a.r, (n + a.slots) * a.C, l, true);
-    }
+    const bool more = n + a.slots < a.N;
+    load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.C, l, more);
+    load_row<DTR, W, NV, FULL>(nr, a.r, (n + a.slots) * a.C, l, more);
     Stream<DT, DTR, W, NV, FULL, WIDE> t;
     t.run(a, l, x, r, scale, seed, n, sm, turn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        Vec<DTR, W> s;
+      Vec<DTR, W> s;
 #pragma unroll
-        for (int e = 0; e < W; ++e) s.set(e, t.s[i][e]);
-        store_row<DTR>(a.s, n * a.C, l, i, s);
-      }
+      for (int e = 0; e < W; ++e) s.set(e, t.s[i][e]);
+      store_row<DTR>(a.s, n * a.C, l, i, s);
+    }
     normalise<WIDE, FULL, W, NV>(t.s, l, a, sm, turn);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        float w[W], b[W];
-        load_weights(a.w, l, i, 1.f, w);
-        load_weights(a.b, l, i, 0.f, b);
-        Vec<DT, W> y;
+      float w[W], b[W];
+      load_weights(a.w, l, i, 1.f, w);
+      load_weights(a.b, l, i, 0.f, b);
+      Vec<DT, W> y;
 #pragma unroll
-        for (int e = 0; e < W; ++e) y.set(e, fmaf(t.s[i][e], w[e], b[e]));
-        store_row<DT>(a.y, n * a.C, l, i, y);
-      }
+      for (int e = 0; e < W; ++e) y.set(e, fmaf(t.s[i][e], w[e], b[e]));
+      store_row<DT>(a.y, n * a.C, l, i, y);
+    }
   }
 }
 
@@ -444,7 +444,7 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
       dy[i] = ndy[i];
       ds[i] = nds[i];
     }
-    if (n + a.slots < a.N) fetch(n + a.slots, true);
+    fetch(n + a.slots, n + a.slots < a.N);   // (zeros behind the last row: those lanes add nothing)
     Stream<DT, DTR, W, NV, FULL, WIDE> t;
     t.run(a, l, x, r, scale, seed, n, sm, turn);
     float d[NV][W];
@@ -452,16 +452,16 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
       const float rstd = normalise<WIDE, FULL, W, NV>(t.s, l, a, sm, turn);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-          float w[W];
-          load_weights(a.w, l, i, 1.f, w);
+        float w[W];
+        load_weights(a.w, l, i, 1.f, w);
 #pragma unroll
-          for (int e = 0; e < W; ++e) {
-            const float g = dy[i][e];
-            sum[0][i][e] = fmaf(g, t.s[i][e], sum[0][i][e]);
-            sum[1][i][e] += g;
-            d[i][e] = g * w[e];
-          }
+        for (int e = 0; e < W; ++e) {
+          const float g = dy[i][e];
+          sum[0][i][e] = fmaf(g, t.s[i][e], sum[0][i][e]);
+          sum[1][i][e] += g;
+          d[i][e] = g * w[e];
         }
+      }
       normalise_back<WIDE, FULL, W, NV>(d, t.s, rstd, l, a, sm, turn);
       each<W, NV>([&](int i, int e) { d[i][e] += ds[i][e]; });   // (zeros without one)
     } else {
@@ -469,33 +469,33 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
     }
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        if (a.s) {
-          Vec<DTR, W> dr;
+      if (a.s) {
+        Vec<DTR, W> dr;
 #pragma unroll
-          for (int e = 0; e < W; ++e) dr.set(e, d[i][e]);
-          store_row<DTR>(a.s, n * a.C, l, i, dr);
-        }
-        float w2[W], c[W];
-        load_weights(a.w2, l, i, 1.f, w2);
-        load_weights(a.gamma, l, i, 1.f, c);
-#pragma unroll
-        for (int e = 0; e < W; ++e) {   // (what was dropped is 0 whatever it was)
-          const bool on = t.keep[i] >> e & 1;
-          const float g = on ? d[i][e] * scale : 0.f, v = on ? t.n2[i][e] : 0.f, dp = g * c[e];
-          sum[2][i][e] = fmaf(g, v * w2[e], sum[2][i][e]);
-          sum[3][i][e] = fmaf(dp, v, sum[3][i][e]);
-          d[i][e] = dp * w2[e];
-        }
+        for (int e = 0; e < W; ++e) dr.set(e, d[i][e]);
+        store_row<DTR>(a.s, n * a.C, l, i, dr);
       }
+      float w2[W], c[W];
+      load_weights(a.w2, l, i, 1.f, w2);
+      load_weights(a.gamma, l, i, 1.f, c);
+#pragma unroll
+      for (int e = 0; e < W; ++e) {   // (what was dropped is 0 whatever it was)
+        const bool on = t.keep[i] >> e & 1;
+        const float g = on ? d[i][e] * scale : 0.f, v = on ? t.n2[i][e] : 0.f, dp = g * c[e];
+        sum[2][i][e] = fmaf(g, v * w2[e], sum[2][i][e]);
+        sum[3][i][e] = fmaf(dp, v, sum[3][i][e]);
+        d[i][e] = dp * w2[e];
+      }
+    }
     if (a.y) {
       if (a.post) normalise_back<WIDE, FULL, W, NV>(d, t.n2, t.rstd2, l, a, sm, turn);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-          Vec<DT, W> dx;
+        Vec<DT, W> dx;
 #pragma unroll
-          for (int e = 0; e < W; ++e) dx.set(e, d[i][e]);
-          store_row<DT>(a.y, n * a.C, l, i, dx);
-        }
+        for (int e = 0; e < W; ++e) dx.set(e, d[i][e]);
+        store_row<DT>(a.y, n * a.C, l, i, dx);
+      }
     }
   }
   if (a.part) leave_sums<W, NV, FULL, 4>(a, l, sum, sm);

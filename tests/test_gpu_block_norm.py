@@ -448,3 +448,42 @@ def test_a_block_in_a_graph(dev):
         # products of 64 and up to 700 terms of fp32 lie between: 2^-14 of the largest value, some
         # 300 roundings of it, and a lost factor or term is far outside
         assert float((b.double().cpu() - c).abs().max()) <= 2.0 ** -14 * float(c.abs().max()), n
+
+
+@pytest.mark.parametrize("dtype", [F32, B16])
+@pytest.mark.parametrize("N,C,G", [(1, 8, 2), (2, 64, 1), (1023, 64, 4), (16411, 1024, 4), (5001, 75, 1), (5003, 75, 5), (3077, 2048, 16),
+                                   (4099, 520, 1), (1537, 1032, 1), (70001, 24, 3), (2500, 4096, 1024), (777, 5000, 1)])
+def test_sums_over_rows_count_every_row_once(dev, N, C, G, dtype):
+    """Whole numbers whose sums over the rows are known: x is 1 or -1, so it is its own norm to
+    8 U of itself (C ones times 1 / C, the root, a product), the gate is open and the
+    gradients are integers up to 3 with signs at random.  A lane adds some hundred terms at
+    most, so partial sums stay within 6 times 2.2 times 10 there and 13 N^0.5 behind: N
+    roundings of at most 130 U and some hundred of 13 N^0.5 U, either way alike, are 0.003 in
+    the root mean square for the longest.  A row lost or counted twice is a whole number off
+    at every channel."""
+    from ssla_amd.norm import gated_norm, residual_norm
+    gen = torch.Generator().manual_seed(N + C)
+    x = (torch.randint(0, 2, (N, C), generator=gen) * 2 - 1).to(dtype)
+    d = (torch.randint(1, 4, (N, C), generator=gen) * (torch.randint(0, 2, (N, C), generator=gen) * 2 - 1)).to(dtype)
+    one = torch.ones(C, device=dev)
+    dw, db = (x.double() * d.double()).sum(0), d.double().sum(0)
+
+    def same(name, got, want):
+        err = (got.double().cpu() - want).abs()
+        assert float(err.max()) <= 0.5, (name, float(err.max()))
+
+    leaves = [t.clone().requires_grad_() for t in (one, 0 * one)]
+    y = gated_norm(x.to(dev), torch.full((N, C), 60.0, dtype=dtype, device=dev), G, *leaves, eps=0.0, activation="sigmoid")
+    for name, got, want in zip(("dw", "db"), torch.autograd.grad(y, leaves, d.to(dev)), (dw, db)):
+        same(name, got, want)
+    if G > 1:
+        return
+    leaves = [t.clone().requires_grad_() for t in (one, 0 * one)]
+    y, s = residual_norm(torch.zeros(N, C, dtype=dtype, device=dev), x.to(dev), *leaves, eps=0.0)
+    for name, got, want in zip(("dw", "db"), torch.autograd.grad(y, leaves, d.to(dev)), (dw, db)):
+        same("residual " + name, got, want)
+    leaves = [t.clone().requires_grad_() for t in (one, one)]
+    y, s = residual_norm(x.to(dev), torch.zeros(N, C, dtype=dtype, device=dev), eps=0.0, scale=leaves[0], post_norm=True,
+                         post_weight=leaves[1])
+    for name, got in zip(("dgamma", "dw2"), torch.autograd.grad(s, leaves, d.to(dev))):
+        same(name, got, dw)
