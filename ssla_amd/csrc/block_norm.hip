@@ -130,6 +130,8 @@ struct Place {
 #pragma unroll
     for (int i = 0; i < NV; ++i) now[i] = live ? has[i] : 0;
   }
+  // The workgroup goes on behind row n (the same for all its threads).
+  __device__ __forceinline__ bool again(int64_t n, const RowArgs &a) const { return n - row + first + a.slots < a.N; }
   __device__ __forceinline__ bool is(int i, int e) const { return FULL ? now[i] != 0 : e < now[i]; }
 };
 
@@ -263,9 +265,11 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void gated_fwd_kernel(co
       x[i] = nx[i];
       z[i] = nz[i];
     }
-    const bool more = n + a.slots < a.N;
-    load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.ldx, l, more);
-    load_row<DT, W, NV, FULL>(nz, a.z, (n + a.slots) * a.ldz, l, more);
+    if (l.again(n, a)) {
+      const bool more = n + a.slots < a.N;
+      load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.ldx, l, more);
+      load_row<DT, W, NV, FULL>(nz, a.z, (n + a.slots) * a.ldz, l, more);
+    }
     float v[NV][W];
     each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
     normalise<WIDE, FULL, W, NV>(v, l, a, sm, turn);
@@ -310,7 +314,7 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void gated_bwd_kernel(co
       z[i] = nz[i];
       dy[i] = ndy[i];
     }
-    fetch(n + a.slots, n + a.slots < a.N);   // (zeros behind the last row: those lanes add nothing)
+    if (l.again(n, a)) fetch(n + a.slots, n + a.slots < a.N);   // (zeros behind the last row: those lanes add nothing)
     float v[NV][W], h[NV][W];
     each<W, NV>([&](int i, int e) { v[i][e] = x[i][e]; });
     const float rstd = normalise<WIDE, FULL, W, NV>(v, l, a, sm, turn);
@@ -388,9 +392,11 @@ __global__ __launch_bounds__(WIDE ? WIDE : kFwdThreads) void residual_fwd_kernel
       x[i] = nx[i];
       r[i] = nr[i];
     }
-    const bool more = n + a.slots < a.N;
-    load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.C, l, more);
-    load_row<DTR, W, NV, FULL>(nr, a.r, (n + a.slots) * a.C, l, more);
+    if (l.again(n, a)) {
+      const bool more = n + a.slots < a.N;
+      load_row<DT, W, NV, FULL>(nx, a.x, (n + a.slots) * a.C, l, more);
+      load_row<DTR, W, NV, FULL>(nr, a.r, (n + a.slots) * a.C, l, more);
+    }
     Stream<DT, DTR, W, NV, FULL, WIDE> t;
     t.run(a, l, x, r, scale, seed, n, sm, turn);
 #pragma unroll
@@ -444,7 +450,7 @@ __global__ __launch_bounds__(WIDE ? WIDE : kBwdThreads) void residual_bwd_kernel
       dy[i] = ndy[i];
       ds[i] = nds[i];
     }
-    fetch(n + a.slots, n + a.slots < a.N);   // (zeros behind the last row: those lanes add nothing)
+    if (l.again(n, a)) fetch(n + a.slots, n + a.slots < a.N);   // (zeros behind the last row: those lanes add nothing)
     Stream<DT, DTR, W, NV, FULL, WIDE> t;
     t.run(a, l, x, r, scale, seed, n, sm, turn);
     float d[NV][W];
