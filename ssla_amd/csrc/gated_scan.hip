@@ -684,22 +684,36 @@ struct StepArgs {
   int32_t *status;
   int n, rows, C, gate;
 };
-template <int DT, int DTG>
+// W channels a thread.
+template <int DT, int DTG, int W>
 __global__ __launch_bounds__(256) void scan_step_kernel(const StepArgs a) {
   const int64_t x = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (x >= static_cast<int64_t>(a.n) * a.C) return;
-  const int64_t i = x / a.C;
-  const int c = static_cast<int>(x % a.C), row = a.at[i];
+  const int cv = a.C / W;
+  if (x >= static_cast<int64_t>(a.n) * cv) return;
+  const int64_t i = x / cv;
+  const int c = static_cast<int>(x - i * cv) * W, row = a.at[i];
+  Vec<DT, W> o;
   if (row < 0 || row >= a.rows || (i > 0 && a.at[i - 1] >= row)) {
-    Elem<DT>::store(a.o, x, 0.f);
+#pragma unroll
+    for (int e = 0; e < W; ++e) o.set(e, 0.f);
+    store_vec<DT, W>(a.o, i * a.C + c, o);
     if (a.status) __hip_atomic_store(a.status, SSLA_ERR_ARG, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     return;
   }
-  float &s = a.state[static_cast<int64_t>(row) * a.C + c];
-  const float g = Elem<DTG>::load(a.g, i * a.ldg + c);
-  const float f = a.gate == kSigmoid ? gate_value<kSigmoid>(g) : a.gate == kLog ? gate_value<kLog>(g) : g;
-  s = fmaf(f, s, Elem<DT>::load(a.u, i * a.ldu + c));
-  Elem<DT>::store(a.o, x, a.q ? s * Elem<DT>::load(a.q, i * a.ldq + c) : s);
+  const Vec<DT, W> u = load_vec<DT, W>(a.u, i * a.ldu + c);
+  const Vec<DTG, W> g = load_vec<DTG, W>(a.g, i * a.ldg + c);
+  Vec<DT, W> q;
+  if (a.q) q = load_vec<DT, W>(a.q, i * a.ldq + c);
+  States<W> &s = *reinterpret_cast<States<W> *>(a.state + static_cast<int64_t>(row) * a.C + c);
+  States<W> h = s;
+#pragma unroll
+  for (int e = 0; e < W; ++e) {
+    const float f = a.gate == kSigmoid ? gate_value<kSigmoid>(g[e]) : a.gate == kLog ? gate_value<kLog>(g[e]) : g[e];
+    h.x[e] = fmaf(f, h.x[e], u[e]);
+    o.set(e, a.q ? h.x[e] * q[e] : h.x[e]);
+  }
+  s = h;
+  store_vec<DT, W>(a.o, i * a.C + c, o);
 }
 
 // --------------------------------------------------------------- launches --
@@ -887,10 +901,17 @@ extern "C" int ssla_sparse_gated_step(const int32_t *row_idx, int n_active, cons
   if (n_active == 0) return SSLA_OK;
   SSLA_CHECK_ARG(row_idx && u && g && o && (state || n_rows == 0), "sparse_gated_step: null pointer");
   StepArgs a{row_idx, u, g, q, ldu, ldg, ldq, state, o, status, n_active, n_rows, C, gate};
-  const int64_t blocks = (static_cast<int64_t>(n_active) * C + 255) / 256;
-#define SSLA_CALL(D, G) \
-  hipLaunchKernelGGL((scan_step_kernel<D, G>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, \
-                     static_cast<hipStream_t>(stream), a)
+  const int W = widest(C, 4, {{u, ldu, dtype}, {g, ldg, g_dtype}, {q, q ? ldq : 0, dtype}, {o, C, dtype}});
+  const int64_t blocks = (static_cast<int64_t>(n_active) * (C / W) + 255) / 256;
+  if (blocks > 0x7fffffff) {
+    set_error("sparse_gated_step: too many workgroups");
+    return SSLA_ERR_UNSUPPORTED;
+  }
+  const dim3 grid(static_cast<unsigned>(blocks)), block(256);
+  const hipStream_t st = static_cast<hipStream_t>(stream);
+#define SSLA_CALL(D, G)                                                                \
+  if (W == 4) hipLaunchKernelGGL((scan_step_kernel<D, G, 4>), grid, block, 0, st, a);   \
+  else hipLaunchKernelGGL((scan_step_kernel<D, G, 1>), grid, block, 0, st, a)
   SSLA_SCAN_TYPES(SSLA_CALL);
 #undef SSLA_CALL
   return launch_status("sparse_gated_step");
