@@ -12,12 +12,12 @@ sample and the ``C / num_groups`` channels of a group, applies the channels'
 weight and bias and an activation, in one pass over the data where a sample
 fits on the chip.  With one group per head it is the norm behind a linear
 attention's output (``[T, H * V]``: every row is a sample; an output gate of a
-second tensor is a product of its own behind it); with ``[B, Hg, Wg, C]`` it is
-the norm of dense event grids.  None of them has a counterpart in the reference, whose
+second tensor is :func:`gated_norm`'s); with ``[B, Hg, Wg, C]`` it is the norm of
+dense event grids.  None of them has a counterpart in the reference, whose
 layers normalise with ``nn.LayerNorm`` (layers/mos_attention.py:101).
 
-The kernels are hand-written gfx950 kernels (``ssla_group_norm_fwd`` /
-``_bwd``); there is no CPU fallback.
+The kernels are hand-written gfx950 kernels (``ssla_group_norm_*``,
+``ssla_gated_norm_*``, ``ssla_residual_norm_*``); there is no CPU fallback.
 """
 from __future__ import annotations
 

@@ -442,3 +442,24 @@ def test_many_sequences(dev):
     check(dev, [1] * 1500, inputs([1] * 1500, 8, B16, F32, "log", seed=1), "log")
     lens = [0] * 2000 + [700] + [0] * 2000
     check(dev, lens, inputs(lens, 8, F32, F32, "value", seed=2), "value")
+
+
+def test_states_off_16_bytes(dev):
+    """Tables, initial states and gradients of final ones that begin at any 4-byte border."""
+    from ssla_amd.scan import gated_scan, sparse_gated_step
+    lens, C = [3, 0, 70, 1], 16
+    x = {n: t.to(dev) for n, t in inputs(lens, C, F32, F32, "sigmoid", seed=7).items()}
+    cu = offsets(lens).to(dev)
+
+    def off(t):
+        return torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+
+    def run(lay):
+        leaves = [x[n].clone().requires_grad_() for n in ("u", "g")] + [lay(x["h0"]).requires_grad_()]
+        out = gated_scan(leaves[0], leaves[1], cu, gate="sigmoid", initial_state=leaves[2], output_final_state=True)
+        return *out, *torch.autograd.grad(out, leaves, (x["do"], lay(x["dht"])))
+
+    assert all(torch.equal(a, b) for a, b in zip(run(off), run(torch.clone)))
+    at, tables = torch.tensor([0, 2], device=dev), [off(x["h0"]), x["h0"].clone()]
+    outs = [sparse_gated_step(at, x["u"][:2], x["g"][:2], t, gate="sigmoid") for t in tables]
+    assert torch.equal(*outs) and torch.equal(*tables)
