@@ -407,8 +407,8 @@ int ssla_diag_scan_bwd(const float *dout, const float *g, const float *h,
  * the forward fills for the backward.  The backward takes dout [T, C] and dht
  * (fp32 [n_seq, C] or NULL) and writes du, dq (dtype; dq only with q), dg
  * (g_dtype), all [T, C], and dh0 (fp32 [n_seq, C], may be NULL).
- * Workspace: ssla_gated_scan_workspace_size bytes, 16-byte aligned, no
- * initialisation, one for each call in flight; 0: none. */
+ * At most 2^30 sequences.  Workspace: ssla_gated_scan_workspace_size bytes, 16-byte
+ * aligned, no initialisation, one for each call in flight; 0: none. */
 enum { SSLA_GATE_VALUE = 0, SSLA_GATE_LOG = 1, SSLA_GATE_SIGMOID = 2 };
 size_t ssla_gated_scan_workspace_size(int64_t T, int C);
 size_t ssla_gated_scan_keep_size(int64_t T, int C);

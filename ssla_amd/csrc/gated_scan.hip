@@ -738,7 +738,8 @@ int check_sizes(const char *what, int n_seq, int64_t T, int C, int gate, int dty
     set_error("%s: rows of more than %d values, or that far apart", what, kMostWidth);
     return SSLA_ERR_UNSUPPORTED;
   }
-  if (T > (1ll << 40) / C || static_cast<int64_t>(n_seq) * C > (1ll << 38)) {
+  // (the kernels add sequences, tiles and threads in 32 bits)
+  if (T > (1ll << 40) / C || static_cast<int64_t>(n_seq) * C > (1ll << 38) || n_seq > 1 << 30) {
     set_error("%s: too many values", what);
     return SSLA_ERR_UNSUPPORTED;
   }
@@ -809,7 +810,7 @@ int launch_scan(const char *what, ScanArgs &a, int W, int R, Kernel kernel, void
     set_error("%s: needs %zu bytes of workspace, got %zu", what, ws_bytes(a.T, a.C), workspace_bytes);
     return SSLA_ERR_WORKSPACE;
   }
-  if (p.tiles * p.cblocks > 0x7fffffff) {
+  if (p.tiles * p.cblocks > 0x3fffffff) {
     set_error("%s: too many workgroups", what);
     return SSLA_ERR_UNSUPPORTED;
   }

@@ -192,7 +192,7 @@ def gated_scan(
     dev = _lib.require_cuda(u, g, q, initial_state)
     cu = _offsets(name, cu_seqlens, dev)
     N, C = cu.numel() - 1, u.shape[1]
-    if N > 0x7fffffff:
+    if N > 1 << 30:
         raise NotImplementedError(f"{name}: too many sequences ({N})")
     if initial_state is not None and (initial_state.shape != (N, C) or not initial_state.is_floating_point()):
         raise ValueError(f"{name}: initial_state must be floating point {(N, C)}, got {tuple(initial_state.shape)} "
@@ -219,7 +219,7 @@ def sparse_gated_step(site_idx: torch.Tensor, u: torch.Tensor, g: torch.Tensor, 
     name = "sparse_gated_step"
     _gated_args(name, u, g, q, gate)
     n, C = u.shape
-    if n > 0x7fffffff:
+    if n > 1 << 30:
         raise NotImplementedError(f"{name}: too many rows ({n})")
     if state.dim() != 2 or state.shape[1] != C or state.dtype != torch.float32 or not state.is_contiguous():
         raise ValueError(f"{name}: state must be contiguous fp32 [n_sites, {C}]")

@@ -93,3 +93,13 @@ def test_tables_refuse():
     for state in (torch.zeros(9, 7), torch.zeros(9, 6).half(), torch.zeros(6, 9).t(), torch.zeros(9, 6, 1)):
         with pytest.raises(ValueError, match="contiguous fp32"):
             sparse_gated_step(torch.arange(4), x, x, state)
+
+
+def test_entries_refuse_more_sequences_than_they_count():
+    lib = _lib.load()
+    n = (1 << 30) + 1
+    assert lib.ssla_gated_scan_fwd(16, 8, 16, 8, None, 0, 16, n, 4, 8, 0, None, 16, None, None, 0, 0, None, 0,
+                                   None) == _lib.SSLA_ERR_UNSUPPORTED
+    assert lib.ssla_gated_scan_bwd(16, 8, 16, 8, None, 0, 16, n, 4, 8, 0, None, 16, 16, None, 16, 16, None, None, 0, 0, None, 0,
+                                   None) == _lib.SSLA_ERR_UNSUPPORTED
+    assert lib.ssla_sparse_gated_step(16, n, 16, 8, 16, 8, None, 0, 16, 5, 8, 0, 16, None, 0, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
