@@ -487,3 +487,23 @@ def test_sums_over_rows_count_every_row_once(dev, N, C, G, dtype):
                          post_weight=leaves[1])
     for name, got in zip(("dgamma", "dw2"), torch.autograd.grad(s, leaves, d.to(dev))):
         same(name, got, dw)
+
+
+def test_rows_past_32_bits(dev):
+    """Behind 2^31 values a tensor rows are read, written, normalised and dropped at their own
+    places: the last are those of a short call on them alone, in both directions."""
+    from ssla_amd.norm import gated_norm, residual_norm
+    N, C, last = (1 << 21) + 9, 1024, slice(-16, None)
+    gen = torch.Generator(device=dev).manual_seed(0)
+    x, r, d = (torch.randn(N, C, generator=gen, device=dev, dtype=B16) for _ in range(3))
+    x.requires_grad_(), r.requires_grad_()
+    for form in (lambda a, b: (gated_norm(a, b, 8),), lambda a, b: residual_norm(a, b, post_norm=True)):
+        def run(*rows):
+            out = form(*rows[:2])
+            return *(o.detach() for o in out), *torch.autograd.grad(out, rows[:2], (rows[2],) * len(out))
+        part = run(*(t.detach()[last].clone().requires_grad_() for t in (x, r)), d[last])
+        for a, b in zip(run(x, r, d), part):
+            assert torch.equal(a[last], b)
+    _, s = residual_norm(x.detach(), torch.zeros_like(r), p=0.25, seed=11, subsequence=3)
+    keep = block.dropout_keep(16 * C, 0.25, 11, 3, first=(N - 16) * C).view(16, C)
+    assert torch.equal(s[last].cpu() != 0, keep & (x.detach()[last].cpu() != 0))

@@ -463,3 +463,30 @@ def test_states_off_16_bytes(dev):
     at, tables = torch.tensor([0, 2], device=dev), [off(x["h0"]), x["h0"].clone()]
     outs = [sparse_gated_step(at, x["u"][:2], x["g"][:2], t, gate="sigmoid") for t in tables]
     assert torch.equal(*outs) and torch.equal(*tables)
+
+
+@pytest.mark.parametrize("dt", [F32, B16])
+def test_steps_in_a_graph(dev, dt):
+    """A single token's step captured once and replayed: the table goes on from replay to
+    replay, with other tokens and other rows, as in eager steps."""
+    from ssla_amd.scan import sparse_gated_step
+    rows, n, C = 50, 9, 40
+    gen = torch.Generator().manual_seed(2)
+    tokens = [[torch.randn(n, C, generator=gen).to(dev, dt) for _ in range(3)] for _ in range(5)]
+    sites = [torch.randperm(rows, generator=gen)[:n].sort().values.int().to(dev) for _ in range(5)]
+    u, g, q = (t.clone() for t in tokens[0])
+    at, state = sites[0].clone(), torch.zeros(rows, C, device=dev)
+    sparse_gated_step(at, u, g, state, q=q, gate="sigmoid")
+    state.zero_()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = sparse_gated_step(at, u, g, state, q=q, gate="sigmoid")
+    table = torch.zeros_like(state)
+    for i, (x, idx) in enumerate(zip(tokens, sites)):
+        for to, t in zip((u, g, q, at), (*x, idx)):
+            to.copy_(t)
+        graph.replay()
+        want = sparse_gated_step(idx, x[0], x[1], table, q=x[2], gate="sigmoid")
+        torch.cuda.synchronize()
+        assert torch.equal(o, want) and torch.equal(state, table), i
