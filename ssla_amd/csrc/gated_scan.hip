@@ -16,6 +16,8 @@
 // from the tiles before: the nearest one whose leaving state is known, and the maps
 // from there on, applied in their order, so the result does not depend on which
 // were known.  A tile with a sequence's start publishes its leaving state at once.
+// Over few channels, where long chains of tiles run at once, 16 tiles are a span that
+// publishes a map and a state of its own (262,144 rows of 64 channels 58 us, without 95).
 // Tiles are handed out in order by a ticket and publish before they wait, so every
 // tile waited for has started and the wait ends.  A word says by itself whether it
 // is there, a map or a state: no fences.
@@ -87,8 +89,8 @@ struct ScanArgs {
   int CT, RG, cblocks;            // lanes of a row, row groups, channel blocks
   int tiles;                      // of rows
   uint32_t *ticket;               // NULL: one tile of rows
-  uint64_t *words;                // [tiles][cblocks CT W]: what a tile says of itself
-  uint32_t *hints;                // [cblocks][tiles]
+  uint64_t *words, *span_words;   // [tiles], [spans][cblocks CT W]: what a tile (spans of more), a span says of itself
+  uint32_t *hints;                // [cblocks][spans]
 };
 
 // ------------------------------------------------------- tiles and sequences --
@@ -182,14 +184,14 @@ __device__ __forceinline__ float apply(uint64_t w, float x) {
   return is_state(w) ? U : apply(__uint_as_float(static_cast<uint32_t>(w)), x, U);
 }
 
-// What a tile has published in a channel block, told by a word of its own next to its
-// neighbours': a wavefront sees 64 tiles at one read.  Only a hint where to look:
-// the words say by themselves whether they are there.
+// What the last tile of a span has published of it in a channel block, told by a word of
+// its own next to its neighbours': a wavefront sees 64 spans at one read.  Only a hint
+// where to look: the words say by themselves whether they are there.
 constexpr uint32_t kNoHint = ~0u, kMapHint = 1, kStateHint = 2;
 
-// The nearest tile before k > 0 whose state is known, with maps from there on; for a
+// The nearest span before k > 0 whose state is known, with maps from there on; for a
 // whole wavefront.
-__device__ __forceinline__ int known_tile(const uint32_t *hints, int k) {
+__device__ __forceinline__ int known_span(const uint32_t *hints, int k) {
   const int lane = threadIdx.x & 63;
   for (int near = k - 1;;) {
     const int t = near - lane;
@@ -197,7 +199,7 @@ __device__ __forceinline__ int known_tile(const uint32_t *hints, int k) {
     const uint64_t states = __ballot(h == kStateHint), nothing = __ballot(h == kNoHint);
     const int s = states ? __builtin_ctzll(states) : 64, n = nothing ? __builtin_ctzll(nothing) : 64;
     if (s < n) return near - s;
-    if (n == 64) near -= 64;   // (tile 0 is known or not there: it stays at 0 or above)
+    if (n == 64) near -= 64;   // (span 0 is known or not there: it stays at 0 or above)
     else __builtin_amdgcn_s_sleep(1);
   }
 }
@@ -244,10 +246,11 @@ __device__ __forceinline__ void enter_groups(const float *A, float *U, const int
   }
 }
 // What the threads share between a tile's maps.
-constexpr int kWords = 64;   // tiles of a round trip
+constexpr int kSpanLog2 = 4, kSpan = 1 << kSpanLog2;   // tiles of a span, where there is more than one
+constexpr int kWords = 48;   // spans of a round trip
 struct TileSmem {
   float A[kMostValues], U[kMostValues];
-  uint64_t words[kWords * kMostLanes * 4];
+  uint64_t words[(kSpan + kWords) * kMostLanes * 4];
   int mark[kMostGroups * kMostRows], fin[kMostGroups * kMostRows], cut[kMostGroups];
   int flags[kBlock];
   int from;
@@ -257,7 +260,11 @@ struct TileSmem {
 // Between a tile's maps, for the whole workgroup: publishes, finds the entering states
 // (`closed`: the tile's first row takes none) and fills U.  The threads from `first` on
 // have a channel each; all of them fetch the words.
-template <bool BACK>
+//
+// 2^SPAN tiles are a span.  Its last tile joins their maps to the span's; the states behind
+// spans come of the states before and the spans' maps, those inside a span of the state
+// before it and its tiles' maps, always in this order: the same bits whoever is first.
+template <bool BACK, int SPAN>
 __device__ __forceinline__ void enter_tile(const ScanArgs &a, TileSmem &sm, float *U, int k, int cb, bool closed, int cw,
                                            int first) {
   const int tid = threadIdx.x, c = tid - first, mine = a.C - cb * cw;   // (channels that exist)
@@ -265,61 +272,95 @@ __device__ __forceinline__ void enter_tile(const ScanArgs &a, TileSmem &sm, floa
   float x = 0.f;
   if (a.ticket) {
     const int64_t wide = static_cast<int64_t>(a.cblocks) * cw;
-    uint64_t *words = a.words + static_cast<int64_t>(cb) * cw;
-    uint32_t *hints = a.hints + static_cast<int64_t>(cb) * a.tiles;
+    const int s = k >> SPAN, in = k - (s << SPAN);
+    const bool last = in + 1 == 1 << SPAN, open = k > 0 && !closed;
+    uint64_t *words = a.words + static_cast<int64_t>(cb) * cw, *above = a.span_words + static_cast<int64_t>(cb) * cw;
+    uint64_t *span = above + s * wide;
+    uint32_t *hints = a.hints + static_cast<int64_t>(cb) * (a.tiles >> SPAN);   // (of the whole spans)
+    // the words of n tiles or spans, from slot `at` on
+    auto fetch = [&](const uint64_t *from, int n, int at, bool state) {
+      const int per = kBlock / cw, i0 = tid / cw, cc = tid - i0 * cw;
+      if (i0 < per && cc < mine)
+        for (int i = i0; i < n; i += 4 * per) {
+          uint64_t w[4];
+          bool there;
+          do {   // (a word may come after its hint)
+            there = true;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int t = i + e * per;
+              w[e] = t < n ? look(from + t * wide + cc) : 0;
+              there = there && w[e] != kNone && (t > 0 || !state || is_state(w[e]));
+            }
+          } while (!there);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (i + e * per < n) sm.words[(at + i + e * per) * cw + cc] = w[e];
+        }
+      __syncthreads();
+    };
+    auto pass = [&](int at, int n) {   // x through n words
+      for (int i = 0; i < n; i += 8) {   // (eight reads on their way at once)
+        uint64_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = sm.words[(at + min(i + e, n - 1)) * cw + c];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (i + e < n) x = apply(w[e], x);
+      }
+    };
     bool known = k == 0;
     Joined j{0.f, 0.f};
     if (c >= 0 && c < 64) {   // (a whole wavefront)
       known |= __any(c < a.RG && sm.cut[c] != 0);
       if (on) {
         j = join_groups<BACK>(sm.A, U, sm.cut, a.RG, cw, c);
-        show(words + k * wide + c, known ? state_word(j.U) : map_word(j.A, j.U));
+        const uint64_t w = known ? state_word(j.U) : map_word(j.A, j.U);
+        if (SPAN > 0) show(words + k * wide + c, w);
+        if (last && (known || SPAN == 0)) show(span + c, w);
       }
-      if (c == 0) show(hints + k, known ? kStateHint : kMapHint);
+      if (last && (known || SPAN == 0) && c == 0) show(hints + s, known ? kStateHint : kMapHint);
     }
     asm volatile("" ::: "memory");   // (published before anything is waited for)
-    if (k > 0 && !closed) {
+    if (open) {
+      if (SPAN > 0 && in > 0) fetch(words + (k - in) * wide, in, 0, false);
       if (c >= 0 && c < 64) {
-        const int from = known_tile(hints, k);
+        bool cut = false;   // (the same for all channels)
+        if (SPAN > 0 && on && last) {
+          Joined m{1.f, 0.f};
+          for (int i = 0; i < in; ++i) {
+            const uint64_t w = sm.words[i * cw + c];
+            cut |= is_state(w);
+            m.U = apply(w, m.U);
+            m.A *= __uint_as_float(static_cast<uint32_t>(w));
+          }
+          j = {m.A * j.A, apply(j.A, m.U, j.U)};
+        } else if (SPAN > 0 && on) {
+          for (int i = 0; i < in; ++i) cut |= is_state(sm.words[i * cw + c]);
+        }
+        if (SPAN > 0) cut = __any(cut);
+        if (SPAN > 0 && last && !known) {
+          if (on) show(span + c, cut ? state_word(j.U) : map_word(j.A, j.U));
+          if (c == 0) show(hints + s, cut ? kStateHint : kMapHint);
+        }
+        known |= cut;
+        const int from = cut ? -1 : known_span(hints, s);
         if (c == 0) sm.from = from;
       }
       __syncthreads();
-      const int per = kBlock / cw, i0 = tid / cw, cc = tid - i0 * cw, from = __builtin_amdgcn_readfirstlane(sm.from);
-      for (int at = from; at < k; at += kWords) {
-        const int n = min(k - at, kWords);
-        if (i0 < per && cc < mine)
-          for (int i = i0; i < n; i += 4 * per) {
-            uint64_t w[4];
-            bool there;
-            do {   // (a word may come after its hint)
-              there = true;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int t = i + e * per;
-                w[e] = t < n ? look(words + (at + t) * wide + cc) : 0;
-                there = there && w[e] != kNone && (t > 0 || at > from || is_state(w[e]));
-              }
-            } while (!there);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (i + e * per < n) sm.words[(i + e * per) * cw + cc] = w[e];
-          }
-        __syncthreads();
-        if (on)
-          for (int i = 0; i < n; i += 8) {   // (eight reads on their way at once)
-            uint64_t w[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) w[e] = sm.words[min(i + e, n - 1) * cw + c];
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (i + e < n) x = apply(w[e], x);
-          }
-        __syncthreads();
+      const int from = __builtin_amdgcn_readfirstlane(sm.from);
+      if (from >= 0)
+        for (int at = from; at < s; at += kWords) {
+          const int n = min(s - at, kWords);
+          fetch(above + at * wide, n, kSpan, at == from);
+          if (on) pass(kSpan, n);
+          if (at + kWords < s) __syncthreads();
+        }
+      if (last && !known) {
+        if (on) show(span + c, state_word(apply(j.A, x, j.U)));
+        if (c == 0) show(hints + s, kStateHint);
       }
-    }
-    if (!known) {
-      if (on) show(words + k * wide + c, state_word(apply(j.A, x, j.U)));
-      if (c == 0) show(hints + k, kStateHint);
+      if (SPAN > 0 && on && in > 0) pass(0, in);
     }
   }
   if (on) enter_groups<BACK>(sm.A, U, sm.cut, a.RG, cw, c, x);
@@ -408,7 +449,7 @@ __device__ __forceinline__ void empty_states(const ScanArgs &a, const float *fro
 // ------------------------------------------------------------------ forward --
 // Two workgroups a CU (128 registers) in 16 bits; fp32 values do without the second one
 // sooner than without registers (8 x 4,096 rows: 130 us, 162 at 128 registers).
-template <int DT, int DTG, int W, bool READ>
+template <int DT, int DTG, int W, bool READ, int SPAN>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(DT == SSLA_F32 ? 2 : 4))) void scan_fwd_kernel(const ScanArgs a) {
   constexpr int R = kFwdRows, B = 4;   // B: rows whose states are read at once
   __shared__ TileSmem sm;
@@ -475,7 +516,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(DT == SS
     if (cl == 0) sm.cut[rg] = reset;
   }
   __syncthreads();
-  enter_tile<false>(a, sm, sm.U, k, cb, some && sm.mark[0] != kInside, cw, 0);
+  enter_tile<false, SPAN>(a, sm, sm.U, k, cb, some && sm.mark[0] != kInside, cw, 0);
   __syncthreads();
   as_read(u);
   if constexpr (READ) as_read(q);
@@ -531,7 +572,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(DT == SS
 }
 
 // ----------------------------------------------------------------- backward --
-template <int DT, int DTG, int W, bool READ>
+template <int DT, int DTG, int W, bool READ, int SPAN>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) void scan_bwd_kernel(const ScanArgs a) {
   constexpr int R = kBwdRows;
   static_assert(R == 4, "rows whose states are read at once");
@@ -617,7 +658,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) voi
   __syncthreads();
   // the first threads take the states forward, those from half on the gradients back
   if (tid < cw && cb * cw + tid < a.C) enter_groups<false>(sm.A, sm.U, sm.cut, a.RG, cw, tid, entering);
-  enter_tile<true>(a, sm, sE, back, cb, some && (sm.mark[rows - 1] == kOutside || sm.fin[rows - 1] >= 0), cw, kBlock / 2);
+  enter_tile<true, SPAN>(a, sm, sE, back, cb, some && (sm.mark[rows - 1] == kOutside || sm.fin[rows - 1] >= 0), cw, kBlock / 2);
   __syncthreads();
   as_read(u);
   as_read(d);
@@ -757,7 +798,7 @@ int check_sizes(const char *what, int n_seq, int64_t T, int C, int gate, int dty
 // row, as many row groups as a workgroup has room for (a power of two, so that a
 // tile is a multiple of kKeepRows rows).
 struct ScanPlan {
-  int CT, RG, cblocks;
+  int CT, RG, cblocks, span;
   int64_t tiles;
 };
 ScanPlan plan_of(int64_t T, int C, int W, int R) {
@@ -768,11 +809,17 @@ ScanPlan plan_of(int64_t T, int C, int W, int R) {
   p.RG = kKeepRows / R;
   while (2 * p.RG * p.CT <= kBlock && p.RG < kMostGroups) p.RG *= 2;
   p.tiles = std::max<int64_t>(1, (T + p.RG * R - 1) / (p.RG * R));
+  // Some 512 workgroups run at once.  Over few channel blocks that is a long chain of tiles
+  // each, which spans shorten (one sequence, spans of 16 against 1: 262,144 rows of 64 channels
+  // 58 us, 95; 65,536 of 96 31, 42; of 256 55, 55); over more blocks spans are one wait more
+  // (65,536 of 1,024 139, 133; 16,384 of 512 32, 30).
+  p.span = p.cblocks <= 4 ? kSpanLog2 : 0;
   return p;
 }
 constexpr size_t kHead = 256;   // the ticket's line
 int64_t word_count(const ScanPlan &p, int W) {   // words and hints
-  return p.tiles * p.cblocks * p.CT * W + (p.tiles * p.cblocks + 1) / 2;
+  const int64_t spans = p.tiles >> p.span;
+  return ((p.span ? p.tiles : 0) + spans) * p.cblocks * p.CT * W + (spans * p.cblocks + 1) / 2;
 }
 size_t ws_bytes(int64_t T, int C) {   // whatever vectors the addresses allow
   int64_t most = 0;
@@ -801,9 +848,9 @@ int widest(int C, int most, std::initializer_list<Rows> all) {
   return 1;
 }
 
-// Sets the plan, clears the words and launches `kernel`.
+// Sets the plan, clears the words and launches `kernel`, or `spans` where there are any.
 template <typename Kernel>
-int launch_scan(const char *what, ScanArgs &a, int W, int R, Kernel kernel, void *workspace, size_t workspace_bytes, hipStream_t st) {
+int launch_scan(const char *what, ScanArgs &a, int W, int R, Kernel kernel, Kernel spans, void *workspace, size_t workspace_bytes, hipStream_t st) {
   const ScanPlan p = plan_of(a.T, a.C, W, R);
   const size_t need = p.tiles > 1 ? kHead + static_cast<size_t>(word_count(p, W)) * 8 : 0;
   if (need && !(workspace && workspace_bytes >= need && aligned(workspace, 16))) {
@@ -818,12 +865,14 @@ int launch_scan(const char *what, ScanArgs &a, int W, int R, Kernel kernel, void
   if (need) {
     const int64_t n = word_count(p, W);
     a.ticket = static_cast<uint32_t *>(workspace);
+    const int64_t wide = static_cast<int64_t>(p.cblocks) * p.CT * W;
     a.words = reinterpret_cast<uint64_t *>(static_cast<char *>(workspace) + kHead);
-    a.hints = reinterpret_cast<uint32_t *>(a.words + p.tiles * p.cblocks * p.CT * W);
+    a.span_words = a.words + (p.span ? p.tiles * wide : 0);
+    a.hints = reinterpret_cast<uint32_t *>(a.span_words + (p.tiles >> p.span) * wide);
     hipLaunchKernelGGL(scan_clear_kernel, dim3(static_cast<unsigned>(std::min<int64_t>((n + 1023) / 1024, 2048))), dim3(256), 0,
                        st, a.ticket, a.words, n);
   }
-  hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(p.tiles * p.cblocks)), dim3(kBlock), 0, st, a);
+  hipLaunchKernelGGL(need && p.span ? spans : kernel, dim3(static_cast<unsigned>(p.tiles * p.cblocks)), dim3(kBlock), 0, st, a);
   return SSLA_OK;
 }
 
@@ -854,8 +903,10 @@ extern "C" int ssla_gated_scan_fwd(const void *u, int64_t ldu, const void *g, in
   const hipStream_t st = static_cast<hipStream_t>(stream);
   int status = SSLA_OK;
 #define SSLA_LAUNCH(D, G, W_) \
-  status = q ? launch_scan("gated_scan_fwd", a, W_, kFwdRows, scan_fwd_kernel<D, G, W_, true>, workspace, workspace_bytes, st) \
-             : launch_scan("gated_scan_fwd", a, W_, kFwdRows, scan_fwd_kernel<D, G, W_, false>, workspace, workspace_bytes, st)
+  status = q ? launch_scan("gated_scan_fwd", a, W_, kFwdRows, scan_fwd_kernel<D, G, W_, true, 0>, scan_fwd_kernel<D, G, W_, true, kSpanLog2>,    \
+                           workspace, workspace_bytes, st)                                                                         \
+             : launch_scan("gated_scan_fwd", a, W_, kFwdRows, scan_fwd_kernel<D, G, W_, false, 0>, scan_fwd_kernel<D, G, W_, false, kSpanLog2>, \
+                           workspace, workspace_bytes, st)
 #define SSLA_CALL(D, G)             \
   if (W == 4) SSLA_LAUNCH(D, G, 4); \
   else SSLA_LAUNCH(D, G, 1)
@@ -886,8 +937,10 @@ extern "C" int ssla_gated_scan_bwd(const void *u, int64_t ldu, const void *g, in
   const hipStream_t st = static_cast<hipStream_t>(stream);
   int status = SSLA_OK;
 #define SSLA_LAUNCH(D, G, W_) \
-  status = q ? launch_scan("gated_scan_bwd", a, W_, kBwdRows, scan_bwd_kernel<D, G, W_, true>, workspace, workspace_bytes, st) \
-             : launch_scan("gated_scan_bwd", a, W_, kBwdRows, scan_bwd_kernel<D, G, W_, false>, workspace, workspace_bytes, st)
+  status = q ? launch_scan("gated_scan_bwd", a, W_, kBwdRows, scan_bwd_kernel<D, G, W_, true, 0>, scan_bwd_kernel<D, G, W_, true, kSpanLog2>,    \
+                           workspace, workspace_bytes, st)                                                                         \
+             : launch_scan("gated_scan_bwd", a, W_, kBwdRows, scan_bwd_kernel<D, G, W_, false, 0>, scan_bwd_kernel<D, G, W_, false, kSpanLog2>, \
+                           workspace, workspace_bytes, st)
 #define SSLA_CALL(D, G)             \
   if (W == 4) SSLA_LAUNCH(D, G, 4); \
   else SSLA_LAUNCH(D, G, 1)

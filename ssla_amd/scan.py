@@ -182,10 +182,10 @@ def gated_scan(
 
     States are fp32; a long sequence is cut along time and the pieces' states are
     joined in their order, so results do not vary from call to call.  Over a piece
-    (up to 512 rows) the gates are multiplied: factors larger than 1 in magnitude
-    hold while such a product stays inside fp32.  Differentiable in u, g, q and the
-    initial state (once, in reverse mode: forward-mode tangents are refused).  Makes
-    no host sync."""
+    (up to 512 rows; 8,192 of up to 256 channels) the gates are multiplied: factors
+    larger than 1 in magnitude hold while such a product stays inside fp32.
+    Differentiable in u, g, q and the initial state (once, in reverse mode:
+    forward-mode tangents are refused).  Makes no host sync."""
     name = "gated_scan"
     _gated_args(name, u, g, q, gate)
     _lib.require_no_tangent(name, u, g, q, initial_state)

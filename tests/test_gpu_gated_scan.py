@@ -490,3 +490,32 @@ def test_steps_in_a_graph(dev, dt):
         want = sparse_gated_step(idx, x[0], x[1], table, q=x[2], gate="sigmoid")
         torch.cuda.synchronize()
         assert torch.equal(o, want) and torch.equal(state, table), i
+
+
+# sequences over many tiles of narrow rows: one, ends on and beside powers of two, short ones between
+@pytest.mark.parametrize("dt,dtg", [(F32, F32), (B16, F32)])
+@pytest.mark.parametrize("lens,C", [([70000], 4), ([8192, 8191, 16385, 1, 0, 20000], 20), ([3, 30000, 0, 2], 7),
+                                    ([1000, 12000], 200)], ids=lambda x: str(x).replace(" ", ""))
+def test_long_narrow(dev, lens, C, dt, dtg):
+    check(dev, lens, inputs(lens, C, dt, dtg, "sigmoid", seed=C), "sigmoid")
+
+
+def test_long_narrow_the_same_every_time(dev):
+    """Gates near 1, so that every state reaches far: repeated calls give the same bits, and
+    offsets that are not in order still end."""
+    from ssla_amd.scan import gated_scan
+    T, C = 200000, 24
+    gen = torch.Generator().manual_seed(8)
+    u, do = (torch.randn(T, C, generator=gen).to(dev) for _ in range(2))
+    u.requires_grad_()
+    g = (torch.randn(T, C, generator=gen) + 9).to(dev).requires_grad_()
+    bad = torch.tensor([0, 150000, 20, 199999, 100000, 7, T], device=dev)
+    want = None
+    for i in range(6):
+        o, ht = gated_scan(u, g, torch.tensor([0, T], device=dev), gate="sigmoid", output_final_state=True)
+        got = o.detach(), ht.detach(), *torch.autograd.grad(o, (u, g), do)
+        if want is not None:
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+        want = got
+        gated_scan(u.detach(), g.detach(), bad, gate="sigmoid", output_final_state=True)
+    torch.cuda.synchronize()
