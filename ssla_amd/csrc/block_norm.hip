@@ -223,11 +223,16 @@ __device__ __forceinline__ void normalise_back(float (&h)[NV][W], const float (&
 
 // Adds the workgroup's sums over rows and leaves them in rows of a.part ([rows][KINDS][C]):
 // a row a workgroup, or a row a slot where a workgroup has not all groups of channels.
+// Lane groups of one group of channels are G apart.  Four or more are added up by all threads,
+// a sum each, fewer by the first lane group for its own channels (forward and backward,
+// us, the first against the second: 16,384 rows of 4 groups of 16 channels 19, 40;
+// 32,768 rows of 1,024 221, 214).
 template <int W, int NV, bool FULL, int KINDS>
 __device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV, FULL> &l, const float (&sum)[KINDS][NV][W], float *sm) {
   const int lanes = blockDim.x, groups = lanes / a.S, mine = threadIdx.x / a.S;   // lane groups
   const bool all = a.G <= groups;
   const int64_t to = all ? static_cast<int64_t>(blockIdx.x) : l.row;
+  const int own = a.G * a.S;   // lanes before the first group of channels comes again
 #pragma unroll
   for (int k = 0; k < KINDS; ++k) {
     __syncthreads();
@@ -236,8 +241,17 @@ __device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV, 
 #pragma unroll
       for (int e = 0; e < W; ++e) sm[(e * NV + i) * lanes + threadIdx.x] = l.has[i] ? sum[k][i][e] : 0.f;
     __syncthreads();
-    // lane groups of one group of channels are G apart: the first adds them up
-    if (mine < a.G && (all || l.on))
+    if (4 * own <= lanes) {
+      for (int o = threadIdx.x; o < own * W * NV; o += lanes) {
+        const uint32_t v = static_cast<uint32_t>(o) / own, at = o - v * own, q = at / a.S, j = at - q * a.S;
+        const uint32_t g = (blockIdx.x * groups + q) % a.G, c = (j + a.S * (v % NV)) * W + v / NV;
+        if (c >= static_cast<uint32_t>(a.per)) continue;
+        float t = 0.f;
+#pragma unroll 8
+        for (int x = at; x < lanes; x += own) t += sm[v * lanes + x];
+        a.part[(to * KINDS + k) * a.C + g * a.per + c] = t;
+      }
+    } else if (mine < a.G && (all || l.on)) {
 #pragma unroll
       for (int i = 0; i < NV; ++i)
 #pragma unroll
@@ -247,6 +261,7 @@ __device__ __forceinline__ void leave_sums(const RowArgs &a, const Place<W, NV, 
             for (int q = mine; q < groups; q += a.G) t += sm[(e * NV + i) * lanes + q * a.S + l.j];
             a.part[(to * KINDS + k) * a.C + l.c[i] + e] = t;
           }
+    }
   }
 }
 
