@@ -558,7 +558,7 @@ struct RowPlan {
 // Wavefronts: the forward's lane groups have a few rows each, the backward's as many as
 // run at once (three workgroups a CU, of wide rows one): their sums over rows go through
 // memory once a workgroup.
-constexpr int64_t kFwdWaves = 8192, kBwdWaves[3] = {3072, 2048, 4096};   // (of 256, 512, 1,024 threads)
+constexpr int64_t kFwdWaves = 256 * 32, kBwdWaves[3] = {256 * 12, 256 * 8, 256 * 16};   // (256 CUs; workgroups of 256, 512, 1,024 threads)
 
 RowPlan plan_of(int64_t N, int per, int G, int W, int dtype, bool bwd) {   // W 0: no vectors
   RowPlan p{};
