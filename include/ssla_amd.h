@@ -407,6 +407,8 @@ int ssla_diag_scan_bwd(const float *dout, const float *g, const float *h,
  * the forward fills for the backward.  The backward takes dout [T, C] and dht
  * (fp32 [n_seq, C] or NULL) and writes du, dq (dtype; dq only with q), dg
  * (g_dtype), all [T, C], and dh0 (fp32 [n_seq, C], may be NULL).
+ * An infinite state (or gradient) goes on with the gates' signs until a gate of 0 makes
+ * it NaN, as row by row.
  * At most 2^30 sequences.  Workspace: ssla_gated_scan_workspace_size bytes, 16-byte
  * aligned, no initialisation, one for each call in flight; 0: none. */
 enum { SSLA_GATE_VALUE = 0, SSLA_GATE_LOG = 1, SSLA_GATE_SIGMOID = 2 };

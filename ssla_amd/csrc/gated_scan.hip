@@ -176,6 +176,13 @@ template <typename T>
 __device__ __forceinline__ void show(T *p, T x) {
   __hip_atomic_store(p, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// A product of gates too small for fp32, none of them 0, is held as +-2^-149 (kFaded: its
+// bits): an infinite state goes on, a finite one is off by 2^-149 of itself at most.
+constexpr uint32_t kFaded = 1;
+// The product A of factors; zero: one of them is 0.
+__device__ __forceinline__ float settled(float A, bool zero) {
+  return A == 0.f && !zero ? __uint_as_float((__float_as_uint(A) & 0x80000000u) | kFaded) : A;
+}
 // (a factor that overflowed must not meet a state of zero)
 __device__ __forceinline__ float apply(float A, float x, float U) { return x == 0.f ? U : fmaf(A, x, U); }
 // The state behind a tile that x enters: the same bits whichever of its words was there.
@@ -252,7 +259,7 @@ struct TileSmem {
   float A[kMostValues], U[kMostValues];
   uint64_t words[(kSpan + kWords) * kMostLanes * 4];
   int mark[kMostGroups * kMostRows], fin[kMostGroups * kMostRows], cut[kMostGroups];
-  int flags[kBlock];
+  int flags[kBlock];   // of a channel: one of its gates is 0; later of empty_states
   int from;
   uint32_t slot;
 };
@@ -315,6 +322,7 @@ __device__ __forceinline__ void enter_tile(const ScanArgs &a, TileSmem &sm, floa
       known |= __any(c < a.RG && sm.cut[c] != 0);
       if (on) {
         j = join_groups<BACK>(sm.A, U, sm.cut, a.RG, cw, c);
+        j.A = settled(j.A, sm.flags[c]);
         const uint64_t w = known ? state_word(j.U) : map_word(j.A, j.U);
         if (SPAN > 0) show(words + k * wide + c, w);
         if (last && (known || SPAN == 0)) show(span + c, w);
@@ -328,13 +336,16 @@ __device__ __forceinline__ void enter_tile(const ScanArgs &a, TileSmem &sm, floa
         bool cut = false;   // (the same for all channels)
         if (SPAN > 0 && on && last) {
           Joined m{1.f, 0.f};
+          bool zero = j.A == 0.f;
           for (int i = 0; i < in; ++i) {
             const uint64_t w = sm.words[i * cw + c];
+            const float f = __uint_as_float(static_cast<uint32_t>(w));
             cut |= is_state(w);
             m.U = apply(w, m.U);
-            m.A *= __uint_as_float(static_cast<uint32_t>(w));
+            m.A *= f;
+            zero |= f == 0.f;
           }
-          j = {m.A * j.A, apply(j.A, m.U, j.U)};
+          j = {settled(m.A * j.A, zero), apply(j.A, m.U, j.U)};
         } else if (SPAN > 0 && on) {
           for (int i = 0; i < in; ++i) cut |= is_state(sm.words[i * cw + c]);
         }
@@ -398,6 +409,21 @@ __device__ __forceinline__ void each(F f) {
   for (int i = 0; i < R; ++i)
 #pragma unroll
     for (int e = 0; e < W; ++e) f(i, e);
+}
+// The products A of a lane's gates(i, e), and a flag for each channel with a gate of 0.
+// A product of 0 is rare enough to look at the gates again (a count of them in
+// join_groups, on every tile's way, is 1 % of a call).
+template <int R, int W, typename F>
+__device__ __forceinline__ void settle(float (&A)[W], int *zeros, F gates) {
+#pragma unroll
+  for (int e = 0; e < W; ++e)
+    if (A[e] == 0.f) {
+      bool zero = false;
+#pragma unroll
+      for (int i = 0; i < R; ++i) zero |= gates(i, e) == 0.f;
+      A[e] = settled(A[e], zero);
+      if (zero) zeros[e] = 1;
+    }
 }
 // W values of a row of states (fp32, at any 4-byte border).
 template <int W>
@@ -473,6 +499,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(DT == SS
   load_rows<DT, W, R>(u, a.u, r0, a.ldu, row, exist - 1, c);
   load_rows<DTG, W, R>(g, a.g, r0, a.ldg, row, exist - 1, c);
   if constexpr (READ) load_rows<DT, W, R>(q, a.q, r0, a.ldq, row, exist - 1, c);
+  if (tid < cw) sm.flags[tid] = 0;   // (mark_rows waits)
   const bool some = mark_rows(a, mine, all, r0, rows, sm.mark, sm.fin);
   float f[R][W];
   by_kind(a.gate, [&](auto kind) { each<R, W>([&](int i, int e) { f[i][e] = gate_value<kind()>(g[i][e]); }); });
@@ -508,6 +535,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(DT == SS
         }
       }
     }
+    settle<R, W>(A, sm.flags + cl * W, [&](int i, int e) { return f[i][e]; });
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       sm.A[rg * cw + cl * W + e] = A[e];
@@ -601,6 +629,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) voi
   if constexpr (READ) load_rows<DT, W, R>(q, a.q, r0, a.ldq, row, exist - 1, c);
   // (the forward left the state that enters the tile)
   const float entering = tid < cw && cb * cw + tid < a.C ? a.keep[r0 / kKeepRows * a.C + cb * cw + tid] : 0.f;
+  if (tid < cw) sm.flags[tid] = 0;   // (mark_rows waits)
   const bool some = mark_rows(a, mine, all, r0, rows, sm.mark, sm.fin);
   Gate f[R][W];
   auto grad_of = [&](int i, int e) { return READ ? d[i][e] * q[READ ? i : 0][e] : d[i][e]; };
@@ -647,6 +676,7 @@ __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(4))) voi
         }
       }
     }
+    settle<R, W>(A, sm.flags + cl * W, [&](int i, int e) { return f[i][e].a; });
 #pragma unroll
     for (int e = 0; e < W; ++e) {
       sm.A[rg * cw + cl * W + e] = A[e];

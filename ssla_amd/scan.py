@@ -184,6 +184,8 @@ def gated_scan(
     joined in their order, so results do not vary from call to call.  Over a piece
     (up to 512 rows; 8,192 of up to 256 channels) the gates are multiplied: factors
     larger than 1 in magnitude hold while such a product stays inside fp32.
+    An infinite state (or gradient) goes on with the gates' signs until a gate of 0
+    (logarithms and logits below about -87 are 0 in fp32) makes it NaN, as row by row.
     Differentiable in u, g, q and the initial state (once, in reverse mode:
     forward-mode tangents are refused).  Makes no host sync."""
     name = "gated_scan"

@@ -519,3 +519,36 @@ def test_long_narrow_the_same_every_time(dev):
         want = got
         gated_scan(u.detach(), g.detach(), bad, gate="sigmoid", output_final_state=True)
     torch.cuda.synchronize()
+
+
+def compare_all(name, got, want, off, dtype):
+    """As compare(), with the same NaN and infinities in the same places."""
+    have = got.double().cpu()
+    assert torch.equal(have.isnan(), want.isnan()), name
+    infinite, finite = want.isinf(), want.isfinite()
+    assert torch.equal(have[infinite], want[infinite]), name
+    compare(name, got.cpu()[finite], want[finite], off[finite], dtype)
+
+
+# tiles of 256 rows (128 in the backward) without spans, of 512 with spans, single channels
+@pytest.mark.parametrize("gate", ["value", "log", "sigmoid"])
+@pytest.mark.parametrize("C,n", [(300, 2500), (8, 20000), (7, 9000)])
+def test_infinite_states_go_on(dev, C, n, gate):
+    """An infinite state, or gradient, stays so through rows whose gates multiply to less
+    than fp32 holds, with the gates' signs, until a gate of exactly 0 makes it NaN; as row by row."""
+    from ssla_amd.scan import gated_scan
+    lens = [400, n, 50]
+    x = inputs(lens, C, F32, F32, gate, seed=11)
+    x["g"] = x["g"] * 0.5 if gate == "value" else x["g"] - 2
+    x["u"][420, 2], x["u"][430, 5], x["h0"][1, 3] = torch.inf, -torch.inf, torch.inf
+    x["u"][1000, 6] = torch.nan
+    x["do"][n + 300, 1], x["dht"][1, 0] = torch.inf, -torch.inf
+    if gate != "sigmoid":
+        x["g"][2000, 2] = x["g"][600, 4] = 0 if gate == "value" else -torch.inf
+    ref = ref_scan(x["u"], x["g"], lens, x["q"], gate, x["h0"], x["do"], x["dht"], EPS)
+    leaves = [x[k].to(dev).requires_grad_() for k in ("u", "g", "q", "h0")]
+    o, ht = gated_scan(*leaves[:2], offsets(lens).to(dev), q=leaves[2], gate=gate, initial_state=leaves[3], output_final_state=True)
+    grads = torch.autograd.grad((o, ht), leaves, (x["do"].to(dev), x["dht"].to(dev)))
+    for k, t in zip(("o", "ht", "du", "dg", "dq", "dh0"), (o.detach(), ht.detach(), *grads)):
+        compare_all(k, t, *ref[k], F32)
+    assert ref["o"][0][420:1900, 2].isinf().all() and ref["du"][0][500:n, 0].isinf().all()
