@@ -407,6 +407,10 @@ int ssla_diag_scan_bwd(const float *dout, const float *g, const float *h,
  * the forward fills for the backward.  The backward takes dout [T, C] and dht
  * (fp32 [n_seq, C] or NULL) and writes du, dq (dtype; dq only with q), dg
  * (g_dtype), all [T, C], and dh0 (fp32 [n_seq, C], may be NULL).
+ * The time axis is cut into pieces (up to 512 rows; up to 8,192 for C <= 256) whose
+ * gates are multiplied: gates larger than 1 in magnitude hold while such a product, and
+ * what the piece sums up from a zero state, stay inside fp32 (a zero state passes any
+ * product, and a gate of 0 empties a finite state whatever the gates beside it).
  * An infinite state (or gradient) goes on with the gates' signs until a gate of 0 makes
  * it NaN, as row by row.
  * At most 2^30 sequences.  Workspace: ssla_gated_scan_workspace_size bytes, 16-byte

@@ -179,9 +179,9 @@ __device__ __forceinline__ void show(T *p, T x) {
 // A product of gates too small for fp32, none of them 0, is held as +-2^-149 (kFaded: its
 // bits): an infinite state goes on, a finite one is off by 2^-149 of itself at most.
 constexpr uint32_t kFaded = 1;
-// The product A of factors; zero: one of them is 0.
+// The product A of factors; zero: one of them is 0 (whatever overflowed beside it).
 __device__ __forceinline__ float settled(float A, bool zero) {
-  return A == 0.f && !zero ? __uint_as_float((__float_as_uint(A) & 0x80000000u) | kFaded) : A;
+  return zero ? 0.f : A == 0.f ? __uint_as_float((__float_as_uint(A) & 0x80000000u) | kFaded) : A;
 }
 // (a factor that overflowed must not meet a state of zero)
 __device__ __forceinline__ float apply(float A, float x, float U) { return x == 0.f ? U : fmaf(A, x, U); }
@@ -411,13 +411,13 @@ __device__ __forceinline__ void each(F f) {
     for (int e = 0; e < W; ++e) f(i, e);
 }
 // The products A of a lane's gates(i, e), and a flag for each channel with a gate of 0.
-// A product of 0 is rare enough to look at the gates again (a count of them in
-// join_groups, on every tile's way, is 1 % of a call).
+// A product of 0 (or 0 times one that overflowed) is rare enough to look at the gates
+// again (a count of them in join_groups, on every tile's way, is 1 % of a call).
 template <int R, int W, typename F>
 __device__ __forceinline__ void settle(float (&A)[W], int *zeros, F gates) {
 #pragma unroll
   for (int e = 0; e < W; ++e)
-    if (A[e] == 0.f) {
+    if (!(fabsf(A[e]) > 0.f)) {
       bool zero = false;
 #pragma unroll
       for (int i = 0; i < R; ++i) zero |= gates(i, e) == 0.f;

@@ -182,8 +182,10 @@ def gated_scan(
 
     States are fp32; a long sequence is cut along time and the pieces' states are
     joined in their order, so results do not vary from call to call.  Over a piece
-    (up to 512 rows; 8,192 of up to 256 channels) the gates are multiplied: factors
-    larger than 1 in magnitude hold while such a product stays inside fp32.
+    (up to 512 rows; up to 8,192 in calls of at most 256 channels) the gates are
+    multiplied: factors larger than 1 in magnitude hold while such a product, and what
+    the piece sums up from a zero state, stay inside fp32 (a zero state passes any
+    product, and a gate of 0 empties a finite state whatever the gates beside it).
     An infinite state (or gradient) goes on with the gates' signs until a gate of 0
     (logarithms and logits below about -87 are 0 in fp32) makes it NaN, as row by row.
     Differentiable in u, g, q and the initial state (once, in reverse mode:

@@ -552,3 +552,69 @@ def test_infinite_states_go_on(dev, C, n, gate):
     for k, t in zip(("o", "ht", "du", "dg", "dq", "dh0"), (o.detach(), ht.detach(), *grads)):
         compare_all(k, t, *ref[k], F32)
     assert ref["o"][0][420:1900, 2].isinf().all() and ref["du"][0][500:n, 0].isinf().all()
+
+
+# two channel blocks or more without spans, with spans, single channels
+@pytest.mark.parametrize("gate", ["value", "log"])
+@pytest.mark.parametrize("C,n", [(300, 2500), (8, 20000), (7, 9000)])
+def test_gates_above_one(dev, C, n, gate):
+    """Gates around 1, whose products grow and fall by up to some powers of ten over a piece
+    of the time axis, in both directions."""
+    lens = [400, n, 50]
+    x = inputs(lens, C, F32, F32, "value", seed=12)
+    g = torch.randn(x["g"].shape, generator=torch.Generator().manual_seed(1)) * 0.02 + 0.0005
+    x["g"] = g if gate == "log" else torch.exp(g) * (1 - 2 * (x["g"] < 0.5).float())
+    assert float((g if gate == "log" else x["g"].abs().log()).cumsum(0).abs().max()) > 5
+    check(dev, lens, x, gate)
+    check(dev, lens, x, gate, read=False, state=False)
+
+
+def row_by_row(x, gate):
+    """One sequence in fp32, for where it passes fp32."""
+    a, slope = (x["g"], 1.0) if gate == "value" else (x["g"].exp(), x["g"].exp())
+    h, states = x["h0"][0], []
+    for t in range(x["u"].shape[0]):
+        states.append(h)
+        h = a[t] * h + x["u"][t]
+    states.append(h)
+    e, grads = x["dht"][0], []
+    for t in range(x["u"].shape[0] - 1, -1, -1):
+        grads.append(x["q"][t] * x["do"][t] + e)
+        e = a[t] * grads[-1]
+    h, s = torch.stack(states), torch.stack(grads[::-1])
+    return {"o": x["q"] * h[1:], "ht": h[-1:], "du": s, "dg": s * h[:-1] * slope, "dq": x["do"] * h[1:], "dh0": e[None]}
+
+
+@pytest.mark.parametrize("gate", ["value", "log"])
+@pytest.mark.parametrize("C,n", [(300, 2500), (8, 20000), (7, 9000)])
+def test_products_past_fp32(dev, C, n, gate):
+    """Gates whose product over a piece of the time axis passes fp32: a state, or gradient, of 0
+    stays 0, and a gate of 0 behind them (before them for gradients) empties any finite
+    state as it does row by row."""
+    from ssla_amd.scan import gated_scan
+    lens = [n]
+    x = inputs(lens, C, F32, F32, "value", seed=13)
+    x["g"] = x["g"].abs()
+    # forward: 1e-30 from row 500 on, times 8^64 over rows 640 .. 703, emptied at row 704
+    x["g"][500] = x["g"][704] = 0
+    x["g"][501:640], x["g"][640:704] = 1, 8
+    x["u"][500], x["u"][501:704] = 1e-30, 0
+    # backward: 1e-30 from row 1299 down, times 8^64 over rows 1164 .. 1101, emptied at row 1100
+    x["g"][1100] = x["g"][1300] = 0
+    x["g"][1101:1165], x["g"][1165:1300] = 8, 1
+    x["u"][1100:1300], x["do"][1100:1299], x["do"][1299] = 0, 0, 1e-30
+    # 0 in either direction through 8^200
+    x["g"][1500] = x["g"][1701] = 0
+    x["g"][1501:1701] = 8
+    x["u"][1500:1701], x["do"][1500:1701] = 0, 0
+    if gate == "log":
+        x["g"] = x["g"].log()
+    ref = ref_scan(x["u"], x["g"], lens, x["q"], gate, x["h0"], x["do"], x["dht"], EPS)
+    rows = row_by_row(x, gate)
+    leaves = [x[k].to(dev).requires_grad_() for k in ("u", "g", "q", "h0")]
+    o, ht = gated_scan(*leaves[:2], offsets(lens).to(dev), q=leaves[2], gate=gate, initial_state=leaves[3], output_final_state=True)
+    grads = torch.autograd.grad((o, ht), leaves, (x["do"].to(dev), x["dht"].to(dev)))
+    for k, t in zip(("o", "ht", "du", "dg", "dq", "dh0"), (o.detach(), ht.detach(), *grads)):
+        compare_all(k, t, torch.where(rows[k].isfinite(), ref[k][0], rows[k].double()), ref[k][1], F32)
+    # (the gradients of rows 639 to 500 are 8^64 = 6e57 of row 703's: infinite in fp32, NaN behind the gate of 0)
+    assert rows["o"].isfinite().all() and rows["du"][704:].isfinite().all() and rows["du"][500:640].isinf().all()
