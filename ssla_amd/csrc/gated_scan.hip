@@ -36,12 +36,14 @@ namespace {
 
 constexpr int kValue = SSLA_GATE_VALUE, kLog = SSLA_GATE_LOG, kSigmoid = SSLA_GATE_SIGMOID;
 
-// e^x with the product x log2(e) in two parts: off by 4 2^-24 at any x whose e^x is a
-// normal number (e^x of one product by up to 100 2^-24).
+// e^x with the product x log2(e) in two parts: off by 4 2^-24 (e^x of one product by up to
+// 100 2^-24) at any x whose e^x is a normal number and, unless UP, at most 2^126.
+template <bool UP>
 __device__ __forceinline__ float exp_of(float x) {
   const float y = x * kLog2e, e = fast_exp2(y);
   const float lo = fmaf(x, 1.925963e-8f, fmaf(x, kLog2e, -y));
-  return fabsf(y) < 126.f ? fmaf(e, lo * 0.6931472f, e) : e;   // (past that 0, infinite or near it)
+  const bool inside = UP ? y >= -126.f && y < 128.f : fabsf(y) <= 126.f;   // (past that 0, infinite or next to it)
+  return inside ? fmaf(e, lo * 0.6931472f, e) : e;
 }
 
 // The gate; and with its derivative, sigmoid's from e^-|g|: both it and 1 - it keep
@@ -50,13 +52,13 @@ struct Gate { float a, slope; };
 template <int KIND>
 __device__ __forceinline__ float gate_value(float g) {
   if constexpr (KIND == kValue) return g;
-  if constexpr (KIND == kLog) return exp_of(g);
-  return __builtin_amdgcn_rcpf(1.f + exp_of(-g));   // (e^-g infinite: 0)
+  if constexpr (KIND == kLog) return exp_of<true>(g);
+  return __builtin_amdgcn_rcpf(1.f + exp_of<false>(-g));   // (e^-g infinite: 0; past 2^126 no normal number)
 }
 template <int KIND>
 __device__ __forceinline__ Gate gate_of(float g) {
   if constexpr (KIND == kSigmoid) {
-    const float t = exp_of(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + t), s = t * r;
+    const float t = exp_of<false>(-fabsf(g)), r = __builtin_amdgcn_rcpf(1.f + t), s = t * r;
     return {g >= 0.f ? r : s, r * s};
   }
   const float a = gate_value<KIND>(g);

@@ -618,3 +618,36 @@ def test_products_past_fp32(dev, C, n, gate):
         compare_all(k, t, torch.where(rows[k].isfinite(), ref[k][0], rows[k].double()), ref[k][1], F32)
     # (the gradients of rows 639 to 500 are 8^64 = 6e57 of row 703's: infinite in fp32, NaN behind the gate of 0)
     assert rows["o"].isfinite().all() and rows["du"][704:].isfinite().all() and rows["du"][500:640].isinf().all()
+
+
+def test_log_gates_to_the_ends_of_fp32(dev):
+    """e^g, and the gate's gradient, wherever e^g is a normal number: off by 4 U of itself (the
+    unit's 2, and two roundings of the correction), the gradient's products of 1 exact."""
+    from ssla_amd.scan import gated_scan, sparse_gated_step
+    g = torch.cat([torch.linspace(lo, hi, 4096) for lo, hi in ((-87.33654, -87), (-87, 87), (87, 88.72283), (-1, 1))])
+    g = g.clamp(min=-87.33654, max=88.72283).view(64, 256).to(dev)
+    want = g.double().exp()
+    assert float(want.min()) >= torch.finfo(F32).tiny and float(want.max()) <= torch.finfo(F32).max
+    none, one = torch.zeros_like(g), torch.ones_like(g)
+    leaf = g.clone().requires_grad_()
+    o, _ = gated_scan(none, leaf, torch.arange(65, device=dev), gate="log", initial_state=one)
+    (dg,) = torch.autograd.grad(o, leaf, one)
+    step = sparse_gated_step(torch.arange(64, device=dev), none, g, one.clone(), gate="log")
+    for name, got in (("scan", o.detach()), ("gradient", dg), ("step", step)):
+        off = (got.double() - want).abs() / want * 2 ** 24
+        assert float(off.max()) <= 4, (name, float(off.max()), float(g.flatten()[off.argmax()]))
+
+
+def test_logits_to_the_end_of_fp32(dev):
+    """The sigmoid of a logit, wherever it is a normal number, by the 10 U of the bound above."""
+    from ssla_amd.scan import gated_scan, sparse_gated_step
+    g = torch.cat([torch.linspace(lo, hi, 4096) for lo, hi in ((-87.33654, -87), (-87, -1), (-1, 1), (1, 120))])
+    g = g.clamp(min=-87.33654).view(64, 256).to(dev)
+    want = 1 / (1 + torch.exp(-g.double()))
+    assert float(want.min()) >= torch.finfo(F32).tiny
+    none, one = torch.zeros_like(g), torch.ones_like(g)
+    o, _ = gated_scan(none, g, torch.arange(65, device=dev), gate="sigmoid", initial_state=one)
+    step = sparse_gated_step(torch.arange(64, device=dev), none, g, one.clone(), gate="sigmoid")
+    for name, got in (("scan", o), ("step", step)):
+        off = (got.double() - want).abs() / want * 2 ** 24
+        assert float(off.max()) <= 10, (name, float(off.max()), float(g.flatten()[off.argmax()]))
