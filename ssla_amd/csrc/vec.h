@@ -13,14 +13,17 @@ struct Vec {
     else Elem<DT>::store(e, i, x);
   }
 };
+// The border that a vector's address lies at: 16 bytes at most, as the callers check.
+template <int DT, int W>
+constexpr size_t vec_border() { return sizeof(Vec<DT, W>) < 16 ? sizeof(Vec<DT, W>) : 16; }
 template <int DT, int W>
 __device__ __forceinline__ Vec<DT, W> load_vec(const void *p, int64_t i) {
-  struct __attribute__((aligned(sizeof(Vec<DT, W>)))) A { Vec<DT, W> v; };
+  struct __attribute__((aligned((vec_border<DT, W>())))) A { Vec<DT, W> v; };
   return reinterpret_cast<const A *>(static_cast<const typename Elem<DT>::T *>(p) + i)->v;
 }
 template <int DT, int W>
 __device__ __forceinline__ void store_vec(void *p, int64_t i, const Vec<DT, W> &x) {
-  struct __attribute__((aligned(sizeof(Vec<DT, W>)))) A { Vec<DT, W> v; };
+  struct __attribute__((aligned((vec_border<DT, W>())))) A { Vec<DT, W> v; };
   reinterpret_cast<A *>(static_cast<typename Elem<DT>::T *>(p) + i)->v = x;
 }
 

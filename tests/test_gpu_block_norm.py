@@ -507,3 +507,28 @@ def test_rows_past_32_bits(dev):
     _, s = residual_norm(x.detach(), torch.zeros_like(r), p=0.25, seed=11, subsequence=3)
     keep = block.dropout_keep(16 * C, 0.25, 11, 3, first=(N - 16) * C).view(16, C)
     assert torch.equal(s[last].cpu() != 0, keep & (x.detach()[last].cpu() != 0))
+
+
+def test_tensors_at_odd_16_byte_borders(dev):
+    """Inputs and outputs of the C entries at 16-byte borders that are no 32-byte ones: a row of
+    8 values of an fp32 stream beside 16-bit ones is 32 bytes."""
+    from ssla_amd import _lib
+    N, C = 37, 96
+    x, r, w, b, gamma, w2, dy, ds = (t.to(dev) for t in residual_case((N, C), B16, F32, seed=9))
+    lib, P, st = _lib.load(), _lib.ptr, _lib.stream_of(x)
+    ws = torch.empty(lib.ssla_residual_norm_bwd_workspace_size(N, C), dtype=torch.uint8, device=dev)
+
+    def run(bytes_off):
+        def lay(t):
+            n = bytes_off // t.element_size()
+            return torch.cat([t.new_zeros(n), t.reshape(-1)])[n:].view(t.shape)
+        a, s, d, e, y, total, dx, dr = map(lay, (x, r, dy, ds, x, r, x, r))
+        sums = [torch.empty_like(w) for _ in range(4)]
+        assert all(t.data_ptr() % 32 == bytes_off for t in (a, s, d, e, y, total, dx, dr))
+        _lib.check(lib.ssla_residual_norm_fwd(P(a), P(s), N, C, 0, P(w), P(b), 1e-5, 1.0, P(gamma), 1, P(w2), 0.0, None, 0,
+                                              P(y), P(total), _lib.SSLA_BF16, _lib.SSLA_F32, st), "fwd")
+        _lib.check(lib.ssla_residual_norm_bwd(P(d), P(e), P(a), P(s), N, C, 0, P(w), 1e-5, 1.0, P(gamma), 1, P(w2), 0.0, None,
+                                              0, P(dx), P(dr), *map(P, sums), _lib.SSLA_BF16, _lib.SSLA_F32, P(ws), ws.numel(),
+                                              st), "bwd")
+        return y, total, dx, dr, *sums
+    assert all(torch.equal(p, q) for p, q in zip(run(0), run(16)))
