@@ -849,6 +849,7 @@ ScanPlan plan_of(int64_t T, int C, int W, int R) {
   return p;
 }
 constexpr size_t kHead = 256;   // the ticket's line
+constexpr int64_t kMostThreads = 0xffffffff;   // of a launch
 int64_t word_count(const ScanPlan &p, int W) {   // words and hints
   const int64_t spans = p.tiles >> p.span;
   return ((p.span ? p.tiles : 0) + spans) * p.cblocks * p.CT * W + (spans * p.cblocks + 1) / 2;
@@ -889,7 +890,7 @@ int launch_scan(const char *what, ScanArgs &a, int W, int R, Kernel kernel, Kern
     set_error("%s: needs %zu bytes of workspace, got %zu", what, ws_bytes(a.T, a.C), workspace_bytes);
     return SSLA_ERR_WORKSPACE;
   }
-  if (p.tiles * p.cblocks > 0x3fffffff) {
+  if (p.tiles * p.cblocks > kMostThreads / kBlock) {
     set_error("%s: too many workgroups", what);
     return SSLA_ERR_UNSUPPORTED;
   }
@@ -995,7 +996,7 @@ extern "C" int ssla_sparse_gated_step(const int32_t *row_idx, int n_active, cons
   StepArgs a{row_idx, u, g, q, ldu, ldg, ldq, state, o, status, n_active, n_rows, C, gate};
   const int W = widest(C, 4, {{u, ldu, dtype}, {g, ldg, g_dtype}, {q, q ? ldq : 0, dtype}, {o, C, dtype}});
   const int64_t blocks = (static_cast<int64_t>(n_active) * (C / W) + 255) / 256;
-  if (blocks > 0x7fffffff) {
+  if (blocks > kMostThreads / 256) {
     set_error("sparse_gated_step: too many workgroups");
     return SSLA_ERR_UNSUPPORTED;
   }

@@ -103,3 +103,21 @@ def test_entries_refuse_more_sequences_than_they_count():
     assert lib.ssla_gated_scan_bwd(16, 8, 16, 8, None, 0, 16, n, 4, 8, 0, None, 16, 16, None, 16, 16, None, None, 0, 0, None, 0,
                                    None) == _lib.SSLA_ERR_UNSUPPORTED
     assert lib.ssla_sparse_gated_step(16, n, 16, 8, 16, 8, None, 0, 16, 5, 8, 0, 16, None, 0, 0, None) == _lib.SSLA_ERR_UNSUPPORTED
+
+
+def test_entries_refuse_more_workgroups_than_a_launch_holds():
+    """A launch's threads are counted in 32 bits: 2^32 rows of one channel are 2^23 tiles of
+    512 rows and 512 threads (twice that in the backward), one more than it holds."""
+    lib = _lib.load()
+    T = 1 << 32
+    size = lib.ssla_gated_scan_workspace_size(T, 1)
+    assert lib.ssla_gated_scan_fwd(16, 1, 16, 1, None, 0, 16, 1, T, 1, 0, None, 16, None, None, 1, 1, 16, size,
+                                   None) == _lib.SSLA_ERR_UNSUPPORTED
+    assert b"workgroups" in lib.ssla_last_error()
+    assert lib.ssla_gated_scan_bwd(16, 1, 16, 1, None, 0, 16, 1, T // 2, 1, 0, None, 16, 16, None, 16, 16, None, None, 1, 1, 16, size,
+                                   None) == _lib.SSLA_ERR_UNSUPPORTED
+    assert b"workgroups" in lib.ssla_last_error()
+    n = 1 << 30   # single tokens, a thread a channel of 5: 5 2^30 threads
+    assert lib.ssla_sparse_gated_step(16, n, 16, 5, 16, 5, None, 0, 16, 5, 5, 0, 16, None, 0, 0,
+                                      None) == _lib.SSLA_ERR_UNSUPPORTED
+    assert b"workgroups" in lib.ssla_last_error()
