@@ -38,9 +38,10 @@ def _seed(name, seed, subsequence, device):
 
 
 def _p(name, p):
+    """p in whole steps of 2^-16 (which fp32 holds)."""
     if not isinstance(p, numbers.Real) or not 0 <= p <= 1:
         raise ValueError(f"{name}: p must lie in [0, 1], got {p!r}")
-    return float(p)
+    return round(float(p) * 65536) / 65536
 
 
 def _drop(x, p, seed, subsequence):

@@ -321,7 +321,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
     elif scale is not None:
         alpha = float(scale)
     w, b, w2 = (_weight(name, nm, t, C) for nm, t in (("weight", weight), ("bias", bias), ("post_weight", post_weight)))
-    p = _p(name, p)
+    steps = _p(name, p)
     tensors = x, residual, weight, bias, scale if gamma is not None else None, post_weight
     _lib.require_no_tangent(name, *tensors)
     dev = _lib.require_cuda(*tensors)
@@ -330,7 +330,7 @@ def residual_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torc
     seed = _seed(name, seed, subsequence, dev) if p > 0 else None
     flat = x.dim() == 2
     rows, r = (_whole(t) if flat else _whole(t).view(-1, C) for t in (x, residual))
-    options = float(eps), KINDS[kind], alpha, int(bool(post_norm)), p, subsequence
+    options = float(eps), KINDS[kind], alpha, int(bool(post_norm)), steps, subsequence
     grad = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
     y, s = (ResidualNormFunction.apply if grad else _residual_forward)(rows, r, w, b, gamma, w2, seed, options)
     return (y, s) if flat else (y.view(x.shape), s.view(x.shape))

@@ -138,3 +138,12 @@ def test_tangents_are_refused():
                 t = list(args)
                 t[i] = forward_ad.make_dual(t[i], torch.ones_like(t[i]))
                 f(*t)
+
+
+def test_probabilities_are_rounded_once():
+    """p counts in steps of 2^-16, t = round(p 2^16): one beside the middle of two steps is not
+    rounded to fp32, which holds the middle, before."""
+    from ssla_amd.dropout import _p
+    for p in (19660.5 / 65536 + 1e-10, 19661.5 / 65536 - 1e-10, 0.1, 0.0, 1.0, 2.0 ** -17 + 1e-12, 2.0 ** -18, 1 - 1e-9):
+        t = round(p * 65536)
+        assert torch.tensor(_p("f", p), dtype=torch.float32).double().item() * 65536 == t, p

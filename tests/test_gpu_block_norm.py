@@ -532,3 +532,17 @@ def test_tensors_at_odd_16_byte_borders(dev):
                                               st), "bwd")
         return y, total, dx, dr, *sums
     assert all(torch.equal(p, q) for p, q in zip(run(0), run(16)))
+
+
+def test_probabilities_beside_the_middle_of_two_steps(dev):
+    """t = round(p 2^16) of the given p, not of its fp32 value: elements whose bits are the step
+    between them stay or go by it."""
+    from ssla_amd.dropout import counter_dropout
+    from ssla_amd.norm import residual_norm
+    n = 1 << 20
+    x = torch.ones(n // 1024, 1024, device=dev)
+    for p in (19660.5 / 65536 + 1e-10, 19661.5 / 65536 - 1e-10):
+        keep = block.dropout_keep(n, p, 6)
+        assert not torch.equal(keep, block.dropout_keep(n, float(torch.tensor(p, dtype=torch.float32)), 6))
+        assert torch.equal((counter_dropout(x, p, 6) != 0).cpu().view(-1), keep)
+        assert torch.equal((residual_norm(x, 0 * x, p=p, seed=6)[1] != 0).cpu().view(-1), keep)
