@@ -555,9 +555,12 @@ struct RowPlan {
   bool full, wide;
   int64_t slots, blocks, rows;   // rows: of sums
 };
-// Wavefronts: the forward's lane groups have a few rows each, the backward's as many as
-// run at once (three workgroups a CU, of wide rows one): their sums over rows go through
-// memory once a workgroup.
+// Wavefronts: the forward's lane groups have a few rows each, the backward's about as many
+// as run at once: their sums over rows go through memory once a workgroup.  Three
+// workgroups a CU fit where a lane has 168 registers or less: all gated ones, and residual
+// ones of 16-bit tensors in vectors of 8 (149 to 168); of fp32 (169 to 200) and some odd
+// widths or vectors of 4 twice (171 to 183) two fit, and a third of the workgroups run behind the
+// others.  Of 1,024 threads one fits.
 constexpr int64_t kFwdWaves = 256 * 32, kBwdWaves[3] = {256 * 12, 256 * 8, 256 * 16};   // (256 CUs; workgroups of 256, 512, 1,024 threads)
 
 RowPlan plan_of(int64_t N, int per, int G, int W, int dtype, bool bwd) {   // W 0: no vectors

@@ -24,7 +24,7 @@
 // The backward does the same from the last tile on; the states it needs come from
 // the forward, which leaves one every 64 rows, and are computed again in between.
 // Measured: 65,536 rows of 1,024 channels, bf16, with q 133 us (4.0 TB/s; vector units
-// busy 40 % of the time, wavefronts waiting 58 %); 8 x 4,096 rows forward 74, backward 127;
+// busy 41 % of the time, wavefronts waiting 58 %); 8 x 4,096 rows forward 74, backward 127;
 // 65,536 sequences of one row 231 with their states (4.6 TB/s); 912 single tokens of
 // 2,048 channels 5.9 (5.1 TB/s).
 #include "vec.h"
@@ -414,7 +414,8 @@ __device__ __forceinline__ void each(F f) {
 }
 // The products A of a lane's gates(i, e), and a flag for each channel with a gate of 0.
 // A product of 0 (or 0 times one that overflowed) is rare enough to look at the gates
-// again (a count of them in join_groups, on every tile's way, is 1 % of a call).
+// again: a count of them in join_groups, on every tile's way, is 1 % of any call, this
+// 2 to 3 % of calls with gates of 0 in most tiles.
 template <int R, int W, typename F>
 __device__ __forceinline__ void settle(float (&A)[W], int *zeros, F gates) {
 #pragma unroll
@@ -475,7 +476,9 @@ __device__ __forceinline__ void empty_states(const ScanArgs &a, const float *fro
 }
 
 // ------------------------------------------------------------------ forward --
-// Two workgroups a CU (128 registers) in 16 bits; fp32 values do without the second one
+// Two workgroups a CU (128 registers; the LDS holds no third) in 16 bits: measured in bf16,
+// which spills none (7 with fp32 gates), while fp16 with a read-out gate spills 10 to 19
+// (65,536 rows of 1,024 channels 150 us, bf16 131).  fp32 values do without the second one
 // sooner than without registers (8 x 4,096 rows: 130 us, 162 at 128 registers).
 template <int DT, int DTG, int W, bool READ, int SPAN>
 __global__ __launch_bounds__(kBlock) __attribute__((amdgpu_waves_per_eu(DT == SSLA_F32 ? 2 : 4))) void scan_fwd_kernel(const ScanArgs a) {
